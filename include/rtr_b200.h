@@ -98,8 +98,8 @@ int rtr_session_create(const rtr_model_config* cfg, int device, rtr_session** ou
 int rtr_session_create_batched(const rtr_model_config* cfg, int device, int32_t max_users, rtr_session** out);
 int rtr_session_destroy(rtr_session* s);
 
-/* Text of the last error of this session (or of the last failed create when
- * s is NULL).  Valid until the next call on the session. */
+/* Text of the last error of this session (when s is NULL: of this thread's last
+ * failed call without a session).  Valid until the next call on the session. */
 const char* rtr_last_error(const rtr_session* s);
 
 /* Issue all work of the session on this cudaStream_t (NULL = session-owned
@@ -292,6 +292,82 @@ int rtr_constraint_process(rtr_session* s, int32_t step, const int64_t* input_id
  *   - blocks until the scores are written. */
 int rtr_constraint_process_static(rtr_session* s, int32_t step, const int64_t* input_ids_dev,
                                   int32_t rows, int32_t cols, const float* scores_dev, float* out_dev);
+
+/* ---- 8-bit KV cache --------------------------------------------------------
+ * K and V of many sequences (users' histories) kept beside or between requests
+ * in a quarter of the fp32 bytes: e4m3 codes in pages, with one float32 scale for
+ * each page and KV head.  No counterpart in the reference, whose prefix lives for
+ * one request (shared_prefix.py:67-89).  These calls need no session: they take
+ * the buffers, a device and a cudaStream_t (NULL: the default stream), enqueue
+ * their kernels and return; every buffer is the caller's and must live until
+ * they ran.  They may be captured into a CUDA graph.  rtr_last_error(NULL) has
+ * the text of a refusal.
+ *
+ * A value is code * scale.  Code [page][head][token][dim] lies at
+ * page * page_stride + head * head_stride + token * head_dim + dim, its scale at
+ * page * scale_stride + head.  head_dim 64 or 128, page 16, 32, 64 or 128 tokens;
+ * strides of codes and their addresses are multiples of 16.  `status` is a device
+ * word that the kernels set bits in (never clear): 1 << 5 a length or row range
+ * that does not fit, 1 << 9 a page number outside [0, pages), 1 << 10 an old scale
+ * that is not positive and finite.  The work concerned is left out (attention:
+ * rows of NaN; where starts itself is at fault those rows are undefined), memory
+ * outside the buffers is never touched. */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t page_stride, head_stride, scale_stride; /* elements */
+  int32_t pages, kv_heads, page, head_dim;
+  uint32_t* status;
+} rtr_kv_cache;
+
+/* Sequences of one call and their rows (device arrays).  Sequence b's i-th page is
+ * table[b * table_stride + i], i < table_width; it holds lens[b] tokens.  Rows
+ * starts[b] .. starts[b + 1] - 1 of the call's `rows` are its rows (starts has
+ * seqs + 1 entries, not decreasing); without starts each has rows / seqs.  Rows
+ * before starts[0] and from starts[seqs] on belong to none and are not touched. */
+typedef struct {
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts;
+  int64_t table_stride;
+  int32_t table_width, seqs, rows;
+} rtr_kv_batch;
+
+/* Quantise k and v rows (row r, head h, dim d at r * token_stride + h * head_stride
+ * + d; RTR_DTYPE_*; addresses and strides multiples of 16 bytes) into the cache as
+ * the last positions of their sequences: lens already counts them.  A page's scale
+ * is the least power of two in [2^-48, 2^48] at which its largest magnitude is at
+ * most 448; a page that already holds older tokens of the sequence keeps its scale
+ * if that is larger, and has their codes rounded again if it is smaller.  Codes are
+ * rounded to nearest even; NaN, infinities and magnitudes above 448 * 2^48 become
+ * NaN.  Codes behind a sequence's last token stay.  The pages that a call writes
+ * must be different ones: two sequences that share such a page leave either's codes. */
+int rtr_kv_write(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const void* k_dev, const void* v_dev,
+                 int32_t dtype, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                 int64_t v_head_stride, int32_t device, void* stream);
+
+/* The reverse: each sequence's last starts[b + 1] - starts[b] tokens as dense rows,
+ * rounded once to dtype. */
+int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_dev, void* v_dev, int32_t dtype,
+                int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                int32_t device, void* stream);
+
+/* out[r][h] = softmax(scale * q[r][h] . K^T) V, K and V [h / (heads / kv_heads)] of
+ * the row's sequence.  causal: a sequence's n rows stand at its last n positions and
+ * see what is not behind them; otherwise each sees all lens[b] tokens.  Rows that see
+ * nothing are 0.  q: row r, head h at r * q_token_stride + h * head_dim; out
+ * [rows][heads][head_dim], same dtype; lse_dev (optional, float32 [rows][heads]):
+ * log of the softmax's sum, minus infinity for rows that see nothing.  fp32 q and
+ * weights enter the tensor cores as fp16 pairs (22 bits); sums are fp32.  V scales
+ * must lie in [2^-48, 2^48] (others make the row NaN).  The workspace must hold
+ * rtr_kv_attention_workspace bytes, aligned to 16, and is free again when the call's
+ * kernels ran: calls that may overlap need one each.  A table row wider than the
+ * sequences need costs idle blocks. */
+int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t heads, int32_t device,
+                               int64_t* bytes);
+int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const void* q_dev, int32_t dtype,
+                     int32_t heads, int64_t q_token_stride, int32_t causal, float scale, void* out_dev, float* lse_dev,
+                     void* workspace_dev, int64_t workspace_bytes, int32_t device, void* stream);
 
 /* ---- synthetic workload --------------------------------------------------- */
 

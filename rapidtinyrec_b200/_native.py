@@ -24,7 +24,8 @@ EXPORTS = (
     'rtr_synth_fill_host', 'rtr_synth_fill_device', 'rtr_launch', 'rtr_wait', 'rtr_get_report',
     'rtr_profile_gemms', 'rtr_constraint_process_static', 'rtr_gemm_check',
     'rtr_session_create_batched', 'rtr_launch_batch', 'rtr_wait_batch', 'rtr_generate_batch',
-    'rtr_debug_wait_control', 'rtr_attention_check',
+    'rtr_debug_wait_control', 'rtr_attention_check', 'rtr_kv_write', 'rtr_kv_read',
+    'rtr_kv_attention_workspace', 'rtr_kv_attention',
 )
 
 
@@ -63,6 +64,19 @@ class ReportC(ctypes.Structure):
 
     def as_dict(self):
         return {name: int(getattr(self, name)) for name, _ in self._fields_}
+
+
+class KvCacheC(ctypes.Structure):
+    _fields_ = [('k', ctypes.c_void_p), ('v', ctypes.c_void_p), ('k_scale', ctypes.c_void_p),
+                ('v_scale', ctypes.c_void_p), ('page_stride', ctypes.c_int64), ('head_stride', ctypes.c_int64),
+                ('scale_stride', ctypes.c_int64), ('pages', ctypes.c_int32), ('kv_heads', ctypes.c_int32),
+                ('page', ctypes.c_int32), ('head_dim', ctypes.c_int32), ('status', ctypes.c_void_p)]
+
+
+class KvBatchC(ctypes.Structure):
+    _fields_ = [('table', ctypes.c_void_p), ('lens', ctypes.c_void_p), ('starts', ctypes.c_void_p),
+                ('table_stride', ctypes.c_int64), ('table_width', ctypes.c_int32), ('seqs', ctypes.c_int32),
+                ('rows', ctypes.c_int32)]
 
 
 class NativeError(RuntimeError):
@@ -115,6 +129,10 @@ def load():
         'rtr_constraint_process_static': (P, I32, P, I32, I32, P, P),
         'rtr_debug_wait_control': (I32, I64, I32),
         'rtr_attention_check': (I32, P, P, P, P, I32, I32, I32, I32, I32),
+        'rtr_kv_write': (P, P, P, P, I32, I64, I64, I64, I64, I32, P),
+        'rtr_kv_read': (P, P, P, P, I32, I64, I64, I64, I64, I32, P),
+        'rtr_kv_attention_workspace': (P, P, I32, I32, ctypes.POINTER(I64)),
+        'rtr_kv_attention': (P, P, P, I32, I32, I64, I32, F, P, P, P, I64, I32, P),
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

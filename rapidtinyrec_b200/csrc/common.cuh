@@ -24,6 +24,8 @@ enum : uint32_t {
   RTR_DEV_TOO_MANY_CAND = 1u << 6,  // candidate buffer overflow
   RTR_DEV_NAN_SCORE = 1u << 7,      // a NaN score (ranked as -inf)
   RTR_DEV_TIMEOUT = 1u << 8,        // a bounded pipeline wait expired (kernel gave up)
+  RTR_DEV_BAD_PAGE = 1u << 9,       // 8-bit KV cache: page number outside the cache
+  RTR_DEV_BAD_SCALE = 1u << 10,     // 8-bit KV cache: scale that is not positive and finite
 };
 
 RTR_DEVICE float warp_sum(float v) {

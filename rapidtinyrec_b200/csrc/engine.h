@@ -7,6 +7,9 @@
 
 namespace rtr {
 
+// Keeps msg for rtr_last_error(NULL) of this thread; returns code.
+int set_error(int code, const char* msg);
+
 enum Epilogue : int { EPI_STORE = 0, EPI_BIAS = 1, EPI_RESID = 2, EPI_SWIGLU = 3, EPI_ROPE = 4 };
 
 // EPI_ROPE (tensor-core GEMM only): the q/k/v projection's epilogue adds the

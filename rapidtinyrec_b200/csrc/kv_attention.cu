@@ -1,0 +1,573 @@
+// Attention over the 8-bit KV cache: softmax(scale q K^T) V of new query rows
+// over sequences whose K and V are e4m3 codes in pages, with one scale a page.
+//
+// Mathematics.  With codes c and scales s the score of key j is
+// scale * s_k(page of j) * (q . ck_j); the scale multiplies the finished dot
+// product, so the codes enter the matrix instructions as they are (e4m3 is exact
+// in fp16).  One pass over the keys keeps, per row, a running maximum M of
+// score * log2(e) + log2(s_v), the weights w_j = 2^(score log2(e) + log2 s_v - M),
+// the sum of w_j cv_j and the softmax's own sum of w_j / s_v: the V scale costs an
+// addition in the exponent, every weight is at most 1 whatever the scales are,
+// and both sums end up relative to the same M.
+//
+// Rows.  The query rows of one KV head are its (token, head of the group) pairs.
+// A block takes a tile of them and a stretch of the sequence's keys; the keys are
+// split over blocks while there are fewer tiles than the GPU has room for, and a
+// second kernel joins the stretches.
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "engine.h"
+#include "kv_cache.cuh"
+#include "kv_host.h"
+
+namespace rtr {
+
+struct KvAttn {
+  KvCache c;
+  KvBatch b;
+  const void* q;
+  int64_t q_token;     // elements between a token's rows; heads are contiguous
+  int heads, group;    // query heads, and those of one KV head
+  int causal;
+  float factor;        // softmax scale * log2(e)
+  void* out;           // [rows][heads][head_dim]
+  float* lse;          // [rows][heads] or null
+  float* part;         // [rows * heads][splits][head_dim] when splits > 1
+  float2* ml;          // [rows * heads][splits]: running maximum, sum
+  int per_seq;         // row tiles of a sequence without starts
+  int chunk, splits;   // keys of a block, and the blocks of a row tile
+};
+
+constexpr int KA_WARPS = 4, KA_ROWS = 8, KA_KEYS = 16, KA_STAGES = 4;
+constexpr int KA_MAX_CHUNK = 2048;  // 32 key groups a warp: their page numbers and scales fit its lanes
+// Weights enter the fp16 operand times 2^12: the largest is 4096, and 2^-24
+// (fp16's smallest) is 2^-36 of it.
+constexpr float KA_LIFT = 12.0f;
+
+template <int D> struct KaCfg {
+  static constexpr int STAGE = 2 * KA_KEYS * D;  // K and V of one key group
+  static constexpr int WARP_BYTES = KA_STAGES * STAGE;
+  static constexpr int LD = D + 4;               // row of the joining buffer, floats
+  static constexpr int RING = KA_WARPS * WARP_BYTES;
+  static constexpr int JOIN = KA_WARPS * KA_ROWS * LD * 4;
+  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+};
+
+RTR_DEVICE float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+RTR_DEVICE void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+RTR_DEVICE uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+RTR_DEVICE uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+RTR_DEVICE float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// Whether one of four codes is NaN (0x7f or 0xff).
+RTR_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// Where 16-byte piece `ch` of key row `row` lies in a stage: pieces are permuted
+// within 128 bytes so that the rows g, g + 1 that eight lanes read of K, and the
+// rows 0, 2, 4, 6 (or 1, 3, 5, 7) that they read of V, lie in different banks.
+template <int D> RTR_DEVICE int ka_at(int row, int ch) {
+  if constexpr (D == 128) {
+    return row * 128 + ((ch ^ (row & 6) ^ ((row & 1) << 2)) << 4);
+  } else {
+    const int line = row >> 1;
+    return line * 128 + (((((row & 1) << 2) + ch) ^ ((line & 3) << 1)) << 4);
+  }
+}
+
+// One block: KA_ROWS query rows, up to `chunk` keys.  Its warps take 16-key groups
+// in turn, each with its own running maximum, and are joined at the end.
+//
+// The products are transposed (keys as the 16 rows of an m16n8k16, query rows as
+// its 8 columns), so a group of up to 8 query heads fills the instruction.  Which
+// dimension sits where in a contraction is free, as long as both operands agree:
+// a lane takes 16 consecutive codes of a key for q . k and, of the keys it needs
+// for P V, 16 consecutive dimensions, so both operands come from shared memory by
+// 16-byte loads and the transposition of V is byte permutes in registers.
+//
+// fp32 queries (and weights) enter as fp16 pairs, hi + lo: 22 significant bits.
+template <typename T, int D>
+__global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const KvAttn a) {
+  using C = KaCfg<D>;
+  constexpr bool PAIR = std::is_same<T, float>::value;
+  constexpr int KW = D / 16;   // 4-code words of a key a lane holds: one q . k instruction each
+  constexpr int VW = D / 32;   // words of a V row a lane holds
+  constexpr int DG = D / 8;    // dimensions of the output a lane holds, for two rows
+  extern __shared__ __align__(128) uint8_t ka_smem[];
+  __shared__ int slot;
+  __shared__ float join_m[KA_WARPS][KA_ROWS], join_l[KA_WARPS][KA_ROWS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+
+  int seq;
+  int64_t item0;
+  if (a.b.starts) {
+    seq = kv_find_seq(a.b, blockIdx.x, a.group, 3, 1, &slot, item0);
+    if (seq < 0) return;
+  } else {
+    seq = (int)blockIdx.x / a.per_seq;
+    item0 = (int64_t)seq * a.per_seq;
+  }
+  int first, count, len;
+  const bool whole = kv_rows(a.b, seq, 0, (int64_t)a.b.table_width << a.c.page_shift, a.c.status, first, count, len);
+  if (!whole) {
+    if (count < 0) return;
+    len = 0;  // a length that does not fit: the sequence's rows become NaN
+  }
+  const int nrows = count * a.group, r0 = (int)(blockIdx.x - item0) * KA_ROWS;
+  if (r0 >= nrows) return;
+  // keys that a row of token t sees
+  auto limit = [&](int row) { return a.causal ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
+  const int kmin = limit(r0), kmax = limit(r0 + KA_ROWS - 1);
+  const int c0 = split * a.chunk, c1 = min(kmax, c0 + a.chunk);
+  if (c1 <= c0 && split > 0) {  // a stretch behind the last key (the first one reports rows that see nothing)
+    if (tid < KA_ROWS && r0 + tid < nrows) {
+      const int rr = r0 + tid;
+      const int64_t rh = (int64_t)(first + rr / a.group) * a.heads + kvh * a.group + rr % a.group;
+      a.ml[rh * a.splits + split] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  const int groups = c1 > c0 ? (c1 - c0 + KA_KEYS - 1) / KA_KEYS : 0;
+  const int n = (groups - warp + KA_WARPS - 1) / KA_WARPS;  // this warp's groups: warp, warp + 4, ...
+
+  // lane i: the page and the scales of this warp's i-th group
+  int64_t at = -1;
+  float ks = 0.f, lvs = 0.f, ivs = 0.f;
+  if (lane < n) {
+    const int key = c0 + KA_KEYS * (warp + KA_WARPS * lane);
+    const int page = kv_page(a.c, a.b, seq, key >> a.c.page_shift);
+    ks = lvs = __int_as_float(0x7fffffff);  // a page that is not there makes the rows NaN
+    if (page >= 0) {
+      at = page * a.c.page_stride + kvh * a.c.head_stride + (int64_t)(key & ((1 << a.c.page_shift) - 1)) * D;
+      ks = a.c.k_scale[page * a.c.scale_stride + kvh];
+      const float vs = a.c.v_scale[page * a.c.scale_stride + kvh];
+      if (vs >= 1.0f / 281474976710656.0f && vs <= 281474976710656.0f) {
+        lvs = log2f(vs);
+        ivs = 1.0f / vs;
+      }
+    }
+  }
+  uint8_t* ring = ka_smem + warp * C::WARP_BYTES;
+  auto issue = [&](int i) {
+    if (i < n) {
+      const int64_t from = __shfl_sync(0xffffffffu, at, i);
+      const int left = c1 - (c0 + KA_KEYS * (warp + KA_WARPS * i));
+      uint8_t* st = ring + (i % KA_STAGES) * C::STAGE;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const int x = lane + 32 * j, row = x / (D / 16), ch = x % (D / 16);
+        const bool there = from >= 0 && row < left;  // keys behind the last are zeros
+        const int64_t off = there ? from + 16 * x : 0;
+        cp_async16(st + ka_at<D>(row, ch), a.c.k + off, there);
+        cp_async16(st + KA_KEYS * D + ka_at<D>(row, ch), a.c.v + off, there);
+      }
+    }
+    cp_async_commit();
+  };
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < KA_STAGES - 1; ++i) issue(i);
+  }
+
+  // this lane's part of query row g: dimensions 16 c .. 16 c + 15 (and 64 more), as
+  // fp16 times a power of two that puts the row's largest value into [2^13, 2^14)
+  uint32_t qh[KW][2], ql[PAIR ? KW : 1][2];
+  float f0, f1;  // back to the score, in units of log2, for rows 2 c and 2 c + 1
+  {
+    float x[D / 4];
+    const int row = r0 + g;
+    if (row < nrows) {
+      const T* p = static_cast<const T*>(a.q) + (int64_t)(first + row / a.group) * a.q_token +
+                   (int64_t)(kvh * a.group + row % a.group) * D + 16 * c;
+#pragma unroll
+      for (int hf = 0; hf < D / 64; ++hf)
+#pragma unroll
+        for (int i = 0; i < 16; i += 16 / sizeof(T)) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p + 64 * hf + i);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (PAIR) {
+              x[16 * hf + i + j] = __uint_as_float(w[j]);
+            } else {
+              x[16 * hf + i + 2 * j] = __uint_as_float(w[j] << 16);
+              x[16 * hf + i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+          }
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    int e = (int)(__float_as_uint(top) >> 23) - 127 - 13;
+    e = top > 0.f && top < INFINITY ? max(-100, e) : 0;
+    const float up = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float back = __uint_as_float((uint32_t)(127 + e) << 23) * a.factor;
+    f0 = __shfl_sync(0xffffffffu, back, 8 * c);
+    f1 = __shfl_sync(0xffffffffu, back, 8 * c + 4);
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float u = x[4 * w + 2 * h] * up, v = x[4 * w + 2 * h + 1] * up;
+        qh[w][h] = pack_f16(u, v);
+        if constexpr (PAIR) {
+          const float2 r = unpack_f16(qh[w][h]);
+          ql[w][h] = pack_f16(u - r.x, v - r.y);
+        }
+      }
+  }
+  const int lim0 = limit(r0 + 2 * c), lim1 = limit(r0 + 2 * c + 1);
+
+  float o[DG / 2][4];  // [dims 2 j, 2 j + 1 of this lane's][row 2 c, row 2 c + 1]
+#pragma unroll
+  for (int j = 0; j < DG / 2; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+  for (int i = 0; i < n; ++i) {
+    cp_async_wait<KA_STAGES - 2>();
+    __syncwarp();
+    issue(i + KA_STAGES - 1);  // into the stage that every lane has read in the last round
+    const uint8_t* kst = ring + (i % KA_STAGES) * C::STAGE;
+    const uint8_t* vst = kst + KA_KEYS * D;
+    const int key0 = c0 + KA_KEYS * (warp + KA_WARPS * i);
+    const float kf = __shfl_sync(0xffffffffu, ks, i), lv = __shfl_sync(0xffffffffu, lvs, i),
+                iv = __shfl_sync(0xffffffffu, ivs, i);
+
+    // scores: rows of the product are keys g and g + 8, columns query rows 2 c, 2 c + 1
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int hf = 0; hf < D / 64; ++hf) {
+      const uint4 ka = *reinterpret_cast<const uint4*>(kst + ka_at<D>(g, c + 4 * hf));
+      const uint4 kb = *reinterpret_cast<const uint4*>(kst + ka_at<D>(g + 8, c + 4 * hf));
+      const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)wa[w]), a1 = e4m3x2_to_f16x2((uint16_t)wb[w]),
+                       a2 = e4m3x2_to_f16x2((uint16_t)(wa[w] >> 16)), a3 = e4m3x2_to_f16x2((uint16_t)(wb[w] >> 16));
+        if constexpr (PAIR) {
+          mma16816(s, a0, a1, a2, a3, qh[4 * hf + w][0], qh[4 * hf + w][1]);
+          mma16816(t, a0, a1, a2, a3, ql[4 * hf + w][0], ql[4 * hf + w][1]);
+        } else {
+          if (w & 1) mma16816(t, a0, a1, a2, a3, qh[4 * hf + w][0], qh[4 * hf + w][1]);
+          else mma16816(s, a0, a1, a2, a3, qh[4 * hf + w][0], qh[4 * hf + w][1]);
+        }
+      }
+    }
+    const float k0 = kf * f0, k1 = kf * f1;
+    s[0] = fmaf(s[0] + t[0], k0, lv);
+    s[1] = fmaf(s[1] + t[1], k1, lv);
+    s[2] = fmaf(s[2] + t[2], k0, lv);
+    s[3] = fmaf(s[3] + t[3], k1, lv);
+    const bool border = key0 + KA_KEYS > kmin;  // some row does not see some key
+    if (border) {
+      if (key0 + g >= lim0) s[0] = -INFINITY;
+      if (key0 + g >= lim1) s[1] = -INFINITY;
+      if (key0 + g + 8 >= lim0) s[2] = -INFINITY;
+      if (key0 + g + 8 >= lim1) s[3] = -INFINITY;
+    }
+    // the running maxima grow rarely: rows are reduced and rescaled only then
+    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > m0 || fmaxf(s[1], s[3]) > m1)) {
+      float x0 = fmaxf(m0, fmaxf(s[0], s[2])), x1 = fmaxf(m1, fmaxf(s[1], s[3]));
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+      }
+      const float r0_ = m0 == x0 ? 1.f : ex2(m0 - x0), r1_ = m1 == x1 ? 1.f : ex2(m1 - x1);
+      m0 = x0;
+      m1 = x1;
+      l0 *= r0_;
+      l1 *= r1_;
+#pragma unroll
+      for (int j = 0; j < DG / 2; ++j) {
+        o[j][0] *= r0_;
+        o[j][1] *= r1_;
+        o[j][2] *= r0_;
+        o[j][3] *= r1_;
+      }
+    }
+    const float u0 = (m0 == -INFINITY ? 0.f : m0) - KA_LIFT, u1 = (m1 == -INFINITY ? 0.f : m1) - KA_LIFT;
+    const float w0 = ex2(s[0] - u0), w1 = ex2(s[1] - u1), w2 = ex2(s[2] - u0), w3 = ex2(s[3] - u1);
+    l0 = fmaf(w0 + w2, iv, l0);
+    l1 = fmaf(w1 + w3, iv, l1);
+    const uint32_t pa = pack_f16(w0, w1), pb = pack_f16(w2, w3);
+    const uint32_t ph0 = transpose8x8(pa), ph1 = transpose8x8(pb);
+    uint32_t pl0 = 0, pl1 = 0;
+    if constexpr (PAIR) {
+      const float2 ra = unpack_f16(pa), rb = unpack_f16(pb);
+      pl0 = transpose8x8(pack_f16(w0 - ra.x, w1 - ra.y));
+      pl1 = transpose8x8(pack_f16(w2 - rb.x, w3 - rb.y));
+    }
+
+    // V: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9, dimensions DG g .. DG g + DG - 1
+    uint32_t v[4][VW];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const int row = 2 * c + (kk & 1) + 8 * (kk >> 1);
+      if constexpr (D == 128) {
+        const uint4 u = *reinterpret_cast<const uint4*>(vst + ka_at<D>(row, g));
+        v[kk][0] = u.x; v[kk][1] = u.y; v[kk][2] = u.z; v[kk][3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(vst + ka_at<D>(row, g >> 1) + 8 * (g & 1));
+        v[kk][0] = u.x; v[kk][1] = u.y;
+      }
+    }
+    bool nans = false;
+    if (border) {
+      // a NaN code of a key that only some rows see must not reach the others
+      // through 0 * NaN: such codes enter the product as 0 and are put back below
+      uint32_t bad = 0;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) bad |= nan_bytes(v[kk][w]);
+      nans = __any_sync(0xffffffffu, bad != 0);
+      if (nans) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) v[kk][w] &= ~((nan_bytes(v[kk][w]) >> 7) * 0xffu);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // dimensions 4 w + 2 h (rows 0 - 7 of the product) and the next one (rows 8 - 15)
+        const uint32_t x = __byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140);
+        const uint32_t y = __byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140);
+        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)(x >> 16)),
+                       a2 = e4m3x2_to_f16x2((uint16_t)y), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+        mma16816(o[2 * w + h], a0, a1, a2, a3, ph0, ph1);
+        if constexpr (PAIR) mma16816(o[2 * w + h], a0, a1, a2, a3, pl0, pl1);
+      }
+    if (nans) {
+      for (int kk = 0; kk < KA_KEYS; ++kk) {
+        const uint8_t* p = vst + ka_at<D>(kk, D == 128 ? g : g >> 1) + (D == 128 ? 0 : 8 * (g & 1));
+#pragma unroll
+        for (int j = 0; j < DG; ++j) {
+          if ((p[j] & 0x7f) != 0x7f) continue;
+          if (key0 + kk < lim0) o[j >> 1][(j & 1) * 2] = __int_as_float(0x7fffffff);
+          if (key0 + kk < lim1) o[j >> 1][(j & 1) * 2 + 1] = __int_as_float(0x7fffffff);
+        }
+      }
+    }
+  }
+
+  // ---- join the warps: rows 2 c and 2 c + 1 of each lane's DG dimensions
+#pragma unroll
+  for (int d = 4; d < 32; d <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  pdl_launch_dependents();
+  float* ob = reinterpret_cast<float*>(ka_smem);
+#pragma unroll
+  for (int j = 0; j < DG / 2; ++j) {
+    float* p = ob + (warp * KA_ROWS + 2 * c) * C::LD + DG * g + 2 * j;
+    *reinterpret_cast<float2*>(p) = make_float2(o[j][0], o[j][2]);
+    *reinterpret_cast<float2*>(p + C::LD) = make_float2(o[j][1], o[j][3]);
+  }
+  if (g == 0) {
+    join_m[warp][2 * c] = m0;
+    join_m[warp][2 * c + 1] = m1;
+    join_l[warp][2 * c] = l0;
+    join_l[warp][2 * c + 1] = l1;
+  }
+  __syncthreads();
+  constexpr int PER = KA_ROWS * D / (KA_WARPS * 32);  // output values a thread: 4 or 8
+  const int row = tid / (D / PER), d0 = tid % (D / PER) * PER, rr = r0 + row;
+  if (rr >= nrows) return;
+  float mt = -INFINITY, lt = 0.f, x[PER];
+#pragma unroll
+  for (int w = 0; w < KA_WARPS; ++w) mt = fmaxf(mt, join_m[w][row]);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) x[j] = 0.f;
+#pragma unroll
+  for (int w = 0; w < KA_WARPS; ++w) {
+    const float mw = join_m[w][row], f = mw == mt ? 1.f : ex2(mw - mt);
+    lt = fmaf(join_l[w][row], f, lt);
+    const float* p = ob + (w * KA_ROWS + row) * C::LD + d0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = fmaf(p[j], f, x[j]);
+  }
+  const bool sees = limit(rr) > c0 || !whole;
+  if (sees && lt == 0.f) lt = __int_as_float(0x7fffffff);  // every visible score is minus infinity: 0 / 0
+  const int64_t rh = (int64_t)(first + rr / a.group) * a.heads + kvh * a.group + rr % a.group;
+  if (a.splits > 1) {
+    float* p = a.part + (rh * a.splits + split) * D + d0;
+#pragma unroll
+    for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+    if (d0 == 0) a.ml[rh * a.splits + split] = make_float2(mt, lt);
+    return;
+  }
+  const float inv = sees ? 1.0f / lt : 0.f;
+  T* p = static_cast<T*>(a.out) + rh * D + d0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) p[j] = from_f32<T>(sees ? x[j] * inv : 0.f);
+  if (a.lse && d0 == 0) a.lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Joins the splits of one (row, head): D threads.
+template <typename T, int D>
+__global__ void __launch_bounds__(D) kv_attn_join_kernel(const KvBatch b, int heads, const float* __restrict__ part,
+                                                         const float2* __restrict__ ml, int splits, T* __restrict__ out,
+                                                         float* __restrict__ lse) {
+  pdl_wait();
+  const int64_t rh = blockIdx.x;
+  const int token = (int)(rh / heads);
+  if (b.starts && (token < b.starts[0] || token >= b.starts[b.seqs])) return;  // no sequence's row: left as it was
+  const int d = threadIdx.x;
+  const float2* m = ml + rh * splits;
+  float mt = -INFINITY;
+  for (int s = 0; s < splits; ++s) mt = fmaxf(mt, m[s].x);
+  float lt = 0.f, x = 0.f;
+  const float* p = part + rh * splits * D + d;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const float2 v = m[s];
+    if (v.y == 0.f) continue;  // nothing seen there, and nothing written to part
+    const float f = v.x == mt ? 1.f : ex2(v.x - mt);
+    lt = fmaf(v.y, f, lt);
+    x = fmaf(p[(int64_t)s * D], f, x);
+  }
+  const bool sees = lt != 0.f;
+  out[rh * D + d] = from_f32<T>(sees ? x / lt : 0.f);
+  if (lse && d == 0) lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+}
+
+// ------------------------------------------------------------------- host
+struct KvAttnPlan {
+  int64_t items;
+  int per_seq, chunk, splits;
+  int64_t workspace;  // bytes
+};
+
+static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, int sms) {
+  KvAttnPlan p;
+  const int group = heads / c->kv_heads;
+  if (b->starts) {
+    p.per_seq = 0;
+    p.items = ((int64_t)b->rows * group >> 3) + b->seqs;
+  } else {
+    p.per_seq = (int)(((int64_t)(b->rows / b->seqs) * group + KA_ROWS - 1) / KA_ROWS);
+    p.items = (int64_t)p.per_seq * b->seqs;
+  }
+  const int64_t most = (int64_t)b->table_width * c->page, base = p.items * c->kv_heads, want = 4 * (int64_t)sms;
+  int64_t splits = base >= want ? 1 : (want + base - 1) / base;
+  int64_t chunk = (most + splits - 1) / splits;
+  chunk = (chunk + 63) / 64 * 64;
+  if (chunk < 256) chunk = 256;
+  if (chunk > KA_MAX_CHUNK) chunk = KA_MAX_CHUNK;
+  p.chunk = (int)chunk;
+  p.splits = (int)((most + chunk - 1) / chunk);
+  p.workspace = p.splits > 1 ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
+  return p;
+}
+
+static const char* kv_attn_check(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads) {
+  if (const char* e = kv_check(c, b)) return e;
+  if (heads < 1 || heads % c->kv_heads) return "heads must be a multiple of kv_heads";
+  if ((int64_t)b->rows * heads > INT32_MAX) return "at most 2^31 - 1 rows x heads in one call";
+  return nullptr;
+}
+
+template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, int64_t items, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kv_attn_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       KaCfg<D>::SMEM);
+  if (e != cudaSuccess) return e;
+  kv_attn_rows_kernel<T, D><<<dim3((unsigned)items, a.c.kv_heads, a.splits), KA_WARPS * 32, KaCfg<D>::SMEM, st>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return launch_pdl(PDL_ATTN, kv_attn_join_kernel<T, D>, dim3((unsigned)(a.b.rows * a.heads)), dim3(D), 0, st, a.b, a.heads,
+                    (const float*)a.part, (const float2*)a.ml, a.splits, static_cast<T*>(a.out), a.lse);
+}
+
+}  // namespace rtr
+
+using namespace rtr;
+
+extern "C" {
+
+int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t heads, int32_t device,
+                               int64_t* bytes) {
+  if (!bytes) return set_error(RTR_ERR_ARG, "null bytes");
+  if (const char* e = kv_attn_check(cache, batch, heads)) return set_error(RTR_ERR_ARG, e);
+  *bytes = 0;
+  if (!batch->rows) return RTR_OK;
+  KvDevice on(device);
+  if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
+  *bytes = kv_attn_plan(cache, batch, heads, on.sms).workspace;
+  return RTR_OK;
+}
+
+int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const void* q_dev, int32_t dtype,
+                     int32_t heads, int64_t q_token_stride, int32_t causal, float scale, void* out_dev, float* lse_dev,
+                     void* workspace_dev, int64_t workspace_bytes, int32_t device, void* stream) {
+  if (const char* e = kv_attn_check(cache, batch, heads)) return set_error(RTR_ERR_ARG, e);
+  if (!batch->rows) return RTR_OK;
+  if (dtype != RTR_DTYPE_F32 && dtype != RTR_DTYPE_BF16)
+    return set_error(RTR_ERR_ARG, "dtype must be float32 or bfloat16");
+  const int size = dtype == RTR_DTYPE_F32 ? 4 : 2;
+  if (!q_dev || !out_dev) return set_error(RTR_ERR_ARG, "null q or out");
+  if ((reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev) | (uintptr_t)(q_token_stride * size)) & 15)
+    return set_error(RTR_ERR_ARG, "q, its stride and out must be multiples of 16 bytes");
+  KvDevice on(device);
+  if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
+  const KvAttnPlan p = kv_attn_plan(cache, batch, heads, on.sms);
+  if (p.items > INT32_MAX || p.splits > 65535 || cache->kv_heads > 65535)
+    return set_error(RTR_ERR_ARG, "too many rows or keys for one call");
+  if (p.workspace && (!workspace_dev || workspace_bytes < p.workspace || (reinterpret_cast<uintptr_t>(workspace_dev) & 15)))
+    return set_error(RTR_ERR_ARG, "workspace missing, too small or not aligned to 16 bytes");
+  KvAttn a;
+  a.c = kv_device_cache(cache);
+  a.b = kv_device_batch(batch);
+  a.q = q_dev;
+  a.q_token = q_token_stride;
+  a.heads = heads;
+  a.group = heads / cache->kv_heads;
+  a.causal = causal != 0;
+  a.factor = scale * 1.4426950408889634f;
+  a.out = out_dev;
+  a.lse = lse_dev;
+  a.part = static_cast<float*>(workspace_dev);
+  a.ml = reinterpret_cast<float2*>(a.part + (int64_t)batch->rows * heads * p.splits * cache->head_dim);
+  a.per_seq = p.per_seq;
+  a.chunk = p.chunk;
+  a.splits = p.splits;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (dtype == RTR_DTYPE_F32)
+    e = cache->head_dim == 128 ? kv_attn_launch<float, 128>(a, p.items, st) : kv_attn_launch<float, 64>(a, p.items, st);
+  else
+    e = cache->head_dim == 128 ? kv_attn_launch<__nv_bfloat16, 128>(a, p.items, st)
+                               : kv_attn_launch<__nv_bfloat16, 64>(a, p.items, st);
+  return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // extern "C"

@@ -129,10 +129,16 @@ struct rtr_session {
   int64_t weight_bytes = 0, device_bytes = 0;
 };
 
-static std::string g_create_error;
+// Text of the last failure of a call without a session, per thread.
+static thread_local char g_error[512];
+int rtr::set_error(int code, const char* msg) {
+  snprintf(g_error, sizeof g_error, "%s", msg);
+  return code;
+}
 
 static int fail(rtr_session* s, int code, const std::string& msg) {
-  if (s) s->err = msg; else g_create_error = msg;
+  if (!s) return set_error(code, msg.c_str());
+  s->err = msg;
   return code;
 }
 
@@ -181,7 +187,7 @@ static void default_rope(const rtr_model_config& c, int n, std::vector<float>& c
 
 extern "C" {
 
-const char* rtr_last_error(const rtr_session* s) { return s ? s->err.c_str() : g_create_error.c_str(); }
+const char* rtr_last_error(const rtr_session* s) { return s ? s->err.c_str() : g_error; }
 
 int rtr_session_create(const rtr_model_config* cfg, int device, rtr_session** out) {
   return rtr_session_create_batched(cfg, device, 1, out);
@@ -207,7 +213,7 @@ int rtr_session_create_batched(const rtr_model_config* cfg, int device, int32_t 
   s->device = device;
   s->max_users = max_users;
   auto bail = [&](int code) {
-    g_create_error = s->err;
+    set_error(RTR_ERR_CUDA, s->err.c_str());
     rtr_session_destroy(s);
     return code;
   };

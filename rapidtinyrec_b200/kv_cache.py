@@ -1,0 +1,215 @@
+"""An 8-bit KV cache in pages, and the operators on it.
+
+``KvCache8`` holds K and V of many sequences as e4m3 codes, ``[pages, kv_heads, page,
+head_dim]``, with one float32 scale for each page and head.  A sequence finds its
+pages through its row of a page table.  Three operators work on the cache, each one
+call into the native library on the current stream: ``write`` quantises new rows into
+the pages, ``read`` gives rows back as the values they stand for, and ``attention``
+attends over the pages as they are.
+
+What the three share: ``table`` int32 ``[seqs, width]`` page numbers, ``lens`` int32
+``[seqs]`` tokens that each sequence holds (the rows of this call included), and
+``starts`` int32 ``[seqs + 1]``: rows ``starts[b] .. starts[b + 1] - 1`` are sequence
+``b``'s; without it every sequence has the same number.  All are device tensors and
+are not read on the host, so nothing here synchronises and every call can be captured
+into a CUDA graph.  What does not fit (a page number outside the cache, a length that
+the table cannot hold) leaves its work undone and sets a bit that ``check`` raises for.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native
+
+PAGES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)
+_DTYPES = {torch.float32: _native.RTR_DTYPE_F32, torch.bfloat16: _native.RTR_DTYPE_BF16}
+_STATUS = {1 << 5: 'a length or row range that does not fit the call or the table',
+           1 << 9: 'a page number outside the cache',
+           1 << 10: 'a scale that is not positive and finite'}
+
+
+class KvCache8:
+    """The cache: ``k``, ``v`` (float8_e4m3fn ``[pages, kv_heads, page, head_dim]``, the last
+    two dimensions contiguous) and ``k_scale``, ``v_scale`` (float32 ``[pages, kv_heads]``).
+
+    Slices of larger tensors serve (one layer's heads of a cache of all layers); k and v
+    must then be sliced alike.
+    """
+
+    def __init__(self, k, v, k_scale, v_scale, status=None):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.float8_e4m3fn or v.dtype != k.dtype:
+            raise ValueError('k and v must be float8_e4m3fn [pages, kv_heads, page, head_dim] of one shape')
+        pages, heads, page, dim = k.shape
+        if page not in PAGES or dim not in HEAD_DIMS:
+            raise ValueError(f'page must be one of {PAGES} tokens and head_dim one of {HEAD_DIMS}')
+        if k.stride() != v.stride() or k.stride(3) != 1 or k.stride(2) != dim:
+            raise ValueError('k and v must have the same strides, tokens and dimensions contiguous')
+        for s in (k_scale, v_scale):
+            if s.shape != (pages, heads) or s.dtype != torch.float32 or s.stride() != k_scale.stride():
+                raise ValueError('scales must be float32 [pages, kv_heads], strided alike')
+        if heads > 1 and k_scale.stride(1) != 1:
+            raise ValueError('the scales of a page must be contiguous')
+        if not (k.is_cuda and len({t.device for t in (k, v, k_scale, v_scale)}) == 1):
+            raise ValueError('the cache must lie on one CUDA device')
+        if status is None:
+            status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self.lib = _native.load()
+        self.k, self.v, self.k_scale, self.v_scale, self.status = k, v, k_scale, v_scale, status
+        self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, dim
+        self.device = k.device
+        self._index = k.device.index
+        # the stride of a dimension with one entry means nothing
+        head_stride = k.stride(1) if heads > 1 else page * dim
+        self._c = _native.KvCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                   k.stride(0) if pages > 1 else heads * head_stride, head_stride,
+                                   k_scale.stride(0) if pages > 1 else heads, pages, heads, page, dim,
+                                   status.data_ptr())
+        self._ref = ctypes.byref(self._c)
+        self._room = {}  # workspace bytes of the call shapes seen
+
+    @classmethod
+    def allocate(cls, pages, kv_heads, page, head_dim, device='cuda'):
+        """An empty cache: codes 0 and scales 1."""
+        dev = torch.device(device)
+        shape = (pages, kv_heads, page, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.ones(shape[:2], dtype=torch.float32, device=dev) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+    def heads(self, first, count):
+        """The cache of ``count`` of its heads from ``first`` on (one layer's, say), same memory."""
+        if not (0 <= first and 0 < count and first + count <= self.kv_heads):
+            raise ValueError('heads outside the cache')
+        cut = slice(first, first + count)
+        return KvCache8(self.k[:, cut], self.v[:, cut], self.k_scale[:, cut], self.v_scale[:, cut], self.status)
+
+    def check(self):
+        """Raise for what earlier calls left undone (synchronises), and forget it."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise _native.NativeError(_native.RTR_ERR_DEVICE, '; '.join(t for b, t in _STATUS.items() if bits & b))
+
+    # ------------------------------------------------------------- plumbing
+    def _batch(self, rows, table, lens, starts):
+        if table.dtype != torch.int32 or table.dim() != 2 or lens.dtype != torch.int32 or lens.dim() != 1 \
+                or table.shape[0] != lens.shape[0]:
+            raise ValueError('table must be int32 [seqs, width] and lens int32 [seqs]')
+        seqs, width = table.shape
+        if (width > 1 and table.stride(1) != 1) or (seqs > 1 and lens.stride(0) != 1):
+            raise ValueError('the rows of table and lens must be contiguous')
+        if table.device != self.device or lens.device != self.device:
+            raise ValueError('table and lens must lie on the cache\'s device')
+        if starts is not None:
+            if starts.dtype != torch.int32 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
+                raise ValueError('starts must be int32 [seqs + 1], contiguous')
+            if starts.device != self.device:
+                raise ValueError('starts must lie on the cache\'s device')
+        elif rows % seqs if seqs else rows:
+            raise ValueError('without starts the rows must be a multiple of the sequences')
+        return _native.KvBatchC(table.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(),
+                                table.stride(0) if seqs > 1 else width, width, seqs, rows)
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _dense(self, x, heads, name):
+        """Rows as the kernels take them: one type, dimensions contiguous, 16-byte steps."""
+        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim or x.device != self.device:
+            raise ValueError(f'{name} must be [rows, {heads}, {self.head_dim}] on the cache\'s device')
+        if x.dtype not in _DTYPES:
+            raise ValueError(f'{name} must be float32 or bfloat16')
+        step = 16 // x.element_size()
+        if x.stride(2) != 1 or x.stride(0) % step or x.stride(1) % step or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+        return x
+
+    # ------------------------------------------------------------ operators
+    def write(self, k, v, table, lens, starts=None):
+        """Quantise rows ``k``, ``v`` ``[rows, kv_heads, head_dim]`` (float32 or bfloat16, any row and
+        head strides) into the pages: the last positions of their sequences.
+
+        A page's scale is the least power of two, from 2^-48 to 2^48, at which its largest
+        magnitude is at most 448.  A page that holds older tokens keeps its scale unless that is
+        too small; then their codes are rounded again.  NaN, infinities and magnitudes above
+        448 * 2^48 are stored as NaN.  Codes behind a sequence's last token stay as they are.
+        No two sequences of a call may write into the same page.
+        """
+        if k.dtype != v.dtype or k.shape != v.shape:
+            raise ValueError('k and v must have one type and shape')
+        k, v = self._dense(k, self.kv_heads, 'k'), self._dense(v, self.kv_heads, 'v')
+        batch = self._batch(k.shape[0], table, lens, starts)
+        code = self.lib.rtr_kv_write(self._ref, ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
+                                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, self._stream())
+        if code:
+            _native.check(code)
+
+    def read(self, rows, table, lens, starts=None, dtype=torch.float32, out=None):
+        """The last tokens of each sequence as ``(k, v)``, ``[rows, kv_heads, head_dim]`` each: the
+        values that the codes stand for, rounded once to ``dtype``.  ``out``: a pair of tensors to
+        fill; rows that belong to no sequence keep what they held (new tensors: undefined there).
+        """
+        shape = (rows, self.kv_heads, self.head_dim)
+        if out is None:
+            if dtype not in _DTYPES:
+                raise ValueError('dtype must be float32 or bfloat16')
+            k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        else:
+            k, v = out
+            if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
+                raise ValueError(f'out must be two tensors {list(shape)} of one type')
+            for x, name in ((k, 'k'), (v, 'v')):
+                if self._dense(x, self.kv_heads, name) is not x:
+                    raise ValueError('out must have contiguous dimensions and rows at multiples of 16 bytes')
+        batch = self._batch(rows, table, lens, starts)
+        code = self.lib.rtr_kv_read(self._ref, ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
+                                    k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, self._stream())
+        if code:
+            _native.check(code)
+        return k, v
+
+    def attention(self, q, table, lens, starts=None, causal=True, scale=None, return_lse=False, out=None):
+        """``softmax(scale q K^T) V`` of the rows ``q`` ``[rows, heads, head_dim]`` (float32 or bfloat16)
+        over their sequences; query head h reads KV head ``h // (heads // kv_heads)``.
+
+        ``causal``: a sequence's rows are its last positions, each sees what is not behind it;
+        otherwise every row sees the whole sequence.  A row that sees nothing is 0.  ``scale``:
+        ``head_dim ** -0.5`` unless given.  Returns ``out`` (a new tensor, or the contiguous one given),
+        with ``return_lse`` also the float32 ``[rows, heads]`` log of the softmax's sum, by which
+        results over several stretches of keys are merged.  Rows that belong to no sequence are not
+        written: a given ``out`` keeps them, new tensors are undefined there.
+        """
+        if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
+            raise ValueError(f'q must be [rows, heads, {self.head_dim}], heads a multiple of {self.kv_heads}')
+        rows, heads = q.shape[:2]
+        q = self._dense(q, heads, 'q')
+        if heads > 1 and q.stride(1) != self.head_dim:
+            q = q.contiguous()
+        batch = self._batch(rows, table, lens, starts)
+        ref = ctypes.byref(batch)
+        key = (rows, heads, batch.seqs, batch.table_width, starts is None)
+        room = self._room.get(key)
+        if room is None:
+            need = ctypes.c_int64()
+            _native.check(self.lib.rtr_kv_attention_workspace(self._ref, ref, heads, self._index, ctypes.byref(need)))
+            if len(self._room) >= 4096:
+                self._room.clear()
+            room = self._room[key] = need.value
+        if out is None:
+            out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise ValueError('out must be contiguous and like q')
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device) if return_lse else None
+        work = torch.empty(room, dtype=torch.uint8, device=self.device) if room else None
+        code = self.lib.rtr_kv_attention(self._ref, ref, q.data_ptr(), _DTYPES[q.dtype], heads, q.stride(0),
+                                         bool(causal), 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
+                                         out.data_ptr(), lse.data_ptr() if return_lse else None,
+                                         work.data_ptr() if room else None, room, self._index, self._stream())
+        if code:
+            _native.check(code)
+        return (out, lse) if return_lse else out
