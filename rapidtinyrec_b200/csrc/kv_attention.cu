@@ -12,8 +12,9 @@
 //
 // Rows.  The query rows of one KV head are its (token, head of the group) pairs.
 // A block takes a tile of them and a stretch of the sequence's keys; the keys are
-// split over blocks while there are fewer tiles than the GPU has room for, and a
-// second kernel joins the stretches.
+// split over blocks while there are fewer tiles than the GPU has room for.  Up to
+// eight stretches are a thread-block cluster, whose blocks join their sums through
+// distributed shared memory; more are joined by a second kernel.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -21,6 +22,7 @@
 #include "engine.h"
 #include "kv_cache.cuh"
 #include "kv_host.h"
+#include "tcgen05.cuh"
 
 namespace rtr {
 
@@ -38,10 +40,11 @@ struct KvAttn {
   float2* ml;          // [rows * heads][splits]: running maximum, sum
   int per_seq;         // row tiles of a sequence without starts
   int chunk, splits;   // keys of a block, and the blocks of a row tile
+  int cluster;         // the blocks of a row tile are one cluster and join among themselves
 };
 
 constexpr int KA_WARPS = 4, KA_ROWS = 8, KA_KEYS = 16, KA_STAGES = 4;
-constexpr int KA_MAX_CHUNK = 2048;  // 32 key groups a warp: their page numbers and scales fit its lanes
+constexpr int KA_MAX_CHUNK = 1024;  // 16 key groups a warp: their page numbers and scales fit its lanes
 // Weights enter the fp16 operand times 2^12: the largest is 4096, and 2^-24
 // (fp16's smallest) is 2^-36 of it.
 constexpr float KA_LIFT = 12.0f;
@@ -65,6 +68,19 @@ RTR_DEVICE void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+RTR_DEVICE float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+RTR_DEVICE float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 RTR_DEVICE uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
@@ -112,6 +128,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   extern __shared__ __align__(128) uint8_t ka_smem[];
   __shared__ int slot;
   __shared__ float join_m[KA_WARPS][KA_ROWS], join_l[KA_WARPS][KA_ROWS];
+  __shared__ __align__(16) float sum_o[KA_ROWS][D];  // this block's sums, read by its cluster
+  __shared__ float2 sum_ml[KA_ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y, split = blockIdx.z;
 
@@ -136,7 +154,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   auto limit = [&](int row) { return a.causal ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
   const int kmin = limit(r0), kmax = limit(r0 + KA_ROWS - 1);
   const int c0 = split * a.chunk, c1 = min(kmax, c0 + a.chunk);
-  if (c1 <= c0 && split > 0) {  // a stretch behind the last key (the first one reports rows that see nothing)
+  if (c1 <= c0 && split > 0 && !a.cluster) {  // a stretch behind the last key (the first one reports rows that see nothing)
     if (tid < KA_ROWS && r0 + tid < nrows) {
       const int rr = r0 + tid;
       const int64_t rh = (int64_t)(first + rr / a.group) * a.heads + kvh * a.group + rr % a.group;
@@ -401,8 +419,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   }
   __syncthreads();
   constexpr int PER = KA_ROWS * D / (KA_WARPS * 32);  // output values a thread: 4 or 8
-  const int row = tid / (D / PER), d0 = tid % (D / PER) * PER, rr = r0 + row;
-  if (rr >= nrows) return;
+  const int row = tid / (D / PER), d0 = tid % (D / PER) * PER;
   float mt = -INFINITY, lt = 0.f, x[PER];
 #pragma unroll
   for (int w = 0; w < KA_WARPS; ++w) mt = fmaxf(mt, join_m[w][row]);
@@ -416,55 +433,146 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
 #pragma unroll
     for (int j = 0; j < PER; ++j) x[j] = fmaf(p[j], f, x[j]);
   }
-  const bool sees = limit(rr) > c0 || !whole;
-  if (sees && lt == 0.f) lt = __int_as_float(0x7fffffff);  // every visible score is minus infinity: 0 / 0
-  const int64_t rh = (int64_t)(first + rr / a.group) * a.heads + kvh * a.group + rr % a.group;
-  if (a.splits > 1) {
+  // every visible score is minus infinity (0 / 0), or the sequence's length did not fit
+  if (lt == 0.f && (limit(r0 + row) > c0 || !whole)) lt = __int_as_float(0x7fffffff);
+  const auto head_row = [&](int rr) {
+    return (int64_t)(first + rr / a.group) * a.heads + kvh * a.group + rr % a.group;
+  };
+  const auto finish = [&](int rr) {
+    const bool sees = lt != 0.f;
+    const float inv = sees ? 1.0f / lt : 0.f;
+    const int64_t rh = head_row(rr);
+    T* p = static_cast<T*>(a.out) + rh * D + d0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) p[j] = from_f32<T>(sees ? x[j] * inv : 0.f);
+    if (a.lse && d0 == 0) a.lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+  };
+  if (a.splits == 1) {
+    if (r0 + row < nrows) finish(r0 + row);
+    return;
+  }
+  if (!a.cluster) {
+    if (r0 + row >= nrows) return;
+    const int64_t rh = head_row(r0 + row);
     float* p = a.part + (rh * a.splits + split) * D + d0;
 #pragma unroll
     for (int j = 0; j < PER; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
     if (d0 == 0) a.ml[rh * a.splits + split] = make_float2(mt, lt);
     return;
   }
-  const float inv = sees ? 1.0f / lt : 0.f;
-  T* p = static_cast<T*>(a.out) + rh * D + d0;
+  // the cluster's blocks share out the rows, each reads the others' sums
 #pragma unroll
-  for (int j = 0; j < PER; ++j) p[j] = from_f32<T>(sees ? x[j] * inv : 0.f);
-  if (a.lse && d0 == 0) a.lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+  for (int j = 0; j < PER; ++j) sum_o[row][d0 + j] = x[j];
+  if (d0 == 0) sum_ml[row] = make_float2(mt, lt);
+  cluster_sync_all();
+  const int mine = split + row * a.splits;
+  if (mine < KA_ROWS && r0 + mine < nrows) {
+    const uint32_t ml_at = smem_addr(&sum_ml[mine]), o_at = smem_addr(&sum_o[mine][d0]);
+    mt = -INFINITY;
+    lt = 0.f;
+    for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, ld_cluster_f32(cluster_map(ml_at, s)));
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      const uint32_t at = cluster_map(ml_at, s), from = cluster_map(o_at, s);
+      const float ms = ld_cluster_f32(at), f = ms == mt ? 1.f : ex2(ms - mt);
+      lt = fmaf(ld_cluster_f32(at + 4), f, lt);
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const float4 v = ld_cluster_f4(from + 4 * j);
+        x[j] = fmaf(v.x, f, x[j]);
+        x[j + 1] = fmaf(v.y, f, x[j + 1]);
+        x[j + 2] = fmaf(v.z, f, x[j + 2]);
+        x[j + 3] = fmaf(v.w, f, x[j + 3]);
+      }
+    }
+    finish(r0 + mine);
+  }
+  cluster_sync_all();  // no block leaves while another may still read its sums
 }
 
-// Joins the splits of one (row, head): D threads.
+// Joins the splits of one (row, head).  KJ_THREADS threads: D / 4 of them cover a
+// split's row, the others take other splits at the same time, so that a row split
+// into hundreds of stretches (one sequence of 128 Ki tokens) costs a few rounds of
+// loads; each split's weight is worked out once.
+constexpr int KJ_THREADS = 256, KJ_MAX = 1024;  // splits whose weights are kept at a time
+
 template <typename T, int D>
-__global__ void __launch_bounds__(D) kv_attn_join_kernel(const KvBatch b, int heads, const float* __restrict__ part,
-                                                         const float2* __restrict__ ml, int splits, T* __restrict__ out,
-                                                         float* __restrict__ lse) {
+__global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch b, int heads,
+                                                                  const float* __restrict__ part,
+                                                                  const float2* __restrict__ ml, int splits,
+                                                                  T* __restrict__ out, float* __restrict__ lse) {
+  constexpr int COLS = D / 4, LANES = KJ_THREADS / COLS;  // 32 x 8 or 16 x 16
+  __shared__ float weight[KJ_MAX];
+  __shared__ float red[2][KJ_THREADS / 32];
+  __shared__ float4 sums[LANES][COLS];
   pdl_wait();
   const int64_t rh = blockIdx.x;
-  const int token = (int)(rh / heads);
+  const int token = (int)(rh / heads), tid = threadIdx.x, col = tid % COLS, sub = tid / COLS;
   if (b.starts && (token < b.starts[0] || token >= b.starts[b.seqs])) return;  // no sequence's row: left as it was
-  const int d = threadIdx.x;
   const float2* m = ml + rh * splits;
-  float mt = -INFINITY;
-  for (int s = 0; s < splits; ++s) mt = fmaxf(mt, m[s].x);
-  float lt = 0.f, x = 0.f;
-  const float* p = part + rh * splits * D + d;
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    const float2 v = m[s];
-    if (v.y == 0.f) continue;  // nothing seen there, and nothing written to part
-    const float f = v.x == mt ? 1.f : ex2(v.x - mt);
-    lt = fmaf(v.y, f, lt);
-    x = fmaf(p[(int64_t)s * D], f, x);
+  const float4* p = reinterpret_cast<const float4*>(part + rh * splits * D) + col;
+  float mt = -INFINITY, lt = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = tid; s < splits; s += KJ_THREADS) mt = fmaxf(mt, m[s].x);
+  mt = warp_max(mt);
+  if ((tid & 31) == 0) red[0][tid >> 5] = mt;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < KJ_THREADS / 32; ++w) mt = fmaxf(mt, red[0][w]);
+  for (int s0 = 0; s0 < splits; s0 += KJ_MAX) {
+    const int n = min(KJ_MAX, splits - s0);
+    if (s0) __syncthreads();
+    for (int s = tid; s < n; s += KJ_THREADS) {
+      const float2 v = m[s0 + s];
+      const float f = v.x == mt ? 1.f : ex2(v.x - mt);
+      // nothing seen there means nothing written to part: no weight, whatever lies there
+      weight[s] = v.y == 0.f ? -1.f : f;
+      lt += v.y == 0.f ? 0.f : v.y * f;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int s = sub; s < n; s += LANES) {
+      const float f = weight[s];
+      if (f < 0.f) continue;
+      const float4 v = p[(int64_t)(s0 + s) * COLS];
+      x.x = fmaf(v.x, f, x.x);
+      x.y = fmaf(v.y, f, x.y);
+      x.z = fmaf(v.z, f, x.z);
+      x.w = fmaf(v.w, f, x.w);
+    }
+  }
+  lt = warp_sum(lt);
+  if ((tid & 31) == 0) red[1][tid >> 5] = lt;
+  sums[sub][col] = x;
+  __syncthreads();
+  if (tid >= COLS) return;
+  lt = 0.f;
+#pragma unroll
+  for (int w = 0; w < KJ_THREADS / 32; ++w) lt += red[1][w];
+#pragma unroll
+  for (int i = 1; i < LANES; ++i) {
+    const float4 v = sums[i][col];
+    x.x += v.x;
+    x.y += v.y;
+    x.z += v.z;
+    x.w += v.w;
   }
   const bool sees = lt != 0.f;
-  out[rh * D + d] = from_f32<T>(sees ? x / lt : 0.f);
-  if (lse && d == 0) lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+  const float inv = sees ? 1.0f / lt : 0.f;
+  T* o = out + rh * D + 4 * col;
+  o[0] = from_f32<T>(sees ? x.x * inv : 0.f);
+  o[1] = from_f32<T>(sees ? x.y * inv : 0.f);
+  o[2] = from_f32<T>(sees ? x.z * inv : 0.f);
+  o[3] = from_f32<T>(sees ? x.w * inv : 0.f);
+  if (lse && tid == 0) lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ------------------------------------------------------------------- host
 struct KvAttnPlan {
   int64_t items;
   int per_seq, chunk, splits;
+  bool cluster;
   int64_t workspace;  // bytes
 };
 
@@ -478,15 +586,22 @@ static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int
     p.per_seq = (int)(((int64_t)(b->rows / b->seqs) * group + KA_ROWS - 1) / KA_ROWS);
     p.items = (int64_t)p.per_seq * b->seqs;
   }
-  const int64_t most = (int64_t)b->table_width * c->page, base = p.items * c->kv_heads, want = 4 * (int64_t)sms;
-  int64_t splits = base >= want ? 1 : (want + base - 1) / base;
-  int64_t chunk = (most + splits - 1) / splits;
+  const int64_t most = (int64_t)b->table_width * c->page, base = p.items * c->kv_heads;
+  // A stretch has at least 512 keys: below that a block is bound by the latency of
+  // finding its pages, and joining costs more than it saves (61 sequences of 30 - 300
+  // keys, 14 heads: 6.2 us in one stretch, 7.8 us in two); at most 1024, so that ragged
+  // batches spread (24 sequences of 6,000 - 32,000 keys: 90.8 us, with 2048 92.3, with
+  // 512 101); between them as many as give two blocks an SM (one sequence of 128 Ki
+  // keys: 22.0 us, with three an SM 23.9, with six 33).
+  const int64_t want = 2 * (int64_t)sms;
+  int64_t chunk = base >= want ? most : most * base / want;
   chunk = (chunk + 63) / 64 * 64;
-  if (chunk < 256) chunk = 256;
+  if (chunk < 512) chunk = 512;
   if (chunk > KA_MAX_CHUNK) chunk = KA_MAX_CHUNK;
   p.chunk = (int)chunk;
   p.splits = (int)((most + chunk - 1) / chunk);
-  p.workspace = p.splits > 1 ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
+  p.cluster = p.splits > 1 && p.splits <= 8;
+  p.workspace = p.splits > 1 && !p.cluster ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
   return p;
 }
 
@@ -497,14 +612,24 @@ static const char* kv_attn_check(const rtr_kv_cache* c, const rtr_kv_batch* b, i
   return nullptr;
 }
 
-template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, int64_t items, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kv_attn_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       KaCfg<D>::SMEM);
+template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, int64_t items, int device, cudaStream_t st) {
+  static std::atomic<uint64_t> done;
+  cudaError_t e = kv_allow_smem(kv_attn_rows_kernel<T, D>, KaCfg<D>::SMEM, done, device);
   if (e != cudaSuccess) return e;
-  kv_attn_rows_kernel<T, D><<<dim3((unsigned)items, a.c.kv_heads, a.splits), KA_WARPS * 32, KaCfg<D>::SMEM, st>>>(a);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
-  return launch_pdl(PDL_ATTN, kv_attn_join_kernel<T, D>, dim3((unsigned)(a.b.rows * a.heads)), dim3(D), 0, st, a.b, a.heads,
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)items, a.c.kv_heads, a.splits);
+  cfg.blockDim = dim3(KA_WARPS * 32);
+  cfg.dynamicSmemBytes = KaCfg<D>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = a.splits;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kv_attn_rows_kernel<T, D>, a);
+  if (e != cudaSuccess || a.splits == 1 || a.cluster) return e;
+  return launch_pdl(PDL_ATTN, kv_attn_join_kernel<T, D>, dim3((unsigned)(a.b.rows * a.heads)), dim3(KJ_THREADS), 0, st, a.b, a.heads,
                     (const float*)a.part, (const float2*)a.ml, a.splits, static_cast<T*>(a.out), a.lse);
 }
 
@@ -560,13 +685,14 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
   a.per_seq = p.per_seq;
   a.chunk = p.chunk;
   a.splits = p.splits;
+  a.cluster = p.cluster;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == RTR_DTYPE_F32)
-    e = cache->head_dim == 128 ? kv_attn_launch<float, 128>(a, p.items, st) : kv_attn_launch<float, 64>(a, p.items, st);
+    e = cache->head_dim == 128 ? kv_attn_launch<float, 128>(a, p.items, device, st) : kv_attn_launch<float, 64>(a, p.items, device, st);
   else
-    e = cache->head_dim == 128 ? kv_attn_launch<__nv_bfloat16, 128>(a, p.items, st)
-                               : kv_attn_launch<__nv_bfloat16, 64>(a, p.items, st);
+    e = cache->head_dim == 128 ? kv_attn_launch<__nv_bfloat16, 128>(a, p.items, device, st)
+                               : kv_attn_launch<__nv_bfloat16, 64>(a, p.items, device, st);
   return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
 }
 

@@ -258,6 +258,16 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvCache c, co
 }
 
 // ------------------------------------------------------------------- host
+int kv_sms(int device, cudaError_t& e) {
+  static std::atomic<int> known[64];
+  if (device >= 0 && device < 64)
+    if (const int n = known[device].load(std::memory_order_relaxed)) return n;
+  int n = 0;
+  e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+  if (e == cudaSuccess && device >= 0 && device < 64) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 const char* kv_check(const rtr_kv_cache* c, const rtr_kv_batch* b) {
   if (!c || !b) return "null cache or batch";
   if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->status) return "null cache buffer";

@@ -4,6 +4,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "kv_cache.cuh"
 
 namespace rtr {
@@ -26,6 +28,18 @@ KvCache kv_device_cache(const rtr_kv_cache* c);
 KvBatch kv_device_batch(const rtr_kv_batch* b);
 KvGrid kv_page_grid(int rows, int seqs, bool starts, int page, int kv_heads, int sms);
 
+// The device's SM count, asked for once (a call would spend 0.3 us on it each time).
+int kv_sms(int device, cudaError_t& e);
+
+// Allows a kernel `bytes` of dynamic shared memory on `device`, the first time (done: a bit a device).
+template <typename F> cudaError_t kv_allow_smem(F* kernel, int bytes, std::atomic<uint64_t>& done, int device) {
+  const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 // Makes `device` the thread's current one for a call and puts the former back.
 struct KvDevice {
   int former = -1, device, sms = 0;
@@ -33,7 +47,7 @@ struct KvDevice {
   explicit KvDevice(int dev) : device(dev) {
     error = cudaGetDevice(&former);
     if (error == cudaSuccess && former != dev) error = cudaSetDevice(dev);
-    if (error == cudaSuccess) error = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (error == cudaSuccess) sms = kv_sms(dev, error);
   }
   ~KvDevice() {
     if (former >= 0 && former != device) cudaSetDevice(former);

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -26,10 +27,16 @@ from . import _native
 
 PAGES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
+_BATCH = struct.Struct('PPPqiii4x')  # rtr_kv_batch; packed bytes cost a third of a ctypes structure
 _DTYPES = {torch.float32: _native.RTR_DTYPE_F32, torch.bfloat16: _native.RTR_DTYPE_BF16}
 _STATUS = {1 << 5: 'a length or row range that does not fit the call or the table',
            1 << 9: 'a page number outside the cache',
            1 << 10: 'a scale that is not positive and finite'}
+
+
+def _stream(index):
+    """The device's current stream (torch.cuda.current_stream without making a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class KvCache8:
@@ -69,6 +76,8 @@ class KvCache8:
                                    k_scale.stride(0) if pages > 1 else heads, pages, heads, page, dim,
                                    status.data_ptr())
         self._ref = ctypes.byref(self._c)
+        self._scale = 1.0 / math.sqrt(dim)
+        self._attend = self.lib.rtr_kv_attention
         self._room = {}  # workspace bytes of the call shapes seen
 
     @classmethod
@@ -96,35 +105,39 @@ class KvCache8:
 
     # ------------------------------------------------------------- plumbing
     def _batch(self, rows, table, lens, starts):
-        if table.dtype != torch.int32 or table.dim() != 2 or lens.dtype != torch.int32 or lens.dim() != 1 \
-                or table.shape[0] != lens.shape[0]:
+        """The call's ``rtr_kv_batch`` (packed)."""
+        shape = table.shape
+        if table.dtype is not torch.int32 or lens.dtype is not torch.int32 or len(shape) != 2 or lens.shape != shape[:1]:
             raise ValueError('table must be int32 [seqs, width] and lens int32 [seqs]')
-        seqs, width = table.shape
-        if (width > 1 and table.stride(1) != 1) or (seqs > 1 and lens.stride(0) != 1):
+        seqs, width = shape
+        step = table.stride()
+        if (width > 1 and step[1] != 1) or (seqs > 1 and lens.stride(0) != 1):
             raise ValueError('the rows of table and lens must be contiguous')
-        if table.device != self.device or lens.device != self.device:
+        index = self._index
+        if table.get_device() != index or lens.get_device() != index:
             raise ValueError('table and lens must lie on the cache\'s device')
-        if starts is not None:
-            if starts.dtype != torch.int32 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
+        if starts is None:
+            if rows % seqs if seqs else rows:
+                raise ValueError('without starts the rows must be a multiple of the sequences')
+            begin = 0
+        else:
+            if starts.dtype is not torch.int32 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
                 raise ValueError('starts must be int32 [seqs + 1], contiguous')
-            if starts.device != self.device:
+            if starts.get_device() != index:
                 raise ValueError('starts must lie on the cache\'s device')
-        elif rows % seqs if seqs else rows:
-            raise ValueError('without starts the rows must be a multiple of the sequences')
-        return _native.KvBatchC(table.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(),
-                                table.stride(0) if seqs > 1 else width, width, seqs, rows)
-
-    def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+            begin = starts.data_ptr()
+        return _BATCH.pack(table.data_ptr(), lens.data_ptr(), begin, step[0] if seqs > 1 else width, width, seqs, rows)
 
     def _dense(self, x, heads, name):
         """Rows as the kernels take them: one type, dimensions contiguous, 16-byte steps."""
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.head_dim or x.device != self.device:
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or x.get_device() != self._index:
             raise ValueError(f'{name} must be [rows, {heads}, {self.head_dim}] on the cache\'s device')
         if x.dtype not in _DTYPES:
             raise ValueError(f'{name} must be float32 or bfloat16')
-        step = 16 // x.element_size()
-        if x.stride(2) != 1 or x.stride(0) % step or x.stride(1) % step or x.data_ptr() % 16:
+        a, b, c = x.stride()
+        step = 4 if x.dtype is torch.float32 else 8
+        if c != 1 or a % step or b % step or x.data_ptr() % 16:
             x = x.clone(memory_format=torch.contiguous_format)
         return x
 
@@ -143,8 +156,8 @@ class KvCache8:
             raise ValueError('k and v must have one type and shape')
         k, v = self._dense(k, self.kv_heads, 'k'), self._dense(v, self.kv_heads, 'v')
         batch = self._batch(k.shape[0], table, lens, starts)
-        code = self.lib.rtr_kv_write(self._ref, ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
-                                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, self._stream())
+        code = self.lib.rtr_kv_write(self._ref, batch, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
+                                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, _stream(self._index))
         if code:
             _native.check(code)
 
@@ -157,7 +170,8 @@ class KvCache8:
         if out is None:
             if dtype not in _DTYPES:
                 raise ValueError('dtype must be float32 or bfloat16')
-            k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+            k = self.k_scale.new_empty(shape, dtype=dtype)
+            v = torch.empty_like(k)
         else:
             k, v = out
             if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
@@ -166,8 +180,8 @@ class KvCache8:
                 if self._dense(x, self.kv_heads, name) is not x:
                     raise ValueError('out must have contiguous dimensions and rows at multiples of 16 bytes')
         batch = self._batch(rows, table, lens, starts)
-        code = self.lib.rtr_kv_read(self._ref, ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
-                                    k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, self._stream())
+        code = self.lib.rtr_kv_read(self._ref, batch, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
+                                    k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, _stream(self._index))
         if code:
             _native.check(code)
         return k, v
@@ -183,33 +197,32 @@ class KvCache8:
         results over several stretches of keys are merged.  Rows that belong to no sequence are not
         written: a given ``out`` keeps them, new tensors are undefined there.
         """
-        if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.kv_heads:
-            raise ValueError(f'q must be [rows, heads, {self.head_dim}], heads a multiple of {self.kv_heads}')
         rows, heads = q.shape[:2]
+        if q.dim() != 3 or heads < 1 or heads % self.kv_heads:
+            raise ValueError(f'q must be [rows, heads, {self.head_dim}], heads a multiple of {self.kv_heads}')
         q = self._dense(q, heads, 'q')
         if heads > 1 and q.stride(1) != self.head_dim:
-            q = q.contiguous()
+            q = q.clone(memory_format=torch.contiguous_format)
         batch = self._batch(rows, table, lens, starts)
-        ref = ctypes.byref(batch)
-        key = (rows, heads, batch.seqs, batch.table_width, starts is None)
+        key = (rows, heads, table.shape, starts is None)
         room = self._room.get(key)
         if room is None:
             need = ctypes.c_int64()
-            _native.check(self.lib.rtr_kv_attention_workspace(self._ref, ref, heads, self._index, ctypes.byref(need)))
+            _native.check(self.lib.rtr_kv_attention_workspace(self._ref, batch, heads, self._index, ctypes.byref(need)))
             if len(self._room) >= 4096:
                 self._room.clear()
             room = self._room[key] = need.value
         if out is None:
-            out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous() \
-                or out.data_ptr() % 16:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != self._index \
+                or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError('out must be contiguous and like q')
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device) if return_lse else None
-        work = torch.empty(room, dtype=torch.uint8, device=self.device) if room else None
-        code = self.lib.rtr_kv_attention(self._ref, ref, q.data_ptr(), _DTYPES[q.dtype], heads, q.stride(0),
-                                         bool(causal), 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
-                                         out.data_ptr(), lse.data_ptr() if return_lse else None,
-                                         work.data_ptr() if room else None, room, self._index, self._stream())
+        lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
+        work = q.new_empty((room,), dtype=torch.uint8) if room else None
+        code = self._attend(self._ref, batch, q.data_ptr(), _DTYPES[q.dtype], heads, q.stride(0), causal,
+                            self._scale if scale is None else scale, out.data_ptr(),
+                            lse.data_ptr() if return_lse else None, work.data_ptr() if room else None, room,
+                            self._index, _stream(self._index))
         if code:
             _native.check(code)
         return (out, lse) if return_lse else out
