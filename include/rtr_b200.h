@@ -363,8 +363,8 @@ int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_de
  * rtr_kv_attention_workspace bytes, aligned to 16, and is free again when the call's
  * kernels ran: calls that may overlap need one each.  A table row wider than the
  * sequences need costs idle blocks. */
-int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t heads, int32_t device,
-                               int64_t* bytes);
+int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t dtype, int32_t heads,
+                               int32_t device, int64_t* bytes);
 int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const void* q_dev, int32_t dtype,
                      int32_t heads, int64_t q_token_stride, int32_t causal, float scale, void* out_dev, float* lse_dev,
                      void* workspace_dev, int64_t workspace_bytes, int32_t device, void* stream);

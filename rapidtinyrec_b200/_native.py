@@ -131,7 +131,7 @@ def load():
         'rtr_attention_check': (I32, P, P, P, P, I32, I32, I32, I32, I32),
         'rtr_kv_write': (P, P, P, P, I32, I64, I64, I64, I64, I32, P),
         'rtr_kv_read': (P, P, P, P, I32, I64, I64, I64, I64, I32, P),
-        'rtr_kv_attention_workspace': (P, P, I32, I32, ctypes.POINTER(I64)),
+        'rtr_kv_attention_workspace': (P, P, I32, I32, I32, ctypes.POINTER(I64)),
         'rtr_kv_attention': (P, P, P, I32, I32, I64, I32, F, P, P, P, I64, I32, P),
     }
     for name, args in sig.items():

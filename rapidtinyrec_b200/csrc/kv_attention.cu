@@ -20,35 +20,14 @@
 #include <type_traits>
 
 #include "engine.h"
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 #include "kv_host.h"
 #include "tcgen05.cuh"
 
 namespace rtr {
 
-struct KvAttn {
-  KvCache c;
-  KvBatch b;
-  const void* q;
-  int64_t q_token;     // elements between a token's rows; heads are contiguous
-  int heads, group;    // query heads, and those of one KV head
-  int causal;
-  float factor;        // softmax scale * log2(e)
-  void* out;           // [rows][heads][head_dim]
-  float* lse;          // [rows][heads] or null
-  float* part;         // [rows * heads][splits][head_dim] when splits > 1
-  float2* ml;          // [rows * heads][splits]: running maximum, sum
-  int per_seq;         // row tiles of a sequence without starts
-  int chunk, splits;   // keys of a block, and the blocks of a row tile
-  int cluster;         // the blocks of a row tile are one cluster and join among themselves
-};
-
 constexpr int KA_WARPS = 4, KA_ROWS = 8, KA_KEYS = 16, KA_STAGES = 4;
 constexpr int KA_MAX_CHUNK = 1024;  // 16 key groups a warp: their page numbers and scales fit its lanes
-// Weights enter the fp16 operand times 2^12: the largest is 4096, and 2^-24
-// (fp16's smallest) is 2^-36 of it.
-constexpr float KA_LIFT = 12.0f;
-
 template <int D> struct KaCfg {
   static constexpr int STAGE = 2 * KA_KEYS * D;  // K and V of one key group
   static constexpr int WARP_BYTES = KA_STAGES * STAGE;
@@ -58,43 +37,17 @@ template <int D> struct KaCfg {
   static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 };
 
-RTR_DEVICE float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 RTR_DEVICE void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-RTR_DEVICE float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-RTR_DEVICE float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
 RTR_DEVICE uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-RTR_DEVICE uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-RTR_DEVICE float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
-// Whether one of four codes is NaN (0x7f or 0xff).
-RTR_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
 // Where 16-byte piece `ch` of key row `row` lies in a stage: pieces are permuted
 // within 128 bytes so that the rows g, g + 1 that eight lanes read of K, and the
 // rows 0, 2, 4, 6 (or 1, 3, 5, 7) that they read of V, lie in different banks.
@@ -174,12 +127,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
     ks = lvs = __int_as_float(0x7fffffff);  // a page that is not there makes the rows NaN
     if (page >= 0) {
       at = page * a.c.page_stride + kvh * a.c.head_stride + (int64_t)(key & ((1 << a.c.page_shift) - 1)) * D;
-      ks = a.c.k_scale[page * a.c.scale_stride + kvh];
-      const float vs = a.c.v_scale[page * a.c.scale_stride + kvh];
-      if (vs >= 1.0f / 281474976710656.0f && vs <= 281474976710656.0f) {
-        lvs = log2f(vs);
-        ivs = 1.0f / vs;
-      }
+      ks = kv_k_scale(a.c.k_scale[page * a.c.scale_stride + kvh]);
+      kv_v_scale(a.c.v_scale[page * a.c.scale_stride + kvh], lvs, ivs);
     }
   }
   uint8_t* ring = ka_smem + warp * C::WARP_BYTES;
@@ -239,10 +188,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
     for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    int e = (int)(__float_as_uint(top) >> 23) - 127 - 13;
-    e = top > 0.f && top < INFINITY ? max(-100, e) : 0;
-    const float up = __uint_as_float((uint32_t)(127 - e) << 23);
-    const float back = __uint_as_float((uint32_t)(127 + e) << 23) * a.factor;
+    const int e = kv_row_exponent(top);
+    const float up = kv_pow2(-e), back = kv_pow2(e) * a.factor;
     f0 = __shfl_sync(0xffffffffu, back, 8 * c);
     f1 = __shfl_sync(0xffffffffu, back, 8 * c + 4);
 #pragma unroll
@@ -570,22 +517,26 @@ __global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch 
 
 // ------------------------------------------------------------------- host
 struct KvAttnPlan {
+  bool tiles;  // 128-row tiles (kv_attention_tile.cu), else KA_ROWS rows a block
   int64_t items;
   int per_seq, chunk, splits;
   bool cluster;
   int64_t workspace;  // bytes
 };
 
-static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, int sms) {
-  KvAttnPlan p;
-  const int group = heads / c->kv_heads;
+static int64_t kv_attn_items(const rtr_kv_batch* b, int group, int shift, int& per_seq) {
   if (b->starts) {
-    p.per_seq = 0;
-    p.items = ((int64_t)b->rows * group >> 3) + b->seqs;
-  } else {
-    p.per_seq = (int)(((int64_t)(b->rows / b->seqs) * group + KA_ROWS - 1) / KA_ROWS);
-    p.items = (int64_t)p.per_seq * b->seqs;
+    per_seq = 0;
+    return ((int64_t)b->rows * group >> shift) + b->seqs;
   }
+  per_seq = (int)(((int64_t)(b->rows / b->seqs) * group + (1 << shift) - 1) >> shift);
+  return (int64_t)per_seq * b->seqs;
+}
+
+// Tiles of 8 rows: stretches and the time to expect, in ns.
+static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int group, bool f32, int sms, int64_t& ns) {
+  KvAttnPlan p = {};
+  p.items = kv_attn_items(b, group, 3, p.per_seq);
   const int64_t most = (int64_t)b->table_width * c->page, base = p.items * c->kv_heads;
   // A stretch has at least 512 keys: below that a block is bound by the latency of
   // finding its pages, and joining costs more than it saves (61 sequences of 30 - 300
@@ -601,6 +552,47 @@ static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   p.chunk = (int)chunk;
   p.splits = (int)((most + chunk - 1) / chunk);
   p.cluster = p.splits > 1 && p.splits <= 8;
+  // measured: 8 rows x 18,500 (fp32 16,000) keys a us at head_dim 128, 55,000 (48,000) at 64
+  const int64_t rate = c->head_dim == 128 ? (f32 ? 16000 : 18500) : f32 ? 48000 : 55000;
+  ns = 5000 + base * most * 1000 / rate + (p.splits > 1 ? 3000 : 0);
+  return p;
+}
+
+// Tiles of 128 rows.
+static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, int group, bool f32, int sms, int64_t& ns) {
+  KvAttnPlan p = {};
+  p.tiles = true;
+  p.items = kv_attn_items(b, group, 7, p.per_seq);
+  const int64_t base = p.items * c->kv_heads;
+  const int64_t all = ((int64_t)b->table_width * c->page + KT_KEYS - 1) / KT_KEYS;
+  // A block costs its key tiles and about six more (q, first and last tile, output), a
+  // cluster's join three, a join through memory eight.  Clusters of three and more fill
+  // about six of seven SMs.
+  int64_t best = INT64_MAX;
+  for (int64_t s = (all * KT_KEYS + KT_MAX_CHUNK - 1) / KT_MAX_CHUNK, end = s + 63; s <= end; ++s) {
+    const int64_t per = (all + s - 1) / s, splits = (all + per - 1) / per;
+    const int64_t wave = splits >= 3 && splits <= 8 ? sms * 6 / 7 : sms;
+    const int64_t cost = (base * splits + wave - 1) / wave * (per + 6) + (splits == 1 ? 0 : splits <= 8 ? 3 : 8);
+    if (cost < best) {
+      best = cost;
+      p.chunk = (int)(per * KT_KEYS);
+      p.splits = (int)splits;
+    }
+  }
+  p.cluster = p.splits > 1 && p.splits <= 8;
+  ns = best * (c->head_dim == 128 ? (f32 ? 1700 : 1400) : f32 ? 1350 : 1150);
+  return p;
+}
+
+// The kernel whose expected time is less.  Measured, 28 / 4 heads of 128, bf16, tiles of
+// 128 against tiles of 8 rows: 8 sequences of 1,200 keys with 2 new tokens 13.6 : 11.9 us,
+// 4 14.1 : 15.1, 16 15.9 : 45; one of 300 keys with 64 14 : 8.4 us, with 256 13 : 20.
+static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, bool f32, int sms) {
+  const int group = heads / c->kv_heads;
+  int64_t rows_ns, tiles_ns;
+  const KvAttnPlan rows = kv_plan_rows(c, b, group, f32, sms, rows_ns);
+  const KvAttnPlan tiles = kv_plan_tiles(c, b, group, f32, sms, tiles_ns);
+  KvAttnPlan p = tiles_ns < rows_ns ? tiles : rows;
   p.workspace = p.splits > 1 && !p.cluster ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
   return p;
 }
@@ -612,25 +604,30 @@ static const char* kv_attn_check(const rtr_kv_cache* c, const rtr_kv_batch* b, i
   return nullptr;
 }
 
-template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, int64_t items, int device, cudaStream_t st) {
-  static std::atomic<uint64_t> done;
-  cudaError_t e = kv_allow_smem(kv_attn_rows_kernel<T, D>, KaCfg<D>::SMEM, done, device);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)items, a.c.kv_heads, a.splits);
-  cfg.blockDim = dim3(KA_WARPS * 32);
-  cfg.dynamicSmemBytes = KaCfg<D>::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = a.splits;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.cluster ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kv_attn_rows_kernel<T, D>, a);
+template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, const KvAttnPlan& p, int device, cudaStream_t st) {
+  cudaError_t e;
+  if (p.tiles) {
+    e = kv_attn_tile(a, p.items, std::is_same<T, float>::value, device, st);
+  } else {
+    static std::atomic<uint64_t> done;
+    e = kv_allow_smem(kv_attn_rows_kernel<T, D>, KaCfg<D>::SMEM, done, device);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.items, a.c.kv_heads, a.splits);
+    cfg.blockDim = dim3(KA_WARPS * 32);
+    cfg.dynamicSmemBytes = KaCfg<D>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = a.splits;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kv_attn_rows_kernel<T, D>, a);
+  }
   if (e != cudaSuccess || a.splits == 1 || a.cluster) return e;
-  return launch_pdl(PDL_ATTN, kv_attn_join_kernel<T, D>, dim3((unsigned)(a.b.rows * a.heads)), dim3(KJ_THREADS), 0, st, a.b, a.heads,
-                    (const float*)a.part, (const float2*)a.ml, a.splits, static_cast<T*>(a.out), a.lse);
+  return launch_pdl(PDL_ATTN, kv_attn_join_kernel<T, D>, dim3((unsigned)(a.b.rows * a.heads)), dim3(KJ_THREADS), 0, st,
+                    a.b, a.heads, (const float*)a.part, (const float2*)a.ml, a.splits, static_cast<T*>(a.out), a.lse);
 }
 
 }  // namespace rtr
@@ -639,15 +636,15 @@ using namespace rtr;
 
 extern "C" {
 
-int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t heads, int32_t device,
-                               int64_t* bytes) {
+int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t dtype, int32_t heads,
+                               int32_t device, int64_t* bytes) {
   if (!bytes) return set_error(RTR_ERR_ARG, "null bytes");
   if (const char* e = kv_attn_check(cache, batch, heads)) return set_error(RTR_ERR_ARG, e);
   *bytes = 0;
   if (!batch->rows) return RTR_OK;
   KvDevice on(device);
   if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
-  *bytes = kv_attn_plan(cache, batch, heads, on.sms).workspace;
+  *bytes = kv_attn_plan(cache, batch, heads, dtype == RTR_DTYPE_F32, on.sms).workspace;
   return RTR_OK;
 }
 
@@ -664,7 +661,7 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
     return set_error(RTR_ERR_ARG, "q, its stride and out must be multiples of 16 bytes");
   KvDevice on(device);
   if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
-  const KvAttnPlan p = kv_attn_plan(cache, batch, heads, on.sms);
+  const KvAttnPlan p = kv_attn_plan(cache, batch, heads, dtype == RTR_DTYPE_F32, on.sms);
   if (p.items > INT32_MAX || p.splits > 65535 || cache->kv_heads > 65535)
     return set_error(RTR_ERR_ARG, "too many rows or keys for one call");
   if (p.workspace && (!workspace_dev || workspace_bytes < p.workspace || (reinterpret_cast<uintptr_t>(workspace_dev) & 15)))
@@ -689,10 +686,10 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == RTR_DTYPE_F32)
-    e = cache->head_dim == 128 ? kv_attn_launch<float, 128>(a, p.items, device, st) : kv_attn_launch<float, 64>(a, p.items, device, st);
+    e = cache->head_dim == 128 ? kv_attn_launch<float, 128>(a, p, device, st) : kv_attn_launch<float, 64>(a, p, device, st);
   else
-    e = cache->head_dim == 128 ? kv_attn_launch<__nv_bfloat16, 128>(a, p.items, device, st)
-                               : kv_attn_launch<__nv_bfloat16, 64>(a, p.items, device, st);
+    e = cache->head_dim == 128 ? kv_attn_launch<__nv_bfloat16, 128>(a, p, device, st)
+                               : kv_attn_launch<__nv_bfloat16, 64>(a, p, device, st);
   return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
 }
 

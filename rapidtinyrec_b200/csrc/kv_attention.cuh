@@ -1,0 +1,79 @@
+// What the two attention kernels over the 8-bit KV cache share
+// (kv_attention.cu: few rows, kv_attention_tile.cu: tiles of 128 rows).
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace rtr {
+
+struct KvAttn {
+  KvCache c;
+  KvBatch b;
+  const void* q;
+  int64_t q_token;     // elements between a token's rows; heads are contiguous
+  int heads, group;    // query heads, and those of one KV head
+  int causal;
+  float factor;        // softmax scale * log2(e)
+  void* out;           // [rows][heads][head_dim]
+  float* lse;          // [rows][heads] or null
+  float* part;         // [rows * heads][splits][head_dim] when splits > 1
+  float2* ml;          // [rows * heads][splits]: running maximum, sum
+  int per_seq;         // row tiles of a sequence without starts
+  int chunk, splits;   // keys of a block, and the blocks of a row tile
+  int cluster;         // the blocks of a row tile are one cluster and join among themselves
+};
+
+// Weights enter the fp16 operand times 2^6: a weight of 2^-24 of the largest (fp16's
+// smallest is 2^-24, so 2^-30 of it) still counts, and a maximum may be exceeded by 2^8
+// before a weight nears fp16's largest, 2^16.
+constexpr float KA_LIFT = 6.0f;
+
+RTR_DEVICE float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+RTR_DEVICE float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+RTR_DEVICE float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+RTR_DEVICE uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+RTR_DEVICE float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// Whether one of four codes is NaN (0x7f or 0xff).
+RTR_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// A K scale: negative ones (and NaN) make what uses them NaN.
+RTR_DEVICE float kv_k_scale(float ks) { return ks >= 0.f ? ks : __int_as_float(0x7fffffff); }
+// A V scale's two uses: log2 of it (an exponent's part) and its reciprocal.  NaN where
+// it lies outside [2^-48, 2^48].
+RTR_DEVICE void kv_v_scale(float vs, float& log2_scale, float& inverse) {
+  const bool fits = vs >= 1.0f / 281474976710656.0f && vs <= 281474976710656.0f;
+  log2_scale = fits ? log2f(vs) : __int_as_float(0x7fffffff);
+  inverse = fits ? 1.0f / vs : 0.f;
+}
+// The power of two that brings a row's largest magnitude into [2^13, 2^14), as its
+// exponent with the sign turned: the row is multiplied by 2^-e, its scores by 2^e.
+RTR_DEVICE int kv_row_exponent(float top) {
+  const int e = (int)(__float_as_uint(top) >> 23) - 127 - 13;
+  return top > 0.f && top < INFINITY ? max(-100, e) : 0;
+}
+RTR_DEVICE float kv_pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// Tiles of 128 rows on the 5th-generation tensor cores (kv_attention_tile.cu).
+constexpr int KT_ROWS = 128, KT_KEYS = 128;
+constexpr int KT_MAX_CHUNK = 8192;  // keys of a block
+cudaError_t kv_attn_tile(const KvAttn& a, int64_t items, bool f32, int device, cudaStream_t st);
+
+}  // namespace rtr

@@ -1,0 +1,777 @@
+// Attention over the 8-bit KV cache for many query rows: tiles of 128 (token,
+// head of the group) rows of one KV head on the 5th-generation tensor cores.
+//
+// The mathematics is that of kv_attention.cu: scores of the codes as they are, one
+// running maximum of score + log2(V scale) a row.  A block walks its keys in tiles of
+// 128; per tile S = Q K^T and O = P V are tcgen05 products with fp32 accumulators in
+// tensor memory.  Warps have one role each:
+//   rows     8 warps: scores to weights, which they write over the scores as the A
+//            operand of P V;
+//   codes    read K and V of the next tiles from the pages into registers, turn them
+//            into fp16 and store them as swizzled operands, V transposed;
+//   products one thread issues whichever product is ready.
+// There are two buffers of K, V, S and O, tile i in buffer i % 2.
+//
+// bf16 rows: two threads a row, each with 64 of a tile's keys, its own maximum, sum and
+// O in tensor memory; the two are joined at the end.  Weights are computed in one pass with
+// the maximum as it stands; only where a score exceeds it by more than 2^8 (weights stay
+// below 2^14) are O and the sum rescaled and the pass repeated.
+// fp32 rows: q and the weights enter as fp16 pairs, two products each.  The tensor core's
+// own accumulation drifts over thousands of keys, so tensor memory sums one tile only: two
+// threads a row (64 scores of the tile each) add it to half of the output's dimensions in
+// registers, by IEEE additions.
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "engine.h"
+#include "kv_attention.cuh"
+#include "kv_host.h"
+#include "tcgen05.cuh"
+
+namespace rtr {
+
+constexpr int KT_ROW_THREADS = 256;
+constexpr int KT_SEGS = KT_MAX_CHUNK / 16;
+constexpr float KT_SLACK = 8.0f;  // log2 by which a maximum may be exceeded (bf16 rows)
+
+template <int D, bool PAIR> struct KtCfg {
+  // code warps: eight keep up with one product a score; beside fp32 rows, whose threads
+  // need 128 registers, there is room for four
+  static constexpr int CODE_WARPS = 4;
+  static constexpr int CODE_THREADS = 32 * CODE_WARPS;
+  static constexpr int THREADS = KT_ROW_THREADS + CODE_THREADS + 32;
+  static constexpr int P_ARRIVALS = PAIR ? 256 : 128;          // row threads of a tile
+  static constexpr int PANELS = D / 64;                        // 128-byte panels of a q or k row
+  static constexpr int Q_PLANE = PANELS * KT_ROWS * 128;
+  static constexpr int Q_BYTES = (PAIR ? 2 : 1) * Q_PLANE;
+  static constexpr int K_BYTES = PANELS * KT_KEYS * 128;       // [panel][key][64 dims]
+  static constexpr int V_BYTES = 2 * D * 128;                  // [64 keys][dim][64 keys]: V transposed
+  static constexpr int Q_OFF = 0, K_OFF = Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES;
+  static constexpr int SEG_OFF = V_OFF + 2 * V_BYTES;          // int64 offsets, then 3 floats a segment
+  static constexpr int ROW_OFF = SEG_OFF + KT_SEGS * 20;       // per row: offset in q, row of out, keys it sees
+  static constexpr int RED_OFF = ROW_OFF + KT_ROWS * 16;       // [2][2][128] maxima
+  static constexpr int BAR_OFF = RED_OFF + 2 * 2 * KT_ROWS * 4;
+  static constexpr int STAGE_LD = D + 4;                       // row of the finished tile (over K and V), floats
+  static_assert(KT_ROWS * STAGE_LD * 4 <= 2 * (K_BYTES + V_BYTES), "the finished tile lies over K and V");
+  static constexpr int SMEM = BAR_OFF + 256 + 1024;            // 1024: alignment of the operands
+};
+
+struct KtBars {
+  uint64_t q_full, k_full[2], v_full[2], s_full[2], p_full[2][2], o_full[2][2], o_free[2];  // p, o: [half][buffer]
+  uint32_t tmem;
+  int abort_flag;
+  int nans;  // V has NaN codes in a tile that not every row sees as a whole
+};
+static_assert(sizeof(KtBars) <= 256, "barriers fit their part of shared memory");
+
+// D[tmem] (+)= A[tmem] . B[smem]^T, kind::f16 (both fp16)
+RTR_DEVICE void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+RTR_DEVICE void tmem_st_words(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+RTR_DEVICE void tmem_st_words(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+RTR_DEVICE void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+RTR_DEVICE void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+// Two fp32 lanes of one instruction.
+RTR_DEVICE uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+RTR_DEVICE uint64_t f2(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
+RTR_DEVICE float2 f2_parts(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+RTR_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+RTR_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+RTR_DEVICE void row_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+RTR_DEVICE uint32_t sw_at(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREADS, 1) kv_attn_tile_kernel(const KvAttn a) {
+  constexpr bool PAIR = std::is_same<T, float>::value;
+  using C = KtCfg<D, PAIR>;
+  constexpr int HD = D / 2;    // dimensions of the output a row thread finishes
+  constexpr int NL = D / 8;    // of those, the ones with the same d % 4
+  extern __shared__ uint8_t kt_smem_raw[];
+  __shared__ int slot;
+  uint8_t* smem = kt_smem_raw + ((1024u - (smem_addr(kt_smem_raw) & 1023u)) & 1023u);
+  uint8_t* qs = smem + C::Q_OFF;
+  int64_t* seg_at = reinterpret_cast<int64_t*>(smem + C::SEG_OFF);
+  float* seg_k = reinterpret_cast<float*>(seg_at + KT_SEGS);
+  float* seg_lv = seg_k + KT_SEGS;
+  float* seg_iv = seg_lv + KT_SEGS;
+  int64_t* row_q = reinterpret_cast<int64_t*>(smem + C::ROW_OFF);
+  int* row_out = reinterpret_cast<int*>(row_q + KT_ROWS);
+  int* row_lim = row_out + KT_ROWS;
+  float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
+  KtBars& bars = *reinterpret_cast<KtBars*>(smem + C::BAR_OFF);
+  volatile int* abort_flag = &bars.abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+
+  int seq;
+  int64_t item0;
+  if (a.b.starts) {
+    seq = kv_find_seq(a.b, blockIdx.x, a.group, 7, 1, &slot, item0);
+    if (seq < 0) return;
+  } else {
+    seq = (int)blockIdx.x / a.per_seq;
+    item0 = (int64_t)seq * a.per_seq;
+  }
+  int first, count, len;
+  const bool whole = kv_rows(a.b, seq, 0, (int64_t)a.b.table_width << a.c.page_shift, a.c.status, first, count, len);
+  if (!whole) {
+    if (count < 0) return;
+    len = 0;  // a length that does not fit: the sequence's rows become NaN
+  }
+  const int nrows = count * a.group, r0 = (int)(blockIdx.x - item0) * KT_ROWS;
+  if (r0 >= nrows) return;
+  const auto limit = [&](int row) { return a.causal ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
+  const int rows = min(KT_ROWS, nrows - r0);
+  const int kmin = limit(r0), kmax = limit(r0 + KT_ROWS - 1);
+  const int c0 = split * a.chunk, c1 = min(kmax, c0 + a.chunk);
+  if (c1 <= c0 && split > 0 && !a.cluster) {  // a stretch behind the last key (the first one reports rows that see nothing)
+    if (tid < rows) {
+      const int token = (r0 + tid) / a.group;
+      const int64_t rh = (int64_t)(first + token) * a.heads + kvh * a.group + (r0 + tid - token * a.group);
+      a.ml[rh * a.splits + split] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+  const int n = c1 > c0 ? (c1 - c0 + KT_KEYS - 1) / KT_KEYS : 0;
+  const int segs = c1 > c0 ? (c1 - c0 + 15) / 16 : 0;  // 16-key segments of the stretch
+
+  if (tid == 0) {
+    mbar_init(smem_addr(&bars.q_full), KT_ROW_THREADS);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&bars.k_full[i]), C::CODE_THREADS);
+      mbar_init(smem_addr(&bars.v_full[i]), C::CODE_THREADS);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_addr(&bars.p_full[h][i]), C::P_ARRIVALS);
+        mbar_init(smem_addr(&bars.o_full[h][i]), 1);
+      }
+      mbar_init(smem_addr(&bars.o_free[i]), KT_ROW_THREADS);
+      mbar_init(smem_addr(&bars.s_full[i]), 1);
+    }
+    bars.nans = 0;
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8 + C::CODE_WARPS) tmem_alloc(smem_addr(&bars.tmem), 512);
+  // the rows' places, by one division each
+  if (const int row = C::THREADS - 1 - tid; row < KT_ROWS) {
+    const int rr = min(r0 + row, nrows - 1), token = rr / a.group, head = kvh * a.group + rr - token * a.group;
+    row_q[row] = (int64_t)(first + token) * a.q_token + (int64_t)head * D;
+    row_out[row] = (first + token) * a.heads + head;
+    row_lim[row] = limit(rr);
+  }
+  // pages and scales of the stretch's 16-key segments (a page is a multiple of 16)
+  for (int s = tid; s < segs; s += C::THREADS) {
+    const int key = c0 + 16 * s;
+    const int page = kv_page(a.c, a.b, seq, key >> a.c.page_shift);
+    int64_t at = kvh * a.c.head_stride;
+    float ks, lv, iv = 0.f;
+    ks = lv = __int_as_float(0x7fffffff);  // a page that is not there makes the rows NaN, whatever codes are read
+    if (page >= 0) {
+      at += page * a.c.page_stride + (int64_t)(key & ((1 << a.c.page_shift) - 1)) * D;
+      ks = kv_k_scale(a.c.k_scale[page * a.c.scale_stride + kvh]);
+      kv_v_scale(a.c.v_scale[page * a.c.scale_stride + kvh], lv, iv);
+    }
+    seg_at[s] = at;
+    seg_k[s] = ks;
+    seg_lv[s] = lv;
+    seg_iv[s] = iv;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  constexpr uint32_t S_COLS = KT_KEYS, O_AT = 2 * S_COLS;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------- rows
+    const int half = warp >> 2, r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    {
+      // q as fp16 (pairs), each row times a power of two; a warp takes 16 rows, LPR lanes a row
+      constexpr int PER = 16 / sizeof(T), LPR = D / PER, RPI = 32 / LPR, BATCH = 8;
+      constexpr int LOADS = 16 / RPI, STEP = LOADS < BATCH ? LOADS : BATCH;
+      const int sub = lane / LPR, col = lane % LPR;
+#pragma unroll
+      for (int base = 0; base < LOADS; base += STEP) {
+        uint4 u[STEP];
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
+          const int row = warp * 16 + (base + j) * RPI + sub;
+          u[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (row < rows) u[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + row_q[row] + col * PER);
+        }
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
+          const int row = warp * 16 + (base + j) * RPI + sub;
+          const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+          float x[PER], top = 0.f;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            if constexpr (PAIR) x[i] = __uint_as_float(w[i]);
+            else x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+            top = fmaxf(top, fabsf(x[i]));
+          }
+#pragma unroll
+          for (int d = 1; d < LPR; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const int e = kv_row_exponent(top);
+          const float up = copysignf(kv_pow2(-e), a.factor);  // the factor back stays positive: see below
+          if (col == 0) red[row] = kv_pow2(e) * fabsf(a.factor);
+          uint32_t hi[PER / 2], lo[PER / 2];
+#pragma unroll
+          for (int i = 0; i < PER / 2; ++i) {
+            hi[i] = pack_f16(x[2 * i] * up, x[2 * i + 1] * up);
+            const float2 b = unpack_f16(hi[i]);
+            lo[i] = pack_f16(x[2 * i] * up - b.x, x[2 * i + 1] * up - b.y);
+          }
+          const int unit = col * PER / 8;
+          uint8_t* at = qs + (unit >> 3) * KT_ROWS * 128 + sw_at(row, unit & 7);
+          if constexpr (PAIR) {
+            at += 8 * (col & 1);
+            *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(at + C::Q_PLANE) = make_uint2(lo[0], lo[1]);
+          } else {
+            *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          }
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(smem_addr(&bars.q_full));
+    }
+    row_barrier();
+    const float f = red[r];  // back to the score, in units of log2; positive
+    row_barrier();
+    const int lim = row_lim[r];
+    uint64_t o[HD / 2];  // pairs; value t * NL + l: dimension half * HD + 4 l + t
+    float m = -INFINITY, l = 0.f;
+
+    if constexpr (PAIR) {
+#pragma unroll
+      for (int i = 0; i < HD / 2; ++i) o[i] = 0;
+      float alpha = 1.f;
+
+      // adds the finished product of tile i, whose weights are relative to the maximum of
+      // that tile; `grew` scales what was summed before it
+      const auto add_product = [&](int i, float grew) {
+        mbar_wait(smem_addr(&bars.o_full[0][i & 1]), (i >> 1) & 1, abort_flag);
+        tc_fence_after();
+        const uint32_t at = tmem + lanes + O_AT + (i & 1) * 128 + half * NL;
+        const uint64_t by = f2(grew, grew);
+        uint32_t v[2][NL];
+        tmem_ld_cols(at, v[0]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          tmem_ld_wait();
+          if (t < 3) tmem_ld_cols(at + (t + 1) * (D / 4), v[(t + 1) & 1]);
+#pragma unroll
+          for (int j = 0; j < NL / 2; ++j)
+            o[t * NL / 2 + j] = f2_fma(o[t * NL / 2 + j], by, f2(v[t & 1][2 * j], v[t & 1][2 * j + 1]));
+        }
+        tc_fence_before();
+        mbar_arrive(smem_addr(&bars.o_free[i & 1]));
+      };
+
+      for (int i = 0; i < n; ++i) {
+        mbar_wait(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1, abort_flag);
+        tc_fence_after();
+        const uint32_t st = tmem + lanes + (i & 1) * S_COLS + half * 64;
+        const int key0 = c0 + i * KT_KEYS + half * 64, seg0 = i * 8 + half * 4;
+        const bool border = key0 + 64 > kmin;
+        float mx = -INFINITY;
+        uint32_t v[2][16];
+        tmem_ld16(st, v[0]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int s = min(seg0 + g, segs - 1);
+          const float kf = f * seg_k[s], lv = seg_lv[s];
+          tmem_ld_wait();
+          if (g < 3) tmem_ld16(st + 16 * (g + 1), v[(g + 1) & 1]);
+          float top = -INFINITY;
+          if (border) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (key0 + 16 * g + j < lim) top = fmaxf(top, __uint_as_float(v[g & 1][j]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; j += 2)
+              top = fmaxf(top, fmaxf(__uint_as_float(v[g & 1][j]), __uint_as_float(v[g & 1][j + 1])));
+          }
+          // kf is positive: the largest product of a segment gives its largest score
+          mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, kf, lv));
+        }
+        float* rm = red + (i & 1) * 2 * KT_ROWS;
+        rm[half * KT_ROWS + r] = mx;
+        row_barrier();
+        const float top = fmaxf(m, fmaxf(rm[r], rm[KT_ROWS + r]));
+        const float grew = alpha;  // of the tile before: scales what came before that tile's product
+        alpha = m == top ? 1.f : ex2(m - top);
+        m = top;
+        l *= alpha;
+        const float u = (m == -INFINITY ? 0.f : m) - KA_LIFT;
+        // 16 keys at a time, the next ones on their way: few registers are left beside o
+        tmem_ld16(st, v[0]);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int s = min(seg0 + g, segs - 1);
+          const float kf = f * seg_k[s], lv = seg_lv[s] - u, iv = seg_iv[s];
+          const uint64_t kf2 = f2(kf, kf), lv2 = f2(lv, lv);
+          tmem_ld_wait();
+          if (g < 3) tmem_ld16(st + 16 * (g + 1), v[(g + 1) & 1]);
+          uint64_t sums = 0;
+          uint32_t w[PAIR ? 16 : 8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float2 x = f2_parts(f2_fma(f2(v[g & 1][2 * j], v[g & 1][2 * j + 1]), kf2, lv2));
+            if (border) {
+              if (key0 + 16 * g + 2 * j >= lim) x.x = -INFINITY;
+              if (key0 + 16 * g + 2 * j + 1 >= lim) x.y = -INFINITY;
+            }
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sums = f2_add(sums, f2(x.x, x.y));
+            w[j] = pack_f16(x.x, x.y);
+            if constexpr (PAIR) {
+              const float2 b = unpack_f16(w[j]);
+              w[8 + j] = pack_f16(x.x - b.x, x.y - b.y);
+            }
+          }
+          const float sum = f2_parts(sums).x + f2_parts(sums).y;
+          l = fmaf(sum, iv, l);
+          tmem_st_words(st + 16 * g, w);  // over the scores just read
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_addr(&bars.p_full[0][i & 1]));
+        if (i > 0) add_product(i - 1, grew);
+      }
+      if (n > 0) add_product(n - 1, alpha);
+      // the row's two halves of the sum
+      row_barrier();
+      red[half * KT_ROWS + r] = l;
+      row_barrier();
+      l = red[r] + red[KT_ROWS + r];
+    } else {
+      const uint32_t ot = tmem + lanes + O_AT + half * 128;
+      for (int i = 0; i < n; ++i) {
+        mbar_wait(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1, abort_flag);
+        tc_fence_after();
+        const uint32_t st = tmem + lanes + (i & 1) * S_COLS + half * 64;
+        const int key0 = c0 + i * KT_KEYS + half * 64, seg0 = i * 8 + half * 4;
+        const bool border = key0 + 64 > kmin;
+        // One pass with the maximum as it stands, which also finds the tile's own; where
+        // that is too far above, a second one with the new maximum.
+        uint32_t w[32];
+        float mx, part_l;
+        const auto weigh = [&](float u) {
+          uint32_t v[2][16];
+          tmem_ld16(st, v[0]);
+          mx = -INFINITY;
+          part_l = 0.f;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int s = min(seg0 + g, segs - 1);
+            const float kf = f * seg_k[s], lv = seg_lv[s], iv = seg_iv[s];
+            const uint64_t kf2 = f2(kf, kf), lv2 = f2(lv - u, lv - u);
+            tmem_ld_wait();
+            uint32_t(&x)[16] = v[g & 1];
+            if (g < 3) tmem_ld16(st + 16 * (g + 1), v[(g + 1) & 1]);
+            if (border) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (key0 + 16 * g + j >= lim) x[j] = 0xff800000u;
+            }
+            float top = -INFINITY;
+            uint64_t sums = 0;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              top = fmaxf(top, fmaxf(fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])),
+                                     fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]))));
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                float2 y = f2_parts(f2_fma(f2(x[j + e], x[j + e + 1]), kf2, lv2));
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+                sums = f2_add(sums, f2(y.x, y.y));
+                w[8 * g + (j + e) / 2] = pack_f16(y.x, y.y);
+              }
+            }
+            part_l = fmaf(f2_parts(sums).x + f2_parts(sums).y, iv, part_l);
+            // the factors are positive: the largest product of a segment gives its largest score
+            mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, kf, lv));
+          }
+        };
+        weigh((m == -INFINITY ? 0.f : m) - KA_LIFT);
+        if (__any_sync(0xffffffffu, mx > m + KT_SLACK)) {  // m may be minus infinity
+          const float top = fmaxf(m, mx), alpha = m == top ? 1.f : ex2(m - top);
+          m = top;
+          l *= alpha;
+          if (i > 0) {
+            mbar_wait(smem_addr(&bars.o_full[half][(i - 1) & 1]), ((i - 1) >> 1) & 1, abort_flag);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t v[16];
+              tmem_ld16(ot + c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+              tmem_st_words(ot + c, v);
+            }
+          }
+          weigh((m == -INFINITY ? 0.f : m) - KA_LIFT);
+        }
+        l += part_l;
+        tmem_st32(st, w);  // over the scores just read
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_addr(&bars.p_full[half][i & 1]));
+      }
+      // join the two halves' sums: each finishes half of the dimensions of every row
+      float* other_l = red + 2 * KT_ROWS;
+      red[half * KT_ROWS + r] = m;
+      other_l[half * KT_ROWS + r] = l;
+      if (n > 0) {
+        mbar_wait(smem_addr(&bars.o_full[0][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag);
+        mbar_wait(smem_addr(&bars.o_full[1][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag);
+      }
+      tc_fence_after();
+      row_barrier();
+      const float m0 = red[r], m1 = red[KT_ROWS + r];
+      m = fmaxf(m0, m1);
+      const float f0 = m0 == m ? 1.f : ex2(m0 - m), f1 = m1 == m ? 1.f : ex2(m1 - m);
+      l = other_l[r] * f0 + other_l[KT_ROWS + r] * f1;
+      const uint64_t f02 = f2(f0, f0), f12 = f2(f1, f1);
+      const uint32_t at = tmem + lanes + O_AT + half * NL;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t v[2][NL];
+        if (n > 0) {
+          tmem_ld_cols(at + t * (D / 4), v[0]);
+          tmem_ld_cols(at + 128 + t * (D / 4), v[1]);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < NL / 2; ++j)
+          o[t * NL / 2 + j] = n > 0 ? f2_fma(f2(v[1][2 * j], v[1][2 * j + 1]), f12,
+                                             f2_fma(f2(v[0][2 * j], v[0][2 * j + 1]), f02, 0)) : 0;
+      }
+    }
+
+    float lt = l;
+    if (bars.nans) {  // NaN codes of V entered the products as 0: put back what the row sees
+      for (int key = max(c0, kmin & ~(KT_KEYS - 1)); key < min(lim, c1); ++key) {
+        const uint8_t* p = a.c.v + seg_at[(key - c0) >> 4] + (key & 15) * D + half * HD;
+#pragma unroll
+        for (int i = 0; i < HD / 2; ++i) {
+          const int d = 4 * (2 * i % NL) + 2 * i / NL;  // of the pair's first value; the second is 4 behind
+          float2 x = f2_parts(o[i]);
+          if ((p[d] & 0x7f) == 0x7f) x.x = __int_as_float(0x7fffffff);
+          if ((p[d + 4] & 0x7f) == 0x7f) x.y = __int_as_float(0x7fffffff);
+          o[i] = f2(x.x, x.y);
+        }
+      }
+    }
+    if (lt == 0.f && (lim > c0 || !whole)) lt = __int_as_float(0x7fffffff);
+    // through shared memory (the operands are done with), for whole lines on the way out
+    float* stage = reinterpret_cast<float*>(smem + C::K_OFF);
+    const auto value = [&](int i) { return i & 1 ? f2_parts(o[i >> 1]).y : f2_parts(o[i >> 1]).x; };
+#pragma unroll
+    for (int j = 0; j < NL; ++j)
+      reinterpret_cast<float4*>(stage + r * C::STAGE_LD + half * HD)[j] =
+          make_float4(value(j), value(NL + j), value(2 * NL + j), value(3 * NL + j));
+    row_barrier();  // red has been read
+    if (half == 0) reinterpret_cast<float2*>(red)[r] = make_float2(m, lt);
+  } else if (warp < 8 + C::CODE_WARPS) {
+    // ------------------------------------------------------------ codes
+    const int cw = warp - 8;
+    constexpr int KP = KT_KEYS * D / 16 / C::CODE_THREADS;  // 16-byte pieces of K a thread: 8 or 4
+    constexpr int LPK = D / 16;                              // threads of a key
+    constexpr int VO = KT_KEYS / 8 * (D / 4) / C::CODE_THREADS;  // (8 keys x 4 dims) blocks of V a thread: 4 or 2
+    // Of K, eight consecutive lanes take four pieces of one panel of two neighbouring keys:
+    // their stores then hit all banks.
+    const int piece = D == 128 ? (lane & 3) + 4 * (lane >> 3 & 1) : lane & 3;
+    const int key_of = cw * (32 / LPK) + (D == 128 ? 2 * (lane >> 4) + (lane >> 2 & 1) : lane >> 2);
+    const int dl = lane % (D / 4);
+    uint4 kr[KP];
+    uint32_t vr[VO][8];
+    // Loads need no conditions: a segment lies in one page as a whole, and what is read of keys
+    // behind the last (or of the last segment again) is masked, NaN codes are taken out below.
+    const auto load_k = [&](int i) {
+#pragma unroll
+      for (int p = 0; p < KP; ++p) {
+        const int rel = i * KT_KEYS + p * (C::CODE_THREADS / LPK) + key_of;
+        kr[p] = __ldg(reinterpret_cast<const uint4*>(a.c.k + seg_at[min(rel >> 4, segs - 1)] + (rel & 15) * D + 16 * piece));
+      }
+    };
+    const auto octet = [&](int v) { return (v * C::CODE_WARPS + cw) * (32 / (D / 4)) + lane / (D / 4); };
+    const auto load_v = [&](int i) {
+#pragma unroll
+      for (int v = 0; v < VO; ++v) {
+        const int rel = i * KT_KEYS + 8 * octet(v);
+        const uint8_t* p = a.c.v + seg_at[min(rel >> 4, segs - 1)] + (rel & 8) * D + 4 * dl;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) vr[v][k] = __ldg(reinterpret_cast<const uint32_t*>(p + k * D));
+      }
+    };
+    if (n > 0) {
+      load_k(0);
+      load_v(0);
+    }
+    for (int i = 0; i < n; ++i) {
+      // S and O of tile i - 2 are done with the buffers
+      if (i >= 2 && !mbar_wait(smem_addr(&bars.s_full[i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      uint8_t* kd = smem + C::K_OFF + (i & 1) * C::K_BYTES;
+#pragma unroll
+      for (int p = 0; p < KP; ++p) {
+        const int key = p * (C::CODE_THREADS / LPK) + key_of;
+        const uint32_t w[4] = {kr[p].x, kr[p].y, kr[p].z, kr[p].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          h[2 * j] = e4m3x2_to_f16x2((uint16_t)w[j]);
+          h[2 * j + 1] = e4m3x2_to_f16x2((uint16_t)(w[j] >> 16));
+        }
+        uint8_t* row = kd + (piece >> 2) * KT_KEYS * 128;
+        const int un = 2 * (piece & 3);
+        *reinterpret_cast<uint4*>(row + sw_at(key, un)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(row + sw_at(key, un + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+      }
+      fence_proxy_async();
+      mbar_arrive(smem_addr(&bars.k_full[i & 1]));
+      if (i + 1 < n) load_k(i + 1);
+      if (i >= 2 && !mbar_wait(smem_addr(&bars.o_full[0][i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      if (!PAIR && i >= 2 && !mbar_wait(smem_addr(&bars.o_full[1][i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      if (c0 + (i + 1) * KT_KEYS > kmin) {
+        // not every row sees every key of the tile: 0 * NaN must not reach the others
+        uint32_t bad = 0;
+#pragma unroll
+        for (int v = 0; v < VO; ++v)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t nb = nan_bytes(vr[v][k]);
+            bad |= nb;
+            vr[v][k] &= ~((nb >> 7) * 0xffu);
+          }
+        if (bad) bars.nans = 1;
+      }
+      uint8_t* vd = smem + C::V_OFF + (i & 1) * C::V_BYTES;
+#pragma unroll
+      for (int v = 0; v < VO; ++v) {
+        const int oc = octet(v);
+        uint32_t h[4][4];  // [dim t][keys 2 j, 2 j + 1]
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = __byte_perm(vr[v][2 * j], vr[v][2 * j + 1], 0x5140);
+          const uint32_t y = __byte_perm(vr[v][2 * j], vr[v][2 * j + 1], 0x7362);
+          h[0][j] = e4m3x2_to_f16x2((uint16_t)x);
+          h[1][j] = e4m3x2_to_f16x2((uint16_t)(x >> 16));
+          h[2][j] = e4m3x2_to_f16x2((uint16_t)y);
+          h[3][j] = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+        }
+        // dimension 4 dl + t becomes row t (D / 4) + dl: consecutive lanes, consecutive rows
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          *reinterpret_cast<uint4*>(vd + (oc >> 3) * D * 128 + sw_at(t * (D / 4) + dl, oc & 7)) =
+              make_uint4(h[t][0], h[t][1], h[t][2], h[t][3]);
+      }
+      fence_proxy_async();
+      mbar_arrive(smem_addr(&bars.v_full[i & 1]));
+      if (i + 1 < n) load_v(i + 1);
+    }
+  } else if (lane == 0) {
+    // --------------------------------------------------------- products
+    constexpr uint32_t id_s = idesc_f16(KT_ROWS, KT_KEYS), id_o = idesc_f16(KT_ROWS, D);
+    const auto issue_s = [&](int i) {
+      const uint8_t* kd = smem + C::K_OFF + (i & 1) * C::K_BYTES;
+#pragma unroll
+      for (int pl = 0; pl < (PAIR ? 2 : 1); ++pl)
+#pragma unroll
+        for (int p = 0; p < C::PANELS; ++p) {
+          const uint64_t qd = sw128_desc(smem_addr(qs + pl * C::Q_PLANE + p * KT_ROWS * 128));
+          const uint64_t kk = sw128_desc(smem_addr(kd + p * KT_KEYS * 128));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16_ss(tmem + (i & 1) * S_COLS, qd + 2 * k, kk + 2 * k, id_s, (pl | p | k) ? 1u : 0u);
+        }
+      mma_commit(smem_addr(&bars.s_full[i & 1]));
+    };
+    // fp32 rows: the whole tile's product, alone in its buffer; bf16 rows: that of one half
+    // of the keys, added to the half's sum
+    const auto issue_o = [&](int i, int h) {
+      const uint8_t* vd = smem + C::V_OFF + (i & 1) * C::V_BYTES;
+      const uint32_t pt = tmem + (i & 1) * S_COLS, ot = tmem + O_AT + (PAIR ? i & 1 : h) * 128;
+#pragma unroll
+      for (int k = 0; k < (PAIR ? 8 : 4); ++k) {  // 16 keys each
+        const int ks = PAIR ? k : 4 * h + k;
+        const uint64_t vv = sw128_desc(smem_addr(vd + (ks >> 2) * D * 128)) + 2 * (ks & 3);
+        if constexpr (PAIR) {
+          const uint32_t p = pt + 16 * k;  // the weights, then their low parts, lie over the scores of their keys
+          mma_f16_ts(ot, p, vv, id_o, k ? 1u : 0u);
+          mma_f16_ts(ot, p + 8, vv, id_o, 1u);
+        } else {
+          mma_f16_ts(ot, pt + 64 * h + 8 * k, vv, id_o, k || i > 0 ? 1u : 0u);
+        }
+      }
+      mma_commit(smem_addr(&bars.o_full[h][i & 1]));
+    };
+    constexpr int HALVES = PAIR ? 1 : 2;
+    int si = 0, oi[2] = {0, 0};  // products issued
+    const auto wait = [&](uint64_t& bar, int i) { return mbar_wait(smem_addr(&bar), (i >> 1) & 1, abort_flag); };
+    bool ok = n == 0 || mbar_wait(smem_addr(&bars.q_full), 0, abort_flag);
+    const auto next_s = [&] {
+      if (si >= n) return true;
+      if (!wait(bars.k_full[si & 1], si)) return false;
+      // S goes over the weights of the tile two before: their products must be done
+      for (int h = 0; h < HALVES; ++h)
+        if (si >= 2 && !wait(bars.o_full[h][si & 1], si - 2)) return false;
+      tc_fence_after();
+      issue_s(si++);
+      return true;
+    };
+    ok = ok && next_s() && next_s();
+    for (int i = 0; i < n && ok; ++i) {
+      for (int h = 0; h < HALVES && ok; ++h) {
+        ok = wait(bars.p_full[h][i & 1], i) && wait(bars.v_full[i & 1], i) &&
+             (!PAIR || i < 2 || wait(bars.o_free[i & 1], i - 2));
+        if (!ok) break;
+        tc_fence_after();
+        issue_o(i, h);
+        oi[h] = i + 1;
+      }
+      ok = ok && next_s();
+    }
+    if (!ok) {
+      atomicOr(a.c.status, RTR_DEV_TIMEOUT);
+      for (int i = si > 2 ? si - 2 : 0; i < si; ++i) mbar_drain(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1);
+      for (int h = 0; h < HALVES; ++h)
+        for (int i = oi[h] > 2 ? oi[h] - 2 : 0; i < oi[h]; ++i)
+          mbar_drain(smem_addr(&bars.o_full[h][i & 1]), (i >> 1) & 1);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8 + C::CODE_WARPS) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  pdl_launch_dependents();
+  // D / 4 threads a row; every warp takes rows in turn
+  const float* stage = reinterpret_cast<const float*>(smem + C::K_OFF);
+  const float2* ml = reinterpret_cast<const float2*>(red);
+  constexpr int LPR = D / 4, RPI = 32 / LPR, WARPS = C::THREADS / 32;
+  const int col = lane % LPR;
+  const auto finish = [&](int row, float m, float l, float4 x) {
+    const int64_t rh = row_out[row];
+    const bool sees = l != 0.f;
+    const float inv = sees ? 1.0f / l : 0.f;
+    x = sees ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+    T* p = static_cast<T*>(a.out) + rh * D + 4 * col;
+    if constexpr (PAIR) {
+      *reinterpret_cast<float4*>(p) = x;
+    } else {
+      const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+      *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(b);
+    }
+    if (a.lse && col == 0) a.lse[rh] = sees ? (m - KA_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  };
+  if (!a.cluster) {
+    for (int row = warp * RPI + lane / LPR; row < rows; row += WARPS * RPI) {
+      const float4 x = *reinterpret_cast<const float4*>(stage + row * C::STAGE_LD + 4 * col);
+      const float2 v = ml[row];
+      if (a.splits == 1) {
+        finish(row, v.x, v.y, x);
+      } else {
+        const int64_t at = (int64_t)row_out[row] * a.splits + split;
+        reinterpret_cast<float4*>(a.part + at * D)[col] = x;
+        if (col == 0) a.ml[at] = v;
+      }
+    }
+    return;
+  }
+  // the cluster's blocks share out the rows, each reads the others' sums
+  cluster_sync_all();
+  for (int row = split + a.splits * (warp * RPI + lane / LPR); row < rows; row += a.splits * WARPS * RPI) {
+    const uint32_t ml_at = smem_addr(&ml[row]), x_at = smem_addr(stage + row * C::STAGE_LD + 4 * col);
+    float mt = -INFINITY, lt = 0.f;
+    for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, ld_cluster_f32(cluster_map(ml_at, s)));
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.splits; ++s) {
+      const uint32_t at = cluster_map(ml_at, s);
+      const float ms = ld_cluster_f32(at), w = ms == mt ? 1.f : ex2(ms - mt);
+      const float4 v = ld_cluster_f4(cluster_map(x_at, s));
+      lt = fmaf(ld_cluster_f32(at + 4), w, lt);
+      x = make_float4(fmaf(v.x, w, x.x), fmaf(v.y, w, x.y), fmaf(v.z, w, x.z), fmaf(v.w, w, x.w));
+    }
+    finish(row, mt, lt, x);
+  }
+  __syncwarp();
+  cluster_sync_all();  // no block leaves while another may still read its sums
+}
+
+template <typename T, int D> static cudaError_t launch_tile(const KvAttn& a, int64_t items, int device, cudaStream_t st) {
+  constexpr int smem = KtCfg<D, std::is_same<T, float>::value>::SMEM;
+  static_assert(smem <= 227 * 1024, "a block's shared memory");
+  static std::atomic<uint64_t> done;
+  const cudaError_t e = kv_allow_smem(kv_attn_tile_kernel<T, D>, smem, done, device);
+  if (e != cudaSuccess) return e;
+  constexpr int threads = KtCfg<D, std::is_same<T, float>::value>::THREADS;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)items, a.c.kv_heads, a.splits);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = a.splits;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv_attn_tile_kernel<T, D>, a);
+}
+
+cudaError_t kv_attn_tile(const KvAttn& a, int64_t items, bool f32, int device, cudaStream_t st) {
+  if (f32)
+    return a.c.head_dim == 128 ? launch_tile<float, 128>(a, items, device, st) : launch_tile<float, 64>(a, items, device, st);
+  return a.c.head_dim == 128 ? launch_tile<__nv_bfloat16, 128>(a, items, device, st)
+                             : launch_tile<__nv_bfloat16, 64>(a, items, device, st);
+}
+
+}  // namespace rtr

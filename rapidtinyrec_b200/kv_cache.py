@@ -204,11 +204,12 @@ class KvCache8:
         if heads > 1 and q.stride(1) != self.head_dim:
             q = q.clone(memory_format=torch.contiguous_format)
         batch = self._batch(rows, table, lens, starts)
-        key = (rows, heads, table.shape, starts is None)
+        key = (rows, heads, table.shape, starts is None, q.dtype)
         room = self._room.get(key)
         if room is None:
             need = ctypes.c_int64()
-            _native.check(self.lib.rtr_kv_attention_workspace(self._ref, batch, heads, self._index, ctypes.byref(need)))
+            _native.check(self.lib.rtr_kv_attention_workspace(self._ref, batch, _DTYPES[q.dtype], heads, self._index,
+                                                                   ctypes.byref(need)))
             if len(self._room) >= 4096:
                 self._room.clear()
             room = self._room[key] = need.value

@@ -71,7 +71,7 @@ def test_rows_that_are_refused():
         assert says in message()
     assert attention(cache(), batch(rows=1 << 30, seqs=1)) == _native.RTR_ERR_ARG and '2^31' in message()
     lib = _native.load()
-    assert lib.rtr_kv_attention_workspace(ctypes.byref(cache()), ctypes.byref(batch()), 8, 0, None) == _native.RTR_ERR_ARG
+    assert lib.rtr_kv_attention_workspace(ctypes.byref(cache()), ctypes.byref(batch()), 0, 8, 0, None) == _native.RTR_ERR_ARG
     assert lib.rtr_kv_write(None, None, A, A, 0, 512, 128, 512, 128, 0, None) == _native.RTR_ERR_ARG
 
 
