@@ -24,40 +24,53 @@
 
 namespace rtr {
 
-constexpr int KV_THREADS = 256;
+constexpr int KV_THREADS = 512;
+constexpr float KV_LARGEST = 448.0f * 281474976710656.0f;  // 448 * 2^48
 
-template <typename T> struct Dense;  // 16 bytes of a dense row
-template <> struct Dense<float> {
-  static constexpr int N = 4;
-  static RTR_DEVICE void load(const float* p, float (&x)[4]) {
-    const float4 u = __ldcs(reinterpret_cast<const float4*>(p));
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-  }
-  static RTR_DEVICE void store(float* p, const float (&x)[4]) {
-    __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
-  }
-};
-template <> struct Dense<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static RTR_DEVICE void load(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// 16 bytes of a dense row, as they come and as values.
+RTR_DEVICE uint4 load16(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
+RTR_DEVICE void values_of(const uint4& u, float (&x)[4]) {
+  x[0] = __uint_as_float(u.x);
+  x[1] = __uint_as_float(u.y);
+  x[2] = __uint_as_float(u.z);
+  x[3] = __uint_as_float(u.w);
+}
+RTR_DEVICE void values_of(const uint4& u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
-  static RTR_DEVICE void store(__nv_bfloat16* p, const float (&x)[8]) {
-    uint32_t w[4];
+}
+// The largest magnitude of 16 bytes of values, as a float's bits.
+template <typename T> RTR_DEVICE uint32_t top_bits(const uint4& u);
+template <> RTR_DEVICE uint32_t top_bits<float>(const uint4& u) {
+  return max(max(u.x & 0x7fffffffu, u.y & 0x7fffffffu), max(u.z & 0x7fffffffu, u.w & 0x7fffffffu));
+}
+template <> RTR_DEVICE uint32_t top_bits<__nv_bfloat16>(const uint4& u) {
+  const uint32_t m = 0x7fff7fffu, a = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+  return max(a << 16, a & 0xffff0000u);
+}
+// The largest of all threads' values (one synchronisation; `red` is free again after the next).
+RTR_DEVICE uint32_t block_max(uint32_t v, uint32_t* red, int warps) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0u);
+}
+RTR_DEVICE void store16(float* p, const float (&x)[4]) {
+  __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+}
+RTR_DEVICE void store16(__nv_bfloat16* p, const float (&x)[8]) {
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
   }
-};
+  __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+}
 
 // N codes of one thread (N = 4 or 8).
 template <int N> struct Codes {
@@ -98,18 +111,25 @@ RTR_DEVICE float least_scale(float amax) {
   return __uint_as_float((uint32_t)(127 + max(-KV_EXP, min(KV_EXP, e))) << 23);
 }
 
-// x / s, exactly rounded: by the reciprocal where s is a power of two (its
-// reciprocal is one too), by a division for scales from elsewhere.
-struct Divider {
-  float s, r;
-  bool pow2;
-  explicit RTR_DEVICE Divider(float by) {
-    s = by;
-    r = 1.0f / by;
-    pow2 = (__float_as_uint(by) & 0x7fffffu) == 0;
-  }
-  RTR_DEVICE float operator()(float x) const { return pow2 ? x * r : __fdiv_rn(x, s); }
-};
+// What the common path leaves, exactly rounded: scales that are no power of two (from
+// elsewhere), values that become NaN; and older codes at a larger scale.
+template <int N> __device__ __noinline__ Codes<N> encode_odd(uint4 raw, float s) {
+  float x[N];
+  values_of(raw, x);
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = fabsf(x[j]) <= KV_LARGEST ? __fdiv_rn(x[j], s) : __int_as_float(0x7fffffff);
+  Codes<N> q;
+  q.set(x);
+  return q;
+}
+template <int N> __device__ __noinline__ Codes<N> encode_again(Codes<N> q, float had, float s) {
+  float x[N];
+  q.get(x);
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = __fdiv_rn(x[j] * had, s);
+  q.set(x);
+  return q;
+}
 
 // The part of a sequence's rows that falls into one of its pages.
 struct PageRows {
@@ -144,116 +164,145 @@ RTR_DEVICE bool kv_page_rows(const KvCache& c, const KvBatch& b, int64_t item, i
   return pr.page >= 0;
 }
 
-// CH 16-byte pieces of the page a thread: page * head_dim = CH * blockDim * N.
-template <typename T, int CH>
-__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvCache c, const KvBatch b, const T* __restrict__ k,
+// A block's threads take CH 16-byte pieces of the page each: page * D = CH * blockDim * N.
+// AHEAD: the next unit's rows are on their way while a unit's maximum is found and its
+// codes are written.  Blocks of one unit are without, in registers that let three of 512
+// threads share an SM (two with eight pieces): 350 fp32 tokens of 56 heads, 13.0 us with
+// the registers of AHEAD, 9.4 us without.
+template <typename T, int D, int CH, bool AHEAD>
+__global__ void __launch_bounds__(KV_THREADS, CH == 4 && !AHEAD ? 3 : 2) kv_write_kernel(const KvCache c, const KvBatch b, const T* __restrict__ k,
                                                               const T* __restrict__ v, const KvRows rs, int per_seq,
                                                               int units) {
-  constexpr int N = Dense<T>::N;
+  constexpr int N = 16 / sizeof(T), DPR = D / N;  // values of a piece, pieces of a row
   __shared__ int slot;
   __shared__ uint32_t red[2][KV_THREADS / 32];
   PageRows pr;
   if (!kv_page_rows(c, b, blockIdx.x, per_seq, &slot, pr)) return;
-  const int tid = threadIdx.x, dpr = c.head_dim / N, warps = blockDim.x >> 5;
-  const int u1 = min(2 * c.kv_heads, (int)(blockIdx.y + 1) * units);
-  for (int u = blockIdx.y * units; u < u1; ++u) {
-    const int head = u >> 1;
-    const T* src = u & 1 ? v + head * rs.v_head : k + head * rs.k_head;
+  const int tid = threadIdx.x, warps = blockDim.x >> 5;
+  const int u0 = blockIdx.y * units, u1 = min(2 * c.kv_heads, u0 + units);
+  const bool kept = pr.lo > 0;  // the page holds older tokens of the sequence
+  const auto scale_of = [&](int u) { return (u & 1 ? c.v_scale : c.k_scale) + pr.page * c.scale_stride + (u >> 1); };
+  const auto load = [&](int u, uint4 (&raw)[CH], float& had) {
+    const T* src = u & 1 ? v + (u >> 1) * rs.v_head : k + (u >> 1) * rs.k_head;
     const int64_t stride = u & 1 ? rs.v_token : rs.k_token;
-    uint8_t* dst = (u & 1 ? c.v : c.k) + pr.page * c.page_stride + head * c.head_stride;
-    float* scale = (u & 1 ? c.v_scale : c.k_scale) + pr.page * c.scale_stride + head;
-    float x[CH][N];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int p = tid + i * blockDim.x, t = p / dpr;
-      if (t >= pr.lo && t < pr.hi) {
-        Dense<T>::load(src + (int64_t)(pr.row0 + t - pr.lo) * stride + (p % dpr) * N, x[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[i][j] = 0.f;
-      }
+      const int p = tid + i * blockDim.x, t = p / DPR;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (t >= pr.lo && t < pr.hi) raw[i] = load16(src + (int64_t)(pr.row0 + t - pr.lo) * stride + (p % DPR) * N);
     }
-    const float had = pr.lo > 0 ? *scale : 0.f;  // of the sequence's older tokens in this page
-    // floats that are not negative order as their bits do
+    had = kept ? *scale_of(u) : 0.f;
+  };
+  uint4 raw[CH], next[AHEAD ? CH : 1];
+  float had, next_had = 0.f;
+  load(u0, raw, had);
+  for (int u = u0; u < u1; ++u) {
+    if constexpr (AHEAD)
+      if (u + 1 < u1) load(u + 1, next, next_had);
+    uint8_t* dst = (u & 1 ? c.v : c.k) + pr.page * c.page_stride + (u >> 1) * c.head_stride;
+    // Magnitudes order as their bits do.  A unit whose largest bits are those of a NaN, an
+    // infinite or a too large value is looked through again without them.
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i) top = max(top, top_bits<T>(raw[i]));
+    top = block_max(top, red[u & 1], warps);
+    const bool odd = top > __float_as_uint(KV_LARGEST);
+    if (odd) {
+      top = 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float a = fabsf(x[i][j]);
-        if (a <= 448.0f * 281474976710656.0f) top = max(top, __float_as_uint(a));
-        else x[i][j] = __int_as_float(0x7fffffff);  // NaN, infinite or too large for the scales
+      for (int i = 0; i < CH; ++i) {
+        float x[N];
+        values_of(raw[i], x);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (fabsf(x[j]) <= KV_LARGEST) top = max(top, __float_as_uint(fabsf(x[j])));
       }
-    top = __reduce_max_sync(0xffffffffu, top);
-    uint32_t* r = red[u & 1];
-    if ((tid & 31) == 0) r[tid >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < warps; ++w) top = max(top, r[w]);
-    float now = least_scale(__uint_as_float(top));
-    if (pr.lo > 0) {
-      if (!(had > 0.f && had < INFINITY)) {
-        if (tid == 0) atomicOr(c.status, RTR_DEV_BAD_SCALE);
-        continue;
-      }
-      now = fmaxf(now, had);
+      __syncthreads();  // every warp has read the first maximum
+      top = block_max(top, red[u & 1], warps);
     }
-    if (tid == 0 && now != had) *scale = now;
-    const Divider over(now);
-    const bool grown = pr.lo > 0 && now > had;
+    float now = least_scale(__uint_as_float(top));
+    const bool fits = !kept || (had > 0.f && had < INFINITY);
+    if (!fits) {
+      if (tid == 0) atomicOr(c.status, RTR_DEV_BAD_SCALE);
+    } else {
+      if (kept) now = fmaxf(now, had);
+      if (tid == 0 && now != had) *scale_of(u) = now;
+      // a power of two has an exact reciprocal
+      const float inverse = 1.0f / now;
+      const bool plain = !odd && (__float_as_uint(now) & 0x7fffffu) == 0;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int p = tid + i * blockDim.x, t = p / dpr;
-      Codes<N> q;
-      if (t >= pr.lo && t < pr.hi) {
+      for (int i = 0; i < CH; ++i) {
+        const int p = tid + i * blockDim.x, t = p / DPR;
+        if (t < pr.lo || t >= pr.hi) continue;
+        Codes<N> q;
+        if (plain) {
+          float x[N];
+          values_of(raw[i], x);
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[i][j] = over(x[i][j]);
-        q.set(x[i]);
-        q.store(dst + (int64_t)p * N);
-      } else if (grown && t < pr.lo) {
-        float y[N];
-        q.load(dst + (int64_t)p * N);
-        q.get(y);
-#pragma unroll
-        for (int j = 0; j < N; ++j) y[j] = over(y[j] * had);
-        q.set(y);
+          for (int j = 0; j < N; ++j) x[j] *= inverse;
+          q.set(x);
+        } else {
+          q = encode_odd<N>(raw[i], now);
+        }
         q.store(dst + (int64_t)p * N);
       }
+      if (kept && now > had) {
+        for (int p = tid; p < pr.lo * DPR; p += blockDim.x) {
+          Codes<N> q;
+          q.load(dst + (int64_t)p * N);
+          encode_again<N>(q, had, now).store(dst + (int64_t)p * N);
+        }
+      }
+    }
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) raw[i] = next[i];
+      had = next_had;
+    } else if (u + 1 < u1) {
+      load(u + 1, raw, had);
     }
   }
 }
 
-template <typename T, int CH>
+template <typename T, int D, int CH>
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvCache c, const KvBatch b, T* __restrict__ k,
                                                              T* __restrict__ v, const KvRows rs, int per_seq,
                                                              int units) {
-  constexpr int N = Dense<T>::N;
+  constexpr int N = 16 / sizeof(T), DPR = D / N;
   __shared__ int slot;
   PageRows pr;
   if (!kv_page_rows(c, b, blockIdx.x, per_seq, &slot, pr)) return;
-  const int tid = threadIdx.x, dpr = c.head_dim / N;
-  const int u1 = min(2 * c.kv_heads, (int)(blockIdx.y + 1) * units);
-  for (int u = blockIdx.y * units; u < u1; ++u) {
-    const int head = u >> 1;
-    T* dst = u & 1 ? v + head * rs.v_head : k + head * rs.k_head;
-    const int64_t stride = u & 1 ? rs.v_token : rs.k_token;
-    const uint8_t* src = (u & 1 ? c.v : c.k) + pr.page * c.page_stride + head * c.head_stride;
-    const float scale = ((u & 1 ? c.v_scale : c.k_scale) + pr.page * c.scale_stride)[head];
-    Codes<N> q[CH];
+  const int tid = threadIdx.x;
+  const int u0 = blockIdx.y * units, u1 = min(2 * c.kv_heads, u0 + units);
+  const auto load = [&](int u, Codes<N> (&q)[CH], float& scale) {
+    const uint8_t* src = (u & 1 ? c.v : c.k) + pr.page * c.page_stride + (u >> 1) * c.head_stride;
+    scale = ((u & 1 ? c.v_scale : c.k_scale) + pr.page * c.scale_stride)[u >> 1];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int p = tid + i * blockDim.x, t = p / dpr;
+      const int p = tid + i * blockDim.x, t = p / DPR;
       if (t >= pr.lo && t < pr.hi) q[i].load(src + (int64_t)p * N);
     }
+  };
+  Codes<N> q[CH], next[CH];
+  float scale, next_scale = 0.f;
+  load(u0, q, scale);
+  for (int u = u0; u < u1; ++u) {
+    if (u + 1 < u1) load(u + 1, next, next_scale);
+    T* dst = u & 1 ? v + (u >> 1) * rs.v_head : k + (u >> 1) * rs.k_head;
+    const int64_t stride = u & 1 ? rs.v_token : rs.k_token;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int p = tid + i * blockDim.x, t = p / dpr;
+      const int p = tid + i * blockDim.x, t = p / DPR;
       if (t < pr.lo || t >= pr.hi) continue;
       float x[N];
       q[i].get(x);
 #pragma unroll
       for (int j = 0; j < N; ++j) x[j] *= scale;
-      Dense<T>::store(dst + (int64_t)(pr.row0 + t - pr.lo) * stride + (p % dpr) * N, x);
+      store16(dst + (int64_t)(pr.row0 + t - pr.lo) * stride + (p % DPR) * N, x);
     }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) q[i] = next[i];
+    scale = next_scale;
   }
 }
 
@@ -329,29 +378,35 @@ KvGrid kv_page_grid(int rows, int seqs, bool starts, int page, int kv_heads, int
   return g;
 }
 
-// Threads and 16-byte pieces a thread for a page of page * head_dim values.
-template <typename T, typename F> static cudaError_t by_pieces(int values, F&& launch) {
-  const int pieces = values / Dense<T>::N;
-  if (pieces <= KV_THREADS) return launch(std::integral_constant<int, 1>{}, pieces);
-  switch (pieces / KV_THREADS) {
-    case 2: return launch(std::integral_constant<int, 2>{}, KV_THREADS);
-    case 4: return launch(std::integral_constant<int, 4>{}, KV_THREADS);
-    case 8: return launch(std::integral_constant<int, 8>{}, KV_THREADS);
-    case 16: return launch(std::integral_constant<int, 16>{}, KV_THREADS);
-  }
-  return cudaErrorInvalidValue;
+// Threads and 16-byte pieces a thread for a page of `pieces` (a power of two from 128 to
+// 4096): four pieces a thread spread a unit's fixed work (maximum, scale, addresses)
+// and leave registers for the next unit's.
+template <typename F> static cudaError_t by_pieces(int pieces, F&& launch) {
+  if (pieces <= 4 * KV_THREADS) return launch(std::integral_constant<int, 4>{}, pieces / 4);
+  return launch(std::integral_constant<int, 8>{}, pieces / 8);
 }
 
-template <typename T, bool WRITE>
+template <typename T, int D, bool WRITE>
 static cudaError_t launch_pages(const KvCache& c, const KvBatch& b, T* k, T* v, const KvRows& r, const KvGrid& g,
                                 cudaStream_t stream) {
-  return by_pieces<T>(c.head_dim << c.page_shift, [&](auto ch, int threads) {
+  return by_pieces((D << c.page_shift) * (int)sizeof(T) / 16, [&](auto ch, int threads) {
     constexpr int CH = decltype(ch)::value;
     const dim3 grid((unsigned)g.items, (unsigned)g.splits);
-    if constexpr (WRITE) kv_write_kernel<T, CH><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
-    else kv_read_kernel<T, CH><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
+    if constexpr (!WRITE) kv_read_kernel<T, D, CH><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
+    else if (CH == 4 && g.units > 1)
+      kv_write_kernel<T, D, CH, CH == 4><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
+    else kv_write_kernel<T, D, CH, false><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
     return cudaGetLastError();
   });
+}
+
+template <typename T>
+static cudaError_t launch_pages(bool write, const KvCache& c, const KvBatch& b, void* k, void* v, const KvRows& r,
+                                const KvGrid& g, cudaStream_t st) {
+  T *kt = static_cast<T*>(k), *vt = static_cast<T*>(v);
+  if (c.head_dim == 128)
+    return write ? launch_pages<T, 128, true>(c, b, kt, vt, r, g, st) : launch_pages<T, 128, false>(c, b, kt, vt, r, g, st);
+  return write ? launch_pages<T, 64, true>(c, b, kt, vt, r, g, st) : launch_pages<T, 64, false>(c, b, kt, vt, r, g, st);
 }
 
 static int pages_call(bool write, const rtr_kv_cache* c, const rtr_kv_batch* b, void* k, void* v, int32_t dtype,
@@ -366,15 +421,8 @@ static int pages_call(bool write, const rtr_kv_cache* c, const rtr_kv_batch* b, 
   const KvCache dc = kv_device_cache(c);
   const KvBatch db = kv_device_batch(b);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
-  if (dtype == RTR_DTYPE_F32) {
-    float *kf = static_cast<float*>(k), *vf = static_cast<float*>(v);
-    e = write ? launch_pages<float, true>(dc, db, kf, vf, r, g, st) : launch_pages<float, false>(dc, db, kf, vf, r, g, st);
-  } else {
-    auto *kh = static_cast<__nv_bfloat16*>(k), *vh = static_cast<__nv_bfloat16*>(v);
-    e = write ? launch_pages<__nv_bfloat16, true>(dc, db, kh, vh, r, g, st)
-              : launch_pages<__nv_bfloat16, false>(dc, db, kh, vh, r, g, st);
-  }
+  const cudaError_t e = dtype == RTR_DTYPE_F32 ? launch_pages<float>(write, dc, db, k, v, r, g, st)
+                                               : launch_pages<__nv_bfloat16>(write, dc, db, k, v, r, g, st);
   return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
 }
 
