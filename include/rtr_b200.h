@@ -369,6 +369,24 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
                      int32_t heads, int64_t q_token_stride, int32_t causal, float scale, void* out_dev, float* lse_dev,
                      void* workspace_dev, int64_t workspace_bytes, int32_t device, void* stream);
 
+/* A request's prefix kept beyond the request, for users who come back (no counterpart in
+ * the reference: its prefix arena holds one request, shared_prefix.py:67-100).
+ * rtr_keep_prefix, between rtr_prefill and the first decode step: quantises the prefix of
+ * every layer into pages of a cache with layers x kv_heads heads (head l * kv_heads + g is
+ * layer l's group g), table_dev [table_width] its page numbers, and copies the final hidden
+ * state of the prompt's last token (hidden elements of the session's type) to hidden_dev.
+ * Blocks until done; a page number outside the cache sets the cache's status word.
+ * rtr_prefill_kept takes rtr_prefill's place for that user: step 0 from the hidden state
+ * (the same scores as at first), then rtr_decode_step 1 - 4 and rtr_read_results as ever,
+ * the prefix's K and V now the 8-bit values.  in_place: the decode steps attend over the
+ * pages (they must stay until rtr_read_results; a page number outside the cache fails the
+ * request); otherwise the pages are read back into the arena first, which needs a decode
+ * attention that reads the arena alone (fp32: the default kernel).  ids: host. */
+int rtr_keep_prefix(rtr_session* s, const rtr_kv_cache* cache, const int32_t* table_dev, int32_t table_width,
+                    void* hidden_dev);
+int rtr_prefill_kept(rtr_session* s, const rtr_kv_cache* cache, const int32_t* table_dev, int32_t table_width,
+                     const int32_t* ids, int32_t L, const void* hidden_dev, int32_t in_place);
+
 /* ---- synthetic workload --------------------------------------------------- */
 
 /* Deterministic synthetic tensor values: element i of stream (seed, tid) is

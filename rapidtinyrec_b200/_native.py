@@ -25,7 +25,7 @@ EXPORTS = (
     'rtr_profile_gemms', 'rtr_constraint_process_static', 'rtr_gemm_check',
     'rtr_session_create_batched', 'rtr_launch_batch', 'rtr_wait_batch', 'rtr_generate_batch',
     'rtr_debug_wait_control', 'rtr_attention_check', 'rtr_kv_write', 'rtr_kv_read',
-    'rtr_kv_attention_workspace', 'rtr_kv_attention',
+    'rtr_kv_attention_workspace', 'rtr_kv_attention', 'rtr_keep_prefix', 'rtr_prefill_kept',
 )
 
 
@@ -133,6 +133,8 @@ def load():
         'rtr_kv_read': (P, P, P, P, I32, I64, I64, I64, I64, I32, P),
         'rtr_kv_attention_workspace': (P, P, I32, I32, I32, ctypes.POINTER(I64)),
         'rtr_kv_attention': (P, P, P, I32, I32, I64, I32, F, P, P, P, I64, I32, P),
+        'rtr_keep_prefix': (P, P, P, I32, P),
+        'rtr_prefill_kept': (P, P, P, I32, P, I32, P, I32),
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

@@ -234,6 +234,15 @@ cudaError_t attention_decode_tc_bf16(const BfPrefillMaps& mp, int layer, int lay
                                      const DecodeUsers& du);
 bool attention_folded_supported(int heads, int kv_heads, int head_dim, bool bf16);
 
+// ---- decode attention over a kept prefix (kv_suffix.cu) ----
+// out = the attention over the prefix (prefix [beams][heads][D] and lse [beams][heads], from
+// rtr_kv_attention) joined with the `t` suffix slots of one user's beams (layout and
+// ancestry as for attention_decode).  fp32: out_big / out_small get the GEMM split.
+cudaError_t kv_suffix_join(const void* q, const void* prefix, const float* lse, const void* k_suffix,
+                           const void* v_suffix, const int32_t* anc, int t, void* out, float* out_big,
+                           float* out_small, int beams, int heads, int kv_heads, int head_dim, float scale,
+                           uint32_t* status, bool bf16, int xfmt, cudaStream_t stream);
+
 // ---- constraints + beam step (beam.cu) ----
 struct DevTables {
   int32_t offsets[3], sizes[3];

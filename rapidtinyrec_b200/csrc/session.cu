@@ -115,6 +115,19 @@ struct rtr_session {
   int L = 0;
   int steps_done = -1;
   bool in_flight = false;
+  // kept prefixes (rtr_keep_prefix): whether the arena holds the request's prefix, and the
+  // pages that decode attention reads instead of the arena
+  bool prefix_in_arena = false;
+  struct {
+    bool on = false;
+    rtr_kv_cache cache{};
+    int width = 0, table_room = 0;
+    int32_t* table = nullptr;   // session copy of the table row
+    void* out = nullptr;        // [beams][heads][D]: the prefix's part of the attention
+    float* lse = nullptr;
+    uint8_t* work = nullptr;
+    int64_t work_bytes = 0;
+  } kept;
   // batched decode (rtr_session_create_batched): up to max_users users share each
   // decode step's GEMMs; user u has its own prefix arena, length, beam state and
   // result.  The per-step entry points serve user 0.
@@ -782,12 +795,41 @@ static cudaError_t prefill_attention(rtr_session* s, int l, const float* kp, con
                            c.head_dim, scale, false, s->stream, s->xfmt);
 }
 
+// One layer's heads of a cache that holds every layer's (head l * kv_heads + g).
+static rtr_kv_cache layer_cache(const rtr_session* s, const rtr_kv_cache& all, int l) {
+  rtr_kv_cache c = all;
+  const int64_t first = (int64_t)l * s->cfg.kv_heads;
+  c.k = static_cast<uint8_t*>(all.k) + first * all.head_stride;
+  c.v = static_cast<uint8_t*>(all.v) + first * all.head_stride;
+  c.k_scale += first;
+  c.v_scale += first;
+  c.kv_heads = s->cfg.kv_heads;
+  c.status = s->d_status;  // a page that does not fit fails the request
+  return c;
+}
+
+// Decode attention of layer l over the kept prefix's pages and the beams' suffixes (user 0).
+// bf16 mode: the prefix's part is rounded to bf16 before the two are joined.
+static cudaError_t kept_attention(rtr_session* s, int l, const void* ks, const void* vs, int t, float* ob, float* os,
+                                  float scale) {
+  const auto& c = s->cfg;
+  const rtr_kv_cache cache = layer_cache(s, s->kept.cache, l);
+  const rtr_kv_batch batch = {s->kept.table, s->d_L, nullptr, s->kept.width, s->kept.width, 1, beams_of(s)};
+  if (rtr_kv_attention(&cache, &batch, s->q, s->bf16 ? RTR_DTYPE_BF16 : RTR_DTYPE_F32, c.heads,
+                       (int64_t)c.heads * c.head_dim, 0, scale, s->kept.out, s->kept.lse, s->kept.work,
+                       s->kept.work_bytes, s->device, s->stream) != RTR_OK)
+    return cudaErrorInvalidValue;
+  return kv_suffix_join(s->q, s->kept.out, s->kept.lse, ks, vs, &s->beam->anc[0][0], t, s->attn, ob, os, beams_of(s),
+                        c.heads, c.kv_heads, c.head_dim, scale, s->d_status, s->bf16, s->xfmt, s->stream);
+}
+
 // Decode attention of layer l: the per-head kernel, the tensor-core kernel
 // (RTR_ATTN=tc) or the folded cluster kernel (RTR_ATTN=folded).
 static cudaError_t decode_attention(rtr_session* s, int l, const void* kp, const void* vp, const void* ks,
                                     const void* vs, int t, float* ob, float* os, float scale, const DecodeUsers& du) {
   const auto& c = s->cfg;
   const int D = c.head_dim;
+  if (s->kept.on) return kept_attention(s, l, ks, vs, t, ob, os, scale);
   if (s->tc_attn_bf16)
     return attention_decode_tc_bf16(s->pbmaps, l, c.layers, s->q, ks, vs, &s->beam->anc[0][0], s->d_L, t, s->attn,
                                     beams_of(s), c.max_prefix, c.heads, c.kv_heads, D, scale, s->d_status, s->stream,
@@ -811,6 +853,13 @@ static cudaError_t decode_attention(rtr_session* s, int l, const void* kp, const
   }
   return attention_decode(s->q, kp, vp, ks, vs, &s->beam->anc[0][0], s->d_L, t, s->attn, ob, os, beams_of(s),
                           c.max_prefix, c.heads, c.kv_heads, D, scale, s->d_status, s->bf16, s->stream, du, s->xfmt);
+}
+
+// Step 0's logits from the final hidden state of the prompt's last token (row 0 of h).
+static cudaError_t first_logits(rtr_session* s) {
+  const int H = s->cfg.hidden, V = s->cfg.vocab;
+  if (s->bf16) return gemm16(s, s->h, s->lm_packed_bf, s->logits, V, nullptr, 1, V, H, EPI_STORE);
+  return gemv_f32(s->h, s->lm_head, s->logits, V, H, s->stream);
 }
 
 // The forward of the bf16 mode: the same launches as the fp32 forward with
@@ -865,7 +914,7 @@ static cudaError_t forward_bf16(rtr_session* s, int t) {
   if (t == 0) {  // the last position only
     const uint16_t* last = reinterpret_cast<const uint16_t*>(s->x) + (size_t)(M - 1) * H;
     FWD_TRY(rms_norm_rows_bf16(last, s->norm_final, s->h, 1, H, c.rms_eps, st));
-    FWD_TRY(gemm16(s, s->h, s->lm_packed_bf, s->logits, V, nullptr, 1, V, H, EPI_STORE));
+    FWD_TRY(first_logits(s));
   } else {
     FWD_TRY(rms_norm_rows_bf16(s->x, s->norm_final, s->h, M, H, c.rms_eps, st));
     FWD_TRY(gemm16(s, s->h, s->lm_packed_bf, s->logits, V, nullptr, M, V, H, EPI_STORE, nullptr,
@@ -920,7 +969,7 @@ static cudaError_t forward(rtr_session* s, int t) {
     }
     if (t == 0) {  // the prefill's last row: explicit norm and the unfolded LM head (GEMV)
       FWD_TRY(rms_norm_rows(s->x + (size_t)(M - 1) * H, s->norm_final, s->h, nullptr, nullptr, 1, H, c.rms_eps, st));
-      FWD_TRY(gemv_f32(s->h, s->lm_head, s->logits, V, H, st));
+      FWD_TRY(first_logits(s));
     } else {
       FWD_TRY(gemm(s, s->x, H, s->lm_head, s->logits, V, nullptr, M, V, H, EPI_STORE, nullptr, &in,
                    s->lse_tail ? s->lse : nullptr));
@@ -961,7 +1010,7 @@ static cudaError_t forward(rtr_session* s, int t) {
   }
   if (t == 0) {
     FWD_TRY(rms_norm_rows(s->x + (size_t)(M - 1) * H, s->norm_final, s->h, nullptr, nullptr, 1, H, c.rms_eps, st));
-    FWD_TRY(gemv_f32(s->h, s->lm_head, s->logits, V, H, st));
+    FWD_TRY(first_logits(s));
   } else {
     FWD_TRY(rms_norm_rows(s->x, s->norm_final, s->h, s->h_big, s->h_small, M, H, c.rms_eps, st, s->xfmt));
     FWD_TRY(gemm(s, s->h, H, s->lm_head, s->logits, V, nullptr, M, V, H, EPI_STORE, nullptr, nullptr,
@@ -1014,6 +1063,8 @@ static int stage_prefill(rtr_session* s, const int32_t* ids, int32_t L, int32_t 
   if (int r = check_prompt(s, ids, L)) return r;
   if (int r = ready(s)) return r;
   CUDA_TRY(s, cudaSetDevice(s->device));
+  s->kept.on = false;
+  s->prefix_in_arena = u == 0;
   s->L = L;
   s->Ls[u] = L;
   s->cur_user = u;
@@ -1046,7 +1097,8 @@ static int check_result(rtr_session* s, const rtr_result* out, int u = 0) {
     CUDA_TRY(s, cudaMemsetAsync(s->tickets, 0, kTickets * sizeof(int), s->stream));
     return fail(s, RTR_ERR_DEVICE, "a bounded pipeline wait ran out (status " + status_hex(st) + ")");
   }
-  if (st & (RTR_DEV_BAD_TOKEN | RTR_DEV_BAD_PARENT | RTR_DEV_BAD_LENGTH | RTR_DEV_TOO_MANY_CAND | RTR_DEV_NAN_SCORE))
+  if (st & (RTR_DEV_BAD_TOKEN | RTR_DEV_BAD_PARENT | RTR_DEV_BAD_LENGTH | RTR_DEV_TOO_MANY_CAND | RTR_DEV_NAN_SCORE |
+            RTR_DEV_BAD_PAGE))
     return fail(s, RTR_ERR_DEVICE, "device bound check failed (status " + status_hex(st) + ")");
   if (st & RTR_DEV_NOT_STOPPED)
     return fail(s, RTR_ERR_DEVICE, "beam search would continue after 5 steps (catalog grammar is not 3 SID tokens + newline + EOS)");
@@ -1072,6 +1124,109 @@ int rtr_prefill(rtr_session* s, const int32_t* ids, int32_t L, int32_t ids_on_de
   return stage_prefill(s, ids, L, ids_on_device);
 }
 
+// A cache that can hold the session's prefix in `width` pages.
+static const char* kept_fits(const rtr_session* s, const rtr_kv_cache* cache, const int32_t* table, int32_t width,
+                             int64_t L) {
+  const auto& c = s->cfg;
+  if (!cache || !table) return "null cache or table";
+  if (cache->kv_heads != c.layers * c.kv_heads || cache->head_dim != c.head_dim)
+    return "the cache must hold layers x kv_heads heads of the model's head_dim";
+  if (width < 1 || (int64_t)width * cache->page < L) return "the table's pages do not hold the prefix";
+  return nullptr;
+}
+
+int rtr_keep_prefix(rtr_session* s, const rtr_kv_cache* cache, const int32_t* table_dev, int32_t table_width,
+                    void* hidden_dev) {
+  if (!s) return RTR_ERR_ARG;
+  if (s->in_flight || s->steps_done != 0 || !s->prefix_in_arena || s->cur_user != 0)
+    return fail(s, RTR_ERR_STATE, "a prefix is kept between rtr_prefill and the first decode step");
+  if (const char* e = kept_fits(s, cache, table_dev, table_width, s->L)) return fail(s, RTR_ERR_ARG, e);
+  if (!hidden_dev) return fail(s, RTR_ERR_ARG, "null hidden state");
+  CUDA_TRY(s, cudaSetDevice(s->device));
+  const auto& c = s->cfg;
+  const int64_t D = c.head_dim, cap = c.max_prefix, kvd = (int64_t)c.kv_heads * D, size = s->bf16 ? 2 : 4;
+  const rtr_kv_batch batch = {table_dev, s->d_L, nullptr, table_width, table_width, 1, s->L};
+  for (int l = 0; l < c.layers; ++l) {
+    rtr_kv_cache layer = layer_cache(s, *cache, l);
+    layer.status = cache->status;
+    const char* k = reinterpret_cast<const char*>(s->kv_prefix) + l * 2 * kvd * cap * size;
+    const char* v = k + kvd * cap * size;
+    if (int r = rtr_kv_write(&layer, &batch, k, v, s->bf16 ? RTR_DTYPE_BF16 : RTR_DTYPE_F32, D, cap * D, D, cap * D,
+                             s->device, s->stream))
+      return fail(s, r, rtr_last_error(nullptr));
+  }
+  CUDA_TRY(s, cudaMemcpyAsync(hidden_dev, s->h, c.hidden * size, cudaMemcpyDeviceToDevice, s->stream));
+  s->launches += c.layers;
+  CUDA_TRY(s, cudaStreamSynchronize(s->stream));
+  return RTR_OK;
+}
+
+int rtr_prefill_kept(rtr_session* s, const rtr_kv_cache* cache, const int32_t* table_dev, int32_t table_width,
+                     const int32_t* ids, int32_t L, const void* hidden_dev, int32_t in_place) {
+  if (!s) return RTR_ERR_ARG;
+  if (s->in_flight) return fail(s, RTR_ERR_STATE, "request in flight");
+  if (int r = check_prompt(s, ids, L)) return r;
+  if (int r = ready(s)) return r;
+  if (const char* e = kept_fits(s, cache, table_dev, table_width, L)) return fail(s, RTR_ERR_ARG, e);
+  if (!hidden_dev) return fail(s, RTR_ERR_ARG, "null hidden state");
+  if (!in_place && (s->tc_attn || s->tc_attn_bf16))
+    return fail(s, RTR_ERR_STATE, "the tensor-core decode attention reads copies of the arena: only in place");
+  CUDA_TRY(s, cudaSetDevice(s->device));
+  const auto& c = s->cfg;
+  const int dtype = s->bf16 ? RTR_DTYPE_BF16 : RTR_DTYPE_F32;
+  const int64_t D = c.head_dim, cap = c.max_prefix, kvd = (int64_t)c.kv_heads * D, size = s->bf16 ? 2 : 4;
+  if (in_place) {
+    auto& k = s->kept;
+    const rtr_kv_cache layer = layer_cache(s, *cache, 0);
+    const rtr_kv_batch batch = {table_dev, s->d_L, nullptr, table_width, table_width, 1, beams_of(s)};
+    int64_t bytes = 0;
+    if (int r = rtr_kv_attention_workspace(&layer, &batch, dtype, c.heads, s->device, &bytes))
+      return fail(s, r, rtr_last_error(nullptr));
+    if (!k.out) {
+      float* out = nullptr;
+      CUDA_TRY(s, dev_alloc(s, &out, (size_t)beams_of(s) * c.heads * D));
+      CUDA_TRY(s, dev_alloc(s, &k.lse, (size_t)beams_of(s) * c.heads));
+      k.out = out;
+    }
+    if (table_width > k.table_room) {
+      CUDA_TRY(s, dev_alloc(s, &k.table, (size_t)table_width));
+      k.table_room = table_width;
+    }
+    if (bytes > k.work_bytes) {
+      CUDA_TRY(s, dev_alloc(s, &k.work, (size_t)bytes));
+      k.work_bytes = bytes;
+    }
+    k.cache = *cache;
+    k.width = table_width;
+    CUDA_TRY(s, cudaMemcpyAsync(k.table, table_dev, table_width * sizeof(int32_t), cudaMemcpyDeviceToDevice, s->stream));
+  }
+  s->step_users = 1;
+  s->L = s->Ls[0] = s->h_L[0] = L;
+  s->cur_user = 0;
+  CUDA_TRY(s, cudaMemcpyAsync(s->d_L, s->h_L, sizeof(int32_t), cudaMemcpyHostToDevice, s->stream));
+  CUDA_TRY(s, cudaMemcpyAsync(s->d_ids, ids, (size_t)L * sizeof(int32_t), cudaMemcpyHostToDevice, s->stream));
+  CUDA_TRY(s, cudaMemsetAsync(s->d_status, 0, sizeof(uint32_t), s->stream));
+  CUDA_TRY(s, beam_reset(s->beam, s->d_ids, s->d_L, beams_of(s), s->stream));
+  CUDA_TRY(s, cudaMemcpyAsync(s->h, hidden_dev, c.hidden * size, cudaMemcpyDeviceToDevice, s->stream));
+  if (!in_place) {
+    const rtr_kv_batch batch = {table_dev, s->d_L, nullptr, table_width, table_width, 1, L};
+    for (int l = 0; l < c.layers; ++l) {
+      const rtr_kv_cache layer = layer_cache(s, *cache, l);
+      char* k = reinterpret_cast<char*>(s->kv_prefix) + l * 2 * kvd * cap * size;
+      if (int r = rtr_kv_read(&layer, &batch, k, k + kvd * cap * size, dtype, D, cap * D, D, cap * D, s->device, s->stream))
+        return fail(s, r, rtr_last_error(nullptr));
+    }
+    s->launches += c.layers;
+  }
+  CUDA_TRY(s, first_logits(s));
+  CUDA_TRY(s, beam_step(s->beam, s->logits, 1, c.vocab, beams_of(s), 0, s->tb, s->d_status, s->stream));
+  s->launches += 2 + kTailKernels;  // beam_reset, the LM head, step tail
+  s->steps_done = 0;
+  s->kept.on = in_place != 0;
+  s->prefix_in_arena = false;  // a kept prefix is not kept again: its codes are in the cache already
+  return RTR_OK;
+}
+
 int rtr_decode_step(rtr_session* s, int32_t t) {
   if (!s) return RTR_ERR_ARG;
   if (t < 1 || t >= NSTEPS) return fail(s, RTR_ERR_ARG, "decode step must be in 1..4");
@@ -1079,6 +1234,7 @@ int rtr_decode_step(rtr_session* s, int32_t t) {
   CUDA_TRY(s, cudaSetDevice(s->device));
   CUDA_TRY(s, decode_and_tail(s, t));
   s->launches += forward_kernels(s, false) + decode_tail_kernels(s);
+  if (s->kept.on) s->launches += (int64_t)s->cfg.layers * (s->kept.work_bytes ? 2 : 1);  // the join(s) beside the attention
   s->steps_done = t;
   return RTR_OK;
 }
@@ -1104,6 +1260,7 @@ static int launch_batch(rtr_session* s, const int32_t* const* ids, const int32_t
   if (int r = ready(s)) return r;
   CUDA_TRY(s, cudaSetDevice(s->device));
   s->step_users = n;
+  s->kept.on = false;  // the graph's attention reads the arena
   if (!s->graphs[n]) {
     cudaGraph_t g = nullptr;
     CUDA_TRY(s, cudaStreamBeginCapture(s->stream, cudaStreamCaptureModeThreadLocal));

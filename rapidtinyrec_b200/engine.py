@@ -10,11 +10,13 @@ the reference's per-user record (``benchmark_inference.py:150-154``).
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import numpy as np
 
 from . import _native
 from .configs import NUM_BEAMS, NUM_STEPS, ModelConfig
+from .kv_cache import KvCache8
 
 
 def rope_table(head_dim: int, theta: float, n_positions: int, dtype=None):
@@ -57,6 +59,14 @@ def weight_order(cfg: ModelConfig):
     if not cfg.tied:
         names.append('lm_head.weight')
     return names
+
+
+class KeptPrefix(NamedTuple):
+    """One user's prefix in a store (``BeamEngine.keep_prefix``)."""
+    store: KvCache8
+    table: object      # int32 [pages] on the engine's device
+    ids: np.ndarray
+    hidden: object     # final hidden state of the last prompt token
 
 
 class BeamEngine:
@@ -207,6 +217,53 @@ class BeamEngine:
     def read_results(self):
         self._check(self.lib.rtr_read_results(self.handle, ctypes.byref(self._result)))
         return self._record()
+
+    # ------------------------------------------------------- kept prefixes
+    def prefix_store(self, pages, page=64):
+        """An 8-bit store for the prefixes of users who may come back: ``pages`` pages of ``page``
+        tokens, every layer's K and V (a quarter of the fp32 arena's bytes per token)."""
+        return KvCache8.allocate(pages, self.cfg.layers * self.cfg.kv_heads, page, self.cfg.head_dim,
+                                 f'cuda:{self.device}')
+
+    def keep_prefix(self, prompt_ids, store, pages):
+        """After ``prefill(prompt_ids)`` and before the first decode step: quantise the prefix into
+        the store's ``pages`` (page numbers, as many as the prompt needs)."""
+        import torch
+        dev = f'cuda:{self.device}'
+        ids = self._ids(prompt_ids)
+        pages = [int(p) for p in pages]
+        if len(set(pages)) < len(pages) or any(not 0 <= p < store.pages for p in pages):
+            raise ValueError('pages must be different page numbers of the store')
+        if store.device.index != self.device:
+            raise ValueError('the store must lie on the engine\'s device')
+        table = torch.tensor(pages, dtype=torch.int32, device=dev)
+        dtype = torch.float32 if self.cfg.dtype == 'fp32' else torch.bfloat16
+        hidden = torch.empty(self.cfg.hidden, dtype=dtype, device=dev)
+        torch.cuda.synchronize(self.device)
+        self._check(self.lib.rtr_keep_prefix(self.handle, store._ref, table.data_ptr(), table.numel(),
+                                             hidden.data_ptr()))
+        store.check()
+        return KeptPrefix(store, table, ids, hidden)
+
+    def generate_and_keep(self, prompt_ids, store, pages):
+        """``generate`` that also keeps the prefix: the record and the ``KeptPrefix``."""
+        self.prefill(prompt_ids)
+        kept = self.keep_prefix(prompt_ids, store, pages)
+        for t in range(1, NUM_STEPS):
+            self.decode_step(t)
+        return self.read_results(), kept
+
+    def generate_kept(self, kept, in_place=True):
+        """A request of a user whose prefix was kept: no prefill.  ``in_place``: decode attention
+        over the 8-bit pages; otherwise the pages are first read back into the arena."""
+        import torch
+        torch.cuda.synchronize(self.device)
+        self._check(self.lib.rtr_prefill_kept(self.handle, kept.store._ref, kept.table.data_ptr(), kept.table.numel(),
+                                              kept.ids.ctypes.data, len(kept.ids), kept.hidden.data_ptr(),
+                                              int(bool(in_place))))
+        for t in range(1, NUM_STEPS):
+            self.decode_step(t)
+        return self.read_results()
 
     def step_scores(self, t):
         """``GenerateBeamOutput.scores[t]``: dense ``[beams, V]`` float32 CUDA tensor."""

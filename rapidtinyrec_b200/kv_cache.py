@@ -30,6 +30,7 @@ HEAD_DIMS = (64, 128)
 _BATCH = struct.Struct('PPPqiii4x')  # rtr_kv_batch; packed bytes cost a third of a ctypes structure
 _DTYPES = {torch.float32: _native.RTR_DTYPE_F32, torch.bfloat16: _native.RTR_DTYPE_BF16}
 _STATUS = {1 << 5: 'a length or row range that does not fit the call or the table',
+           1 << 8: 'a bounded wait of a kernel that ran out',
            1 << 9: 'a page number outside the cache',
            1 << 10: 'a scale that is not positive and finite'}
 
@@ -177,8 +178,8 @@ class KvCache8:
             if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
                 raise ValueError(f'out must be two tensors {list(shape)} of one type')
             for x, name in ((k, 'k'), (v, 'v')):
-                if self._dense(x, self.kv_heads, name) is not x:
-                    raise ValueError('out must have contiguous dimensions and rows at multiples of 16 bytes')
+                if self._dense(x, self.kv_heads, name) is not x or any(n > 1 and not d for n, d in zip(shape, x.stride())):
+                    raise ValueError('out must have contiguous dimensions and rows of their own at multiples of 16 bytes')
         batch = self._batch(rows, table, lens, starts)
         code = self.lib.rtr_kv_read(self._ref, batch, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
                                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, _stream(self._index))

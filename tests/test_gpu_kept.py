@@ -1,0 +1,160 @@
+"""Kept prefixes: a user's prefilled K and V quantised into a store of 8-bit pages, later
+requests without a prefill (``BeamEngine.keep_prefix`` / ``generate_kept``).
+
+Two independent paths read a kept prefix - decode attention over the pages, and the pages
+read back into the arena for the ordinary decode attention - so they check each other; a
+model whose K and V are exact in 8 bits (constant V, zero K) has to give the unkept
+request's record.  fp32 scores of two kernels agree within the parity tests' 1e-4."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+SCORE_TOL = 1e-4
+
+
+@pytest.fixture(scope='module', autouse=True)
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.fail('CUDA device required for -m gpu tests')
+
+
+def make_engine(tiny, weights=None, dtype='fp32', **kw):
+    from rapidtinyrec_b200.constraints import GpuSidConstraintTables
+    from rapidtinyrec_b200.engine import BeamEngine
+    c = tiny['cfg'].with_dtype(dtype)
+    tables = GpuSidConstraintTables(tiny['constraints'], c.root, c.newline, c.eos)
+    return BeamEngine(c, tiny['weights'] if weights is None else weights, tables, max_prefix=128, **kw)
+
+
+@pytest.fixture(scope='module')
+def engine(tiny):
+    e = make_engine(tiny)
+    yield e
+    e.close()
+
+
+def prompts(tiny, n=3):
+    return [u.prompt_token_ids for u in tiny['users'][:n]]
+
+
+def same(a, b, tol=SCORE_TOL):
+    assert a['token_ids'] == b['token_ids'] and a['beam_indices'] == b['beam_indices']
+    for key in ('sequence_logp', 'transition_logp'):
+        assert np.abs(np.array(a[key]) - np.array(b[key])).max() <= tol, key
+
+
+def pages_for(ids, page):
+    return -(-len(ids) // page)
+
+
+@pytest.mark.parametrize('page', [16, 64])
+def test_both_ways_of_reading_a_kept_prefix_agree(tiny, engine, page):
+    store = engine.prefix_store(64, page)
+    free = list(range(63, -1, -1))
+    kept, first, scores = [], [], []
+    for ids in prompts(tiny):
+        plain = engine.generate(ids)
+        record, k = engine.generate_and_keep(ids, store, [free.pop() for _ in range(pages_for(ids, page))])
+        assert record == plain  # keeping changes nothing
+        kept.append(k)
+        engine.prefill(ids)
+        first.append(engine.step_scores(0))
+    for ids, k, want in zip(prompts(tiny), kept, first):
+        over_pages = engine.generate_kept(k)
+        assert torch.equal(engine.step_scores(0), want)  # step 0 comes from the same hidden state
+        back = engine.generate_kept(k, in_place=False)
+        assert torch.equal(engine.step_scores(0), want)
+        same(over_pages, back)
+        scores.append(over_pages)
+    for k, want in zip(reversed(kept), reversed(scores)):  # in any order, again and again
+        assert engine.generate_kept(k) == want
+    ids = prompts(tiny)[0]
+    assert engine.generate(ids) == engine.generate(ids)
+    engine.generate_kept(kept[1])
+    plain = engine.generate(ids)  # the captured graph reads the arena as before
+    same(plain, engine.generate_and_keep(ids, store, [free.pop() for _ in range(pages_for(ids, page))])[0], 0)
+
+
+@pytest.mark.parametrize('heads', [4, 12])
+def test_a_prefix_that_is_exact_in_8_bits_gives_the_same_record(tiny, heads):
+    """K = 0 and V = a bias of e4m3 values per layer and head: nothing is rounded, so a page, layer
+    or head taken for another shows."""
+    import dataclasses
+    from rapidtinyrec_b200 import workload
+    cfg = dataclasses.replace(tiny['cfg'], heads=heads)
+    weights = dict(workload.synth_weights(cfg, seed=3, backend='numpy'))
+    g = torch.Generator().manual_seed(5)
+    for name in list(weights):
+        if '.k_proj.' in name or name.endswith('v_proj.weight'):
+            weights[name] = torch.zeros_like(weights[name])
+        if name.endswith('v_proj.bias'):
+            weights[name] = torch.randint(-7, 8, weights[name].shape, generator=g).float() / 8
+    e = make_engine({**tiny, 'cfg': cfg}, weights)
+    store = e.prefix_store(20, 16)
+    for n, ids in enumerate(prompts(tiny, 2)):
+        count = pages_for(ids, 16)
+        record, kept = e.generate_and_keep(ids, store, range(n * 10, n * 10 + count))
+        same(e.generate_kept(kept), record)
+        same(e.generate_kept(kept, in_place=False), record)
+    e.close()
+
+
+def test_bf16_prefixes(tiny, monkeypatch):
+    """bf16 sessions: their default decode attention reads copies of the arena, so only in place;
+    with the per-head kernel both ways, within the differences of the framework's own bf16
+    attention kernels (every operation rounds to bf16: up to 0.017 on this model; bound 0.1)."""
+    from rapidtinyrec_b200._native import NativeError
+    ids = prompts(tiny)[0]
+    count = pages_for(ids, 64)
+    e = make_engine(tiny, dtype='bf16')
+    store = e.prefix_store(8)
+    record, kept = e.generate_and_keep(ids, store, range(count))
+    a = e.generate_kept(kept)
+    if e.report()['decode_attention'] == 1:
+        with pytest.raises(NativeError, match='in place'):
+            e.generate_kept(kept, in_place=False)
+    assert e.generate_kept(kept) == a
+    assert np.abs(np.array(a['sequence_logp']) - np.array(record['sequence_logp'])).max() < 1  # the right prefix
+    e.close()
+    monkeypatch.setenv('RTR_ATTN', 'rows')
+    e = make_engine(tiny, dtype='bf16')
+    store = e.prefix_store(8)
+    _, kept = e.generate_and_keep(ids, store, range(count))
+    a, b = e.generate_kept(kept), e.generate_kept(kept, in_place=False)
+    assert np.abs(np.array(a['sequence_logp']) - np.array(b['sequence_logp'])).max() <= 0.1
+    e.close()
+
+
+def test_calls_out_of_order_and_what_does_not_fit(tiny, engine):
+    from rapidtinyrec_b200._native import RTR_ERR_ARG, RTR_ERR_DEVICE, RTR_ERR_STATE, NativeError
+    from rapidtinyrec_b200.kv_cache import KvCache8
+    ids = prompts(tiny)[0]
+    count = pages_for(ids, 64)
+    store = engine.prefix_store(8)
+    plain = engine.generate(ids)
+
+    def refused(code, call):
+        with pytest.raises(NativeError) as e:
+            call()
+        assert e.value.code == code, e.value
+
+    refused(RTR_ERR_STATE, lambda: engine.keep_prefix(ids, store, range(count)))  # after a whole request
+    engine.prefill(ids)
+    refused(RTR_ERR_ARG, lambda: engine.keep_prefix(ids, store, range(count - 1)))
+    refused(RTR_ERR_ARG, lambda: engine.keep_prefix(ids, KvCache8.allocate(8, 2, 64, 64), range(count)))
+    for bad in ([0, 0], [0, 8], [-1, 0]):
+        with pytest.raises(ValueError):
+            engine.keep_prefix(ids, store, bad)
+    kept = engine.keep_prefix(ids, store, range(count))
+    engine.decode_step(1)
+    refused(RTR_ERR_STATE, lambda: engine.keep_prefix(ids, store, range(count)))
+    refused(RTR_ERR_ARG, lambda: engine.generate_kept(kept._replace(table=kept.table[:count - 1])))
+    refused(RTR_ERR_ARG, lambda: engine.generate_kept(kept._replace(ids=kept.ids[:2])))
+    refused(RTR_ERR_DEVICE, lambda: engine.generate_kept(kept._replace(table=kept.table + 8)))
+    record = engine.generate_kept(kept)
+    refused(RTR_ERR_STATE, lambda: engine.keep_prefix(ids, store, range(count)))
+    assert engine.generate_kept(kept) == record
+    assert engine.generate(ids) == plain
+    store.check()
