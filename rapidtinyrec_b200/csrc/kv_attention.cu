@@ -587,6 +587,11 @@ static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   return p;
 }
 
+// What a block of 128 rows needs for 128 keys.
+static int kv_tile_ns(const rtr_kv_cache* c, bool f32) {
+  return c->head_dim == 128 ? (f32 ? 1700 : 1400) : f32 ? 1350 : 1150;
+}
+
 // Tiles of 128 rows.
 static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, int group, bool f32, int sms, int64_t& ns) {
   KvAttnPlan p = {};
@@ -598,7 +603,7 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
   // cluster's join three, a join through memory eight.  Clusters of three and more fill
   // about six of seven SMs.
   int64_t best = INT64_MAX;
-  for (int64_t s = (all * KT_KEYS + KT_MAX_CHUNK - 1) / KT_MAX_CHUNK, end = s + 63; s <= end; ++s) {
+  for (int64_t s = (all * KT_KEYS + KT_MAX_CHUNK - 1) / KT_MAX_CHUNK, end = s + 63; s <= end && s <= all; ++s) {
     const int64_t per = (all + s - 1) / s, splits = (all + per - 1) / per;
     const int64_t wave = splits >= 3 && splits <= 8 ? sms * 6 / 7 : sms;
     const int64_t cost = (base * splits + wave - 1) / wave * (per + 6) + (splits == 1 ? 0 : splits <= 8 ? 3 : 8);
@@ -609,7 +614,7 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
     }
   }
   p.cluster = p.splits > 1 && p.splits <= 8;
-  ns = best * (c->head_dim == 128 ? (f32 ? 1700 : 1400) : f32 ? 1350 : 1150);
+  ns = best * kv_tile_ns(c, f32);
   return p;
 }
 
@@ -619,9 +624,11 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
 static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, bool f32, int sms) {
   const int group = heads / c->kv_heads;
   int64_t rows_ns, tiles_ns;
-  const KvAttnPlan rows = kv_plan_rows(c, b, group, f32, sms, rows_ns);
-  const KvAttnPlan tiles = kv_plan_tiles(c, b, group, f32, sms, tiles_ns);
-  KvAttnPlan p = tiles_ns < rows_ns ? tiles : rows;
+  KvAttnPlan p = kv_plan_rows(c, b, group, f32, sms, rows_ns);
+  if (rows_ns > 7 * kv_tile_ns(c, f32)) {  // what one key tile costs at least
+    const KvAttnPlan tiles = kv_plan_tiles(c, b, group, f32, sms, tiles_ns);
+    if (tiles_ns < rows_ns) p = tiles;
+  }
   p.workspace = p.splits > 1 && !p.cluster ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
   return p;
 }

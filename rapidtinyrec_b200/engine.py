@@ -240,7 +240,7 @@ class BeamEngine:
         dtype = torch.float32 if self.cfg.dtype == 'fp32' else torch.bfloat16
         hidden = torch.empty(self.cfg.hidden, dtype=dtype, device=dev)
         torch.cuda.synchronize(self.device)
-        self._check(self.lib.rtr_keep_prefix(self.handle, store._ref, table.data_ptr(), table.numel(),
+        self._check(self.lib.rtr_keep_prefix(self.handle, store._at, table.data_ptr(), table.numel(),
                                              hidden.data_ptr()))
         store.check()
         return KeptPrefix(store, table, ids, hidden)
@@ -258,7 +258,7 @@ class BeamEngine:
         over the 8-bit pages; otherwise the pages are first read back into the arena."""
         import torch
         torch.cuda.synchronize(self.device)
-        self._check(self.lib.rtr_prefill_kept(self.handle, kept.store._ref, kept.table.data_ptr(), kept.table.numel(),
+        self._check(self.lib.rtr_prefill_kept(self.handle, kept.store._at, kept.table.data_ptr(), kept.table.numel(),
                                               kept.ids.ctypes.data, len(kept.ids), kept.hidden.data_ptr(),
                                               int(bool(in_place))))
         for t in range(1, NUM_STEPS):

@@ -19,7 +19,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-import struct
 
 import torch
 
@@ -27,7 +26,6 @@ from . import _native
 
 PAGES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
-_BATCH = struct.Struct('PPPqiii4x')  # rtr_kv_batch; packed bytes cost a third of a ctypes structure
 _DTYPES = {torch.float32: _native.RTR_DTYPE_F32, torch.bfloat16: _native.RTR_DTYPE_BF16}
 _STATUS = {1 << 5: 'a length or row range that does not fit the call or the table',
            1 << 8: 'a bounded wait of a kernel that ran out',
@@ -35,9 +33,23 @@ _STATUS = {1 << 5: 'a length or row range that does not fit the call or the tabl
            1 << 10: 'a scale that is not positive and finite'}
 
 
-def _stream(index):
-    """The device's current stream (torch.cuda.current_stream without making a Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(index)
+_call = None
+
+
+def _load():
+    """The calls' C++ module (kv_call.cpp), bound to the library's entry points."""
+    global _call
+    if _call is None:
+        lib = _native.load()
+        try:
+            from . import _kv_call
+        except ImportError as e:
+            raise ImportError('_kv_call.so is not built; run `python -m rapidtinyrec_b200.build`') from e
+        entries = (lib.rtr_kv_write, lib.rtr_kv_read, lib.rtr_kv_attention, lib.rtr_kv_attention_workspace,
+                   lib.rtr_last_error)
+        _kv_call.setup(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), _native.NativeError)
+        _call = _kv_call
+    return _call
 
 
 class KvCache8:
@@ -65,7 +77,7 @@ class KvCache8:
             raise ValueError('the cache must lie on one CUDA device')
         if status is None:
             status = torch.zeros(1, dtype=torch.int32, device=k.device)
-        self.lib = _native.load()
+        self._call = _load()
         self.k, self.v, self.k_scale, self.v_scale, self.status = k, v, k_scale, v_scale, status
         self.pages, self.kv_heads, self.page, self.head_dim = pages, heads, page, dim
         self.device = k.device
@@ -76,10 +88,8 @@ class KvCache8:
                                    k.stride(0) if pages > 1 else heads * head_stride, head_stride,
                                    k_scale.stride(0) if pages > 1 else heads, pages, heads, page, dim,
                                    status.data_ptr())
-        self._ref = ctypes.byref(self._c)
+        self._at = ctypes.addressof(self._c)
         self._scale = 1.0 / math.sqrt(dim)
-        self._attend = self.lib.rtr_kv_attention
-        self._room = {}  # workspace bytes of the call shapes seen
 
     @classmethod
     def allocate(cls, pages, kv_heads, page, head_dim, device='cuda'):
@@ -104,44 +114,6 @@ class KvCache8:
             self.status.zero_()
             raise _native.NativeError(_native.RTR_ERR_DEVICE, '; '.join(t for b, t in _STATUS.items() if bits & b))
 
-    # ------------------------------------------------------------- plumbing
-    def _batch(self, rows, table, lens, starts):
-        """The call's ``rtr_kv_batch`` (packed)."""
-        shape = table.shape
-        if table.dtype is not torch.int32 or lens.dtype is not torch.int32 or len(shape) != 2 or lens.shape != shape[:1]:
-            raise ValueError('table must be int32 [seqs, width] and lens int32 [seqs]')
-        seqs, width = shape
-        step = table.stride()
-        if (width > 1 and step[1] != 1) or (seqs > 1 and lens.stride(0) != 1):
-            raise ValueError('the rows of table and lens must be contiguous')
-        index = self._index
-        if table.get_device() != index or lens.get_device() != index:
-            raise ValueError('table and lens must lie on the cache\'s device')
-        if starts is None:
-            if rows % seqs if seqs else rows:
-                raise ValueError('without starts the rows must be a multiple of the sequences')
-            begin = 0
-        else:
-            if starts.dtype is not torch.int32 or starts.shape != (seqs + 1,) or not starts.is_contiguous():
-                raise ValueError('starts must be int32 [seqs + 1], contiguous')
-            if starts.get_device() != index:
-                raise ValueError('starts must lie on the cache\'s device')
-            begin = starts.data_ptr()
-        return _BATCH.pack(table.data_ptr(), lens.data_ptr(), begin, step[0] if seqs > 1 else width, width, seqs, rows)
-
-    def _dense(self, x, heads, name):
-        """Rows as the kernels take them: one type, dimensions contiguous, 16-byte steps."""
-        shape = x.shape
-        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or x.get_device() != self._index:
-            raise ValueError(f'{name} must be [rows, {heads}, {self.head_dim}] on the cache\'s device')
-        if x.dtype not in _DTYPES:
-            raise ValueError(f'{name} must be float32 or bfloat16')
-        a, b, c = x.stride()
-        step = 4 if x.dtype is torch.float32 else 8
-        if c != 1 or a % step or b % step or x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)
-        return x
-
     # ------------------------------------------------------------ operators
     def write(self, k, v, table, lens, starts=None):
         """Quantise rows ``k``, ``v`` ``[rows, kv_heads, head_dim]`` (float32 or bfloat16, any row and
@@ -153,39 +125,17 @@ class KvCache8:
         448 * 2^48 are stored as NaN.  Codes behind a sequence's last token stay as they are.
         No two sequences of a call may write into the same page.
         """
-        if k.dtype != v.dtype or k.shape != v.shape:
-            raise ValueError('k and v must have one type and shape')
-        k, v = self._dense(k, self.kv_heads, 'k'), self._dense(v, self.kv_heads, 'v')
-        batch = self._batch(k.shape[0], table, lens, starts)
-        code = self.lib.rtr_kv_write(self._ref, batch, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
-                                     k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, _stream(self._index))
-        if code:
-            _native.check(code)
+        self._call.write(self._at, self._index, k, v, table, lens, starts)
 
     def read(self, rows, table, lens, starts=None, dtype=torch.float32, out=None):
         """The last tokens of each sequence as ``(k, v)``, ``[rows, kv_heads, head_dim]`` each: the
         values that the codes stand for, rounded once to ``dtype``.  ``out``: a pair of tensors to
         fill; rows that belong to no sequence keep what they held (new tensors: undefined there).
         """
-        shape = (rows, self.kv_heads, self.head_dim)
-        if out is None:
-            if dtype not in _DTYPES:
-                raise ValueError('dtype must be float32 or bfloat16')
-            k = self.k_scale.new_empty(shape, dtype=dtype)
-            v = torch.empty_like(k)
-        else:
-            k, v = out
-            if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
-                raise ValueError(f'out must be two tensors {list(shape)} of one type')
-            for x, name in ((k, 'k'), (v, 'v')):
-                if self._dense(x, self.kv_heads, name) is not x or any(n > 1 and not d for n, d in zip(shape, x.stride())):
-                    raise ValueError('out must have contiguous dimensions and rows of their own at multiples of 16 bytes')
-        batch = self._batch(rows, table, lens, starts)
-        code = self.lib.rtr_kv_read(self._ref, batch, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
-                                    k.stride(0), k.stride(1), v.stride(0), v.stride(1), self._index, _stream(self._index))
-        if code:
-            _native.check(code)
-        return k, v
+        if dtype not in _DTYPES:
+            raise ValueError('dtype must be float32 or bfloat16')
+        return self._call.read(self._at, self._index, rows, table, lens, starts, _DTYPES[dtype],
+                               out if out is None else tuple(out))
 
     def attention(self, q, table, lens, starts=None, causal=True, scale=None, return_lse=False, out=None):
         """``softmax(scale q K^T) V`` of the rows ``q`` ``[rows, heads, head_dim]`` (float32 or bfloat16)
@@ -198,33 +148,5 @@ class KvCache8:
         results over several stretches of keys are merged.  Rows that belong to no sequence are not
         written: a given ``out`` keeps them, new tensors are undefined there.
         """
-        rows, heads = q.shape[:2]
-        if q.dim() != 3 or heads < 1 or heads % self.kv_heads:
-            raise ValueError(f'q must be [rows, heads, {self.head_dim}], heads a multiple of {self.kv_heads}')
-        q = self._dense(q, heads, 'q')
-        if heads > 1 and q.stride(1) != self.head_dim:
-            q = q.clone(memory_format=torch.contiguous_format)
-        batch = self._batch(rows, table, lens, starts)
-        key = (rows, heads, table.shape, starts is None, q.dtype)
-        room = self._room.get(key)
-        if room is None:
-            need = ctypes.c_int64()
-            _native.check(self.lib.rtr_kv_attention_workspace(self._ref, batch, _DTYPES[q.dtype], heads, self._index,
-                                                                   ctypes.byref(need)))
-            if len(self._room) >= 4096:
-                self._room.clear()
-            room = self._room[key] = need.value
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != self._index \
-                or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError('out must be contiguous and like q')
-        lse = q.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
-        work = q.new_empty((room,), dtype=torch.uint8) if room else None
-        code = self._attend(self._ref, batch, q.data_ptr(), _DTYPES[q.dtype], heads, q.stride(0), causal,
-                            self._scale if scale is None else scale, out.data_ptr(),
-                            lse.data_ptr() if return_lse else None, work.data_ptr() if room else None, room,
-                            self._index, _stream(self._index))
-        if code:
-            _native.check(code)
-        return (out, lse) if return_lse else out
+        return self._call.attention(self._at, self._index, q, table, lens, starts, causal,
+                                    self._scale if scale is None else scale, return_lse, out)

@@ -75,6 +75,22 @@ def test_rows_that_are_refused():
     assert lib.rtr_kv_write(None, None, A, A, 0, 512, 128, 512, 128, 0, None) == _native.RTR_ERR_ARG
 
 
+def test_the_call_module_loads_and_refuses():
+    from rapidtinyrec_b200 import kv_cache
+    call = kv_cache._load()
+    c = cache()
+    t = torch.zeros(2, 2, 128)
+    for bad in ((t, t, t, t, None), (None, t, t, t, None), (t, t.double(), t, t, None), (t, t[:1], t, t, None)):
+        with pytest.raises(ValueError):
+            call.write(ctypes.addressof(c), 0, *bad)  # tensors on the CPU, of wrong types or shapes
+    with pytest.raises(ValueError, match='arguments'):
+        call.attention(ctypes.addressof(c), 0, t)
+    with pytest.raises(ValueError, match='pair'):
+        call.read(ctypes.addressof(c), 0, 2, t, t, None, 0, t)
+    with pytest.raises(TypeError):
+        call.write('cache', 0, t, t, t, t, None)
+
+
 def test_nothing_to_do_is_done_without_a_device():
     for b in (batch(rows=0), batch(rows=0, seqs=0, table=None, lens=None)):
         assert write(cache(), b) == _native.RTR_OK
