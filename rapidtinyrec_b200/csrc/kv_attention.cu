@@ -85,6 +85,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   __shared__ float2 sum_ml[KA_ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y, split = blockIdx.z;
+  pdl_launch_dependents();
+  pdl_wait();
 
   int seq;
   int64_t item0;
@@ -378,7 +380,6 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   }
   cp_async_wait<0>();
   __syncthreads();
-  pdl_launch_dependents();
   float* ob = reinterpret_cast<float*>(ka_smem);
 #pragma unroll
   for (int j = 0; j < DG / 2; ++j) {
@@ -482,6 +483,7 @@ __global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch 
   __shared__ float weight[KJ_MAX];
   __shared__ float red[2][KJ_THREADS / 32];
   __shared__ float4 sums[LANES][COLS];
+  pdl_launch_dependents();
   pdl_wait();
   const int64_t rh = blockIdx.x;
   const int token = (int)(rh / heads), tid = threadIdx.x, col = tid % COLS, sub = tid / COLS;
@@ -648,18 +650,8 @@ template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, 
     static std::atomic<uint64_t> done;
     e = kv_allow_smem(kv_attn_rows_kernel<T, D>, KaCfg<D>::SMEM, done, device);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.items, a.c.kv_heads, a.splits);
-    cfg.blockDim = dim3(KA_WARPS * 32);
-    cfg.dynamicSmemBytes = KaCfg<D>::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = a.splits;
-    cfg.attrs = attr;
-    cfg.numAttrs = a.cluster ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kv_attn_rows_kernel<T, D>, a);
+    e = kv_launch(kv_attn_rows_kernel<T, D>, dim3((unsigned)p.items, a.c.kv_heads, a.splits), KA_WARPS * 32,
+                  KaCfg<D>::SMEM, a.cluster ? a.splits : 1, st, a);
   }
   if (e != cudaSuccess || a.splits == 1 || a.cluster) return e;
   const auto join = [&](auto kernel, int threads) {

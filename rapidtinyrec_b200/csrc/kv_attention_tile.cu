@@ -141,6 +141,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   volatile int* abort_flag = &bars.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.y, split = blockIdx.z;
+  pdl_launch_dependents();
+  pdl_wait();
 
   int seq;
   int64_t item0;
@@ -692,7 +694,6 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  pdl_launch_dependents();
   // D / 4 threads a row; every warp takes rows in turn
   const float* stage = reinterpret_cast<const float*>(smem + C::K_OFF);
   const float2* ml = reinterpret_cast<const float2*>(red);
@@ -753,18 +754,8 @@ template <typename T, int D> static cudaError_t launch_tile(const KvAttn& a, int
   const cudaError_t e = kv_allow_smem(kv_attn_tile_kernel<T, D>, smem, done, device);
   if (e != cudaSuccess) return e;
   constexpr int threads = KtCfg<D, std::is_same<T, float>::value>::THREADS;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)items, a.c.kv_heads, a.splits);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = a.splits;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.cluster ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kv_attn_tile_kernel<T, D>, a);
+  return kv_launch(kv_attn_tile_kernel<T, D>, dim3((unsigned)items, a.c.kv_heads, a.splits), threads, smem,
+                   a.cluster ? a.splits : 1, st, a);
 }
 
 cudaError_t kv_attn_tile(const KvAttn& a, int64_t items, bool f32, int device, cudaStream_t st) {

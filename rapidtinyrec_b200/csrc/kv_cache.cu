@@ -177,6 +177,8 @@ __global__ void __launch_bounds__(KV_THREADS, CH == 4 && !AHEAD ? 3 : 2) kv_writ
   __shared__ int slot;
   __shared__ uint32_t red[2][KV_THREADS / 32];
   PageRows pr;
+  pdl_launch_dependents();
+  pdl_wait();
   if (!kv_page_rows(c, b, blockIdx.x, per_seq, &slot, pr)) return;
   const int tid = threadIdx.x, warps = blockDim.x >> 5;
   const int u0 = blockIdx.y * units, u1 = min(2 * c.kv_heads, u0 + units);
@@ -271,6 +273,8 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvCache c, co
   constexpr int N = 16 / sizeof(T), DPR = D / N;
   __shared__ int slot;
   PageRows pr;
+  pdl_launch_dependents();
+  pdl_wait();
   if (!kv_page_rows(c, b, blockIdx.x, per_seq, &slot, pr)) return;
   const int tid = threadIdx.x;
   const int u0 = blockIdx.y * units, u1 = min(2 * c.kv_heads, u0 + units);
@@ -392,11 +396,10 @@ static cudaError_t launch_pages(const KvCache& c, const KvBatch& b, T* k, T* v, 
   return by_pieces((D << c.page_shift) * (int)sizeof(T) / 16, [&](auto ch, int threads) {
     constexpr int CH = decltype(ch)::value;
     const dim3 grid((unsigned)g.items, (unsigned)g.splits);
-    if constexpr (!WRITE) kv_read_kernel<T, D, CH><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
-    else if (CH == 4 && g.units > 1)
-      kv_write_kernel<T, D, CH, CH == 4><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
-    else kv_write_kernel<T, D, CH, false><<<grid, threads, 0, stream>>>(c, b, k, v, r, g.per_seq, g.units);
-    return cudaGetLastError();
+    const auto run = [&](auto kernel) { return kv_launch(kernel, grid, threads, 0, 1, stream, c, b, k, v, r, g.per_seq, g.units); };
+    if constexpr (!WRITE) return run(kv_read_kernel<T, D, CH>);
+    else if (CH == 4 && g.units > 1) return run(kv_write_kernel<T, D, CH, CH == 4>);
+    else return run(kv_write_kernel<T, D, CH, false>);
   });
 }
 
