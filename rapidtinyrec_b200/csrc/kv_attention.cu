@@ -97,18 +97,35 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
     seq = (int)blockIdx.x / a.per_seq;
     item0 = (int64_t)seq * a.per_seq;
   }
-  int first, count, len;
-  const bool whole = kv_rows(a.b, seq, 0, (int64_t)a.b.table_width << a.c.page_shift, a.c.status, first, count, len);
-  if (!whole) {
-    if (count < 0) return;
-    len = 0;  // a length that does not fit: the sequence's rows become NaN
-  }
+  // What needs no other load's result is loaded first: the length, this lane's page
+  // number and its part of the query rows.
+  int first, count, len = a.b.lens[seq];
+  if (!kv_rows(a.b, seq, a.c.status, first, count)) return;
   const int nrows = count * a.group, r0 = (int)(blockIdx.x - item0) * KA_ROWS;
   if (r0 >= nrows) return;
+  const int c0 = split * a.chunk;
+  // lane 2 i + h: the h-th 16 keys of this warp's i-th group (a page is a multiple of 16)
+  const int key_at = c0 + KA_KEYS * (warp + KA_WARPS * (lane >> 1)) + 16 * (lane & 1);
+  const int page = a.b.table[(int64_t)seq * a.b.table_stride + min(key_at >> a.c.page_shift, a.b.table_width - 1)];
+  uint4 raw[D * sizeof(T) / 64];  // dimensions 16 c .. 16 c + 15 (and 64 more) of query row g
+  {
+    const int row = r0 + g, token = row / a.group;
+    const T* p = static_cast<const T*>(a.q) + (int64_t)(first + token) * a.q_token +
+                 (int64_t)(kvh * a.group + row - token * a.group) * D + 16 * c;
+    constexpr int PER = sizeof(T);  // 16-byte loads of 16 values
+#pragma unroll
+    for (int i = 0; i < D / 64 * PER; ++i)
+      raw[i] = row < nrows ? *reinterpret_cast<const uint4*>(p + 64 * (i / PER) + 16 / PER * (i % PER))
+                           : make_uint4(0u, 0u, 0u, 0u);
+  }
+  const bool whole = kv_len_fits(a.c, a.b, len, 0);
+  if (!whole) len = 0;  // the sequence's rows become NaN
   // keys that a row of token t sees
-  auto limit = [&](int row) { return a.causal ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
+  const auto limit = [&](int row) {
+    return a.causal && count > 1 ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len;
+  };
   const int kmin = limit(r0), kmax = limit(r0 + KA_ROWS - 1);
-  const int c0 = split * a.chunk, c1 = min(kmax, c0 + a.chunk);
+  const int c1 = min(kmax, c0 + a.chunk);
   if (c1 <= c0 && split > 0 && !a.cluster) {  // a stretch behind the last key (the first one reports rows that see nothing)
     if (tid < KA_ROWS && r0 + tid < nrows) {
       const int rr = r0 + tid;
@@ -120,19 +137,16 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   const int groups = c1 > c0 ? (c1 - c0 + KA_KEYS - 1) / KA_KEYS : 0;
   const int n = (groups - warp + KA_WARPS - 1) / KA_WARPS;  // this warp's groups: warp, warp + 4, ...
 
-  // lane 2 i + h: the page and the scales of the h-th 16 keys of this warp's i-th group
-  // (a page is a multiple of 16).  Where there are none the last ones stand in, masked.
-  int64_t at = 0;
-  float ks = 0.f, lvs = 0.f, ivs = 0.f;
-  if (lane < 2 * n) {
-    const int key = min(c0 + KA_KEYS * (warp + KA_WARPS * (lane >> 1)) + 16 * (lane & 1), (c1 - 1) & ~15);
-    const int page = kv_page(a.c, a.b, seq, key >> a.c.page_shift);
-    ks = lvs = __int_as_float(0x7fffffff);  // a page that is not there makes the rows NaN
-    at = kvh * a.c.head_stride;
-    if (page >= 0) {
-      at += page * a.c.page_stride + (int64_t)(key & ((1 << a.c.page_shift) - 1)) * D;
-      ks = kv_k_scale(a.c.k_scale[page * a.c.scale_stride + kvh]);
-      kv_v_scale(a.c.v_scale[page * a.c.scale_stride + kvh], lvs, ivs);
+  int64_t at = kvh * a.c.head_stride;
+  float ks = 0.f, vs = 0.f;  // where there are no keys: scores are masked
+  if (key_at < c1) {
+    if (page >= 0 && page < a.c.pages) {
+      at += page * a.c.page_stride + (int64_t)(key_at & ((1 << a.c.page_shift) - 1)) * D;
+      ks = a.c.k_scale[page * a.c.scale_stride + kvh];
+      vs = a.c.v_scale[page * a.c.scale_stride + kvh];
+    } else {
+      atomicOr(a.c.status, RTR_DEV_BAD_PAGE);
+      ks = __int_as_float(0x7fffffff);  // the rows that see the page become NaN
     }
   }
   uint8_t* ring = ka_smem + warp * C::WARP_BYTES;
@@ -160,35 +174,23 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
     for (int i = 0; i < KA_STAGES - 1; ++i) issue(i);
   }
 
-  // this lane's part of query row g: dimensions 16 c .. 16 c + 15 (and 64 more), as
-  // fp16 times a power of two that puts the row's largest value into [2^13, 2^14)
+  float lvs = 0.f, ivs = 0.f;
+  if (key_at < c1) {
+    ks = kv_k_scale(ks);
+    kv_v_scale(vs, lvs, ivs);
+  }
+
+  // the query rows as fp16 times a power of two that puts a row's largest value into [2^13, 2^14)
   uint32_t qh[KW][2], ql[PAIR ? KW : 1][2];
   float f0, f1;  // back to the score, in units of log2, for rows 2 c and 2 c + 1
   {
     float x[D / 4];
-    const int row = r0 + g;
-    if (row < nrows) {
-      const T* p = static_cast<const T*>(a.q) + (int64_t)(first + row / a.group) * a.q_token +
-                   (int64_t)(kvh * a.group + row % a.group) * D + 16 * c;
 #pragma unroll
-      for (int hf = 0; hf < D / 64; ++hf)
-#pragma unroll
-        for (int i = 0; i < 16; i += 16 / sizeof(T)) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p + 64 * hf + i);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (PAIR) {
-              x[16 * hf + i + j] = __uint_as_float(w[j]);
-            } else {
-              x[16 * hf + i + 2 * j] = __uint_as_float(w[j] << 16);
-              x[16 * hf + i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
-          }
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+    for (int i = 0; i < D / 4; ++i) {
+      const uint4& u = raw[i * sizeof(T) / 16];
+      const uint32_t w = (&u.x)[i * sizeof(T) % 16 / 4];
+      if constexpr (PAIR) x[i] = __uint_as_float(w);
+      else x[i] = __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     }
     float top = 0.f;
 #pragma unroll

@@ -153,12 +153,10 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     seq = (int)blockIdx.x / a.per_seq;
     item0 = (int64_t)seq * a.per_seq;
   }
-  int first, count, len;
-  const bool whole = kv_rows(a.b, seq, 0, (int64_t)a.b.table_width << a.c.page_shift, a.c.status, first, count, len);
-  if (!whole) {
-    if (count < 0) return;
-    len = 0;  // a length that does not fit: the sequence's rows become NaN
-  }
+  int first, count, len = a.b.lens[seq];
+  if (!kv_rows(a.b, seq, a.c.status, first, count)) return;
+  const bool whole = kv_len_fits(a.c, a.b, len, 0);
+  if (!whole) len = 0;  // the sequence's rows become NaN
   const int nrows = count * a.group, r0 = (int)(blockIdx.x - item0) * KT_ROWS;
   if (r0 >= nrows) return;
   const auto limit = [&](int row) { return a.causal ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };

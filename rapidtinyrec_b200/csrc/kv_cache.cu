@@ -151,8 +151,9 @@ RTR_DEVICE bool kv_page_rows(const KvCache& c, const KvBatch& b, int64_t item, i
     seq = (int)(item / per_seq);
     item0 = (int64_t)seq * per_seq;
   }
-  int first, count, len;
-  if (!kv_rows(b, seq, 1, (int64_t)b.table_width << c.page_shift, c.status, first, count, len)) return false;
+  int first, count;
+  const int len = b.lens[seq];
+  if (!kv_rows(b, seq, c.status, first, count) || !kv_len_fits(c, b, len, count)) return false;
   const int begin = len - count;
   const int64_t nth = (begin >> c.page_shift) + (item - item0);
   const int64_t p0 = nth << c.page_shift;

@@ -42,30 +42,27 @@ struct KvBatch {
   int32_t table_width, seqs, rows;
 };
 
-// The rows of one sequence: first row and count; false (with the status bit)
-// when starts (then count is -1) or lens do not fit the call.  `capacity`: tokens
-// of a table row.
-RTR_DEVICE bool kv_rows(const KvBatch& b, int seq, int need_rows_in_len, int64_t capacity, uint32_t* status, int& first,
-                        int& count, int& len) {
-  if (b.starts) {
-    first = b.starts[seq];
-    const int end = b.starts[seq + 1];
-    if (first < 0 || end < first || end > b.rows) {
-      atomicOr(status, RTR_DEV_BAD_LENGTH);
-      count = -1;
-      return false;
-    }
-    count = end - first;
-  } else {
+// The rows of one sequence: first row and count; false (with the status bit) when starts
+// does not fit the call.
+RTR_DEVICE bool kv_rows(const KvBatch& b, int seq, uint32_t* status, int& first, int& count) {
+  if (!b.starts) {
     count = b.rows / b.seqs;
     first = seq * count;
+    return true;
   }
-  len = b.lens[seq];
-  if (len < 0 || len > capacity || (need_rows_in_len && count > len)) {
-    atomicOr(status, RTR_DEV_BAD_LENGTH);
-    return false;
-  }
-  return true;
+  first = b.starts[seq];
+  const int end = b.starts[seq + 1];
+  count = end - first;
+  if (first >= 0 && end >= first && end <= b.rows) return true;
+  atomicOr(status, RTR_DEV_BAD_LENGTH);
+  return false;
+}
+
+// Whether a sequence's length fits its table row and holds `least` tokens.
+RTR_DEVICE bool kv_len_fits(const KvCache& c, const KvBatch& b, int len, int least) {
+  if (len >= least && len <= (int64_t)b.table_width << c.page_shift) return true;
+  atomicOr(c.status, RTR_DEV_BAD_LENGTH);
+  return false;
 }
 
 // Which sequence a work item belongs to, when sequence b's items are those from
