@@ -49,8 +49,8 @@ template <int D, bool PAIR> struct KtCfg {
   static constexpr int V_BYTES = 2 * D * 128;                  // [64 keys][dim][64 keys]: V transposed
   static constexpr int Q_OFF = 0, K_OFF = Q_BYTES, V_OFF = K_OFF + 2 * K_BYTES;
   static constexpr int SEG_OFF = V_OFF + 2 * V_BYTES;          // int64 offsets, then 3 floats a segment
-  static constexpr int ROW_OFF = SEG_OFF + KT_SEGS * 20;       // per row: offset in q, row of out, keys it sees
-  static constexpr int RED_OFF = ROW_OFF + KT_ROWS * 16;       // [2][2][128] maxima
+  static constexpr int ROW_OFF = SEG_OFF + KT_SEGS * 20;       // per row: row of out, keys it sees
+  static constexpr int RED_OFF = ROW_OFF + KT_ROWS * 8;        // [2][2][128] maxima
   static constexpr int BAR_OFF = RED_OFF + 2 * 2 * KT_ROWS * 4;
   static constexpr int STAGE_LD = D + 4;                       // row of the finished tile (over K and V), floats
   static_assert(KT_ROWS * STAGE_LD * 4 <= 2 * (K_BYTES + V_BYTES), "the finished tile lies over K and V");
@@ -133,8 +133,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   float* seg_k = reinterpret_cast<float*>(seg_at + KT_SEGS);
   float* seg_lv = seg_k + KT_SEGS;
   float* seg_iv = seg_lv + KT_SEGS;
-  int64_t* row_q = reinterpret_cast<int64_t*>(smem + C::ROW_OFF);
-  int* row_out = reinterpret_cast<int*>(row_q + KT_ROWS);
+  int* row_out = reinterpret_cast<int*>(smem + C::ROW_OFF);
   int* row_lim = row_out + KT_ROWS;
   float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
   KtBars& bars = *reinterpret_cast<KtBars*>(smem + C::BAR_OFF);
@@ -153,16 +152,39 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     seq = (int)blockIdx.x / a.per_seq;
     item0 = (int64_t)seq * a.per_seq;
   }
+  // What needs no other load's result is loaded first: the length, the code warps' page
+  // numbers and the row warps' q.
   int first, count, len = a.b.lens[seq];
   if (!kv_rows(a.b, seq, a.c.status, first, count)) return;
-  const bool whole = kv_len_fits(a.c, a.b, len, 0);
-  if (!whole) len = 0;  // the sequence's rows become NaN
   const int nrows = count * a.group, r0 = (int)(blockIdx.x - item0) * KT_ROWS;
   if (r0 >= nrows) return;
-  const auto limit = [&](int row) { return a.causal ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
-  const int rows = min(KT_ROWS, nrows - r0);
-  const int kmin = limit(r0), kmax = limit(r0 + KT_ROWS - 1);
-  const int c0 = split * a.chunk, c1 = min(kmax, c0 + a.chunk);
+  const int rows = min(KT_ROWS, nrows - r0), c0 = split * a.chunk;
+  constexpr int QPER = 16 / sizeof(T), QLPR = D / QPER, QRPI = 32 / QLPR;  // q: values of 16 bytes, lanes of a row, rows of a load
+  constexpr int QLOADS = 16 / QRPI, QSTEP = QLOADS < 8 ? QLOADS : 8;
+  uint4 q0[QSTEP];
+  int my_q = 0, my_out = 0, my_token = 0;  // lane i of a row warp: its i-th row's place (i < 16)
+  if (warp < 8) {
+    const int rr = min(r0 + warp * 16 + (lane & 15), nrows - 1);
+    my_token = rr / a.group;
+    const int head = kvh * a.group + rr - my_token * a.group;
+    my_q = head * D;
+    my_out = (first + my_token) * a.heads + head;
+  }
+  const auto load_q = [&](int base, uint4 (&u)[QSTEP]) {
+#pragma unroll
+    for (int j = 0; j < QSTEP; ++j) {
+      const int row = (base + j) * QRPI + lane / QLPR;
+      const int64_t at = (int64_t)(first + __shfl_sync(0xffffffffu, my_token, row)) * a.q_token +
+                         __shfl_sync(0xffffffffu, my_q, row) + (lane % QLPR) * QPER;
+      u[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (warp * 16 + row < rows) u[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at);
+    }
+  };
+  if (warp < 8) load_q(0, q0);
+  const bool whole = kv_len_fits(a.c, a.b, len, 0);
+  if (!whole) len = 0;  // the sequence's rows become NaN
+  const auto limit = [&](int row) { return a.causal && count > 1 ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
+  const int kmin = limit(r0), kmax = limit(r0 + KT_ROWS - 1), c1 = min(kmax, c0 + a.chunk);
   if (c1 <= c0 && split > 0 && !a.cluster) {  // a stretch behind the last key (the first one reports rows that see nothing)
     if (tid < rows) {
       const int token = (r0 + tid) / a.group;
@@ -191,15 +213,13 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8 + C::CODE_WARPS) tmem_alloc(smem_addr(&bars.tmem), 512);
-  // the rows' places, by one division each
-  if (const int row = C::THREADS - 1 - tid; row < KT_ROWS) {
-    const int rr = min(r0 + row, nrows - 1), token = rr / a.group, head = kvh * a.group + rr - token * a.group;
-    row_q[row] = (int64_t)(first + token) * a.q_token + (int64_t)head * D;
-    row_out[row] = (first + token) * a.heads + head;
-    row_lim[row] = limit(rr);
+  if (warp < 8 && lane < 16) {
+    row_out[warp * 16 + lane] = my_out;
+    row_lim[warp * 16 + lane] = a.causal ? max(0, len - count + my_token + 1) : len;
   }
   // pages and scales of the stretch's 16-key segments (a page is a multiple of 16)
-  for (int s = tid; s < segs; s += C::THREADS) {
+  for (int s = tid - KT_ROW_THREADS; s < segs; s += C::THREADS - KT_ROW_THREADS) {
+    if (s < 0) break;
     const int key = c0 + 16 * s;
     const int page = kv_page(a.c, a.b, seq, key >> a.c.page_shift);
     int64_t at = kvh * a.c.head_stride;
@@ -226,18 +246,17 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     const int half = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     {
-      // q as fp16 (pairs), each row times a power of two; a warp takes 16 rows, LPR lanes a row
-      constexpr int PER = 16 / sizeof(T), LPR = D / PER, RPI = 32 / LPR, BATCH = 8;
-      constexpr int LOADS = 16 / RPI, STEP = LOADS < BATCH ? LOADS : BATCH;
+      // q as fp16 (pairs), each row times a power of two; a warp takes 16 rows
+      constexpr int PER = QPER, LPR = QLPR, RPI = QRPI, LOADS = QLOADS, STEP = QSTEP;
       const int sub = lane / LPR, col = lane % LPR;
+      uint4 u[STEP];
 #pragma unroll
       for (int base = 0; base < LOADS; base += STEP) {
-        uint4 u[STEP];
+        if (base == 0) {
 #pragma unroll
-        for (int j = 0; j < STEP; ++j) {
-          const int row = warp * 16 + (base + j) * RPI + sub;
-          u[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (row < rows) u[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + row_q[row] + col * PER);
+          for (int j = 0; j < STEP; ++j) u[j] = q0[j];
+        } else {
+          load_q(base, u);
         }
 #pragma unroll
         for (int j = 0; j < STEP; ++j) {
