@@ -445,27 +445,17 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   cluster_sync_all();
   const int mine = split + row * a.splits;
   if (mine < KA_ROWS && r0 + mine < nrows) {
-    const uint32_t ml_at = smem_addr(&sum_ml[mine]), o_at = smem_addr(&sum_o[mine][d0]);
-    mt = -INFINITY;
-    lt = 0.f;
-    for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, ld_cluster_f32(cluster_map(ml_at, s)));
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const uint32_t at = cluster_map(ml_at, s), from = cluster_map(o_at, s);
-      const float ms = ld_cluster_f32(at), f = ms == mt ? 1.f : ex2(ms - mt);
-      lt = fmaf(ld_cluster_f32(at + 4), f, lt);
-#pragma unroll
-      for (int j = 0; j < PER; j += 4) {
-        const float4 v = ld_cluster_f4(from + 4 * j);
-        x[j] = fmaf(v.x, f, x[j]);
-        x[j + 1] = fmaf(v.y, f, x[j + 1]);
-        x[j + 2] = fmaf(v.z, f, x[j + 2]);
-        x[j + 3] = fmaf(v.w, f, x[j + 3]);
-      }
+    for (int j = 0; j < PER; j += 4) {
+      const float4 v = kv_join_cluster(smem_addr(&sum_ml[mine]), smem_addr(&sum_o[mine][d0 + j]), a.splits, mt, lt);
+      x[j] = v.x;
+      x[j + 1] = v.y;
+      x[j + 2] = v.z;
+      x[j + 3] = v.w;
     }
     finish(r0 + mine);
   }
+  __syncwarp();
   cluster_sync_all();  // no block leaves while another may still read its sums
 }
 
@@ -584,7 +574,7 @@ static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   if (chunk > KA_MAX_CHUNK) chunk = KA_MAX_CHUNK;
   p.chunk = (int)chunk;
   p.splits = (int)((most + chunk - 1) / chunk);
-  p.cluster = p.splits > 1 && p.splits <= 8;
+  p.cluster = p.splits > 1 && p.splits <= KV_CLUSTER;
   // measured: 8 rows x 18,500 (fp32 16,000) keys a us at head_dim 128, 55,000 (48,000) at 64
   const int64_t rate = c->head_dim == 128 ? (f32 ? 16000 : 18500) : f32 ? 48000 : 55000;
   ns = 5000 + base * most * 1000 / rate + (p.splits > 1 ? 3000 : 0);
@@ -617,7 +607,7 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
       p.splits = (int)splits;
     }
   }
-  p.cluster = p.splits > 1 && p.splits <= 8;
+  p.cluster = p.splits > 1 && p.splits <= KV_CLUSTER;
   ns = best * kv_tile_ns(c, f32);
   return p;
 }
@@ -640,6 +630,7 @@ static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int
 static const char* kv_attn_check(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads) {
   if (const char* e = kv_check(c, b)) return e;
   if (heads < 1 || heads % c->kv_heads) return "heads must be a multiple of kv_heads";
+  if (heads > 16384) return "at most 16384 heads";
   if ((int64_t)b->rows * heads > INT32_MAX) return "at most 2^31 - 1 rows x heads in one call";
   return nullptr;
 }
@@ -706,6 +697,7 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
   a.q_token = q_token_stride;
   a.heads = heads;
   a.group = heads / cache->kv_heads;
+  a.group_inverse = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   a.causal = causal != 0;
   a.factor = scale * 1.4426950408889634f;
   a.out = out_dev;

@@ -3,8 +3,11 @@
 #pragma once
 
 #include "kv_cache.cuh"
+#include "tcgen05.cuh"
 
 namespace rtr {
+
+constexpr int KV_CLUSTER = 8;  // stretches that one cluster joins
 
 struct KvAttn {
   KvCache c;
@@ -12,6 +15,7 @@ struct KvAttn {
   const void* q;
   int64_t q_token;     // elements between a token's rows; heads are contiguous
   int heads, group;    // query heads, and those of one KV head
+  uint32_t group_inverse;  // ceil(2^32 / group): see kv_div
   int causal;
   float factor;        // softmax scale * log2(e)
   void* out;           // [rows][heads][head_dim]
@@ -28,15 +32,19 @@ struct KvAttn {
 // before a weight nears fp16's largest, 2^16.
 constexpr float KA_LIFT = 6.0f;
 
+// v / group for v < 2^32 / group (v is a row's place within some tiles): one multiplication.
+// A group of one has no 32-bit inverse.
+RTR_DEVICE int kv_div(const KvAttn& a, int v) { return a.group == 1 ? v : (int)__umulhi((uint32_t)v, a.group_inverse); }
+
+// The sums of a cluster's blocks for one row: their joined maximum and sum, and four
+// columns.  ml_at: this block's (maximum, sum), x_at: its columns; all loads are issued before
+// any is used (one after the other they cost 250 cycles each).
+RTR_DEVICE float4 kv_join_cluster(uint32_t ml_at, uint32_t x_at, int splits, float& m, float& l);
+
 RTR_DEVICE float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
-}
-RTR_DEVICE float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
 }
 RTR_DEVICE float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
@@ -45,6 +53,35 @@ RTR_DEVICE float4 ld_cluster_f4(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+RTR_DEVICE float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+RTR_DEVICE float4 kv_join_cluster(uint32_t ml_at, uint32_t x_at, int splits, float& m, float& l) {
+  float2 ml[KV_CLUSTER];
+  float4 v[KV_CLUSTER];
+#pragma unroll
+  for (int s = 0; s < KV_CLUSTER; ++s) {
+    if (s >= splits) break;
+    ml[s] = ld_cluster_f2(cluster_map(ml_at, s));
+    v[s] = ld_cluster_f4(cluster_map(x_at, s));
+  }
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int s = 0; s < KV_CLUSTER; ++s)
+    if (s < splits) m = fmaxf(m, ml[s].x);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int s = 0; s < KV_CLUSTER; ++s) {
+    if (s >= splits) break;
+    const float w = ml[s].x == m ? 1.f : ex2(ml[s].x - m);
+    l = fmaf(ml[s].y, w, l);
+    x = make_float4(fmaf(v[s].x, w, x.x), fmaf(v[s].y, w, x.y), fmaf(v[s].z, w, x.z), fmaf(v[s].w, w, x.w));
+  }
+  return x;
 }
 RTR_DEVICE uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);

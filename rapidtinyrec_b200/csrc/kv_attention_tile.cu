@@ -162,22 +162,22 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   constexpr int QPER = 16 / sizeof(T), QLPR = D / QPER, QRPI = 32 / QLPR;  // q: values of 16 bytes, lanes of a row, rows of a load
   constexpr int QLOADS = 16 / QRPI, QSTEP = QLOADS < 8 ? QLOADS : 8;
   uint4 q0[QSTEP];
-  int my_q = 0, my_out = 0, my_token = 0;  // lane i of a row warp: its i-th row's place (i < 16)
-  if (warp < 8) {
-    const int rr = min(r0 + warp * 16 + (lane & 15), nrows - 1);
-    my_token = rr / a.group;
-    const int head = kvh * a.group + rr - my_token * a.group;
-    my_q = head * D;
-    my_out = (first + my_token) * a.heads + head;
-  }
+  const int token0 = r0 / a.group, head0 = r0 - token0 * a.group;  // of the tile's first row
+  // token and head (of the group) of a row of the tile
+  const auto place = [&](int row, int& token, int& head) {
+    const int t = kv_div(a, head0 + min(row, rows - 1));
+    token = token0 + t;
+    head = head0 + min(row, rows - 1) - t * a.group;
+  };
   const auto load_q = [&](int base, uint4 (&u)[QSTEP]) {
 #pragma unroll
     for (int j = 0; j < QSTEP; ++j) {
-      const int row = (base + j) * QRPI + lane / QLPR;
-      const int64_t at = (int64_t)(first + __shfl_sync(0xffffffffu, my_token, row)) * a.q_token +
-                         __shfl_sync(0xffffffffu, my_q, row) + (lane % QLPR) * QPER;
-      u[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (warp * 16 + row < rows) u[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at);
+      const int row = warp * 16 + (base + j) * QRPI + lane / QLPR;
+      int token, head;
+      place(row, token, head);
+      const T* p = static_cast<const T*>(a.q) + (int64_t)(first + token) * a.q_token +
+                   (kvh * a.group + head) * D + (lane % QLPR) * QPER;
+      u[j] = row < rows ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
   if (warp < 8) load_q(0, q0);
@@ -213,9 +213,11 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8 + C::CODE_WARPS) tmem_alloc(smem_addr(&bars.tmem), 512);
-  if (warp < 8 && lane < 16) {
-    row_out[warp * 16 + lane] = my_out;
-    row_lim[warp * 16 + lane] = a.causal ? max(0, len - count + my_token + 1) : len;
+  if (tid < KT_ROWS) {
+    int token, head;
+    place(tid, token, head);
+    row_out[tid] = (first + token) * a.heads + kvh * a.group + head;
+    row_lim[tid] = a.causal ? max(0, len - count + token + 1) : len;
   }
   // pages and scales of the stretch's 16-key segments (a page is a multiple of 16)
   for (int s = tid - KT_ROW_THREADS; s < segs; s += C::THREADS - KT_ROW_THREADS) {
@@ -269,8 +271,9 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             else x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
             top = fmaxf(top, fabsf(x[i]));
           }
-#pragma unroll
-          for (int d = 1; d < LPR; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          // magnitudes order as their bits do
+          top = __uint_as_float(__reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (sub * LPR),
+                                                  __float_as_uint(top)));
           const int e = kv_row_exponent(top);
           const float up = copysignf(kv_pow2(-e), a.factor);  // the factor back stays positive: see below
           if (col == 0) red[row] = kv_pow2(e) * fabsf(a.factor);
@@ -457,6 +460,24 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, kf, lv));
           }
         };
+        if (i == 0) {
+          // nothing to go by: the maximum alone first
+          uint32_t v[2][32];
+          tmem_ld32(st, v[0]);
+          tmem_ld32(st + 32, v[1]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int s = min(seg0 + g, segs - 1);
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float x = __uint_as_float(v[g >> 1][16 * (g & 1) + j]);
+              top = fmaxf(top, key0 + 16 * g + j < lim ? x : -INFINITY);
+            }
+            m = fmaxf(m, top == -INFINITY ? top : fmaf(top, f * seg_k[s], seg_lv[s]));
+          }
+        }
         weigh((m == -INFINITY ? 0.f : m) - KA_LIFT);
         if (__any_sync(0xffffffffu, mx > m + KT_SLACK)) {  // m may be minus infinity
           const float top = fmaxf(m, mx), alpha = m == top ? 1.f : ex2(m - top);
@@ -747,17 +768,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   // the cluster's blocks share out the rows, each reads the others' sums
   cluster_sync_all();
   for (int row = split + a.splits * (warp * RPI + lane / LPR); row < rows; row += a.splits * WARPS * RPI) {
-    const uint32_t ml_at = smem_addr(&ml[row]), x_at = smem_addr(stage + row * C::STAGE_LD + 4 * col);
-    float mt = -INFINITY, lt = 0.f;
-    for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, ld_cluster_f32(cluster_map(ml_at, s)));
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; ++s) {
-      const uint32_t at = cluster_map(ml_at, s);
-      const float ms = ld_cluster_f32(at), w = ms == mt ? 1.f : ex2(ms - mt);
-      const float4 v = ld_cluster_f4(cluster_map(x_at, s));
-      lt = fmaf(ld_cluster_f32(at + 4), w, lt);
-      x = make_float4(fmaf(v.x, w, x.x), fmaf(v.y, w, x.y), fmaf(v.z, w, x.z), fmaf(v.w, w, x.w));
-    }
+    float mt, lt;
+    const float4 x = kv_join_cluster(smem_addr(&ml[row]), smem_addr(stage + row * C::STAGE_LD + 4 * col), a.splits, mt, lt);
     finish(row, mt, lt, x);
   }
   __syncwarp();
