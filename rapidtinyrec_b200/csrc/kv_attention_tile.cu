@@ -52,8 +52,12 @@ template <int D, bool PAIR> struct KtCfg {
   static constexpr int ROW_OFF = SEG_OFF + KT_SEGS * 20;       // per row: row of out, keys it sees
   static constexpr int RED_OFF = ROW_OFF + KT_ROWS * 8;        // [2][2][128] maxima
   static constexpr int BAR_OFF = RED_OFF + 2 * 2 * KT_ROWS * 4;
-  static constexpr int STAGE_LD = D + 4;                       // row of the finished tile (over K and V), floats
-  static_assert(KT_ROWS * STAGE_LD * 4 <= 2 * (K_BYTES + V_BYTES), "the finished tile lies over K and V");
+  // the finished tile (rows of STAGE_LD floats) lies over the last operands, what a cluster's
+  // blocks send each other over the first
+  static constexpr int STAGE_LD = D + 4;
+  static constexpr int STAGE_OFF = SEG_OFF - KT_ROWS * STAGE_LD * 4;
+  static constexpr int RECV_ROWS = KT_ROWS + KV_CLUSTER;       // ceil(128 / splits) rows from each block
+  static_assert(RECV_ROWS * D * 4 + RECV_ROWS * 8 <= STAGE_OFF, "both lie over the operands");
   static constexpr int SMEM = BAR_OFF + 256 + 1024;            // 1024: alignment of the operands
 };
 
@@ -115,6 +119,13 @@ RTR_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+RTR_DEVICE void st_cluster_f4(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+RTR_DEVICE void st_cluster_f2(uint32_t addr, float2 v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
 }
 RTR_DEVICE void row_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 RTR_DEVICE uint32_t sw_at(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
@@ -551,7 +562,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     }
     if (lt == 0.f && (lim > c0 || !whole)) lt = __int_as_float(0x7fffffff);
     // through shared memory (the operands are done with), for whole lines on the way out
-    float* stage = reinterpret_cast<float*>(smem + C::K_OFF);
+    float* stage = reinterpret_cast<float*>(smem + C::STAGE_OFF);
     const auto value = [&](int i) { return i & 1 ? f2_parts(o[i >> 1]).y : f2_parts(o[i >> 1]).x; };
 #pragma unroll
     for (int j = 0; j < NL; ++j)
@@ -733,7 +744,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     tmem_dealloc(tmem, 512);
   }
   // D / 4 threads a row; every warp takes rows in turn
-  const float* stage = reinterpret_cast<const float*>(smem + C::K_OFF);
+  const float* stage = reinterpret_cast<const float*>(smem + C::STAGE_OFF);
   const float2* ml = reinterpret_cast<const float2*>(red);
   constexpr int LPR = D / 4, RPI = 32 / LPR, WARPS = C::THREADS / 32;
   const int col = lane % LPR;
@@ -765,15 +776,44 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     }
     return;
   }
-  // the cluster's blocks share out the rows, each reads the others' sums
-  cluster_sync_all();
-  for (int row = split + a.splits * (warp * RPI + lane / LPR); row < rows; row += a.splits * WARPS * RPI) {
-    float mt, lt;
-    const float4 x = kv_join_cluster(smem_addr(&ml[row]), smem_addr(stage + row * C::STAGE_LD + 4 * col), a.splits, mt, lt);
-    finish(row, mt, lt, x);
+  // The cluster's blocks share out the rows: block `row % splits` gets the row from all of
+  // them.  Stores into the other blocks' shared memory need no answer; reading it the other way
+  // round, 64 KB a block, took 6,100 cycles, this 3,000.
+  cluster_sync_all();  // every block is done with its operands
+  const int inverse = (65536 + a.splits - 1) / a.splits;  // row / splits = row * inverse >> 16 for these few rows
+  const int each = ((KT_ROWS - 1) * inverse >> 16) + 1;
+  const uint32_t recv = smem_addr(smem), recv_ml = recv + C::RECV_ROWS * D * 4;
+  for (int row = warp * RPI + lane / LPR; row < rows; row += WARPS * RPI) {
+    const int nth = row * inverse >> 16, to = row - nth * a.splits, slot_at = split * each + nth;
+    st_cluster_f4(cluster_map(recv + (slot_at * D + 4 * col) * 4, to),
+                  *reinterpret_cast<const float4*>(stage + row * C::STAGE_LD + 4 * col));
+    if (col == 0) st_cluster_f2(cluster_map(recv_ml + slot_at * 8, to), ml[row]);
   }
   __syncwarp();
-  cluster_sync_all();  // no block leaves while another may still read its sums
+  cluster_sync_all();
+  const float4* sent = reinterpret_cast<const float4*>(smem);
+  const float2* sent_ml = reinterpret_cast<const float2*>(smem + C::RECV_ROWS * D * 4);
+  for (int i = warp * RPI + lane / LPR; split + i * a.splits < rows; i += WARPS * RPI) {
+    float2 p[KV_CLUSTER];
+    float4 v[KV_CLUSTER];
+    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int s = 0; s < KV_CLUSTER; ++s) {
+      if (s >= a.splits) break;
+      p[s] = sent_ml[s * each + i];
+      v[s] = sent[(s * each + i) * (D / 4) + col];
+      mt = fmaxf(mt, p[s].x);
+    }
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < KV_CLUSTER; ++s) {
+      if (s >= a.splits) break;
+      const float w = p[s].x == mt ? 1.f : ex2(p[s].x - mt);
+      lt = fmaf(p[s].y, w, lt);
+      x = make_float4(fmaf(v[s].x, w, x.x), fmaf(v[s].y, w, x.y), fmaf(v[s].z, w, x.z), fmaf(v[s].w, w, x.w));
+    }
+    finish(split + i * a.splits, mt, lt, x);
+  }
 }
 
 template <typename T, int D> static cudaError_t launch_tile(const KvAttn& a, int64_t items, int device, cudaStream_t st) {
