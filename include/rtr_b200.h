@@ -341,7 +341,8 @@ typedef struct {
  * if that is larger, and has their codes rounded again if it is smaller.  Codes are
  * rounded to nearest even; NaN, infinities and magnitudes above 448 * 2^48 become
  * NaN.  Codes behind a sequence's last token stay.  The pages that a call writes
- * must be different ones: two sequences that share such a page leave either's codes. */
+ * must be different ones: where two sequences write into one page, its codes and scale
+ * are some of either's. */
 int rtr_kv_write(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const void* k_dev, const void* v_dev,
                  int32_t dtype, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
                  int64_t v_head_stride, int32_t device, void* stream);
@@ -358,8 +359,9 @@ int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_de
  * nothing are 0.  q: row r, head h at r * q_token_stride + h * head_dim; out
  * [rows][heads][head_dim], same dtype; lse_dev (optional, float32 [rows][heads]):
  * log of the softmax's sum, minus infinity for rows that see nothing.  fp32 q and
- * weights enter the tensor cores as fp16 pairs (22 bits); sums are fp32.  V scales
- * must lie in [2^-48, 2^48] (others make the row NaN).  The workspace must hold
+ * weights enter the tensor cores as fp16 pairs (22 bits); sums are fp32.  A row
+ * that sees a page whose V scale is outside [2^-48, 2^48], whose K scale is negative or
+ * whose number is outside the cache is NaN.  The workspace must hold
  * rtr_kv_attention_workspace bytes, aligned to 16, and is free again when the call's
  * kernels ran: calls that may overlap need one each.  A table row wider than the
  * sequences need costs idle blocks. */

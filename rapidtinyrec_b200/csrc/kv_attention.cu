@@ -467,10 +467,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
 constexpr int KJ_MAX = 1024;  // splits whose weights are kept at a time
 
 template <typename T, int D, int KJ_THREADS>
-__global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch b, int heads,
-                                                                  const float* __restrict__ part,
-                                                                  const float2* __restrict__ ml, int splits,
-                                                                  T* __restrict__ out, float* __restrict__ lse) {
+__global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch b, int heads, const float* part,
+                                                                  const float2* ml, int splits, T* out, float* lse) {
   constexpr int COLS = D / 4, LANES = KJ_THREADS / COLS;
   __shared__ float weight[KJ_MAX];
   __shared__ float red[2][KJ_THREADS / 32];

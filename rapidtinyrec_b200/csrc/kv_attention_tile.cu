@@ -433,7 +433,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         // that is too far above, a second one with the new maximum.
         uint32_t w[32];
         float mx, part_l;
-        const auto weigh = [&](float u) {
+        const auto weigh_keys = [&](float u, auto at_border) {
+          constexpr bool BORDER = decltype(at_border)::value;
           uint32_t v[2][16];
           tmem_ld16(st, v[0]);
           mx = -INFINITY;
@@ -446,20 +447,22 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             tmem_ld_wait();
             uint32_t(&x)[16] = v[g & 1];
             if (g < 3) tmem_ld16(st + 16 * (g + 1), v[(g + 1) & 1]);
-            if (border) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (key0 + 16 * g + j >= lim) x[j] = 0xff800000u;
-            }
             float top = -INFINITY;
             uint64_t sums = 0;
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
-              top = fmaxf(top, fmaxf(fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])),
-                                     fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]))));
+              float z[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                z[e] = BORDER && key0 + 16 * g + j + e >= lim ? -INFINITY : __uint_as_float(x[j + e]);
+              top = fmaxf(top, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
 #pragma unroll
               for (int e = 0; e < 4; e += 2) {
                 float2 y = f2_parts(f2_fma(f2(x[j + e], x[j + e + 1]), kf2, lv2));
+                if constexpr (BORDER) {  // after the product: the scales of a page that the row does not see may be anything
+                  if (key0 + 16 * g + j + e >= lim) y.x = -INFINITY;
+                  if (key0 + 16 * g + j + e + 1 >= lim) y.y = -INFINITY;
+                }
                 y.x = ex2(y.x);
                 y.y = ex2(y.y);
                 sums = f2_add(sums, f2(y.x, y.y));
@@ -470,6 +473,11 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             // the factors are positive: the largest product of a segment gives its largest score
             mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, kf, lv));
           }
+        };
+        const auto weigh = [&] {
+          const float u = (m == -INFINITY ? 0.f : m) - KA_LIFT;
+          if (border) weigh_keys(u, std::true_type{});
+          else weigh_keys(u, std::false_type{});
         };
         if (i == 0) {
           // nothing to go by: the maximum alone first
@@ -489,7 +497,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             m = fmaxf(m, top == -INFINITY ? top : fmaf(top, f * seg_k[s], seg_lv[s]));
           }
         }
-        weigh((m == -INFINITY ? 0.f : m) - KA_LIFT);
+        weigh();
         if (__any_sync(0xffffffffu, mx > m + KT_SLACK)) {  // m may be minus infinity
           const float top = fmaxf(m, mx), alpha = m == top ? 1.f : ex2(m - top);
           m = top;
@@ -507,7 +515,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
               tmem_st_words(ot + c, v);
             }
           }
-          weigh((m == -INFINITY ? 0.f : m) - KA_LIFT);
+          weigh();
         }
         l += part_l;
         tmem_st32(st, w);  // over the scores just read

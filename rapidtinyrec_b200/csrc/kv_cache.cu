@@ -171,8 +171,8 @@ RTR_DEVICE bool kv_page_rows(const KvCache& c, const KvBatch& b, int64_t item, i
 // threads share an SM (two with eight pieces): 350 fp32 tokens of 56 heads, 13.0 us with
 // the registers of AHEAD, 9.4 us without.
 template <typename T, int D, int CH, bool AHEAD>
-__global__ void __launch_bounds__(KV_THREADS, CH == 4 && !AHEAD ? 3 : 2) kv_write_kernel(const KvCache c, const KvBatch b, const T* __restrict__ k,
-                                                              const T* __restrict__ v, const KvRows rs, int per_seq,
+__global__ void __launch_bounds__(KV_THREADS, CH == 4 && !AHEAD ? 3 : 2) kv_write_kernel(const KvCache c, const KvBatch b, const T* k,
+                                                              const T* v, const KvRows rs, int per_seq,
                                                               int units) {
   constexpr int N = 16 / sizeof(T), DPR = D / N;  // values of a piece, pieces of a row
   __shared__ int slot;
@@ -268,8 +268,8 @@ __global__ void __launch_bounds__(KV_THREADS, CH == 4 && !AHEAD ? 3 : 2) kv_writ
 }
 
 template <typename T, int D, int CH>
-__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvCache c, const KvBatch b, T* __restrict__ k,
-                                                             T* __restrict__ v, const KvRows rs, int per_seq,
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvCache c, const KvBatch b, T* k,
+                                                             T* v, const KvRows rs, int per_seq,
                                                              int units) {
   constexpr int N = 16 / sizeof(T), DPR = D / N;
   __shared__ int slot;

@@ -14,6 +14,7 @@ What the three share: ``table`` int32 ``[seqs, width]`` page numbers, ``lens`` i
 are not read on the host, so nothing here synchronises and every call can be captured
 into a CUDA graph.  What does not fit (a page number outside the cache, a length that
 the table cannot hold) leaves its work undone and sets a bit that ``check`` raises for.
+The operators serve inference: their results carry no gradient.
 """
 from __future__ import annotations
 

@@ -422,6 +422,98 @@ def test_nan_stays_with_the_rows_that_see_it(dtype, counts):
     assert torch.equal(nan, want)
 
 
+# ------------------------------------------------------------- 128-row tiles
+# Sizes at which the tiles of 128 rows are expected to be the faster ones by a wide margin:
+# some thousand rows a KV head over more than a thousand keys.
+TILED = [(12, 2, 128), (14, 2, 64)]
+
+
+@pytest.mark.parametrize('heads,kv,dim', TILED)
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('causal', [True, False])
+def test_tiles_of_128_rows(heads, kv, dim, dtype, causal):
+    """Ragged sequences, some with more rows than tokens or none; one longer than a block's keys."""
+    counts = [700, 0, 1, 300, 129, 1400]
+    lens = [1300, 900, 0, 120, 9000, 1500]
+    pages = sum(-(-t // 64) for t in lens) + 1
+    cache = filled(pages, kv, 64, dim, seed=heads + dim + 2)
+    table = tables(lens, 64, pages, seed=46)
+    g = torch.Generator().manual_seed(47)
+    q = (2 * torch.randn(sum(counts), heads, dim, generator=g)).to(dtype).cuda()
+    check_attention(cache, q, table, lens, counts, causal, starts=cuts(counts))
+    for scale in (0.0, -0.05):
+        check_attention(cache, q[:1400], table[:1], lens[:1], [1400], causal, scale=scale)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('tokens', [1100, 9000])
+def test_tiles_of_an_own_length(dtype, tokens):
+    """Rows of one sequence, scales 2^60 apart and no powers of two, tiny and huge queries."""
+    cache = filled(80, 2, 128, 128, seed=48)
+    table = tables([tokens], 128, 80, seed=49)
+    g = torch.Generator().manual_seed(50)
+    cache.v_scale.copy_(torch.exp2(torch.randint(-30, 30, (80, 2), generator=g).float()))
+    cache.k_scale.copy_(torch.rand(80, 2, generator=g) * 0.01 + 0.001)
+    for size in (1e-30, 1.0, 30.0):
+        q = (torch.randn(1000, 12, 128, generator=g) * size).to(dtype).cuda()
+        check_attention(cache, q, table, [tokens], [1000], True)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_tiles_keep_nan_with_the_rows_that_see_it(dtype):
+    n, tokens, page = 1000, 1300, 32
+    cache = filled(50, 1, page, 64, seed=51)
+    table = tables([tokens], page, 50, seed=52)
+    pages = table.tolist()[0]
+    q = torch.randn(n, 14, 64, generator=torch.Generator().manual_seed(53)).to(dtype).cuda()
+    before = cache.attention(q, table, ints([tokens]))
+    code = cache.v.view(torch.uint8)
+    code[pages[1100 // page], 0, 1100 % page, 5] = 0xff       # V of token 1100, dimension 5
+    cache.k.view(torch.uint8)[pages[1250 // page], 0, 1250 % page, 7] = 0x7f  # K of token 1250
+    code[pages[-1], 0, tokens % page:] = 0x7f                 # behind the last token
+    cache.k.view(torch.uint8)[pages[-1], 0, tokens % page:] = 0x7f
+    cache.v_scale[pages[1280 // page]] = 0.0                  # tokens 1280 ..
+    out = cache.attention(q, table, ints([tokens]))
+    nan = out.isnan()
+    first = tokens - n  # the token of row 0
+    assert not nan[:1100 - first].any() and torch.equal(out[:1100 - first], before[:1100 - first])
+    some = nan[1100 - first:1250 - first]
+    assert some[:, :, 5].all() and some.sum() == some.shape[0] * 14
+    assert nan[1250 - first:].all()
+    # the row at token 1279 sees all but the page without a scale; what it sees has the NaN
+    ok = torch.ones(64, dtype=torch.bool)
+    ok[5] = False
+    assert torch.equal(out[1100 - first:1250 - first][..., ok], before[1100 - first:1250 - first][..., ok])
+    # queries that are NaN or infinite spoil their own rows alone
+    q[1, 2, 3], q[130, 0, 0] = NAN, math.inf
+    nan = cache.attention(q[:700], table, ints([1000])).isnan()
+    want = torch.zeros_like(nan)
+    want[1, 2] = want[130, 0] = True
+    assert torch.equal(nan, want)
+    # a page number outside the cache, in the last page: the rows before it are whole
+    from rapidtinyrec_b200._native import NativeError
+    table[0, 1000 // page - 1] = 50
+    out = cache.attention(q[:700], table, ints([1000]))
+    with pytest.raises(NativeError, match='page'):
+        cache.check()
+    behind = (1000 // page - 1) * page - (1000 - 700)  # the first row that sees it
+    assert out[behind:].isnan().all() and not out[131:behind].isnan().any()
+
+
+def test_bad_k_scales_make_their_rows_nan():
+    cache = filled(4, 1, 16, 64, seed=54)
+    table = ints([[0, 1], [2, 3]])
+    q = torch.randn(2, 2, 64, generator=torch.Generator().manual_seed(55)).cuda()
+    for bad in (-1.0, NAN):
+        cache.k_scale[1] = bad
+        out = cache.attention(q, table, ints([20, 20]))
+        assert out[0].isnan().all() and not out[1].isnan().any()
+        assert not cache.attention(q, table, ints([16, 20])).isnan().any()
+    cache.k_scale[1] = 0.0  # a page of equal scores
+    check_attention(cache, q, table, [20, 20], [1, 1], True)
+    check_attention(cache, q, table, [20, 20], [1, 1], True, scale=-0.3)
+
+
 def test_bad_v_scales_make_their_rows_nan():
     cache = filled(4, 1, 16, 64, seed=27)
     table = ints([[0, 1], [2, 3]])
