@@ -9,7 +9,7 @@
 //            operand of P V;
 //   codes    read K and V of the next tiles from the pages into registers, turn them
 //            into fp16 and store them as swizzled operands, V transposed;
-//   products one thread issues whichever product is ready.
+//   products one thread issues the products.
 // There are two buffers of K, V, S and O, tile i in buffer i % 2.
 //
 // bf16 rows: two threads a row, each with 64 of a tile's keys, its own maximum, sum and
@@ -69,13 +69,24 @@ struct KtBars {
 };
 static_assert(sizeof(KtBars) <= 256, "barriers fit their part of shared memory");
 
-// D[tmem] (+)= A[tmem] . B[smem]^T, kind::f16 (both fp16)
-RTR_DEVICE void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A . B[smem]^T, kind::f16 (both fp16), A in shared or tensor memory;
+// descriptors as low words and their common high word.
+RTR_DEVICE void mma_f16_ss_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+RTR_DEVICE void mma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
 RTR_DEVICE void tmem_st_words(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -677,65 +688,73 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     }
   } else if (lane == 0) {
     // --------------------------------------------------------- products
+    // One thread's instructions stand between a tile's weights and the next scores: buffers are
+    // compile-time numbers and descriptors their low words from a common base, so that a
+    // product costs little more than its issue.
     constexpr uint32_t id_s = idesc_f16(KT_ROWS, KT_KEYS), id_o = idesc_f16(KT_ROWS, D);
-    const auto issue_s = [&](int i) {
-      const uint8_t* kd = smem + C::K_OFF + (i & 1) * C::K_BYTES;
+    constexpr int HALVES = PAIR ? 1 : 2;
+    const uint64_t base = sw128_desc(smem_addr(smem));
+    const uint32_t lo = (uint32_t)base, hi = (uint32_t)(base >> 32);
+    int si = 0, oi[2] = {0, 0};  // products issued
+    const auto wait = [&](uint64_t& bar, int i) { return mbar_wait(smem_addr(&bar), (i >> 1) & 1, abort_flag); };
+    const auto issue_s = [&](auto buffer) {
+      constexpr int B = decltype(buffer)::value;
+      tc_fence_after();
 #pragma unroll
       for (int pl = 0; pl < (PAIR ? 2 : 1); ++pl)
 #pragma unroll
-        for (int p = 0; p < C::PANELS; ++p) {
-          const uint64_t qd = sw128_desc(smem_addr(qs + pl * C::Q_PLANE + p * KT_ROWS * 128));
-          const uint64_t kk = sw128_desc(smem_addr(kd + p * KT_KEYS * 128));
+        for (int p = 0; p < C::PANELS; ++p)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_f16_ss(tmem + (i & 1) * S_COLS, qd + 2 * k, kk + 2 * k, id_s, (pl | p | k) ? 1u : 0u);
-        }
-      mma_commit(smem_addr(&bars.s_full[i & 1]));
+            mma_f16_ss_lo(tmem + B * S_COLS, lo + (C::Q_OFF + pl * C::Q_PLANE + p * KT_ROWS * 128) / 16 + 2 * k,
+                          lo + (C::K_OFF + B * C::K_BYTES + p * KT_KEYS * 128) / 16 + 2 * k, hi, id_s, pl || p || k);
+      mma_commit(smem_addr(&bars.s_full[B]));
+      ++si;
     };
     // fp32 rows: the whole tile's product, alone in its buffer; bf16 rows: that of one half
     // of the keys, added to the half's sum
-    const auto issue_o = [&](int i, int h) {
-      const uint8_t* vd = smem + C::V_OFF + (i & 1) * C::V_BYTES;
-      const uint32_t pt = tmem + (i & 1) * S_COLS, ot = tmem + O_AT + (PAIR ? i & 1 : h) * 128;
+    const auto issue_o = [&](auto buffer, auto half, bool add) {
+      constexpr int B = decltype(buffer)::value, H = decltype(half)::value;
+      tc_fence_after();
 #pragma unroll
       for (int k = 0; k < (PAIR ? 8 : 4); ++k) {  // 16 keys each
-        const int ks = PAIR ? k : 4 * h + k;
-        const uint64_t vv = sw128_desc(smem_addr(vd + (ks >> 2) * D * 128)) + 2 * (ks & 3);
+        const int ks = PAIR ? k : 4 * H + k;
+        const uint32_t v = lo + (C::V_OFF + B * C::V_BYTES + (ks >> 2) * D * 128) / 16 + 2 * (ks & 3);
         if constexpr (PAIR) {
-          const uint32_t p = pt + 16 * k;  // the weights, then their low parts, lie over the scores of their keys
-          mma_f16_ts(ot, p, vv, id_o, k ? 1u : 0u);
-          mma_f16_ts(ot, p + 8, vv, id_o, 1u);
+          const uint32_t p = tmem + B * S_COLS + 16 * k;  // the weights, then their low parts, lie over the scores
+          mma_f16_ts_lo(tmem + O_AT + B * 128, p, v, hi, id_o, k > 0);
+          mma_f16_ts_lo(tmem + O_AT + B * 128, p + 8, v, hi, id_o, true);
         } else {
-          mma_f16_ts(ot, pt + 64 * h + 8 * k, vv, id_o, k || i > 0 ? 1u : 0u);
+          mma_f16_ts_lo(tmem + O_AT + H * 128, tmem + B * S_COLS + 64 * H + 8 * k, v, hi, id_o, k > 0 || add);
         }
       }
-      mma_commit(smem_addr(&bars.o_full[h][i & 1]));
+      mma_commit(smem_addr(&bars.o_full[H][B]));
+      ++oi[H];
     };
-    constexpr int HALVES = PAIR ? 1 : 2;
-    int si = 0, oi[2] = {0, 0};  // products issued
-    const auto wait = [&](uint64_t& bar, int i) { return mbar_wait(smem_addr(&bar), (i >> 1) & 1, abort_flag); };
-    bool ok = n == 0 || mbar_wait(smem_addr(&bars.q_full), 0, abort_flag);
-    const auto next_s = [&] {
-      if (si >= n) return true;
-      if (!wait(bars.k_full[si & 1], si)) return false;
-      // S goes over the weights of the tile two before: their products must be done
-      for (int h = 0; h < HALVES; ++h)
-        if (si >= 2 && !wait(bars.o_full[h][si & 1], si - 2)) return false;
-      tc_fence_after();
-      issue_s(si++);
+    const auto tile = [&](int i, auto buffer) {
+      constexpr int B = decltype(buffer)::value;
+      if (!wait(bars.v_full[B], i) || (PAIR && i >= 2 && !wait(bars.o_free[B], i - 2))) return false;
+      if (!wait(bars.p_full[0][B], i)) return false;
+      issue_o(buffer, std::integral_constant<int, 0>{}, i > 0);
+      if constexpr (!PAIR) {
+        if (!wait(bars.p_full[1][B], i)) return false;
+        issue_o(buffer, std::integral_constant<int, 1>{}, i > 0);
+      }
+      if (i + 2 >= n) return true;
+      // the next scores of this buffer go over the weights: their products must be done
+      if (!wait(bars.k_full[B], i + 2) || !wait(bars.o_full[0][B], i)) return false;
+      if (!PAIR && !wait(bars.o_full[1][B], i)) return false;
+      issue_s(buffer);
       return true;
     };
-    ok = ok && next_s() && next_s();
-    for (int i = 0; i < n && ok; ++i) {
-      for (int h = 0; h < HALVES && ok; ++h) {
-        ok = wait(bars.p_full[h][i & 1], i) && wait(bars.v_full[i & 1], i) &&
-             (!PAIR || i < 2 || wait(bars.o_free[i & 1], i - 2));
-        if (!ok) break;
-        tc_fence_after();
-        issue_o(i, h);
-        oi[h] = i + 1;
-      }
-      ok = ok && next_s();
+    const std::integral_constant<int, 0> even{};
+    const std::integral_constant<int, 1> odd{};
+    bool ok = n == 0 || mbar_wait(smem_addr(&bars.q_full), 0, abort_flag);
+    if (n > 0 && ok && (ok = wait(bars.k_full[0], 0))) issue_s(even);
+    if (n > 1 && ok && (ok = wait(bars.k_full[1], 1))) issue_s(odd);
+    for (int i = 0; i < n && ok; i += 2) {
+      ok = tile(i, even);
+      if (ok && i + 1 < n) ok = tile(i + 1, odd);
     }
     if (!ok) {
       atomicOr(a.c.status, RTR_DEV_TIMEOUT);
