@@ -362,8 +362,8 @@ int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_de
  * weights enter the tensor cores as fp16 pairs (22 bits); sums are fp32.  A row
  * that sees a page whose V scale is outside [2^-48, 2^48], whose K scale is negative or
  * whose number is outside the cache is NaN.  The workspace must hold
- * rtr_kv_attention_workspace bytes, aligned to 16, and is free again when the call's
- * kernels ran: calls that may overlap need one each.  A table row wider than the
+ * rtr_kv_attention_workspace bytes (the same batch, dtype and heads), aligned to 16, and is
+ * free again when the call's kernels ran: calls that may overlap need one each.  A table row wider than the
  * sequences need costs idle blocks. */
 int rtr_kv_attention_workspace(const rtr_kv_cache* cache, const rtr_kv_batch* batch, int32_t dtype, int32_t heads,
                                int32_t device, int64_t* bytes);

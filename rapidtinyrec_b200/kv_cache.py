@@ -147,7 +147,9 @@ class KvCache8:
         ``head_dim ** -0.5`` unless given.  Returns ``out`` (a new tensor, or the contiguous one given),
         with ``return_lse`` also the float32 ``[rows, heads]`` log of the softmax's sum, by which
         results over several stretches of keys are merged.  Rows that belong to no sequence are not
-        written: a given ``out`` keeps them, new tensors are undefined there.
+        written: a given ``out`` keeps them, new tensors are undefined there.  The work is laid out
+        for sequences as long as a row of ``table``: where they are much shorter, pass a slice of it
+        (``table[:, :n]``).
         """
         return self._call.attention(self._at, self._index, q, table, lens, starts, causal,
                                     self._scale if scale is None else scale, return_lse, out)

@@ -526,6 +526,22 @@ def test_bad_v_scales_make_their_rows_nan():
 
 
 # -------------------------------------------- rows, pages and lengths that do not fit
+def test_what_a_table_holds_behind_a_length_is_not_used():
+    cache = filled(40, 2, 16, 64, seed=56)
+    lens = [20, 0, 33, 300]
+    table = tables(lens, 16, 40, seed=57, width=70)
+    need = torch.tensor([-(-t // 16) for t in lens], device='cuda')
+    wild = torch.where(torch.arange(70, device='cuda') < need[:, None], table, -(1 << 30)).to(torch.int32)
+    q = torch.randn(4, 4, 64, device='cuda')
+    out, _ = check_attention(cache, q, table, lens, [1] * 4, True)
+    assert torch.equal(cache.attention(q, wild, ints(lens)), out)
+    assert torch.equal(cache.attention(q, wild[:, :19], ints(lens)), cache.attention(q, table[:, :19], ints(lens)))
+    x = torch.randn(3, 2, 64, device='cuda')
+    cache.write(x, x, wild[[0, 2, 3]], ints([20, 33, 300]))
+    cache.read(3, wild[[0, 2, 3]], ints([20, 33, 300]))
+    cache.check()
+
+
 def test_rows_of_no_sequence_stay():
     cache = filled(8, 2, 16, 64, seed=29)
     table = tables([20, 30], 16, 8, seed=30)
