@@ -74,6 +74,8 @@ class KvCache8:
                 raise ValueError('scales must be float32 [pages, kv_heads], strided alike')
         if heads > 1 and k_scale.stride(1) != 1:
             raise ValueError('the scales of a page must be contiguous')
+        if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or status.device != k.device):
+            raise ValueError('status must be one int32 on the cache\'s device')
         if not (k.is_cuda and len({t.device for t in (k, v, k_scale, v_scale)}) == 1):
             raise ValueError('the cache must lie on one CUDA device')
         if status is None:

@@ -109,6 +109,15 @@ def test_python_refuses_wrong_caches():
             KvCache8(*bad)
 
 
+def test_python_refuses_wrong_status_words():
+    code = torch.zeros(3, 2, 16, 64, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    scale = torch.ones(3, 2)
+    for bad in (torch.zeros(1), torch.zeros(1, dtype=torch.int64), torch.zeros(2, dtype=torch.int32),
+                torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int32, device='meta')):
+        with pytest.raises(ValueError, match='status'):
+            KvCache8(code, code, scale, scale, bad)
+
+
 @pytest.mark.parametrize('page', [16, 32, 64, 128])
 def test_page_items_cover_every_page_once(page):
     """A sequence's items start at starts[b] // page + 2 b, without starts there are
