@@ -328,7 +328,9 @@ const char* kv_check(const rtr_kv_cache* c, const rtr_kv_batch* b) {
   if (c->head_dim != 64 && c->head_dim != 128) return "head_dim must be 64 or 128";
   if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return "page must be 16, 32, 64 or 128 tokens";
   if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 16384) return "the cache needs pages and 1 to 16384 KV heads";
-  if (c->head_stride < (int64_t)c->page * c->head_dim || c->page_stride < c->head_stride || c->scale_stride < 1)
+  const int64_t one = (int64_t)c->page * c->head_dim;  // codes of a page's head
+  if (c->head_stride < one || c->page_stride < one || c->scale_stride < c->kv_heads ||
+      (c->kv_heads > 1 && (c->page_stride - one) / (c->kv_heads - 1) < c->head_stride))
     return "cache strides overlap";
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | (uintptr_t)c->page_stride |
        (uintptr_t)c->head_stride) & 15)

@@ -49,6 +49,16 @@ def test_caches_that_are_refused(change, says):
         assert says in message()
 
 
+@pytest.mark.parametrize('change', [dict(page_stride=4 * 16 * 128 - 16), dict(scale_stride=3),
+                                    dict(head_stride=1 << 62, page_stride=(1 << 63) - 16)])
+def test_pages_that_share_memory_are_refused(change):
+    for call in (write, attention):
+        assert call(cache(**change), batch()) == _native.RTR_ERR_ARG
+        assert 'overlap' in message()
+    for fits in (dict(page_stride=7 * 16 * 128, head_stride=2 * 16 * 128), dict(kv_heads=1, page_stride=16 * 128)):
+        assert write(cache(**fits), batch(rows=0)) == _native.RTR_OK
+
+
 @pytest.mark.parametrize('change,says', [
     (dict(table=None), 'null table'), (dict(lens=None), 'null table'), (dict(seqs=-1), 'negative'),
     (dict(rows=-1), 'negative'), (dict(table_width=0), 'table rows'), (dict(table_stride=7), 'table rows'),
