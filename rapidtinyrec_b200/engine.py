@@ -257,6 +257,10 @@ class BeamEngine:
         """A request of a user whose prefix was kept: no prefill.  ``in_place``: decode attention
         over the 8-bit pages; otherwise the pages are first read back into the arena."""
         import torch
+        want = torch.float32 if self.cfg.dtype == 'fp32' else torch.bfloat16
+        if kept.store.device.index != self.device or kept.hidden.dtype != want or \
+                kept.hidden.numel() != self.cfg.hidden:
+            raise ValueError('the prefix was kept on another device, or by an engine of another model or type')
         torch.cuda.synchronize(self.device)
         self._check(self.lib.rtr_prefill_kept(self.handle, kept.store._at, kept.table.data_ptr(), kept.table.numel(),
                                               kept.ids.ctypes.data, len(kept.ids), kept.hidden.data_ptr(),

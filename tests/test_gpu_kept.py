@@ -158,3 +158,22 @@ def test_calls_out_of_order_and_what_does_not_fit(tiny, engine):
     assert engine.generate_kept(kept) == record
     assert engine.generate(ids) == plain
     store.check()
+
+
+def test_prefixes_of_another_engine(tiny, engine):
+    """Another engine of the model and type takes a kept prefix; one of another type has a hidden
+    state of another size and refuses it."""
+    ids = prompts(tiny)[1]
+    store = engine.prefix_store(8)
+    record, kept = engine.generate_and_keep(ids, store, range(pages_for(ids, 64)))
+    again = engine.generate_kept(kept)
+    e = make_engine(tiny)
+    assert e.generate_kept(kept) == again
+    e.close()
+    e = make_engine(tiny, dtype='bf16')
+    with pytest.raises(ValueError, match='another'):
+        e.generate_kept(kept)
+    e.close()
+    with pytest.raises(ValueError, match='another'):
+        engine.generate_kept(kept._replace(hidden=kept.hidden[:-1]))
+    assert engine.generate_kept(kept) == again
