@@ -70,6 +70,8 @@ class KeptPrefix(NamedTuple):
 
 
 class BeamEngine:
+    _prefilled = None  # the prompt of the last prefill()
+
     def __init__(self, cfg: ModelConfig, weights, tables, max_prefix: int, device: int = 0,
                  num_beams: int = NUM_BEAMS, max_users: int = 1):
         import torch
@@ -210,6 +212,7 @@ class BeamEngine:
     def prefill(self, prompt_ids):
         ids = self._ids(prompt_ids)
         self._check(self.lib.rtr_prefill(self.handle, ids.ctypes.data, len(ids), 0))
+        self._prefilled = ids.copy()
 
     def decode_step(self, t):
         self._check(self.lib.rtr_decode_step(self.handle, t))
@@ -230,7 +233,9 @@ class BeamEngine:
         the store's ``pages`` (page numbers, as many as the prompt needs)."""
         import torch
         dev = f'cuda:{self.device}'
-        ids = self._ids(prompt_ids)
+        ids = self._ids(prompt_ids).copy()
+        if self._prefilled is not None and not np.array_equal(ids, self._prefilled):
+            raise ValueError('the prompt is not the one prefilled last')
         pages = [int(p) for p in pages]
         if len(set(pages)) < len(pages) or any(not 0 <= p < store.pages for p in pages):
             raise ValueError('pages must be different page numbers of the store')

@@ -177,3 +177,17 @@ def test_prefixes_of_another_engine(tiny, engine):
     with pytest.raises(ValueError, match='another'):
         engine.generate_kept(kept._replace(hidden=kept.hidden[:-1]))
     assert engine.generate_kept(kept) == again
+
+
+def test_a_prompt_that_was_not_prefilled_is_not_kept(tiny, engine):
+    ids = list(prompts(tiny)[0])
+    store = engine.prefix_store(8)
+    engine.prefill(ids)
+    for wrong in (ids[:-1], ids + ids[-1:], ids[:-1] + [ids[-1] + 1]):
+        with pytest.raises(ValueError, match='prefilled'):
+            engine.keep_prefix(wrong, store, range(pages_for(wrong, 64)))
+    given = np.array(ids, dtype=np.int32)
+    kept = engine.keep_prefix(given, store, range(pages_for(ids, 64)))
+    record = engine.generate_kept(kept)
+    given[:] = 0  # the kept prompt is a copy
+    assert engine.generate_kept(kept) == record
