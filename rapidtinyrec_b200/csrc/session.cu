@@ -1172,6 +1172,8 @@ int rtr_prefill_kept(rtr_session* s, const rtr_kv_cache* cache, const int32_t* t
   if (!in_place && (s->tc_attn || s->tc_attn_bf16))
     return fail(s, RTR_ERR_STATE, "the tensor-core decode attention reads copies of the arena: only in place");
   CUDA_TRY(s, cudaSetDevice(s->device));
+  s->steps_done = -1;  // whatever fails from here on, no decode step follows the former request
+  s->kept.on = s->prefix_in_arena = false;  // a kept prefix is not kept again: its codes are in the cache already
   const auto& c = s->cfg;
   const int dtype = s->bf16 ? RTR_DTYPE_BF16 : RTR_DTYPE_F32;
   const int64_t D = c.head_dim, cap = c.max_prefix, kvd = (int64_t)c.kv_heads * D, size = s->bf16 ? 2 : 4;
@@ -1223,7 +1225,6 @@ int rtr_prefill_kept(rtr_session* s, const rtr_kv_cache* cache, const int32_t* t
   s->launches += 2 + kTailKernels;  // beam_reset, the LM head, step tail
   s->steps_done = 0;
   s->kept.on = in_place != 0;
-  s->prefix_in_arena = false;  // a kept prefix is not kept again: its codes are in the cache already
   return RTR_OK;
 }
 

@@ -191,3 +191,23 @@ def test_a_prompt_that_was_not_prefilled_is_not_kept(tiny, engine):
     record = engine.generate_kept(kept)
     given[:] = 0  # the kept prompt is a copy
     assert engine.generate_kept(kept) == record
+
+
+def test_a_refused_kept_prefix_ends_the_former_request(tiny, engine):
+    from rapidtinyrec_b200._native import RTR_ERR_ARG, RTR_ERR_STATE, NativeError
+    from rapidtinyrec_b200.kv_cache import KvCache8
+    ids = prompts(tiny)[2]
+    store = engine.prefix_store(8)
+    record, kept = engine.generate_and_keep(ids, store, range(pages_for(ids, 64)))
+    odd = KvCache8(store.k, store.v, store.k_scale, store.v_scale)
+    odd._c.page_stride += 8  # refused on the host, after the session began the request
+    for in_place in (True, False):
+        engine.prefill(ids)
+        with pytest.raises(NativeError, match='16 bytes') as e:
+            engine.generate_kept(kept._replace(store=odd), in_place=in_place)
+        assert e.value.code == RTR_ERR_ARG
+        with pytest.raises(NativeError) as e:
+            engine.decode_step(1)
+        assert e.value.code == RTR_ERR_STATE
+    assert engine.generate(ids) == record
+    store.check()
