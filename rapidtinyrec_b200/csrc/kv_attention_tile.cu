@@ -25,15 +25,10 @@
 #include <type_traits>
 
 #include "engine.h"
-#include "kv_attention.cuh"
+#include "kv_attention_tile.cuh"
 #include "kv_host.h"
-#include "tcgen05.cuh"
 
 namespace rtr {
-
-constexpr int KT_ROW_THREADS = 256;
-constexpr int KT_SEGS = KT_MAX_CHUNK / 16;
-constexpr float KT_SLACK = 8.0f;  // log2 by which a maximum may be exceeded (bf16 rows)
 
 template <int D, bool PAIR> struct KtCfg {
   // code warps: eight keep up with one product a score; beside fp32 rows, whose threads
@@ -69,68 +64,6 @@ struct KtBars {
 };
 static_assert(sizeof(KtBars) <= 256, "barriers fit their part of shared memory");
 
-// D[tmem] (+)= A . B[smem]^T, kind::f16 (both fp16), A in shared or tensor memory;
-// descriptors as low words and their common high word.
-RTR_DEVICE void mma_f16_ss_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
-}
-RTR_DEVICE void mma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
-}
-RTR_DEVICE void tmem_st_words(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-RTR_DEVICE void tmem_st_words(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-RTR_DEVICE void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
-RTR_DEVICE void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
-}
-// Two fp32 lanes of one instruction.
-RTR_DEVICE uint64_t f2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-RTR_DEVICE uint64_t f2(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
-RTR_DEVICE float2 f2_parts(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-RTR_DEVICE uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-RTR_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 RTR_DEVICE void st_cluster_f4(uint32_t addr, float4 v) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
@@ -139,7 +72,6 @@ RTR_DEVICE void st_cluster_f2(uint32_t addr, float2 v) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
 }
 RTR_DEVICE void row_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-RTR_DEVICE uint32_t sw_at(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREADS, 1) kv_attn_tile_kernel(const KvAttn a) {
@@ -241,24 +173,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     row_out[tid] = (first + token) * a.heads + kvh * a.group + head;
     row_lim[tid] = a.causal ? max(0, len - count + token + 1) : len;
   }
-  // pages and scales of the stretch's 16-key segments (a page is a multiple of 16)
-  for (int s = tid - KT_ROW_THREADS; s < segs; s += C::THREADS - KT_ROW_THREADS) {
-    if (s < 0) break;
-    const int key = c0 + 16 * s;
-    const int page = kv_page(a.c, a.b, seq, key >> a.c.page_shift);
-    int64_t at = kvh * a.c.head_stride;
-    float ks, lv, iv = 0.f;
-    ks = lv = __int_as_float(0x7fffffff);  // a page that is not there makes the rows NaN, whatever codes are read
-    if (page >= 0) {
-      at += page * a.c.page_stride + (int64_t)(key & ((1 << a.c.page_shift) - 1)) * D;
-      ks = kv_k_scale(a.c.k_scale[page * a.c.scale_stride + kvh]);
-      kv_v_scale(a.c.v_scale[page * a.c.scale_stride + kvh], lv, iv);
-    }
-    seg_at[s] = at;
-    seg_k[s] = ks;
-    seg_lv[s] = lv;
-    seg_iv[s] = iv;
-  }
+  if (tid >= KT_ROW_THREADS)
+    kt_segments(a, seq, kvh, c0, segs, tid - KT_ROW_THREADS, C::THREADS - KT_ROW_THREADS, seg_at, seg_k, seg_lv, seg_iv);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -591,100 +507,26 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     if (half == 0) reinterpret_cast<float2*>(red)[r] = make_float2(m, lt);
   } else if (warp < 8 + C::CODE_WARPS) {
     // ------------------------------------------------------------ codes
-    const int cw = warp - 8;
-    constexpr int KP = KT_KEYS * D / 16 / C::CODE_THREADS;  // 16-byte pieces of K a thread: 8 or 4
-    constexpr int LPK = D / 16;                              // threads of a key
-    constexpr int VO = KT_KEYS / 8 * (D / 4) / C::CODE_THREADS;  // (8 keys x 4 dims) blocks of V a thread: 4 or 2
-    // Of K, eight consecutive lanes take four pieces of one panel of two neighbouring keys:
-    // their stores then hit all banks.
-    const int piece = D == 128 ? (lane & 3) + 4 * (lane >> 3 & 1) : lane & 3;
-    const int key_of = cw * (32 / LPK) + (D == 128 ? 2 * (lane >> 4) + (lane >> 2 & 1) : lane >> 2);
-    const int dl = lane % (D / 4);
-    uint4 kr[KP];
-    uint32_t vr[VO][8];
-    // Loads need no conditions: a segment lies in one page as a whole, and what is read of keys
-    // behind the last (or of the last segment again) is masked, NaN codes are taken out below.
-    const auto load_k = [&](int i) {
-#pragma unroll
-      for (int p = 0; p < KP; ++p) {
-        const int rel = i * KT_KEYS + p * (C::CODE_THREADS / LPK) + key_of;
-        kr[p] = __ldg(reinterpret_cast<const uint4*>(a.c.k + seg_at[min(rel >> 4, segs - 1)] + (rel & 15) * D + 16 * piece));
-      }
-    };
-    const auto octet = [&](int v) { return (v * C::CODE_WARPS + cw) * (32 / (D / 4)) + lane / (D / 4); };
-    const auto load_v = [&](int i) {
-#pragma unroll
-      for (int v = 0; v < VO; ++v) {
-        const int rel = i * KT_KEYS + 8 * octet(v);
-        const uint8_t* p = a.c.v + seg_at[min(rel >> 4, segs - 1)] + (rel & 8) * D + 4 * dl;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) vr[v][k] = __ldg(reinterpret_cast<const uint32_t*>(p + k * D));
-      }
-    };
+    KtCodes<D, C::CODE_WARPS> codes(a.c, seg_at, segs, warp - 8, lane);
     if (n > 0) {
-      load_k(0);
-      load_v(0);
+      codes.load_k(0);
+      codes.load_v(0);
     }
     for (int i = 0; i < n; ++i) {
       // S and O of tile i - 2 are done with the buffers
       if (i >= 2 && !mbar_wait(smem_addr(&bars.s_full[i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
-      uint8_t* kd = smem + C::K_OFF + (i & 1) * C::K_BYTES;
-#pragma unroll
-      for (int p = 0; p < KP; ++p) {
-        const int key = p * (C::CODE_THREADS / LPK) + key_of;
-        const uint32_t w[4] = {kr[p].x, kr[p].y, kr[p].z, kr[p].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          h[2 * j] = e4m3x2_to_f16x2((uint16_t)w[j]);
-          h[2 * j + 1] = e4m3x2_to_f16x2((uint16_t)(w[j] >> 16));
-        }
-        uint8_t* row = kd + (piece >> 2) * KT_KEYS * 128;
-        const int un = 2 * (piece & 3);
-        *reinterpret_cast<uint4*>(row + sw_at(key, un)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(row + sw_at(key, un + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
-      }
+      codes.put_k(smem + C::K_OFF + (i & 1) * C::K_BYTES);
       fence_proxy_async();
       mbar_arrive(smem_addr(&bars.k_full[i & 1]));
-      if (i + 1 < n) load_k(i + 1);
+      if (i + 1 < n) codes.load_k(i + 1);
       if (i >= 2 && !mbar_wait(smem_addr(&bars.o_full[0][i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
       if (!PAIR && i >= 2 && !mbar_wait(smem_addr(&bars.o_full[1][i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
-      if (c0 + (i + 1) * KT_KEYS > kmin) {
-        // not every row sees every key of the tile: 0 * NaN must not reach the others
-        uint32_t bad = 0;
-#pragma unroll
-        for (int v = 0; v < VO; ++v)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t nb = nan_bytes(vr[v][k]);
-            bad |= nb;
-            vr[v][k] &= ~((nb >> 7) * 0xffu);
-          }
-        if (bad) bars.nans = 1;
-      }
-      uint8_t* vd = smem + C::V_OFF + (i & 1) * C::V_BYTES;
-#pragma unroll
-      for (int v = 0; v < VO; ++v) {
-        const int oc = octet(v);
-        uint32_t h[4][4];  // [dim t][keys 2 j, 2 j + 1]
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t x = __byte_perm(vr[v][2 * j], vr[v][2 * j + 1], 0x5140);
-          const uint32_t y = __byte_perm(vr[v][2 * j], vr[v][2 * j + 1], 0x7362);
-          h[0][j] = e4m3x2_to_f16x2((uint16_t)x);
-          h[1][j] = e4m3x2_to_f16x2((uint16_t)(x >> 16));
-          h[2][j] = e4m3x2_to_f16x2((uint16_t)y);
-          h[3][j] = e4m3x2_to_f16x2((uint16_t)(y >> 16));
-        }
-        // dimension 4 dl + t becomes row t (D / 4) + dl: consecutive lanes, consecutive rows
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          *reinterpret_cast<uint4*>(vd + (oc >> 3) * D * 128 + sw_at(t * (D / 4) + dl, oc & 7)) =
-              make_uint4(h[t][0], h[t][1], h[t][2], h[t][3]);
-      }
+      // not every row sees every key of the tile: 0 * NaN must not reach the others
+      if (c0 + (i + 1) * KT_KEYS > kmin && codes.drop_nans()) bars.nans = 1;
+      codes.put_v(smem + C::V_OFF + (i & 1) * C::V_BYTES);
       fence_proxy_async();
       mbar_arrive(smem_addr(&bars.v_full[i & 1]));
-      if (i + 1 < n) load_v(i + 1);
+      if (i + 1 < n) codes.load_v(i + 1);
     }
   } else if (lane == 0) {
     // --------------------------------------------------------- products
