@@ -71,7 +71,6 @@ RTR_DEVICE void st_cluster_f4(uint32_t addr, float4 v) {
 RTR_DEVICE void st_cluster_f2(uint32_t addr, float2 v) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
 }
-RTR_DEVICE void row_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREADS, 1) kv_attn_tile_kernel(const KvAttn a) {
@@ -92,7 +91,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
   KtBars& bars = *reinterpret_cast<KtBars*>(smem + C::BAR_OFF);
   volatile int* abort_flag = &bars.abort_flag;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const int kvh = blockIdx.y, split = blockIdx.z;
   pdl_launch_dependents();
   pdl_wait();
@@ -178,7 +177,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars.tmem;
+  const uint32_t tmem = uniform(bars.tmem);
   constexpr uint32_t S_COLS = KT_KEYS, O_AT = 2 * S_COLS;
 
   if (warp < 8) {
@@ -528,9 +527,10 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       mbar_arrive(smem_addr(&bars.v_full[i & 1]));
       if (i + 1 < n) codes.load_v(i + 1);
     }
-  } else if (lane == 0) {
+  } else {
     // --------------------------------------------------------- products
-    // One thread's instructions stand between a tile's weights and the next scores: buffers are
+    const uint32_t leader = elect_leader();
+    // The warp's instructions stand between a tile's weights and the next scores: buffers are
     // compile-time numbers and descriptors their low words from a common base, so that a
     // product costs little more than its issue.
     constexpr uint32_t id_s = idesc_f16(KT_ROWS, KT_KEYS), id_o = idesc_f16(KT_ROWS, D);
@@ -548,9 +548,9 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         for (int p = 0; p < C::PANELS; ++p)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_f16_ss_lo(tmem + B * S_COLS, lo + (C::Q_OFF + pl * C::Q_PLANE + p * KT_ROWS * 128) / 16 + 2 * k,
+            mma_f16_ss_lo(leader, tmem + B * S_COLS, lo + (C::Q_OFF + pl * C::Q_PLANE + p * KT_ROWS * 128) / 16 + 2 * k,
                           lo + (C::K_OFF + B * C::K_BYTES + p * KT_KEYS * 128) / 16 + 2 * k, hi, id_s, pl || p || k);
-      mma_commit(smem_addr(&bars.s_full[B]));
+      if (leader) mma_commit(smem_addr(&bars.s_full[B]));
       ++si;
     };
     // fp32 rows: the whole tile's product, alone in its buffer; bf16 rows: that of one half
@@ -564,13 +564,13 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         const uint32_t v = lo + (C::V_OFF + B * C::V_BYTES + (ks >> 2) * D * 128) / 16 + 2 * (ks & 3);
         if constexpr (PAIR) {
           const uint32_t p = tmem + B * S_COLS + 16 * k;  // the weights, then their low parts, lie over the scores
-          mma_f16_ts_lo(tmem + O_AT + B * 128, p, v, hi, id_o, k > 0);
-          mma_f16_ts_lo(tmem + O_AT + B * 128, p + 8, v, hi, id_o, true);
+          mma_f16_ts_lo(leader, tmem + O_AT + B * 128, p, v, hi, id_o, k > 0);
+          mma_f16_ts_lo(leader, tmem + O_AT + B * 128, p + 8, v, hi, id_o, true);
         } else {
-          mma_f16_ts_lo(tmem + O_AT + H * 128, tmem + B * S_COLS + 64 * H + 8 * k, v, hi, id_o, k > 0 || add);
+          mma_f16_ts_lo(leader, tmem + O_AT + H * 128, tmem + B * S_COLS + 64 * H + 8 * k, v, hi, id_o, k > 0 || add);
         }
       }
-      mma_commit(smem_addr(&bars.o_full[H][B]));
+      if (leader) mma_commit(smem_addr(&bars.o_full[H][B]));
       ++oi[H];
     };
     const auto tile = [&](int i, auto buffer) {
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       if (ok && i + 1 < n) ok = tile(i + 1, odd);
     }
     if (!ok) {
-      atomicOr(a.c.status, RTR_DEV_TIMEOUT);
+      if (leader) atomicOr(a.c.status, RTR_DEV_TIMEOUT);
       for (int i = si > 2 ? si - 2 : 0; i < si; ++i) mbar_drain(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1);
       for (int h = 0; h < HALVES; ++h)
         for (int i = oi[h] > 2 ? oi[h] - 2 : 0; i < oi[h]; ++i)

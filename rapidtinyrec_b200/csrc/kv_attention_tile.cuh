@@ -12,24 +12,34 @@ constexpr int KT_ROW_THREADS = 256;
 constexpr int KT_SEGS = KT_MAX_CHUNK / 16;
 constexpr float KT_SLACK = 8.0f;  // log2 by which a maximum may be exceeded (bf16 rows)
 
+// The products' warp runs as a whole, and one of its threads (the leader) issues: where the
+// compiler sees that a warp does not diverge, descriptors and addresses stay in uniform
+// registers, which the instructions take; one thread in a branch of its own moved each of
+// them there first (a product of 16 keys took 70 cycles to issue, now 20 - 30).
+RTR_DEVICE int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+RTR_DEVICE uint32_t elect_leader() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
 // D[tmem] (+)= A . B[smem]^T, kind::f16 (both fp16), A in shared or tensor memory;
 // descriptors as low words and their common high word.
-RTR_DEVICE void mma_f16_ss_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
+RTR_DEVICE void mma_f16_ss_lo(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
       "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add)
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add), "r"(leader)
       : "memory");
 }
-RTR_DEVICE void mma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
+RTR_DEVICE void mma_f16_ts_lo(uint32_t leader, uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
       "mov.b64 b, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add)
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)add), "r"(leader)
       : "memory");
 }
 RTR_DEVICE void tmem_st_words(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -74,6 +84,8 @@ RTR_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The row threads of a block.
+RTR_DEVICE void row_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // Byte of a 16-byte unit of a 128-byte row in a 128B-swizzled operand.
 RTR_DEVICE uint32_t sw_at(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
 
