@@ -538,11 +538,12 @@ __global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch 
 
 // ------------------------------------------------------------------- host
 struct KvAttnPlan {
-  bool tiles;  // 128-row tiles (kv_attention_tile.cu), else KA_ROWS rows a block
+  int tile_rows;  // 128 (kv_attention_tile.cu), 256 (kv_attention_wide.cu) or 0: 8 rows a block
   int64_t items;
   int per_seq, chunk, splits;
   bool cluster;
-  int64_t workspace;  // bytes
+  int64_t whole, tails;  // 256-row tiles: items that are one block, items of `splits` blocks
+  int64_t workspace;     // bytes
 };
 
 static int64_t kv_attn_items(const rtr_kv_batch* b, int group, int shift, int& per_seq) {
@@ -573,21 +574,21 @@ static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   p.chunk = (int)chunk;
   p.splits = (int)((most + chunk - 1) / chunk);
   p.cluster = p.splits > 1 && p.splits <= KV_CLUSTER;
-  // measured: 8 rows x 18,500 (fp32 16,000) keys a us at head_dim 128, 55,000 (48,000) at 64
-  const int64_t rate = c->head_dim == 128 ? (f32 ? 16000 : 18500) : f32 ? 48000 : 55000;
+  // measured: 8 rows x 18,500 (fp32 16,000) keys a us at head_dim 128, 45,000 (35,000) at 64
+  const int64_t rate = c->head_dim == 128 ? (f32 ? 16000 : 18500) : f32 ? 35000 : 45000;
   ns = 5000 + base * most * 1000 / rate + (p.splits > 1 ? 3000 : 0);
   return p;
 }
 
 // What a block of 128 rows needs for 128 keys.
 static int kv_tile_ns(const rtr_kv_cache* c, bool f32) {
-  return c->head_dim == 128 ? (f32 ? 1700 : 1400) : f32 ? 1350 : 1150;
+  return c->head_dim == 128 ? (f32 ? 1700 : 1100) : f32 ? 1350 : 1150;
 }
 
 // Tiles of 128 rows.
 static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, int group, bool f32, int sms, int64_t& ns) {
   KvAttnPlan p = {};
-  p.tiles = true;
+  p.tile_rows = KT_ROWS;
   p.items = kv_attn_items(b, group, 7, p.per_seq);
   const int64_t base = p.items * c->kv_heads;
   const int64_t all = ((int64_t)b->table_width * c->page + KT_KEYS - 1) / KT_KEYS;
@@ -597,8 +598,8 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
   int64_t best = INT64_MAX;
   for (int64_t s = (all * KT_KEYS + KT_MAX_CHUNK - 1) / KT_MAX_CHUNK, end = s + 63; s <= end && s <= all; ++s) {
     const int64_t per = (all + s - 1) / s, splits = (all + per - 1) / per;
-    const int64_t wave = splits >= 3 && splits <= 8 ? sms * 6 / 7 : sms;
-    const int64_t cost = (base * splits + wave - 1) / wave * (per + 6) + (splits == 1 ? 0 : splits <= 8 ? 3 : 8);
+    const int64_t wave = splits >= 3 && splits <= KV_CLUSTER ? sms * 6 / 7 : sms;
+    const int64_t cost = (base * splits + wave - 1) / wave * (per + 6) + (splits == 1 ? 0 : splits <= KV_CLUSTER ? 3 : 8);
     if (cost < best) {
       best = cost;
       p.chunk = (int)(per * KT_KEYS);
@@ -610,18 +611,58 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
   return p;
 }
 
+// What a block of 256 rows needs for 128 keys, and for its start and end in these units.
+constexpr int KW_TILE_NS = 1920, KW_BLOCK = 8;
+
+// Tiles of 256 rows.  Items that fill all SMs are blocks of their own; what is left is split
+// along its keys, so that the last wave is a short one, and joined through memory.
+static KvAttnPlan kv_plan_wide(const rtr_kv_cache* c, const rtr_kv_batch* b, int group, int sms, int64_t& ns) {
+  KvAttnPlan p = {};
+  p.tile_rows = KW_ROWS;
+  p.items = kv_attn_items(b, group, 8, p.per_seq);
+  const int64_t base = p.items * c->kv_heads;
+  const int64_t all = ((int64_t)b->table_width * c->page + KT_KEYS - 1) / KT_KEYS, most = KW_MAX_CHUNK / KT_KEYS;
+  const int64_t waves = all > most ? 0 : base / sms;
+  int64_t best = INT64_MAX;
+  for (int64_t s = (all + most - 1) / most, end = s + 63; s <= end && s <= all; ++s) {
+    const int64_t per = (all + s - 1) / s, splits = (all + per - 1) / per, left = base - waves * sms;
+    const int64_t cost = waves * (all + KW_BLOCK) + (left * splits + sms - 1) / sms * (per + KW_BLOCK) + (splits == 1 ? 0 : 6);
+    if (cost < best) {
+      best = cost;
+      p.whole = splits == 1 ? base : waves * sms;
+      p.chunk = (int)(per * KT_KEYS);
+      p.splits = (int)splits;
+    }
+  }
+  p.tails = base - p.whole;
+  ns = best * KW_TILE_NS;
+  return p;
+}
+
 // The kernel whose expected time is less.  Measured, 28 / 4 heads of 128, bf16, tiles of
-// 128 against tiles of 8 rows: 8 sequences of 1,200 keys with 2 new tokens 13.6 : 11.9 us,
-// 4 14.1 : 15.1, 16 15.9 : 45; one of 300 keys with 64 14 : 8.4 us, with 256 13 : 20.
+// 128 against tiles of 8 rows: 8 sequences of 1,200 keys with 2 new tokens 12.7 : 11.0 us,
+// 4 12.9 : 12.7, 16 14.7 : 37.7; one of 300 keys with 64 11.3 : 8.4 us, with 256 11.3 : 15.6.
+// Tiles of 256 against 128: 32 sequences of 4,096 keys with 64 163 : 190 us, 4 of 512 keys with
+// 256 21.5 : 24.1, one of 4,096 with 1,024 80 : 86, with 512 57 : 47.
 static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, bool f32, int sms) {
   const int group = heads / c->kv_heads;
   int64_t rows_ns, tiles_ns;
   KvAttnPlan p = kv_plan_rows(c, b, group, f32, sms, rows_ns);
   if (rows_ns > 7 * kv_tile_ns(c, f32)) {  // what one key tile costs at least
     const KvAttnPlan tiles = kv_plan_tiles(c, b, group, f32, sms, tiles_ns);
-    if (tiles_ns < rows_ns) p = tiles;
+    if (tiles_ns < rows_ns) {
+      p = tiles;
+      if (!f32 && c->head_dim == 128) {
+        int64_t wide_ns;
+        const KvAttnPlan wide = kv_plan_wide(c, b, group, sms, wide_ns);
+        if (wide_ns < tiles_ns && wide.whole + wide.tails * wide.splits <= INT32_MAX / KW_ROWS) p = wide;
+      }
+    }
   }
-  p.workspace = p.splits > 1 && !p.cluster ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
+  if (p.tile_rows == KW_ROWS)
+    p.workspace = p.tails * KW_ROWS * (p.splits * (int64_t)(c->head_dim * 4 + 8) + 4);
+  else
+    p.workspace = p.splits > 1 && !p.cluster ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
   return p;
 }
 
@@ -635,7 +676,13 @@ static const char* kv_attn_check(const rtr_kv_cache* c, const rtr_kv_batch* b, i
 
 template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, const KvAttnPlan& p, int device, cudaStream_t st) {
   cudaError_t e;
-  if (p.tiles) {
+  if (p.tile_rows == KW_ROWS) {
+    const int64_t rows = p.tails * KW_ROWS * p.splits;
+    KvAttn w = a;
+    w.ml = reinterpret_cast<float2*>(a.part + rows * D);
+    return kv_attn_wide(w, KwShare{(int)p.whole, (int)p.tails, reinterpret_cast<int*>(w.ml + rows)}, device, st);
+  }
+  if (p.tile_rows) {
     e = kv_attn_tile(a, p.items, std::is_same<T, float>::value, device, st);
   } else {
     static std::atomic<uint64_t> done;

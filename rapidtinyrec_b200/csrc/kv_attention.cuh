@@ -113,4 +113,15 @@ constexpr int KT_ROWS = 128, KT_KEYS = 128;
 constexpr int KT_MAX_CHUNK = 8192;  // keys of a block
 cudaError_t kv_attn_tile(const KvAttn& a, int64_t items, bool f32, int device, cudaStream_t st);
 
+// Two such tiles a block, bf16 rows (kv_attention_wide.cu).  Of the items (256 rows and a KV
+// head) the first `whole` have a block each, the `tails` others a.splits blocks, each a
+// stretch of a.chunk keys: a.part and a.ml are [tails][256][splits].
+constexpr int KW_ROWS = 2 * KT_ROWS;
+constexpr int KW_MAX_CHUNK = 16384;  // keys of a block
+struct KwShare {
+  int whole, tails;
+  int* row;  // [tails][256]: the (row, head) of out, -1 for none
+};
+cudaError_t kv_attn_wide(const KvAttn& a, const KwShare& w, int device, cudaStream_t st);
+
 }  // namespace rtr

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   const bool whole = kv_len_fits(a.c, a.b, len, 0);
   if (!whole) len = 0;  // the sequence's rows become NaN
   const auto limit = [&](int row) { return a.causal && count > 1 ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
-  const int kmin = limit(r0), kmax = limit(r0 + KT_ROWS - 1), c1 = min(kmax, c0 + a.chunk);
+  const int kmin = limit(r0), kmax = limit(r0 + KT_ROWS - 1), c1 = c0 + min(kmax - c0, a.chunk);
   if (c1 <= c0 && split > 0 && !a.cluster) {  // a stretch behind the last key (the first one reports rows that see nothing)
     if (tid < rows) {
       const int token = (r0 + tid) / a.group;

@@ -17,6 +17,18 @@ constexpr float KT_SLACK = 8.0f;  // log2 by which a maximum may be exceeded (bf
 // registers, which the instructions take; one thread in a branch of its own moved each of
 // them there first (a product of 16 keys took 70 cycles to issue, now 20 - 30).
 RTR_DEVICE int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// Whether a barrier's phase is complete, without waiting.
+RTR_DEVICE bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 RTR_DEVICE uint32_t elect_leader() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));

@@ -16,6 +16,7 @@ for equality.  Attention's tolerance counts its roundings, per output value:
   most n / 16 + 8 steps, all relative to the largest |v|;
 * the output's own rounding is half a step of its type.
 """
+import ctypes
 import math
 
 import pytest
@@ -498,6 +499,140 @@ def test_tiles_keep_nan_with_the_rows_that_see_it(dtype):
         cache.check()
     behind = (1000 // page - 1) * page - (1000 - 700)  # the first row that sees it
     assert out[behind:].isnan().all() and not out[131:behind].isnan().any()
+
+
+# ------------------------------------------------------------- 256-row tiles
+# bf16, head_dim 128: enough rows to fill the GPU with blocks of 256, some of them split along
+# the keys and joined (more than 148 blocks or more than 16,384 keys).
+def tails(cache, q, table, lens, starts=None):
+    """Whether the call is one of 256-row tiles with split ones: 4 bytes for each of their rows beside
+    the sums' 8 + 4 * head_dim."""
+    from rapidtinyrec_b200 import _native
+    b = _native.KvBatchC(table.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(), table.shape[1],
+                         table.shape[1], table.shape[0], q.shape[0])
+    need = ctypes.c_int64()
+    assert _native.load().rtr_kv_attention_workspace(ctypes.byref(cache._c), ctypes.byref(b), _native.RTR_DTYPE_BF16,
+                                                     q.shape[1], 0, ctypes.byref(need)) == 0
+    return need.value % 520 != 0
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('page', [16, 128])
+def test_tiles_of_256_rows(causal, page):
+    """Ragged sequences as in the test of 128 rows: whole blocks, and split ones at the end."""
+    counts = [500, 0, 1, 300, 129, 400]
+    lens = [1300, 900, 0, 120, 9000, 1500]
+    pages = sum(-(-t // page) for t in lens) + 1
+    cache = filled(pages, 4, page, 128, seed=page + 60)
+    table = tables(lens, page, pages, seed=61)
+    g = torch.Generator().manual_seed(62)
+    q = (2 * torch.randn(sum(counts), 28, 128, generator=g)).bfloat16().cuda()
+    assert tails(cache, q, table, ints(lens), cuts(counts))
+    check_attention(cache, q, table, lens, counts, causal, starts=cuts(counts))
+    # rows in front of and behind the sequences', in a tensor of NaN
+    starts = cuts(counts, first=3)
+    wide = torch.cat((q[:3], q, q[:5]))
+    out = torch.full_like(wide, NAN)
+    cache.attention(wide, table, ints(lens), starts=starts, causal=causal, out=out)
+    assert out[:3].isnan().all() and out[-5:].isnan().all() and not out[3:-5].isnan().any()
+
+
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('rows', [1300, 1290])
+def test_tiles_of_256_rows_without_starts(causal, rows):
+    """Whole blocks only; the last block has both of its tiles, or one."""
+    cache = filled(40, 4, 64, 128, seed=63)
+    table = tables([2000], 64, 40, seed=64)
+    q = (2 * torch.randn(rows, 28, 128, generator=torch.Generator().manual_seed(65))).bfloat16().cuda()
+    for scale in (None, 0.0, -0.05):
+        out, _ = check_attention(cache, q, table, [2000], [rows], causal, **({} if scale is None else dict(scale=scale)))
+    # again, on another stream and from a captured graph
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        stream.wait_stream(torch.cuda.default_stream())
+        assert torch.equal(cache.attention(q, table, ints([2000]), causal=causal, scale=-0.05), out)
+    torch.cuda.synchronize()
+    lens, given = ints([2000]), torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attention(q, table, lens, causal=causal, scale=-0.05, out=given)
+    for _ in range(2):
+        given.fill_(NAN)
+        graph.replay()
+        assert torch.equal(given, out)
+
+
+@pytest.mark.parametrize('size', [1e-30, 1.0, 30.0])
+def test_tiles_of_256_rows_over_many_keys(size):
+    """More keys than one block takes; scales 2^60 apart and no powers of two, tiny and huge
+    queries; rows that see nothing of the last stretches; a row that sees a single key."""
+    cache = filled(140, 4, 128, 128, seed=66)
+    g = torch.Generator().manual_seed(67)
+    cache.v_scale.copy_(torch.exp2(torch.randint(-30, 30, (140, 4), generator=g).float()))
+    cache.k_scale.copy_(torch.rand(140, 4, generator=g) * 0.01 + 0.001)
+    table = tables([17000], 128, 140, seed=68)
+    q = (torch.randn(400, 28, 128, generator=g) * size).bfloat16().cuda()
+    assert tails(cache, q, table, ints([17000]))
+    check_attention(cache, q, table, [17000], [400], True)
+    if size == 1.0:
+        for length in (400, 399, 1, 0, 129):  # of a table row for many more
+            check_attention(cache, q, table, [length], [400], True)
+            check_attention(cache, q, table, [length], [400], False)
+
+
+@pytest.mark.parametrize('n,tokens,heads,kv,page', [(1300, 2000, 28, 4, 32), (1000, 17000, 12, 2, 128)])
+def test_tiles_of_256_rows_keep_nan_with_the_rows_that_see_it(n, tokens, heads, kv, page):
+    """Rows that do not see a NaN stay as they are up to when their maximum was taken: every
+    fp16 weight may round otherwise, 2^-11 of it each time (V is at most 448 * 2^-6 = 7), then the
+    output's bf16."""
+    from rapidtinyrec_b200._native import NativeError
+    pages = -(-tokens // page)
+    cache = filled(pages, kv, page, 128, seed=69)
+    table = tables([tokens], page, pages, seed=70)
+    ids = table.tolist()[0]
+    q = torch.randn(n, heads, 128, generator=torch.Generator().manual_seed(71)).bfloat16().cuda()
+    before = cache.attention(q, table, ints([tokens]))
+
+    def same(a, b):
+        return ((a.float() - b.float()).abs() <= 7 * 2.0 ** -10 + 1e-5 + b.float().abs() * 2.0 ** -8).all()
+
+    t0 = tokens - n  # the token of row 0
+    v_at, k_at, bad = tokens - 200, tokens - 150, (tokens - 40) // page * page
+    cache.v.view(torch.uint8)[ids[v_at // page], :, v_at % page, 5] = 0xff
+    out = cache.attention(q, table, ints([tokens]))
+    nan = out.isnan()
+    want = torch.zeros_like(nan)
+    want[v_at - t0:, :, 5] = True
+    assert torch.equal(nan, want) and same(out[~want], before[~want])
+    cache.k.view(torch.uint8)[ids[k_at // page], :, k_at % page, 7] = 0x7f
+    nan = cache.attention(q, table, ints([tokens])).isnan()
+    want[k_at - t0:] = True
+    assert torch.equal(nan, want)
+    # behind the last token nothing counts
+    last = tokens % page
+    if last:
+        cache.v.view(torch.uint8)[ids[-1], :, last:] = 0x7f
+        cache.k.view(torch.uint8)[ids[-1], :, last:] = 0x7f
+    assert torch.equal(cache.attention(q, table, ints([tokens])).isnan(), want)
+    # a query with a NaN or an infinite value spoils its own row
+    q[1, 2, 3], q[130, 0, 0], q[40] = NAN, math.inf, -math.inf
+    nan = cache.attention(q, table, ints([tokens])).isnan()
+    want[1, 2] = want[130, 0] = want[40] = True
+    assert torch.equal(nan, want)
+    # a page without a scale, then one outside the cache: the rows that see it
+    cache.v_scale[ids[bad // page]] = 0.0
+    want[bad - t0:] = True
+    assert torch.equal(cache.attention(q, table, ints([tokens])).isnan(), want)
+    first = (t0 + 600) // page * page
+    table[0, first // page] = pages
+    want[first - t0:] = True
+    assert torch.equal(cache.attention(q, table, ints([tokens])).isnan(), want)
+    with pytest.raises(NativeError, match='page'):
+        cache.check()
+    # a length that the table cannot hold
+    assert cache.attention(q, table, ints([pages * page + 1])).isnan().all()
+    with pytest.raises(NativeError, match='length'):
+        cache.check()
 
 
 def test_bad_k_scales_make_their_rows_nan():
