@@ -462,8 +462,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
 // Joins the splits of one (row, head).  D / 4 threads cover a split's row, the others take
 // other splits at the same time, so that a row split into hundreds of stretches (one
 // sequence of 128 Ki tokens) costs a few rounds of loads; each split's weight is worked
-// out once.  256 threads for up to 32 splits, 1024 for more (147 splits: 22.1 us for the whole
-// call with 256, 19.9 us with 1024).
+// out once.  256 threads for up to 32 splits, 1024 for more (147 splits: the whole call is
+// 2.2 us faster with 1024).
 constexpr int KJ_MAX = 1024;  // splits whose weights are kept at a time
 
 template <typename T, int D, int KJ_THREADS>
@@ -562,10 +562,10 @@ static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   const int64_t most = (int64_t)b->table_width * c->page, base = p.items * c->kv_heads;
   // A stretch has at least 512 keys: below that a block is bound by the latency of
   // finding its pages, and joining costs more than it saves (61 sequences of 30 - 300
-  // keys, 14 heads: 6.2 us in one stretch, 7.8 us in two); at most 1024, so that ragged
-  // batches spread (24 sequences of 6,000 - 32,000 keys: 90.8 us, with 2048 92.3, with
-  // 512 101); between them as many as give two blocks an SM (one sequence of 128 Ki
-  // keys: 22.0 us, with three an SM 23.9, with six 33).
+  // keys, 14 heads: 5.4 us in one stretch, 5.8 in three); at most 1024, which a warp's lanes
+  // can hold the pages of and at which ragged batches spread (24 sequences of 6,000 -
+  // 32,000 keys: 89.8 us, with 512 100.5); between them as many as give two blocks an SM (one
+  // sequence of 128 Ki keys: 19.1 us, with three an SM 19.0, with 512 keys 23.0).
   const int64_t want = 2 * (int64_t)sms;
   int64_t chunk = base >= want ? most : most * base / want;
   chunk = (chunk + 63) / 64 * 64;
