@@ -141,8 +141,9 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   if (warp < 8) load_q(0, q0);
   const bool whole = kv_len_fits(a.c, a.b, len, 0);
   if (!whole) len = 0;  // the sequence's rows become NaN
-  const auto limit = [&](int row) { return a.causal && count > 1 ? max(0, len - count + min(row, nrows - 1) / a.group + 1) : len; };
-  const int kmin = limit(r0), kmax = limit(r0 + KT_ROWS - 1), c1 = c0 + min(kmax - c0, a.chunk);
+  // keys that a row of the tile sees; of all rows, the least and the most
+  const auto limit = [&](int row) { return a.causal ? max(0, len - count + token0 + kv_div(a, head0 + min(row, rows - 1)) + 1) : len; };
+  const int kmin = limit(0), kmax = limit(rows - 1), c1 = c0 + min(kmax - c0, a.chunk);
   if (c1 <= c0 && split > 0 && !a.cluster) {  // a stretch behind the last key (the first one reports rows that see nothing)
     if (tid < rows) {
       const int token = (r0 + tid) / a.group;
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     int token, head;
     place(tid, token, head);
     row_out[tid] = (first + token) * a.heads + kvh * a.group + head;
-    row_lim[tid] = a.causal ? max(0, len - count + token + 1) : len;
+    row_lim[tid] = limit(tid);
   }
   if (tid >= KT_ROW_THREADS)
     kt_segments(a, seq, kvh, c0, segs, tid - KT_ROW_THREADS, C::THREADS - KT_ROW_THREADS, seg_at, seg_k, seg_lv, seg_iv);
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     {
       // q as fp16 (pairs), each row times a power of two; a warp takes 16 rows
       constexpr int PER = QPER, LPR = QLPR, RPI = QRPI, LOADS = QLOADS, STEP = QSTEP;
-      const int sub = lane / LPR, col = lane % LPR;
+      const int sub = lane / LPR, col = lane % LPR, unit = col * PER / 8;
       uint4 u[STEP];
 #pragma unroll
       for (int base = 0; base < LOADS; base += STEP) {
@@ -202,23 +203,40 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         } else {
           load_q(base, u);
         }
+        uint32_t top[STEP];  // magnitudes order as their bits do
 #pragma unroll
         for (int j = 0; j < STEP; ++j) {
-          const int row = warp * 16 + (base + j) * RPI + sub;
+          const uint32_t m = PAIR ? 0x7fffffffu : 0x7fff7fffu, w[4] = {u[j].x & m, u[j].y & m, u[j].z & m, u[j].w & m};
+          if constexpr (PAIR) {
+            top[j] = max(max(w[0], w[1]), max(w[2], w[3]));
+          } else {
+            const uint32_t t = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+            top[j] = max(t << 16, t & 0xffff0000u);
+          }
+        }
+        if constexpr (LPR == 32) {
+#pragma unroll
+          for (int j = 0; j < STEP; ++j) top[j] = __reduce_max_sync(0xffffffffu, top[j]);
+        } else {
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+        }
+        // the row's place in the operand: RPI rows on, 128 RPI bytes on and other swizzle bits
+        uint8_t* const at = qs + (unit >> 3) * KT_ROWS * 128 + (warp * 16 + base * RPI + sub) * 128 + (PAIR ? 8 * (col & 1) : 0);
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
           const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-          float x[PER], top = 0.f;
+          float x[PER];
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             if constexpr (PAIR) x[i] = __uint_as_float(w[i]);
             else x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-            top = fmaxf(top, fabsf(x[i]));
           }
-          // magnitudes order as their bits do
-          top = __uint_as_float(__reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (sub * LPR),
-                                                  __float_as_uint(top)));
-          const int e = kv_row_exponent(top);
+          const int e = kv_row_exponent(__uint_as_float(top[j]));
           const float up = copysignf(kv_pow2(-e), a.factor);  // the factor back stays positive: see below
-          if (col == 0) red[row] = kv_pow2(e) * fabsf(a.factor);
+          if (col == 0) red[warp * 16 + (base + j) * RPI + sub] = kv_pow2(e) * fabsf(a.factor);
           uint32_t hi[PER / 2], lo[PER / 2];
 #pragma unroll
           for (int i = 0; i < PER / 2; ++i) {
@@ -226,14 +244,12 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             const float2 b = unpack_f16(hi[i]);
             lo[i] = pack_f16(x[2 * i] * up - b.x, x[2 * i + 1] * up - b.y);
           }
-          const int unit = col * PER / 8;
-          uint8_t* at = qs + (unit >> 3) * KT_ROWS * 128 + sw_at(row, unit & 7);
+          uint8_t* to = at + j * RPI * 128 + ((((unit & 7) ^ sub) ^ ((base + j) * RPI & 7)) << 4);
           if constexpr (PAIR) {
-            at += 8 * (col & 1);
-            *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(at + C::Q_PLANE) = make_uint2(lo[0], lo[1]);
+            *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(to + C::Q_PLANE) = make_uint2(lo[0], lo[1]);
           } else {
-            *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           }
         }
       }
