@@ -673,6 +673,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   const int inverse = (65536 + a.splits - 1) / a.splits;  // row / splits = row * inverse >> 16 for these few rows
   const int each = ((KT_ROWS - 1) * inverse >> 16) + 1;
   const uint32_t recv = smem_addr(smem), recv_ml = recv + C::RECV_ROWS * D * 4;
+#pragma unroll 4
   for (int row = warp * RPI + lane / LPR; row < rows; row += WARPS * RPI) {
     const int nth = row * inverse >> 16, to = row - nth * a.splits, slot_at = split * each + nth;
     st_cluster_f4(cluster_map(recv + (slot_at * D + 4 * col) * 4, to),
@@ -688,12 +689,13 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     float4 v[KV_CLUSTER];
     float mt = -INFINITY, lt = 0.f;
 #pragma unroll
-    for (int s = 0; s < KV_CLUSTER; ++s) {
-      if (s >= a.splits) break;
-      p[s] = sent_ml[s * each + i];
-      v[s] = sent[(s * each + i) * (D / 4) + col];
-      mt = fmaxf(mt, p[s].x);
+    for (int s = 0; s < KV_CLUSTER; ++s) {  // without a break: all loads first
+      const int from = min(s, a.splits - 1) * each + i;
+      p[s] = sent_ml[from];
+      v[s] = sent[from * (D / 4) + col];
     }
+#pragma unroll
+    for (int s = 0; s < KV_CLUSTER; ++s) mt = fmaxf(mt, p[s].x);
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int s = 0; s < KV_CLUSTER; ++s) {
