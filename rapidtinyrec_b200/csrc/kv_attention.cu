@@ -612,7 +612,7 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
 }
 
 // What a block of 256 rows needs for 128 keys, and for its start and end in these units.
-constexpr int KW_TILE_NS = 1920, KW_BLOCK = 8;
+constexpr int KW_TILE_NS = 1750, KW_BLOCK = 7;
 
 // Tiles of 256 rows.  Items that fill all SMs are blocks of their own; what is left is split
 // along its keys, so that the last wave is a short one, and joined through memory.
@@ -626,7 +626,7 @@ static KvAttnPlan kv_plan_wide(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   int64_t best = INT64_MAX;
   for (int64_t s = (all + most - 1) / most, end = s + 63; s <= end && s <= all; ++s) {
     const int64_t per = (all + s - 1) / s, splits = (all + per - 1) / per, left = base - waves * sms;
-    const int64_t cost = waves * (all + KW_BLOCK) + (left * splits + sms - 1) / sms * (per + KW_BLOCK) + (splits == 1 ? 0 : 6);
+    const int64_t cost = waves * (all + KW_BLOCK) + (left * splits + sms - 1) / sms * (per + KW_BLOCK) + (splits == 1 ? 0 : 3);
     if (cost < best) {
       best = cost;
       p.whole = splits == 1 ? base : waves * sms;
@@ -642,8 +642,8 @@ static KvAttnPlan kv_plan_wide(const rtr_kv_cache* c, const rtr_kv_batch* b, int
 // The kernel whose expected time is less.  Measured, 28 / 4 heads of 128, bf16, tiles of
 // 128 against tiles of 8 rows: 8 sequences of 1,200 keys with 2 new tokens 12.7 : 11.0 us,
 // 4 12.9 : 12.7, 16 14.7 : 37.7; one of 300 keys with 64 11.3 : 8.4 us, with 256 11.3 : 15.6.
-// Tiles of 256 against 128: 32 sequences of 4,096 keys with 64 163 : 190 us, 4 of 512 keys with
-// 256 21.5 : 24.1, one of 4,096 with 1,024 80 : 86, with 512 57 : 47.
+// Tiles of 256 against 128: 32 sequences of 4,096 keys with 64 154 : 190 us, 4 of 512 keys with
+// 256 20.0 : 22.9, one of 4,096 with 1,024 74 : 86, with 512 57 : 47.
 static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, bool f32, int sms) {
   const int group = heads / c->kv_heads;
   int64_t rows_ns, tiles_ns;

@@ -10,10 +10,10 @@
 // maximum as it stands; only where a score exceeds it by more than 2^8 (weights stay below
 // 2^14) are O and the sum rescaled and the pass repeated.
 //
-// 128 keys take a block 3,500 cycles (exponentials alone 2,048, products 2,048; one row tile by
-// itself 2,600: a thread's chain of loads, exponentials and stores), its start and end about
-// eight times that.  8 x 1,024 rows over 6,000 keys, 28 / 4 heads: 673 us, 1,058 TFLOP/s, tiles
-// of 128 rows 749; 1,024 rows over 30,000 keys 459 : 600; at head_dim 64 no difference.
+// 128 keys take a block some 3,200 cycles (exponentials alone 2,048, products 2,048; one row
+// tile by itself 2,600: a thread's chain of loads, exponentials and stores), its start and end
+// about seven times that.  8 x 1,024 rows over 6,000 keys, 28 / 4 heads: 597 us, 1,181 TFLOP/s,
+// tiles of 128 rows 749; 1,024 rows over 30,000 keys 425 : 600; at head_dim 64 no difference.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -26,7 +26,7 @@
 namespace rtr {
 
 constexpr int KW_SEGS = KW_MAX_CHUNK / 16;
-constexpr int KW_JOIN = 32;  // rows of a block that joins
+constexpr int KW_JOIN = 8;  // rows of a block that joins, a warp each
 
 struct KwCfg {
   static constexpr int D = 128;
@@ -488,38 +488,36 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
   }
 }
 
-// Joins the stretches of the items that were split: a warp takes a row at a time.
-__global__ void __launch_bounds__(256) kv_attn_wide_join_kernel(const KvAttn a, const KwShare w) {
+// Joins the stretches of the items that were split: a warp has a row.
+__global__ void __launch_bounds__(32 * KW_JOIN) kv_attn_wide_join_kernel(const KvAttn a, const KwShare w) {
   constexpr int D = KwCfg::D;
   static_assert(D == 4 * 32, "a lane has four columns");
   pdl_launch_dependents();
   pdl_wait();
   const int col = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < KW_JOIN; i += 8) {
-    const int64_t row = (int64_t)blockIdx.x * KW_JOIN + i;
-    const int rh = w.row[row];
-    if (rh < 0) continue;
-    const float2* ml = a.ml + row * a.splits;
-    const float4* part = reinterpret_cast<const float4*>(a.part + row * a.splits * D) + col;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s].x);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int64_t row = (int64_t)blockIdx.x * KW_JOIN + (threadIdx.x >> 5);
+  const int rh = w.row[row];
+  if (rh < 0) return;
+  const float2* ml = a.ml + row * a.splits;
+  const float4* part = reinterpret_cast<const float4*>(a.part + row * a.splits * D) + col;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s].x);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
-      const float2 p = ml[s];
-      if (p.y == 0.f) continue;  // nothing seen there means nothing written to part
-      const float f = p.x == m ? 1.f : ex2(p.x - m);
-      const float4 v = part[s * 32];
-      l = fmaf(p.y, f, l);
-      x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
-    }
-    const bool sees = l != 0.f;
-    const float inv = sees ? 1.0f / l : 0.f;
-    x = sees ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
-    const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
-    reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)rh * D)[col] = *reinterpret_cast<const uint2*>(b);
-    if (a.lse && col == 0) a.lse[rh] = sees ? (m - KA_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 p = ml[s];
+    if (p.y == 0.f) continue;  // nothing seen there means nothing written to part
+    const float f = p.x == m ? 1.f : ex2(p.x - m);
+    const float4 v = part[s * 32];
+    l = fmaf(p.y, f, l);
+    x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
   }
+  const bool sees = l != 0.f;
+  const float inv = sees ? 1.0f / l : 0.f;
+  x = sees ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+  reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)rh * D)[col] = *reinterpret_cast<const uint2*>(b);
+  if (a.lse && col == 0) a.lse[rh] = sees ? (m - KA_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 cudaError_t kv_attn_wide(const KvAttn& a, const KwShare& w, int device, cudaStream_t st) {
@@ -529,7 +527,7 @@ cudaError_t kv_attn_wide(const KvAttn& a, const KwShare& w, int device, cudaStre
   if (e != cudaSuccess) return e;
   e = kv_launch(kv_attn_wide_kernel, dim3(w.whole + w.tails * a.splits), KwCfg::THREADS, KwCfg::SMEM, 1, st, a, w);
   if (e != cudaSuccess || !w.tails) return e;
-  return kv_launch(kv_attn_wide_join_kernel, dim3(w.tails * (KW_ROWS / KW_JOIN)), 256, 0, 1, st, a, w);
+  return kv_launch(kv_attn_wide_join_kernel, dim3(w.tails * (KW_ROWS / KW_JOIN)), 32 * KW_JOIN, 0, 1, st, a, w);
 }
 
 }  // namespace rtr
