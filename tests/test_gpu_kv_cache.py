@@ -562,6 +562,21 @@ def test_tiles_of_256_rows_without_starts(causal, rows):
         assert torch.equal(given, out)
 
 
+@pytest.mark.parametrize('heads,kv,rows', [(16, 16, 2300), (40, 1, 900), (300, 1, 130)])
+def test_tiles_of_256_rows_of_other_groups(heads, kv, rows):
+    """One head a group, more than a tile's half and more than a tile; q, K and V slices of larger
+    tensors."""
+    whole = filled(50, kv + 3, 32, 128, seed=72)
+    cache = whole.heads(2, kv)
+    table = tables([1300], 32, 50, seed=73)
+    g = torch.Generator().manual_seed(74)
+    fused = torch.randn(rows, heads + 5, 128, generator=g).bfloat16().cuda()
+    q = fused[:, 3:3 + heads]
+    out, _ = check_attention(cache, q, table, [1300], [rows], True)
+    assert torch.equal(cache.attention(q.contiguous(), table, ints([1300])), out)
+    check_attention(cache, q, table, [1300], [rows], False, scale=0.3)
+
+
 @pytest.mark.parametrize('size', [1e-30, 1.0, 30.0])
 def test_tiles_of_256_rows_over_many_keys(size):
     """More keys than one block takes; scales 2^60 apart and no powers of two, tiny and huge
