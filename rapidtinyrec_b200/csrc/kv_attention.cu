@@ -17,6 +17,8 @@
 // distributed shared memory; more are joined by a second kernel.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "engine.h"
@@ -555,6 +557,15 @@ static int64_t kv_attn_items(const rtr_kv_batch* b, int group, int shift, int& p
   return (int64_t)per_seq * b->seqs;
 }
 
+// Of the tiles that a ragged call may have (a sequence's last one is half full on average),
+// as many as it will hardly exceed: planned for the most there can be, 5 sequences of 3,000 - 6,000 keys with 33 -
+// 135 rows take 31.1 us instead of 27.9.
+static int64_t kv_likely_items(const rtr_kv_batch* b, int group, int shift, int64_t items) {
+  if (!b->starts) return items;
+  const double mean = (double)b->rows * group / (1 << shift) + 0.5 * b->seqs;
+  return std::min(items, std::max((int64_t)b->seqs, (int64_t)std::ceil(mean + std::sqrt(b->seqs / 12.0))));
+}
+
 // Tiles of 8 rows: stretches and the time to expect, in ns.
 static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int group, bool f32, int sms, int64_t& ns) {
   KvAttnPlan p = {};
@@ -590,7 +601,7 @@ static KvAttnPlan kv_plan_tiles(const rtr_kv_cache* c, const rtr_kv_batch* b, in
   KvAttnPlan p = {};
   p.tile_rows = KT_ROWS;
   p.items = kv_attn_items(b, group, 7, p.per_seq);
-  const int64_t base = p.items * c->kv_heads;
+  const int64_t base = kv_likely_items(b, group, 7, p.items) * c->kv_heads;
   const int64_t all = ((int64_t)b->table_width * c->page + KT_KEYS - 1) / KT_KEYS;
   // A block costs its key tiles and about six more (q, first and last tile, output), a
   // cluster's join three, a join through memory eight.  Clusters of three and more fill
