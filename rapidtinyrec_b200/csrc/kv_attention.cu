@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
         const float u = x[4 * w + 2 * h] * up, v = x[4 * w + 2 * h + 1] * up;
         qh[w][h] = pack_f16(u, v);
         if constexpr (PAIR) {
-          const float2 r = unpack_f16(qh[w][h]);
-          ql[w][h] = pack_f16(u - r.x, v - r.y);
+          const float2 r = rest_f16(qh[w][h], u, v);
+          ql[w][h] = pack_f16(r.x, r.y);
         }
       }
   }
@@ -314,9 +314,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
       ph[h][0] = transpose8x8(pa);
       ph[h][1] = transpose8x8(pb);
       if constexpr (PAIR) {
-        const float2 ra = unpack_f16(pa), rb = unpack_f16(pb);
-        pl[h][0] = transpose8x8(pack_f16(w0 - ra.x, w1 - ra.y));
-        pl[h][1] = transpose8x8(pack_f16(w2 - rb.x, w3 - rb.y));
+        const float2 ra = rest_f16(pa, w0, w1), rb = rest_f16(pb, w2, w3);
+        pl[h][0] = transpose8x8(pack_f16(ra.x, ra.y));
+        pl[h][1] = transpose8x8(pack_f16(rb.x, rb.y));
       }
     }
 

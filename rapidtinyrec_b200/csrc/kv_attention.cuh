@@ -87,7 +87,15 @@ RTR_DEVICE uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-RTR_DEVICE float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// What is left of two values beside their fp16 parts: exact, in one instruction each.
+RTR_DEVICE float2 rest_f16(uint32_t parts, float lo, float hi) {
+  float2 r;
+  asm("{\n\t.reg .f16 a, b, minus;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 minus, 0xBC00;\n\t"
+      "fma.rn.f32.f16 %0, a, minus, %3;\n\tfma.rn.f32.f16 %1, b, minus, %4;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(parts), "f"(lo), "f"(hi));
+  return r;
+}
 // Whether one of four codes is NaN (0x7f or 0xff).
 RTR_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 

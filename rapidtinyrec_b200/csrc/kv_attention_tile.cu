@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
 #pragma unroll
           for (int i = 0; i < PER / 2; ++i) {
             hi[i] = pack_f16(x[2 * i] * up, x[2 * i + 1] * up);
-            const float2 b = unpack_f16(hi[i]);
-            lo[i] = pack_f16(x[2 * i] * up - b.x, x[2 * i + 1] * up - b.y);
+            const float2 b = rest_f16(hi[i], x[2 * i] * up, x[2 * i + 1] * up);
+            lo[i] = pack_f16(b.x, b.y);
           }
           uint8_t* to = at + j * RPI * 128 + ((((unit & 7) ^ sub) ^ ((base + j) * RPI & 7)) << 4);
           if constexpr (PAIR) {
@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             sums = f2_add(sums, f2(x.x, x.y));
             w[j] = pack_f16(x.x, x.y);
             if constexpr (PAIR) {
-              const float2 b = unpack_f16(w[j]);
-              w[8 + j] = pack_f16(x.x - b.x, x.y - b.y);
+              const float2 b = rest_f16(w[j], x.x, x.y);
+              w[8 + j] = pack_f16(b.x, b.y);
             }
           }
           const float sum = f2_parts(sums).x + f2_parts(sums).y;
