@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         }
         float* rm = red + (i & 1) * 2 * KT_ROWS;
         rm[half * KT_ROWS + r] = mx;
-        row_barrier();
+        halves_barrier(warp & 3);
         const float top = fmaxf(m, fmaxf(rm[r], rm[KT_ROWS + r]));
         const float grew = alpha;  // of the tile before: scales what came before that tile's product
         alpha = m == top ? 1.f : ex2(m - top);
@@ -364,9 +364,9 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       }
       if (n > 0) add_product(n - 1, alpha);
       // the row's two halves of the sum
-      row_barrier();
+      halves_barrier(warp & 3);
       red[half * KT_ROWS + r] = l;
-      row_barrier();
+      halves_barrier(warp & 3);
       l = red[r] + red[KT_ROWS + r];
     } else {
       const uint32_t ot = tmem + lanes + O_AT + half * 128;

@@ -98,6 +98,8 @@ RTR_DEVICE uint64_t f2_add(uint64_t a, uint64_t b) {
 }
 // The row threads of a block.
 RTR_DEVICE void row_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// The two warps that have the halves of the same rows.
+RTR_DEVICE void halves_barrier(int warp) { asm volatile("bar.sync %0, 64;" ::"r"(2 + warp) : "memory"); }
 // Byte of a 16-byte unit of a 128-byte row in a 128B-swizzled operand.
 RTR_DEVICE uint32_t sw_at(int row, int unit) { return row * 128 + ((unit ^ (row & 7)) << 4); }
 
