@@ -24,7 +24,7 @@
 // What bounds it is the chain of a tile, weights - O - S (about 2,600 cycles for 128 keys at
 // head_dim 128, of which exponentials need 1,024 and products 1,024).  2 x 1,024 rows over 6,000
 // keys: 28 / 4 heads of 128, bf16, 221 us (797 TFLOP/s; kv_attention_wide.cu 183); 12 / 2, fp32,
-// 155 us; 14 / 2 of 64 92 (bf16) and 160 us (fp32).  50 beams over 719 keys, 28 / 4, 11.5 us.
+// 149 us; 14 / 2 of 64 94 (bf16) and 149 us (fp32).  50 beams over 719 keys, 28 / 4, 11.5 us.
 #include <cuda_runtime.h>
 
 #include <type_traits>
