@@ -54,7 +54,7 @@ def _compile_calls() -> None:
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-w',
            f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', *[f'-I{p}' for p in include],
            str(CSRC / 'kv_call.cpp'), '-o', str(tmp), f"-L{root / 'lib'}", '-lc10', '-lc10_cuda', '-ltorch_cpu',
-           '-ltorch_python']
+           '-ltorch_cuda', '-ltorch_python']
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f'compiling kv_call.cpp failed:\n{res.stdout}\n{res.stderr}')

@@ -6,8 +6,7 @@
 // The module links against torch only; setup() hands it the C entry points' addresses.
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstdarg>
@@ -107,6 +106,11 @@ bool dense(const Cache& cache, const at::Tensor& x, int64_t heads, const char* n
 
 int32_t type_of(const at::Tensor& x) { return x.scalar_type() == at::kFloat ? RTR_DTYPE_F32 : RTR_DTYPE_BF16; }
 
+// A new tensor on the cache's device, by its allocator without a pass through the dispatcher.
+at::Tensor room_for(const Cache& cache, at::IntArrayRef size, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(size, type, at::Device(at::kCUDA, (c10::DeviceIndex)cache.index), std::nullopt));
+}
+
 at::Tensor copied(const at::Tensor& x) { return x.clone(at::MemoryFormat::Contiguous); }
 
 template <typename F> PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F&& body) {
@@ -145,9 +149,9 @@ PyObject* call_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (rows < 0) refuse("negative row count");
     at::Tensor k, v;
     if (a[7] == Py_None) {
-      const auto options = at::TensorOptions().dtype(dtype ? at::kBFloat16 : at::kFloat).device(at::kCUDA, cache.index);
-      k = at::empty({rows, heads, dim}, options);
-      v = at::empty({rows, heads, dim}, options);
+      const at::ScalarType type = dtype ? at::kBFloat16 : at::kFloat;
+      k = room_for(cache, {rows, heads, dim}, type);
+      v = room_for(cache, {rows, heads, dim}, type);
     } else {
       if (!PyTuple_Check(a[7]) || PyTuple_GET_SIZE(a[7]) != 2) refuse("out must be a pair of tensors");
       k = tensor(PyTuple_GET_ITEM(a[7], 0), "out");
@@ -186,7 +190,7 @@ PyObject* call_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (PyErr_Occurred()) throw Raised{};
     at::Tensor out, lse, work;
     if (a[9] == Py_None) {
-      out = at::empty({rows, heads, dim}, q.options());
+      out = room_for(cache, {rows, heads, dim}, q.scalar_type());
     } else {
       out = tensor(a[9], "out");
       if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || !cache.here(out) || !out.is_contiguous() ||
@@ -195,8 +199,8 @@ PyObject* call_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     int64_t room = 0;
     check(kv_workspace(cache.c, &b, type_of(q), (int32_t)heads, cache.index, &room));
-    if (with_lse) lse = at::empty({rows, heads}, q.options().dtype(at::kFloat));
-    if (room) work = at::empty({room}, q.options().dtype(at::kByte));
+    if (with_lse) lse = room_for(cache, {rows, heads}, at::kFloat);
+    if (room) work = room_for(cache, {room}, at::kByte);
     check(kv_attention(cache.c, &b, q.data_ptr(), type_of(q), (int32_t)heads, q.stride(0), causal, (float)scale,
                        out.data_ptr(), with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
                        room ? work.data_ptr() : nullptr, room, cache.index, cache.stream()));
