@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
       if (!wait(bars.v_full[B], i >> 1)) return false;
       if (!step(i, buffer, next, c0_) || !step(i, buffer, next, c1_)) return false;
       if (!step(i, buffer, next, c2_) || !step(i, buffer, next, c3_)) return false;
-      if (leader) {  // tile i's V, the next tile's K
+      if (leader && i + 2 < n) {  // tile i's V, the next tile's K; nothing arrives for which no one waits
         mma_commit(smem_addr(&bars.v_free[B]));
         mma_commit(smem_addr(&bars.k_free[B ^ 1]));
       }
