@@ -360,8 +360,10 @@ int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_de
  * nothing are 0.  q: row r, head h at r * q_token_stride + h * head_dim; out
  * [rows][heads][head_dim], same dtype; lse_dev (optional, float32 [rows][heads]):
  * log of the softmax's sum, minus infinity for rows that see nothing.  fp32 q and
- * weights enter the tensor cores as fp16 pairs (22 bits); sums are fp32.  A row
- * that sees a page whose V scale is outside [2^-48, 2^48], whose K scale is negative or
+ * weights enter the tensor cores as fp16 pairs: 22 bits, or for small ones half a step of 2^-38
+ * of the largest q of the row, of 2^-39 of the largest weight (times V scale) among 128 keys.
+ * bf16 rows' weights are one fp16 value: 11 bits, or half a step of 2^-34 of the row's largest.
+ * Sums are fp32.  A row that sees a page whose V scale is outside [2^-48, 2^48], whose K scale is negative or
  * whose number is outside the cache is NaN.  The workspace must hold
  * rtr_kv_attention_workspace bytes (the same batch, dtype and heads), aligned to 16, and is
  * free again when the call's kernels ran: calls that may overlap need one each.  A table row wider than the

@@ -45,6 +45,14 @@ RTR_DEVICE void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same, from zeros.
+RTR_DEVICE void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "{\n\t.reg .f32 z;\n\tmov.f32 z, 0f00000000;\n\t"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {z, z, z, z};\n\t}"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 RTR_DEVICE uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -72,7 +80,8 @@ template <int D> RTR_DEVICE int ka_at(int row, int ch) {
 // for P V, 16 consecutive dimensions, so both operands come from shared memory by
 // 16-byte loads and the transposition of V is byte permutes in registers.
 //
-// fp32 queries (and weights) enter as fp16 pairs, hi + lo: 22 significant bits.
+// fp32 queries (and weights) enter as fp16 pairs, hi + lo: 22 significant bits.  The weights' low
+// parts have a product of their own, times KA_LOW, which is added to the sums by IEEE operations.
 template <typename T, int D>
 __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const KvAttn a) {
   using C = KaCfg<D>;
@@ -315,8 +324,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
       ph[h][1] = transpose8x8(pb);
       if constexpr (PAIR) {
         const float2 ra = rest_f16(pa, w0, w1), rb = rest_f16(pb, w2, w3);
-        pl[h][0] = transpose8x8(pack_f16(ra.x, ra.y));
-        pl[h][1] = transpose8x8(pack_f16(rb.x, rb.y));
+        pl[h][0] = transpose8x8(pack_f16(ra.x * KA_LOW, ra.y * KA_LOW));
+        pl[h][1] = transpose8x8(pack_f16(rb.x * KA_LOW, rb.y * KA_LOW));
       }
     }
 
@@ -360,7 +369,12 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
           const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)(x >> 16)),
                          a2 = e4m3x2_to_f16x2((uint16_t)y), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
           mma16816(o[2 * w + e], a0, a1, a2, a3, ph[h][0], ph[h][1]);
-          if constexpr (PAIR) mma16816(o[2 * w + e], a0, a1, a2, a3, pl[h][0], pl[h][1]);
+          if constexpr (PAIR) {
+            float low[4];
+            mma16816_first(low, a0, a1, a2, a3, pl[h][0], pl[h][1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[2 * w + e][j] = fmaf(low[j], 1.0f / KA_LOW, o[2 * w + e][j]);
+          }
         }
     }
     if (nans) {
@@ -413,6 +427,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
 #pragma unroll
     for (int j = 0; j < PER; ++j) x[j] = fmaf(p[j], f, x[j]);
   }
+  mt -= KA_LIFT;  // what the sums are relative to
   // every visible score is minus infinity (0 / 0), or the sequence's length did not fit
   if (lt == 0.f && (limit(r0 + row) > c0 || !whole)) lt = __int_as_float(0x7fffffff);
   const auto head_row = [&](int rr) {
@@ -425,7 +440,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
     T* p = static_cast<T*>(a.out) + rh * D + d0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) p[j] = from_f32<T>(sees ? x[j] * inv : 0.f);
-    if (a.lse && d0 == 0) a.lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+    if (a.lse && d0 == 0) a.lse[rh] = sees ? (mt + log2f(lt)) * 0.6931471805599453f : -INFINITY;
   };
   if (a.splits == 1) {
     if (r0 + row < nrows) finish(r0 + row);
@@ -535,7 +550,7 @@ __global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch 
   o[1] = from_f32<T>(sees ? x.y * inv : 0.f);
   o[2] = from_f32<T>(sees ? x.z * inv : 0.f);
   o[3] = from_f32<T>(sees ? x.w * inv : 0.f);
-  if (lse && tid == 0) lse[rh] = sees ? (mt - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+  if (lse && tid == 0) lse[rh] = sees ? (mt + log2f(lt)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ------------------------------------------------------------------- host

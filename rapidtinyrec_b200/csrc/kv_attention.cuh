@@ -1,5 +1,5 @@
-// What the two attention kernels over the 8-bit KV cache share
-// (kv_attention.cu: few rows, kv_attention_tile.cu: tiles of 128 rows).
+// What the attention kernels over the 8-bit KV cache share (kv_attention.cu: few rows,
+// kv_attention_tile.cu: tiles of 128 rows, kv_attention_wide.cu: two such tiles a block).
 #pragma once
 
 #include "kv_cache.cuh"
@@ -21,16 +21,21 @@ struct KvAttn {
   void* out;           // [rows][heads][head_dim]
   float* lse;          // [rows][heads] or null
   float* part;         // [rows * heads][splits][head_dim] when splits > 1
-  float2* ml;          // [rows * heads][splits]: running maximum, sum
+  float2* ml;          // [rows * heads][splits]: log2 of the unit of part and of the sum, sum
   int per_seq;         // row tiles of a sequence without starts
   int chunk, splits;   // keys of a block, and the blocks of a row tile
   int cluster;         // the blocks of a row tile are one cluster and join among themselves
 };
 
-// Weights enter the fp16 operand times 2^6: a weight of 2^-24 of the largest (fp16's
-// smallest is 2^-24, so 2^-30 of it) still counts, and a maximum may be exceeded by 2^8
-// before a weight nears fp16's largest, 2^16.
-constexpr float KA_LIFT = 6.0f;
+// Weights enter the fp16 operands relative to 2^(maximum - lift): the lift brings the largest
+// near fp16's largest, 2^16, since what lies below fp16's smallest normal value, 2^-14, is
+// rounded to multiples of 2^-24 and a few keys that outweigh thousands of others (whose values
+// may be 0) must not cost those their precision.  Where the maximum is always the running one,
+// the lift is 15: weights down to 2^-29 of the largest keep the operand's 11 bits.
+constexpr float KA_LIFT = 15.0f;
+// The low parts of pairs enter times 2^11, as large as the high ones, where their product has
+// an accumulator of its own: 22 bits down to the same 2^-29.
+constexpr float KA_LOW = 2048.0f;
 
 // v / group for v < 2^32 / group (v is a row's place within some tiles): one multiplication.
 // A group of one has no 32-bit inverse.

@@ -14,12 +14,15 @@
 //
 // bf16 rows: two threads a row, each with 64 of a tile's keys, its own maximum, sum and
 // O in tensor memory; the two are joined at the end.  Weights are computed in one pass with
-// the maximum as it stands; only where a score exceeds it by more than 2^8 (weights stay
-// below 2^14) are O and the sum rescaled and the pass repeated.
+// the maximum as it stands; only where a score exceeds it by more than 2^KT_SLACK (weights stay
+// below 2^15) are O and the sum rescaled and the pass repeated.
 // fp32 rows: q and the weights enter as fp16 pairs, two products each.  The tensor core's
 // own accumulation drifts over thousands of keys, so tensor memory sums one tile only: two
 // threads a row (64 scores of the tile each) add it to half of the output's dimensions in
-// registers, by IEEE additions.
+// registers, by IEEE operations.  Weights are relative to their own tile's maximum, which the
+// addition makes up for: the low parts of a pair keep 22 bits down to 2^-17 of the largest
+// weight of 128 keys (tensor memory has no room for a product of their own), whatever other
+// tiles hold.
 //
 // What bounds it is the chain of a tile, weights - O - S (about 2,600 cycles for 128 keys at
 // head_dim 128, of which exponentials need 1,024 and products 1,024).  2 x 1,024 rows over 6,000
@@ -81,6 +84,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREADS, 1) kv_attn_tile_kernel(const KvAttn a) {
   constexpr bool PAIR = std::is_same<T, float>::value;
   using C = KtCfg<D, PAIR>;
+  constexpr float LIFT = PAIR ? KA_LIFT : KT_LIFT;
   constexpr int HD = D / 2;    // dimensions of the output a row thread finishes
   constexpr int NL = D / 8;    // of those, the ones with the same d % 4
   extern __shared__ uint8_t kt_smem_raw[];
@@ -266,15 +270,14 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     if constexpr (PAIR) {
 #pragma unroll
       for (int i = 0; i < HD / 2; ++i) o[i] = 0;
-      float alpha = 1.f;
+      float keep = 1.f, take = 1.f;  // factors of what was summed before the last tile, and of that tile
 
-      // adds the finished product of tile i, whose weights are relative to the maximum of
-      // that tile; `grew` scales what was summed before it
-      const auto add_product = [&](int i, float grew) {
+      // adds the finished product of tile i, whose weights are relative to that tile's maximum
+      const auto add_product = [&](int i, float keep_, float take_) {
         mbar_wait(smem_addr(&bars.o_full[0][i & 1]), (i >> 1) & 1, abort_flag);
         tc_fence_after();
         const uint32_t at = tmem + lanes + O_AT + (i & 1) * 128 + half * NL;
-        const uint64_t by = f2(grew, grew);
+        const uint64_t old2 = f2(keep_, keep_), new2 = f2(take_, take_);
         uint32_t v[2][NL];
         tmem_ld_cols(at, v[0]);
 #pragma unroll
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
           if (t < 3) tmem_ld_cols(at + (t + 1) * (D / 4), v[(t + 1) & 1]);
 #pragma unroll
           for (int j = 0; j < NL / 2; ++j)
-            o[t * NL / 2 + j] = f2_fma(o[t * NL / 2 + j], by, f2(v[t & 1][2 * j], v[t & 1][2 * j + 1]));
+            o[t * NL / 2 + j] = f2_fma(f2(v[t & 1][2 * j], v[t & 1][2 * j + 1]), new2, f2_mul(o[t * NL / 2 + j], old2));
         }
         tc_fence_before();
         mbar_arrive(smem_addr(&bars.o_free[i & 1]));
@@ -320,12 +323,13 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         float* rm = red + (i & 1) * 2 * KT_ROWS;
         rm[half * KT_ROWS + r] = mx;
         halves_barrier(warp & 3);
-        const float top = fmaxf(m, fmaxf(rm[r], rm[KT_ROWS + r]));
-        const float grew = alpha;  // of the tile before: scales what came before that tile's product
-        alpha = m == top ? 1.f : ex2(m - top);
-        m = top;
-        l *= alpha;
-        const float u = (m == -INFINITY ? 0.f : m) - KA_LIFT;
+        const float top = fmaxf(rm[r], rm[KT_ROWS + r]), all = fmaxf(m, top);
+        const float kept = keep, took = take;  // of the tile before
+        keep = m == all ? 1.f : ex2(m - all);
+        take = top == all ? 1.f : ex2(top - all);
+        m = all;
+        float part_l = 0.f;
+        const float u = (top == -INFINITY ? 0.f : top) - LIFT;
         // 16 keys at a time, the next ones on their way: few registers are left beside o
         tmem_ld16(st, v[0]);
 #pragma unroll
@@ -354,15 +358,16 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
             }
           }
           const float sum = f2_parts(sums).x + f2_parts(sums).y;
-          l = fmaf(sum, iv, l);
+          part_l = fmaf(sum, iv, part_l);
           tmem_st_words(st + 16 * g, w);  // over the scores just read
         }
+        l = fmaf(part_l, take, l * keep);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_addr(&bars.p_full[0][i & 1]));
-        if (i > 0) add_product(i - 1, grew);
+        if (i > 0) add_product(i - 1, kept, took);
       }
-      if (n > 0) add_product(n - 1, alpha);
+      if (n > 0) add_product(n - 1, keep, take);
       // the row's two halves of the sum
       halves_barrier(warp & 3);
       red[half * KT_ROWS + r] = l;
@@ -422,7 +427,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
           }
         };
         const auto weigh = [&] {
-          const float u = (m == -INFINITY ? 0.f : m) - KA_LIFT;
+          const float u = (m == -INFINITY ? 0.f : m) - LIFT;
           if (border) weigh_keys(u, std::true_type{});
           else weigh_keys(u, std::false_type{});
         };
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       reinterpret_cast<float4*>(stage + r * C::STAGE_LD + half * HD)[j] =
           make_float4(value(j), value(NL + j), value(2 * NL + j), value(3 * NL + j));
     row_barrier();  // red has been read
-    if (half == 0) reinterpret_cast<float2*>(red)[r] = make_float2(m, lt);
+    if (half == 0) reinterpret_cast<float2*>(red)[r] = make_float2(m - LIFT, lt);
   } else if (warp < 8 + C::CODE_WARPS) {
     // ------------------------------------------------------------ codes
     KtCodes<D, C::CODE_WARPS> codes(a.c, seg_at, segs, warp - 8, lane);
@@ -650,7 +655,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
       *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(b);
     }
-    if (a.lse && col == 0) a.lse[rh] = sees ? (m - KA_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    if (a.lse && col == 0) a.lse[rh] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   };
   if (!a.cluster) {
     for (int row = warp * RPI + lane / LPR; row < rows; row += WARPS * RPI) {

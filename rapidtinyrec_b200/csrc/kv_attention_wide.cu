@@ -7,8 +7,8 @@
 // other's sum and next scores, and the two tiles' threads take turns at the exponential unit;
 // codes are converted once for 256 rows.  Tensor memory: S and O of either tile, 128 columns
 // each; a half's weights lie over its scores.  Weights are computed in one pass with the
-// maximum as it stands; only where a score exceeds it by more than 2^8 (weights stay below
-// 2^14) are O and the sum rescaled and the pass repeated.
+// maximum as it stands; only where a score exceeds it by more than 2^KT_SLACK (weights stay below
+// 2^15) are O and the sum rescaled and the pass repeated.
 //
 // 128 keys take a block some 3,200 cycles (exponentials alone 2,048, products 2,048; one row
 // tile by itself 2,600: a thread's chain of loads, exponentials and stores), its start and end
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
           }
         };
         const auto weigh = [&] {
-          const float u = (m == -INFINITY ? 0.f : m) - KA_LIFT;
+          const float u = (m == -INFINITY ? 0.f : m) - KT_LIFT;
           if (border) weigh_keys(u, std::true_type{});
           else weigh_keys(u, std::false_type{});
         };
@@ -329,8 +329,8 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
     uint8_t* stage = smem + tid * (alone ? C::STAGE_LD16 : C::STAGE_LD32);
     const int64_t rh = row_out[tid];
     if (tid < rows) {
-      if (!alone) a.ml[(int64_t)(tail * KW_ROWS + tid) * a.splits + split] = make_float2(m, lt);
-      else if (a.lse) a.lse[rh] = sees ? (m - KA_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
+      if (!alone) a.ml[(int64_t)(tail * KW_ROWS + tid) * a.splits + split] = make_float2(m - KT_LIFT, lt);
+      else if (a.lse) a.lse[rh] = sees ? (m - KT_LIFT + log2f(lt)) * 0.6931471805599453f : -INFINITY;
     }
     if (active) {
       const int nan0 = bars.nans ? max(c0, kmin & ~(KT_KEYS - 1)) : INT_MAX;
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(32 * KW_JOIN) kv_attn_wide_join_kernel(const K
   x = sees ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
   const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
   reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)rh * D)[col] = *reinterpret_cast<const uint2*>(b);
-  if (a.lse && col == 0) a.lse[rh] = sees ? (m - KA_LIFT + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  if (a.lse && col == 0) a.lse[rh] = sees ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 cudaError_t kv_attn_wide(const KvAttn& a, const KwShare& w, int device, cudaStream_t st) {

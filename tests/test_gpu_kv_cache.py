@@ -650,6 +650,61 @@ def test_tiles_of_256_rows_keep_nan_with_the_rows_that_see_it(n, tokens, heads, 
         cache.check()
 
 
+# ------------------------------------------- keys that outweigh all others together
+# One row, stretches of one cluster, stretches joined by a kernel; tiles of 128 and 256 rows.
+OUTWEIGHED = [(torch.float32, 12, 2, 128, 1, 700), (torch.float32, 14, 2, 64, 3, 3000), (torch.float32, 12, 2, 128, 2, 20000),
+              (torch.bfloat16, 12, 2, 128, 1, 700), (torch.bfloat16, 14, 2, 64, 3, 3000), (torch.bfloat16, 12, 2, 128, 2, 20000),
+              (torch.float32, 12, 2, 128, 1000, 2300), (torch.float32, 14, 2, 64, 1000, 2300),
+              (torch.bfloat16, 14, 2, 64, 1000, 2300), (torch.bfloat16, 28, 4, 128, 1300, 2000)]
+
+
+@pytest.mark.parametrize('dtype,heads,kv,dim,rows,tokens', OUTWEIGHED)
+@pytest.mark.parametrize('by', ['score', 'scale'])
+def test_keys_beside_one_that_outweighs_them(dtype, heads, kv, dim, rows, tokens, by):
+    """One key (or one page's V scale) outweighs all others by up to 2^26 (fp32: 2^32) and its V is 0: the
+    output is what the others give.  All V are positive, so every error is relative to the output.
+
+    Scores are one exact product: x = 45 in units of log2 at most, and the six roundings of its factors
+    and of the exponent move a weight by 6 * 2^-24 * 64 * ln 2 < 2^-15.  A weight has 22 bits (2^-22;
+    one fp16 value: 2^-12), or is off by half a step of the operand: 2^-40 of the largest of its 128 keys
+    (fp32; the other tiles' weights are exact to 22 bits, and where one row's running maximum counts
+    for all keys it is 2^-51) and 2^-35 of the row's largest (bf16).  Positive
+    terms are added in at most tokens / 16 + 64 steps of 2^-22; the output's own rounding comes last.
+    """
+    page, most = 32, 32 if dtype == torch.float32 else 26
+    pages = -(-tokens // page)
+    cache = filled(pages, kv, page, dim, seed=80)
+    g = torch.Generator().manual_seed(81)
+    table = tables([tokens], page, pages, seed=82)
+    ids = table.tolist()[0]
+    cache.v.copy_((torch.randint(8, 449, cache.v.shape, generator=g).float()).to(F8))
+    cache.v_scale.fill_(2.0 ** -7)
+    cache.k_scale.fill_(2.0 ** -3)
+    # log2 of the factor, for each row: eighths, which bf16 holds and 2^x does not make round numbers of
+    more = torch.randint(8 * (most - 10), 8 * most, (rows, heads), generator=g).double() / 8
+    for at in (0, tokens // 2, tokens - 1):
+        v, vs = cache.v.clone(), cache.v_scale.clone()
+        cache.k.zero_()
+        q = torch.zeros(rows, heads, dim, device='cuda')
+        if by == 'score':
+            cache.k[ids[at // page], :, at % page, 0] = 8.0  # times 2^-3: the score is scale * q
+            cache.v[ids[at // page], :, at % page] = 0.0
+            q[..., 0] = more.float().cuda()
+        else:
+            cache.v[ids[at // page]] = 0.0
+            cache.v_scale[ids[at // page]] = 1.3 * 2.0 ** (most - 8)  # and the others' weights no round numbers
+        out, lse = cache.attention(q.to(dtype), table, ints([tokens]), causal=False, scale=math.log(2.0), return_lse=True)
+        want, want_lse, _, _ = plain_attention(q.to(dtype).double(), cache, table.tolist(), [tokens], [rows], False, math.log(2.0))
+        low = 2.0 ** (most - 40) * min(1.0, 256 / tokens) if dtype == torch.float32 else 2.0 ** (most - 35)
+        rel = 2.0 ** -15 + (2.0 ** -22 if dtype == torch.float32 else 2.0 ** -12) + low + (tokens / 16 + 64) * 2.0 ** -22
+        off = (out.double() - want).abs() / want
+        assert off.max() <= rel + torch.finfo(dtype).eps / 2, (at, off.max())
+        assert (lse.double() - want_lse).abs().max() <= rel + want_lse.abs().max() * 2.0 ** -22
+        cache.v.copy_(v)
+        cache.v_scale.copy_(vs)
+    cache.check()
+
+
 def test_bad_k_scales_make_their_rows_nan():
     cache = filled(4, 1, 16, 64, seed=54)
     table = ints([[0, 1], [2, 3]])
