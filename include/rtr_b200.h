@@ -380,7 +380,8 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
  * every layer into pages of a cache with layers x kv_heads heads (head l * kv_heads + g is
  * layer l's group g), table_dev [table_width] its page numbers, and copies the final hidden
  * state of the prompt's last token (hidden elements of the session's type) to hidden_dev.
- * Blocks until done; a page number outside the cache sets the cache's status word.
+ * Blocks until done; a prefill that failed on the device is refused (RTR_ERR_DEVICE) and nothing
+ * written; a page number outside the cache sets the cache's status word.
  * rtr_prefill_kept takes rtr_prefill's place for that user: step 0 from the hidden state
  * (the same scores as at first), then rtr_decode_step 1 - 4 and rtr_read_results as ever,
  * the prefix's K and V now the 8-bit values.  in_place: the decode steps attend over the

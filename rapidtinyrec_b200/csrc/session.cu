@@ -1088,9 +1088,8 @@ static std::string status_hex(uint32_t st) {
   return b;
 }
 
-static int check_result(rtr_session* s, const rtr_result* out, int u = 0) {
-  const DevResult& r = s->hres[u];
-  const uint32_t st = r.status;
+// The error that a status word's bits stand for, if any.
+static int check_status(rtr_session* s, uint32_t st) {
   if (st & RTR_DEV_TIMEOUT) {
     // the aborted GEMMs keep their split-K tickets whole; re-arm them anyway so
     // no count left by an interrupted launch can reach the next request
@@ -1104,6 +1103,13 @@ static int check_result(rtr_session* s, const rtr_result* out, int u = 0) {
     return fail(s, RTR_ERR_DEVICE, "beam search would continue after 5 steps (catalog grammar is not 3 SID tokens + newline + EOS)");
   if (st & RTR_DEV_STOPPED_EARLY)
     return fail(s, RTR_ERR_DEVICE, "beam search stopped before 5 steps");
+  return RTR_OK;
+}
+
+static int check_result(rtr_session* s, const rtr_result* out, int u = 0) {
+  const DevResult& r = s->hres[u];
+  const uint32_t st = r.status;
+  if (int e = check_status(s, st)) return e;
   const int B = beams_of(s);
   if (out) {
     if (out->token_ids) memcpy(out->token_ids, r.token_ids, sizeof(int32_t) * B * NSTEPS);
@@ -1143,6 +1149,11 @@ int rtr_keep_prefix(rtr_session* s, const rtr_kv_cache* cache, const int32_t* ta
   if (const char* e = kept_fits(s, cache, table_dev, table_width, s->L)) return fail(s, RTR_ERR_ARG, e);
   if (!hidden_dev) return fail(s, RTR_ERR_ARG, "null hidden state");
   CUDA_TRY(s, cudaSetDevice(s->device));
+  // A prefill that failed is not kept: rtr_prefill_kept does not run it again and would not notice.
+  uint32_t status = 0;
+  CUDA_TRY(s, cudaMemcpyAsync(&status, s->d_status, sizeof status, cudaMemcpyDeviceToHost, s->stream));
+  CUDA_TRY(s, cudaStreamSynchronize(s->stream));
+  if (int e = check_status(s, status)) return e;
   const auto& c = s->cfg;
   const int64_t D = c.head_dim, cap = c.max_prefix, kvd = (int64_t)c.kv_heads * D, size = s->bf16 ? 2 : 4;
   const rtr_kv_batch batch = {table_dev, s->d_L, nullptr, table_width, table_width, 1, s->L};

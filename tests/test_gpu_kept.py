@@ -193,6 +193,37 @@ def test_a_prompt_that_was_not_prefilled_is_not_kept(tiny, engine):
     assert engine.generate_kept(kept) == record
 
 
+@pytest.mark.parametrize('fault', ['token', 'wait'])
+def test_a_prefill_that_failed_is_not_kept(tiny, engine, fault):
+    """A token outside the vocabulary, or a bounded wait that ran out: the store stays as it was, and
+    the engine serves on."""
+    from rapidtinyrec_b200 import _native
+    ids = list(prompts(tiny)[0])
+    store = engine.prefix_store(8)
+    pages = range(pages_for(ids, 64))
+    record, kept = engine.generate_and_keep(ids, store, pages)
+    again = engine.generate_kept(kept)
+    before = store.k.view(torch.uint8).clone(), store.k_scale.clone()
+    wrong = list(ids)
+    if fault == 'token':
+        wrong[1] = tiny['cfg'].vocab
+        engine.prefill(wrong)
+    else:
+        _native.wait_control(0, 4_000_000, withhold_activation_copies=True)
+        try:
+            engine.prefill(wrong)
+            torch.cuda.synchronize()
+        finally:
+            _native.wait_control(0)
+    with pytest.raises(_native.NativeError) as e:
+        engine.keep_prefix(wrong, store, pages)
+    assert e.value.code == _native.RTR_ERR_DEVICE
+    assert torch.equal(store.k.view(torch.uint8), before[0]) and torch.equal(store.k_scale, before[1])
+    assert engine.generate_kept(kept) == again
+    assert engine.generate(ids) == record
+    assert engine.generate_and_keep(ids, store, pages)[0] == record
+
+
 def test_a_refused_kept_prefix_ends_the_former_request(tiny, engine):
     from rapidtinyrec_b200._native import RTR_ERR_ARG, RTR_ERR_STATE, NativeError
     from rapidtinyrec_b200.kv_cache import KvCache8
