@@ -311,8 +311,8 @@ int rtr_constraint_process_static(rtr_session* s, int32_t step, const int64_t* i
  * word that the kernels set bits in (never clear): 1 << 5 a length or row range
  * that does not fit, 1 << 9 a page number outside [0, pages), 1 << 10 an old scale
  * that is not positive and finite.  The work concerned is left out (attention:
- * rows of NaN; where starts itself is at fault those rows are undefined), memory
- * outside the buffers is never touched. */
+ * rows of NaN; where starts itself is at fault the whole call is left out and no row written),
+ * memory outside the buffers is never touched. */
 typedef struct {
   void *k, *v;
   float *k_scale, *v_scale;

@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   int seq;
   int64_t item0;
   if (a.b.starts) {
-    seq = kv_find_seq(a.b, blockIdx.x, a.group, 3, 1, &slot, item0);
+    seq = kv_find_seq(a.b, blockIdx.x, a.group, 3, 1, a.c.status, &slot, item0);
+    if (a.refused && tid == 0) *a.refused = seq == -2;  // every block says the same
     if (seq < 0) return;
   } else {
     seq = (int)blockIdx.x / a.per_seq;
@@ -484,8 +485,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
 constexpr int KJ_MAX = 1024;  // splits whose weights are kept at a time
 
 template <typename T, int D, int KJ_THREADS>
-__global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch b, int heads, const float* part,
-                                                                  const float2* ml, int splits, T* out, float* lse) {
+__global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch b, const int* refused, int heads,
+                                                                  const float* part, const float2* ml, int splits,
+                                                                  T* out, float* lse) {
   constexpr int COLS = D / 4, LANES = KJ_THREADS / COLS;
   __shared__ float weight[KJ_MAX];
   __shared__ float red[2][KJ_THREADS / 32];
@@ -494,7 +496,8 @@ __global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch 
   pdl_wait();
   const int64_t rh = blockIdx.x;
   const int token = (int)(rh / heads), tid = threadIdx.x, col = tid % COLS, sub = tid / COLS;
-  if (b.starts && (token < b.starts[0] || token >= b.starts[b.seqs])) return;  // no sequence's row: left as it was
+  // no sequence's row, or nothing to join: left as it was
+  if (b.starts && (*refused || token < b.starts[0] || token >= b.starts[b.seqs])) return;
   const float2* m = ml + rh * splits;
   const float4* p = reinterpret_cast<const float4*>(part + rh * splits * D) + col;
   float mt = -INFINITY, lt = 0.f;
@@ -687,8 +690,9 @@ static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   }
   if (p.tile_rows == KW_ROWS)
     p.workspace = p.tails * KW_ROWS * (p.splits * (int64_t)(c->head_dim * 4 + 8) + 4);
-  else
-    p.workspace = p.splits > 1 && !p.cluster ? (int64_t)b->rows * heads * p.splits * (c->head_dim * 4 + 8) : 0;
+  else  // with starts, room for KvAttn::refused behind the sums
+    p.workspace = p.splits > 1 && !p.cluster
+                      ? ((int64_t)b->rows * heads * p.splits + (b->starts != nullptr)) * (c->head_dim * 4 + 8) : 0;
   return p;
 }
 
@@ -719,8 +723,9 @@ template <typename T, int D> static cudaError_t kv_attn_launch(const KvAttn& a, 
   }
   if (e != cudaSuccess || a.splits == 1 || a.cluster) return e;
   const auto join = [&](auto kernel, int threads) {
-    return launch_pdl(PDL_ATTN, kernel, dim3((unsigned)(a.b.rows * a.heads)), dim3(threads), 0, st, a.b, a.heads,
-                      (const float*)a.part, (const float2*)a.ml, a.splits, static_cast<T*>(a.out), a.lse);
+    return launch_pdl(PDL_ATTN, kernel, dim3((unsigned)(a.b.rows * a.heads)), dim3(threads), 0, st, a.b,
+                      (const int*)a.refused, a.heads, (const float*)a.part, (const float2*)a.ml, a.splits,
+                      static_cast<T*>(a.out), a.lse);
   };
   return a.splits <= 32 ? join(kv_attn_join_kernel<T, D, 256>, 256) : join(kv_attn_join_kernel<T, D, 1024>, 1024);
 }
@@ -775,6 +780,8 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
   a.lse = lse_dev;
   a.part = static_cast<float*>(workspace_dev);
   a.ml = reinterpret_cast<float2*>(a.part + (int64_t)batch->rows * heads * p.splits * cache->head_dim);
+  a.refused = batch->starts && p.splits > 1 && !p.cluster && p.tile_rows != KW_ROWS
+                  ? reinterpret_cast<int*>(a.ml + (int64_t)batch->rows * heads * p.splits) : nullptr;
   a.per_seq = p.per_seq;
   a.chunk = p.chunk;
   a.splits = p.splits;

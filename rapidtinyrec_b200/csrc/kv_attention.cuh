@@ -21,6 +21,7 @@ struct KvAttn {
   void* out;           // [rows][heads][head_dim]
   float* lse;          // [rows][heads] or null
   float* part;         // [rows * heads][splits][head_dim] when splits > 1
+  int* refused;        // with starts, and stretches that a kernel joins: whether the call is refused
   float2* ml;          // [rows * heads][splits]: log2 of the unit of part and of the sum, sum
   int per_seq;         // row tiles of a sequence without starts
   int chunk, splits;   // keys of a block, and the blocks of a row tile

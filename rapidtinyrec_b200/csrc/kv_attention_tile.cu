@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   int seq;
   int64_t item0;
   if (a.b.starts) {
-    seq = kv_find_seq(a.b, blockIdx.x, a.group, 7, 1, &slot, item0);
+    seq = kv_find_seq(a.b, blockIdx.x, a.group, 7, 1, a.c.status, &slot, item0);
+    if (a.refused && tid == 0) *a.refused = seq == -2;  // every block says the same
     if (seq < 0) return;
   } else {
     seq = (int)blockIdx.x / a.per_seq;

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
   int seq, first = 0, count = 0;
   int64_t item0 = 0;
   if (a.b.starts) {
-    seq = kv_find_seq(a.b, item, a.group, 8, 1, &slot, item0);
+    seq = kv_find_seq(a.b, item, a.group, 8, 1, a.c.status, &slot, item0);
   } else {
     seq = item / a.per_seq;
     item0 = (int64_t)seq * a.per_seq;

@@ -145,7 +145,7 @@ RTR_DEVICE bool kv_page_rows(const KvCache& c, const KvBatch& b, int64_t item, i
   int seq;
   int64_t item0;
   if (b.starts) {
-    seq = kv_find_seq(b, item, 1, c.page_shift, 2, slot, item0);
+    seq = kv_find_seq(b, item, 1, c.page_shift, 2, c.status, slot, item0);
     if (seq < 0) return false;
   } else {
     seq = (int)(item / per_seq);

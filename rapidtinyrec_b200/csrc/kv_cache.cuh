@@ -43,7 +43,7 @@ struct KvBatch {
 };
 
 // The rows of one sequence: first row and count; false (with the status bit) when starts
-// does not fit the call.
+// does not fit the call (kv_find_seq has looked; this is what the addresses come from).
 RTR_DEVICE bool kv_rows(const KvBatch& b, int seq, uint32_t* status, int& first, int& count) {
   if (!b.starts) {
     count = b.rows / b.seqs;
@@ -67,18 +67,25 @@ RTR_DEVICE bool kv_len_fits(const KvCache& c, const KvBatch& b, int len, int lea
 
 // Which sequence a work item belongs to, when sequence b's items are those from
 // (starts[b] * num >> shift) + b * extra on: found by all threads of the block, each
-// looking at some sequences.  -1 for an item behind the last sequence's.  (At most one
-// sequence matches while starts is sorted; where it is not, kv_rows refuses the
-// rows or the result is one of the matches.)
-RTR_DEVICE int kv_find_seq(const KvBatch& b, int64_t item, int num, int shift, int extra, int* slot, int64_t& item0) {
+// looking at some sequences.  -1 for an item behind the last sequence's.  Where any of
+// starts does not fit the call the call is refused: -2 for every item, and the status bit.
+// (Some sequences of such a call match no item, others match one another's.)
+RTR_DEVICE int kv_find_seq(const KvBatch& b, int64_t item, int num, int shift, int extra, uint32_t* status, int* slot,
+                           int64_t& item0) {
   if (threadIdx.x == 0) *slot = -1;
   __syncthreads();
+  bool wrong = false;
   for (int s = threadIdx.x; s < b.seqs; s += blockDim.x) {
-    const int64_t lo = ((int64_t)b.starts[s] * num >> shift) + (int64_t)s * extra;
-    const int64_t hi = ((int64_t)b.starts[s + 1] * num >> shift) + (int64_t)(s + 1) * extra;
+    const int first = b.starts[s], end = b.starts[s + 1];
+    wrong |= first < 0 || end < first || end > b.rows;
+    const int64_t lo = ((int64_t)first * num >> shift) + (int64_t)s * extra;
+    const int64_t hi = ((int64_t)end * num >> shift) + (int64_t)(s + 1) * extra;
     if (item >= lo && item < hi) *slot = s;
   }
-  __syncthreads();
+  if (__syncthreads_or(wrong)) {
+    if (threadIdx.x == 0) atomicOr(status, RTR_DEV_BAD_LENGTH);
+    return -2;
+  }
   const int seq = *slot;
   if (seq >= 0) item0 = ((int64_t)b.starts[seq] * num >> shift) + (int64_t)seq * extra;
   return seq;

@@ -13,7 +13,9 @@ What the three share: ``table`` int32 ``[seqs, width]`` page numbers, ``lens`` i
 ``b``'s; without it every sequence has the same number.  All are device tensors and
 are not read on the host, so nothing here synchronises and every call can be captured
 into a CUDA graph.  What does not fit (a page number outside the cache, a length that
-the table cannot hold) leaves its work undone and sets a bit that ``check`` raises for.
+the table cannot hold) leaves its work undone and sets a bit that ``check`` raises for:
+attention's rows of that sequence become NaN.  ``starts`` that decrease, or leave the call's
+rows, leave out the whole call: no row and no page is written.
 The operators serve inference: their results carry no gradient.
 """
 from __future__ import annotations

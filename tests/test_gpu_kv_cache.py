@@ -816,6 +816,40 @@ def test_what_does_not_fit_is_left_out_and_reported(fault):
         assert ((out[4:].double() - want[0]).abs() <= want[2]).all()
 
 
+@pytest.mark.parametrize('starts,rows', [([0, 300, 100, 400], 400), ([5000, 5002, 5004, 5006], 10),
+                                         ([0, 4, 400, 100], 400), ([0, 100, 200, 401], 400), ([-1, 100, 200, 400], 400),
+                                         ([400, 300, 200, 100], 400), ([0, -(1 << 31), (1 << 31) - 1, 400], 400)])
+@pytest.mark.parametrize('width', [25, 600])
+def test_starts_that_do_not_fit_leave_out_the_whole_call(starts, rows, width):
+    """Also where no work item, or more than one, would match a sequence; tables so wide that stretches
+    are joined by a kernel."""
+    from rapidtinyrec_b200._native import NativeError
+    cache = filled(80, 2, 16, 128, seed=83)
+    table = tables([400, 400, 400], 16, 80, seed=84, width=width)
+    lens, bad = ints([400, 400, 400]), ints(starts)
+    x = torch.randn(rows, 2, 128, device='cuda')
+    before = [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    calls = [lambda: cache.write(x, x, table, lens, starts=bad)]
+    outs = []
+    for dtype in DTYPES:
+        for heads in (2, 8, 64):
+            q = torch.randn(rows, heads, 128, device='cuda').to(dtype)
+            outs.append(torch.full_like(q, 7.0))
+            calls.append(lambda q=q, out=outs[-1]: cache.attention(q, table, lens, starts=bad, out=out))
+    outs += [torch.full_like(x, 7.0), torch.full_like(x, 7.0)]
+    calls.append(lambda: cache.read(rows, table, lens, starts=bad, out=outs[-2:]))
+    for call in calls:
+        call()
+        with pytest.raises(NativeError, match='row range'):
+            cache.check()
+    assert all((out == 7).all() for out in outs)
+    for t, was in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), before):
+        assert torch.equal(t.view(torch.uint8), was)
+    # the next call, with starts that fit
+    q = torch.randn(9, 8, 128, device='cuda')
+    check_attention(cache, q, table, [400] * 3, [4, 0, 5], True, starts=ints([0, 4, 4, 9]))
+
+
 def test_python_refuses_what_the_kernels_cannot_take():
     cache = filled(4, 2, 16, 64, seed=32)
     q, x = torch.randn(2, 4, 64, device='cuda'), torch.randn(2, 2, 64, device='cuda')
