@@ -67,6 +67,8 @@ class KeptPrefix(NamedTuple):
     table: object      # int32 [pages] on the engine's device
     ids: np.ndarray
     hidden: object     # final hidden state of the last prompt token
+    pages: tuple = ()  # the table's numbers, and what says whose pages they are (KvCache8.kept)
+    owner: object = None
 
 
 class BeamEngine:
@@ -230,7 +232,8 @@ class BeamEngine:
 
     def keep_prefix(self, prompt_ids, store, pages):
         """After ``prefill(prompt_ids)`` and before the first decode step: quantise the prefix into
-        the store's ``pages`` (page numbers, as many as the prompt needs)."""
+        the store's ``pages`` (page numbers, as many as the prompt needs).  A ``KeptPrefix`` that held
+        one of them before ends with that: ``generate_kept`` refuses it."""
         import torch
         dev = f'cuda:{self.device}'
         ids = self._ids(prompt_ids).copy()
@@ -247,8 +250,10 @@ class BeamEngine:
         torch.cuda.synchronize(self.device)
         self._check(self.lib.rtr_keep_prefix(self.handle, store._at, table.data_ptr(), table.numel(),
                                              hidden.data_ptr()))
+        owner = object()
+        store.kept.update(dict.fromkeys(pages, owner))
         store.check()
-        return KeptPrefix(store, table, ids, hidden)
+        return KeptPrefix(store, table, ids, hidden, tuple(pages), owner)
 
     def generate_and_keep(self, prompt_ids, store, pages):
         """``generate`` that also keeps the prefix: the record and the ``KeptPrefix``."""
@@ -260,8 +265,12 @@ class BeamEngine:
 
     def generate_kept(self, kept, in_place=True):
         """A request of a user whose prefix was kept: no prefill.  ``in_place``: decode attention
-        over the 8-bit pages; otherwise the pages are first read back into the arena."""
+        over the 8-bit pages; otherwise the pages are first read back into the arena.  The pages must
+        be as ``keep_prefix`` left them: those that a later ``keep_prefix`` took are noticed, what else is
+        written to the store is not."""
         import torch
+        if any(kept.store.kept.get(p, kept.owner) is not kept.owner for p in kept.pages):
+            raise ValueError('pages of the prefix were given to another one since it was kept')
         want = torch.float32 if self.cfg.dtype == 'fp32' else torch.bfloat16
         if kept.store.device.index != self.device or kept.hidden.dtype != want or \
                 kept.hidden.numel() != self.cfg.hidden:

@@ -94,6 +94,7 @@ class KvCache8:
                                    k_scale.stride(0) if pages > 1 else heads, pages, heads, page, dim,
                                    status.data_ptr())
         self._at = ctypes.addressof(self._c)
+        self.kept = {}  # page number -> what the last prefix kept there is known by (BeamEngine.keep_prefix)
         self._scale = 1.0 / math.sqrt(dim)
 
     @classmethod

@@ -179,6 +179,34 @@ def test_prefixes_of_another_engine(tiny, engine):
     assert engine.generate_kept(kept) == again
 
 
+def test_a_prefix_whose_pages_were_given_away_is_refused(tiny, engine):
+    from rapidtinyrec_b200._native import NativeError
+    a, b = prompts(tiny)[:2]
+    store = engine.prefix_store(8, 16)
+    n = max(pages_for(a, 16), pages_for(b, 16))
+    assert n < 8
+    _, first = engine.generate_and_keep(a, store, range(n))
+    record = engine.generate_kept(first)
+    # what refuses to be kept takes no pages
+    with pytest.raises(NativeError):
+        engine.keep_prefix(a, store, range(n))
+    assert engine.generate_kept(first) == record
+    engine.prefill(b)
+    with pytest.raises(NativeError):
+        engine.keep_prefix(b, store, [0])
+    assert engine.generate_kept(first) == record
+    for count in (n, 1):  # all of its pages, or one
+        _, second = engine.generate_and_keep(b, store, list(range(count - 1, -1, -1)) + list(range(7, 7 - (n - count), -1)))
+        for in_place in (True, False):
+            with pytest.raises(ValueError, match='given to another'):
+                engine.generate_kept(first, in_place=in_place)
+        other = engine.generate_kept(second)
+        _, first = engine.generate_and_keep(a, store, range(n))
+        assert engine.generate_kept(first) == record != other
+        with pytest.raises(ValueError, match='given to another'):
+            engine.generate_kept(second)
+
+
 def test_a_prompt_that_was_not_prefilled_is_not_kept(tiny, engine):
     ids = list(prompts(tiny)[0])
     store = engine.prefix_store(8)
