@@ -10,6 +10,8 @@ the reference's per-user record (``benchmark_inference.py:150-154``).
 from __future__ import annotations
 
 import ctypes
+import dataclasses
+import hashlib
 from typing import NamedTuple
 
 import numpy as np
@@ -61,6 +63,14 @@ def weight_order(cfg: ModelConfig):
     return names
 
 
+def model_key(cfg: ModelConfig, tensors):
+    """What a model is known by: its shapes and constants, and 4,096 values spread over each weight."""
+    import torch
+    fields = {k: v for k, v in dataclasses.asdict(cfg).items() if k != 'name'}
+    some = torch.cat([t.reshape(-1)[::max(1, t.numel() // 4096)] for t in tensors])
+    return hashlib.sha256(repr(sorted(fields.items())).encode() + some.cpu().numpy().tobytes()).hexdigest()
+
+
 class KeptPrefix(NamedTuple):
     """One user's prefix in a store (``BeamEngine.keep_prefix``)."""
     store: KvCache8
@@ -69,10 +79,12 @@ class KeptPrefix(NamedTuple):
     hidden: object     # final hidden state of the last prompt token
     pages: tuple = ()  # the table's numbers, and what says whose pages they are (KvCache8.kept)
     owner: object = None
+    model: object = None  # model_key of the engine that kept it
 
 
 class BeamEngine:
     _prefilled = None  # the prompt of the last prefill()
+    _model = None      # model_key of the weights, once loaded
 
     def __init__(self, cfg: ModelConfig, weights, tables, max_prefix: int, device: int = 0,
                  num_beams: int = NUM_BEAMS, max_users: int = 1):
@@ -145,6 +157,7 @@ class BeamEngine:
             torch.cuda.synchronize(self.device)
         self._check(self.lib.rtr_load_weights(self.handle, ptrs, len(tensors), _native.RTR_DTYPE_F32,
                                               int(bool(on_device))))
+        self._model = model_key(self.cfg, tensors)
 
     def close(self):
         if getattr(self, 'handle', None) and self.handle.value:
@@ -253,7 +266,7 @@ class BeamEngine:
         owner = object()
         store.kept.update(dict.fromkeys(pages, owner))
         store.check()
-        return KeptPrefix(store, table, ids, hidden, tuple(pages), owner)
+        return KeptPrefix(store, table, ids, hidden, tuple(pages), owner, self._model)
 
     def generate_and_keep(self, prompt_ids, store, pages):
         """``generate`` that also keeps the prefix: the record and the ``KeptPrefix``."""
@@ -273,7 +286,7 @@ class BeamEngine:
             raise ValueError('pages of the prefix were given to another one since it was kept')
         want = torch.float32 if self.cfg.dtype == 'fp32' else torch.bfloat16
         if kept.store.device.index != self.device or kept.hidden.dtype != want or \
-                kept.hidden.numel() != self.cfg.hidden:
+                kept.hidden.numel() != self.cfg.hidden or kept.model not in (None, self._model):
             raise ValueError('the prefix was kept on another device, or by an engine of another model or type')
         torch.cuda.synchronize(self.device)
         self._check(self.lib.rtr_prefill_kept(self.handle, kept.store._at, kept.table.data_ptr(), kept.table.numel(),

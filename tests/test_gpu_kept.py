@@ -179,6 +179,28 @@ def test_prefixes_of_another_engine(tiny, engine):
     assert engine.generate_kept(kept) == again
 
 
+def test_prefixes_of_another_model_of_the_same_shapes(tiny, engine):
+    """Other weights, or another rope: refused.  The same weights given on the device: taken."""
+    import dataclasses
+    ids = prompts(tiny)[1]
+    store = engine.prefix_store(8)
+    _, kept = engine.generate_and_keep(ids, store, range(pages_for(ids, 64)))
+    again = engine.generate_kept(kept)
+    last = sorted(n for n in tiny['weights'] if n.endswith('k_proj.weight'))[-1]
+    other = dict(tiny['weights'])
+    other[last] = other[last] * 1.01
+    cfg = dataclasses.replace(tiny['cfg'], rope_theta=tiny['cfg'].rope_theta / 10)
+    for model, weights in ((tiny, other), ({**tiny, 'cfg': cfg}, None)):
+        e = make_engine(model, weights)
+        for in_place in (True, False):
+            with pytest.raises(ValueError, match='another'):
+                e.generate_kept(kept, in_place=in_place)
+        e.close()
+    e = make_engine(tiny, {n: w.cuda() for n, w in tiny['weights'].items()})
+    assert e.generate_kept(kept) == again
+    e.close()
+
+
 def test_a_prefix_whose_pages_were_given_away_is_refused(tiny, engine):
     from rapidtinyrec_b200._native import NativeError
     a, b = prompts(tiny)[:2]
