@@ -306,8 +306,8 @@ int rtr_constraint_process_static(rtr_session* s, int32_t step, const int64_t* i
  * A value is code * scale.  Code [page][head][token][dim] lies at
  * page * page_stride + head * head_stride + token * head_dim + dim, its scale at
  * page * scale_stride + head.  head_dim 64 or 128, page 16, 32, 64 or 128 tokens;
- * strides of codes and their addresses are multiples of 16, and a page's last head
- * ends before the next page.  `status` is a device
+ * strides of codes and their addresses are multiples of 16, and either a page's last head
+ * ends before the next page or a head's last page before the next head.  `status` is a device
  * word that the kernels set bits in (never clear): 1 << 5 a length or row range
  * that does not fit, 1 << 9 a page number outside [0, pages), 1 << 10 an old scale
  * that is not positive and finite.  The work concerned is left out (attention:

@@ -329,8 +329,10 @@ const char* kv_check(const rtr_kv_cache* c, const rtr_kv_batch* b) {
   if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128) return "page must be 16, 32, 64 or 128 tokens";
   if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 16384) return "the cache needs pages and 1 to 16384 KV heads";
   const int64_t one = (int64_t)c->page * c->head_dim;  // codes of a page's head
-  if (c->head_stride < one || c->page_stride < one || c->scale_stride < c->kv_heads ||
-      (c->kv_heads > 1 && (c->page_stride - one) / (c->kv_heads - 1) < c->head_stride))
+  if (c->head_stride < one || c->page_stride < one || c->scale_stride < c->kv_heads) return "cache strides overlap";
+  // the heads of a page before the next page, or the pages of a head before the next head
+  if (c->kv_heads > 1 && (c->page_stride - one) / (c->kv_heads - 1) < c->head_stride &&
+      c->pages > 1 && (c->head_stride - one) / (c->pages - 1) < c->page_stride)
     return "cache strides overlap";
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | (uintptr_t)c->page_stride |
        (uintptr_t)c->head_stride) & 15)

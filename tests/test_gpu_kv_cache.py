@@ -306,6 +306,29 @@ def test_strides_of_rows_and_of_the_cache():
     assert torch.equal(one.attention(shifted, table, ints(total), starts=cuts(total)), out)
 
 
+def test_a_cache_with_its_heads_outermost():
+    from rapidtinyrec_b200.kv_cache import KvCache8
+    a = filled(40, 3, 32, 64, seed=85)
+    turned = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (a.k, a.v)]
+    assert turned[0].stride(1) > turned[0].stride(0)
+    b = KvCache8(*turned, a.k_scale.clone(), a.v_scale.clone())
+    counts, lens = [3, 40, 1], [90, 500, 33]
+    table = tables(lens, 32, 40, seed=86)
+    x = torch.randn(44, 3, 64, device='cuda')
+    for cache in (a, b):
+        cache.write(x, 2 * x, table, ints(lens), starts=cuts(counts))
+    assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.v_scale, b.v_scale)
+    for one, two in zip(*(c.read(44, table, ints(lens), starts=cuts(counts)) for c in (a, b))):
+        assert torch.equal(one, two)
+    for dtype in DTYPES:
+        q = torch.randn(44, 12, 64, device='cuda').to(dtype)
+        out, _ = check_attention(b, q, table, lens, counts, True, starts=cuts(counts))
+        assert torch.equal(out, a.attention(q, table, ints(lens), starts=cuts(counts)))
+    cut = b.heads(1, 2)
+    q = torch.randn(1500, 12, 64, device='cuda')
+    check_attention(cut, q, table[1:2], [500], [1500], False)
+
+
 # --------------------------------------------------------------- attention
 @pytest.mark.parametrize('heads,kv,dim', SHAPES)
 @pytest.mark.parametrize('dtype', DTYPES)

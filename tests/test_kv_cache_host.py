@@ -59,6 +59,19 @@ def test_pages_that_share_memory_are_refused(change):
         assert write(cache(**fits), batch(rows=0)) == _native.RTR_OK
 
 
+def test_heads_may_lie_outermost():
+    """[heads][pages][page][dim], as one buffer a head: nothing overlaps."""
+    one = 16 * 128
+    for fits in (dict(page_stride=one, head_stride=9 * one), dict(page_stride=2 * one, head_stride=40 * one),
+                 dict(page_stride=16 * one, head_stride=one, pages=1), dict(page_stride=one, head_stride=one, pages=1)):
+        assert write(cache(**fits), batch(rows=0)) == _native.RTR_OK, message()
+        assert attention(cache(**fits), batch(rows=0)) == _native.RTR_OK, message()
+    for bad in (dict(page_stride=one, head_stride=9 * one - 16), dict(page_stride=one + 16, head_stride=9 * one),
+                dict(page_stride=one, head_stride=2 * one), dict(page_stride=one - 16, head_stride=9 * one)):
+        for call in (write, attention):
+            assert call(cache(**bad), batch()) == _native.RTR_ERR_ARG and 'overlap' in message()
+
+
 @pytest.mark.parametrize('change,says', [
     (dict(table=None), 'null table'), (dict(lens=None), 'null table'), (dict(seqs=-1), 'negative'),
     (dict(rows=-1), 'negative'), (dict(table_width=0), 'table rows'), (dict(table_stride=7), 'table rows'),
