@@ -14,6 +14,7 @@
 // copy; the prefix length lives in device memory so the graph serves every L.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -126,7 +127,7 @@ struct rtr_session {
     void* out = nullptr;        // [beams][heads][D]: the prefix's part of the attention
     float* lse = nullptr;
     uint8_t* work = nullptr;
-    int64_t work_bytes = 0;
+    int64_t work_bytes = 0, work_used = 0;  // room, and what this request's attention takes (0: no join kernel)
   } kept;
   // batched decode (rtr_session_create_batched): up to max_users users share each
   // decode step's GEMMs; user u has its own prefix arena, length, beam state and
@@ -176,6 +177,21 @@ static cudaError_t dev_alloc(rtr_session* s, T** p, size_t count) {
   s->device_bytes += (int64_t)(count * sizeof(T) + 256);
   *p = static_cast<T*>(raw);
   return cudaSuccess;
+}
+
+// Room for `count` elements where *p has `room` (0: none yet): the former buffer is given back,
+// once what still uses it has run.
+template <typename T>
+static cudaError_t dev_grow(rtr_session* s, T** p, size_t room, size_t count) {
+  if (*p) {
+    cudaError_t e = cudaStreamSynchronize(s->stream);
+    if (e == cudaSuccess) e = cudaFree(*p);
+    if (e != cudaSuccess) return e;
+    s->allocs.erase(std::find(s->allocs.begin(), s->allocs.end(), static_cast<void*>(*p)));
+    s->device_bytes -= (int64_t)(room * sizeof(T) + 256);
+    *p = nullptr;
+  }
+  return dev_alloc(s, p, count);
 }
 
   // split-K tickets: one per output tile
@@ -1198,17 +1214,20 @@ int rtr_prefill_kept(rtr_session* s, const rtr_kv_cache* cache, const int32_t* t
     if (!k.out) {
       float* out = nullptr;
       CUDA_TRY(s, dev_alloc(s, &out, (size_t)beams_of(s) * c.heads * D));
-      CUDA_TRY(s, dev_alloc(s, &k.lse, (size_t)beams_of(s) * c.heads));
       k.out = out;
     }
+    if (!k.lse) CUDA_TRY(s, dev_alloc(s, &k.lse, (size_t)beams_of(s) * c.heads));
     if (table_width > k.table_room) {
-      CUDA_TRY(s, dev_alloc(s, &k.table, (size_t)table_width));
+      const int room = std::exchange(k.table_room, 0);
+      CUDA_TRY(s, dev_grow(s, &k.table, room, table_width));
       k.table_room = table_width;
     }
     if (bytes > k.work_bytes) {
-      CUDA_TRY(s, dev_alloc(s, &k.work, (size_t)bytes));
+      const int64_t room = std::exchange(k.work_bytes, 0);
+      CUDA_TRY(s, dev_grow(s, &k.work, room, bytes));
       k.work_bytes = bytes;
     }
+    k.work_used = bytes;
     k.cache = *cache;
     k.width = table_width;
     CUDA_TRY(s, cudaMemcpyAsync(k.table, table_dev, table_width * sizeof(int32_t), cudaMemcpyDeviceToDevice, s->stream));
@@ -1246,7 +1265,7 @@ int rtr_decode_step(rtr_session* s, int32_t t) {
   CUDA_TRY(s, cudaSetDevice(s->device));
   CUDA_TRY(s, decode_and_tail(s, t));
   s->launches += forward_kernels(s, false) + decode_tail_kernels(s);
-  if (s->kept.on) s->launches += (int64_t)s->cfg.layers * (s->kept.work_bytes ? 2 : 1);  // the join(s) beside the attention
+  if (s->kept.on) s->launches += (int64_t)s->cfg.layers * (s->kept.work_used ? 2 : 1);  // the join(s) beside the attention
   s->steps_done = t;
   return RTR_OK;
 }

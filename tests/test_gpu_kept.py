@@ -179,6 +179,35 @@ def test_prefixes_of_another_engine(tiny, engine):
     assert engine.generate_kept(kept) == again
 
 
+def test_wider_tables_give_back_what_narrower_ones_took(tiny):
+    """Tables of more pages than the prompt needs, each wider than the last: the session ends up with
+    the room of the widest alone; and a narrow one's launches are counted as its own."""
+    ids = prompts(tiny)[0]
+    n = pages_for(ids, 16)
+    bytes_, launches = [], []
+    for widths in ([n, n + 1, 600, 900, 1300], [1300]):
+        e = make_engine(tiny)
+        store = e.prefix_store(1300, 16)
+        records = []
+        for w in widths:
+            kept = e.generate_and_keep(ids, store, range(w))[1]
+            records.append(e.generate_kept(kept))
+        for r in records[1:]:
+            same(r, records[0])
+        bytes_.append(e.report()['device_bytes'])
+        before = e.report()['kernel_launches']
+        e.generate_kept(kept)
+        launches.append(e.report()['kernel_launches'] - before)
+        kept = e.generate_and_keep(ids, store, range(n))[1]
+        before = e.report()['kernel_launches']
+        same(e.generate_kept(kept), records[0])
+        launches.append(e.report()['kernel_launches'] - before)
+        e.close()
+    assert bytes_[0] == bytes_[1]
+    assert launches[0] == launches[2] and launches[1] == launches[3]
+    assert launches[0] - launches[1] == 4 * tiny['cfg'].layers  # the wide ones' join kernel
+
+
 def test_prefixes_of_another_model_of_the_same_shapes(tiny, engine):
     """Other weights, or another rope: refused.  The same weights given on the device: taken."""
     import dataclasses
