@@ -429,12 +429,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
     for (int j = 0; j < PER; ++j) x[j] = fmaf(p[j], f, x[j]);
   }
   mt -= KA_LIFT;  // what the sums are relative to
-  // every visible score is minus infinity (0 / 0), or the sequence's length did not fit
-  if (lt == 0.f && (limit(r0 + row) > c0 || !whole)) lt = __int_as_float(0x7fffffff);
+  if (!whole) lt = __int_as_float(0x7fffffff);  // the sequence's length did not fit
+  else if (lt == 0.f && limit(r0 + row) > c0) mt = KV_ALL_LOW;
   const auto head_row = [&](int rr) {
     return (int64_t)(first + rr / a.group) * a.heads + kvh * a.group + rr % a.group;
   };
   const auto finish = [&](int rr) {
+    lt = kv_whole_sum(mt, lt);
     const bool sees = lt != 0.f;
     const float inv = sees ? 1.0f / lt : 0.f;
     const int64_t rh = head_row(rr);
@@ -538,6 +539,7 @@ __global__ void __launch_bounds__(KJ_THREADS) kv_attn_join_kernel(const KvBatch 
   lt = 0.f;
 #pragma unroll
   for (int w = 0; w < KJ_THREADS / 32; ++w) lt += red[1][w];
+  lt = kv_whole_sum(mt, lt);
 #pragma unroll
   for (int i = 1; i < LANES; ++i) {
     const float4 v = sums[i][col];

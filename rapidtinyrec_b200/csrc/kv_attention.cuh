@@ -38,6 +38,12 @@ constexpr float KA_LIFT = 15.0f;
 // an accumulator of its own: 22 bits down to the same 2^-29.
 constexpr float KA_LOW = 2048.0f;
 
+// A row's sum l, in units of 2^m.  A row that sees nothing has m = -infinity and l = 0; one that
+// sees keys whose scores are all minus infinity (products beyond float's range) has KV_ALL_LOW and
+// l = 0: nothing beside a stretch that has more, NaN (0 / 0) where all stretches are so.
+constexpr float KV_ALL_LOW = -3.402823466e+38f;
+RTR_DEVICE float kv_whole_sum(float m, float l) { return l == 0.f && m != -INFINITY ? __int_as_float(0x7fffffff) : l; }
+
 // v / group for v < 2^32 / group (v is a row's place within some tiles): one multiplication.
 // A group of one has no 32-bit inverse.
 RTR_DEVICE int kv_div(const KvAttn& a, int v) { return a.group == 1 ? v : (int)__umulhi((uint32_t)v, a.group_inverse); }

@@ -507,7 +507,6 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       }
     }
 
-    float lt = l;
     if (bars.nans) {  // NaN codes of V entered the products as 0: put back what the row sees
       for (int key = max(c0, kmin & ~(KT_KEYS - 1)); key < min(lim, c1); ++key) {
         const uint8_t* p = a.c.v + seg_at[(key - c0) >> 4] + (key & 15) * D + half * HD;
@@ -521,7 +520,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
         }
       }
     }
-    if (lt == 0.f && (lim > c0 || !whole)) lt = __int_as_float(0x7fffffff);
+    if (!whole) l = __int_as_float(0x7fffffff);  // the sequence's length did not fit
+    else if (l == 0.f && lim > c0) m = KV_ALL_LOW;
     // through shared memory (the operands are done with), for whole lines on the way out
     float* stage = reinterpret_cast<float*>(smem + C::STAGE_OFF);
     const auto value = [&](int i) { return i & 1 ? f2_parts(o[i >> 1]).y : f2_parts(o[i >> 1]).x; };
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       reinterpret_cast<float4*>(stage + r * C::STAGE_LD + half * HD)[j] =
           make_float4(value(j), value(NL + j), value(2 * NL + j), value(3 * NL + j));
     row_barrier();  // red has been read
-    if (half == 0) reinterpret_cast<float2*>(red)[r] = make_float2(m - LIFT, lt);
+    if (half == 0) reinterpret_cast<float2*>(red)[r] = make_float2(m - LIFT, l);
   } else if (warp < 8 + C::CODE_WARPS) {
     // ------------------------------------------------------------ codes
     KtCodes<D, C::CODE_WARPS> codes(a.c, seg_at, segs, warp - 8, lane);
@@ -646,6 +646,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   const int col = lane % LPR;
   const auto finish = [&](int row, float m, float l, float4 x) {
     const int64_t rh = row_out[row];
+    l = kv_whole_sum(m, l);
     const bool sees = l != 0.f;
     const float inv = sees ? 1.0f / l : 0.f;
     x = sees ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);

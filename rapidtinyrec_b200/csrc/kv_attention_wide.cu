@@ -321,8 +321,9 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
     if (n > 0 && active) mbar_wait(smem_addr(&bars.o_full[g][1]), (n - 1) & 1, abort_flag);
     tc_fence_after();
     row_barrier();  // both tiles are done with the operands
-    float lt = l;
-    if (lt == 0.f && (lim > c0 || !whole)) lt = __int_as_float(0x7fffffff);
+    if (!whole) l = __int_as_float(0x7fffffff);  // the sequence's length did not fit
+    else if (l == 0.f && lim > c0) m = KV_ALL_LOW;
+    const float lt = alone ? kv_whole_sum(m, l) : l;
     // A whole item: finished values as bf16; a stretch: sums as they are.
     const bool sees = lt != 0.f;
     const float inv = !alone ? 1.f : sees ? 1.0f / lt : 0.f;
@@ -512,6 +513,7 @@ __global__ void __launch_bounds__(32 * KW_JOIN) kv_attn_wide_join_kernel(const K
     l = fmaf(p.y, f, l);
     x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
   }
+  l = kv_whole_sum(m, l);
   const bool sees = l != 0.f;
   const float inv = sees ? 1.0f / l : 0.f;
   x = sees ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);

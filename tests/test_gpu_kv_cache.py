@@ -728,6 +728,40 @@ def test_keys_beside_one_that_outweighs_them(dtype, heads, kv, dim, rows, tokens
     cache.check()
 
 
+@pytest.mark.parametrize('dtype,heads,kv,dim,rows,tokens', OUTWEIGHED)
+@pytest.mark.parametrize('low', ['first', 'last'])
+def test_scores_beyond_float_in_some_pages(dtype, heads, kv, dim, rows, tokens, low):
+    """Most pages hold K so large that every score is minus infinity in float (2^75 * 448 * 2^48 * dim), the
+    others zeros: the output is the mean of their V, whichever block has which.  Weights are equal and
+    exact or one fp16 value (2^-12), their positive terms added in tokens / 16 + 64 steps of 2^-22."""
+    page = 32
+    pages = -(-tokens // page)
+    cache = filled(pages, kv, page, dim, seed=87)
+    g = torch.Generator().manual_seed(88)
+    table = tables([tokens], page, pages, seed=89)
+    ids = table.tolist()[0]
+    cache.v.copy_((torch.randint(8, 449, cache.v.shape, generator=g).float()).to(F8))
+    cache.v_scale.fill_(2.0 ** -7)
+    cache.k.zero_()
+    cut = pages * 17 // 20 if low == 'first' else pages * 3 // 20
+    for p in ids[:cut] if low == 'first' else ids[cut:]:
+        cache.k[p], cache.k_scale[p] = 448.0, 2.0 ** 48
+    q = torch.full((rows, heads, dim), -2.0 ** 75, device='cuda').to(dtype)
+    out, lse = cache.attention(q, table, ints([tokens]), causal=False, return_lse=True)
+    v = gather(cache.v, cache.v_scale, ids, tokens)
+    v = v[cut * page:] if low == 'first' else v[:cut * page]
+    want = v.mean(0).repeat_interleave(heads // kv, 0)
+    rel = (0.0 if dtype == torch.float32 else 2.0 ** -12) + (tokens / 16 + 64) * 2.0 ** -22
+    off = ((out.double() - want).abs() / want).max()
+    assert off <= rel + torch.finfo(dtype).eps / 2, off
+    assert (lse.double() - math.log(len(v))).abs().max() <= rel + 2.0 ** -20
+    # where no key is left that counts, 0 / 0
+    cache.k.fill_(448.0)
+    cache.k_scale.fill_(2.0 ** 48)
+    assert cache.attention(q, table, ints([tokens]), causal=False).isnan().all()
+    cache.check()
+
+
 def test_bad_k_scales_make_their_rows_nan():
     cache = filled(4, 1, 16, 64, seed=54)
     table = ints([[0, 1], [2, 3]])
