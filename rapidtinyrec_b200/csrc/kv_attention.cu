@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   constexpr int VW = D / 32;   // words of a V row a lane holds
   constexpr int DG = D / 8;    // dimensions of the output a lane holds, for two rows
   extern __shared__ __align__(128) uint8_t ka_smem[];
-  __shared__ int slot;
+  __shared__ int slot[2];
   __shared__ float join_m[KA_WARPS][KA_ROWS], join_l[KA_WARPS][KA_ROWS];
   __shared__ __align__(16) float sum_o[KA_ROWS][D];  // this block's sums, read by its cluster
   __shared__ float2 sum_ml[KA_ROWS];
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
   int seq;
   int64_t item0;
   if (a.b.starts) {
-    seq = kv_find_seq(a.b, blockIdx.x, a.group, 3, 1, a.c.status, &slot, item0);
+    seq = kv_find_seq(a.b, blockIdx.x, a.group, 3, 1, a.c.status, slot, item0);
     if (a.refused && tid == 0) *a.refused = seq == -2;  // every block says the same
     if (seq < 0) return;
   } else {

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   constexpr int HD = D / 2;    // dimensions of the output a row thread finishes
   constexpr int NL = D / 8;    // of those, the ones with the same d % 4
   extern __shared__ uint8_t kt_smem_raw[];
-  __shared__ int slot;
+  __shared__ int slot[2];
   uint8_t* smem = kt_smem_raw + ((1024u - (smem_addr(kt_smem_raw) & 1023u)) & 1023u);
   uint8_t* qs = smem + C::Q_OFF;
   int64_t* seg_at = reinterpret_cast<int64_t*>(smem + C::SEG_OFF);
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   int seq;
   int64_t item0;
   if (a.b.starts) {
-    seq = kv_find_seq(a.b, blockIdx.x, a.group, 7, 1, a.c.status, &slot, item0);
+    seq = kv_find_seq(a.b, blockIdx.x, a.group, 7, 1, a.c.status, slot, item0);
     if (a.refused && tid == 0) *a.refused = seq == -2;  // every block says the same
     if (seq < 0) return;
   } else {

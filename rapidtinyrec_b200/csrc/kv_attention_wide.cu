@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
   using C = KwCfg;
   constexpr int D = C::D;
   extern __shared__ uint8_t kw_smem_raw[];
-  __shared__ int slot;
+  __shared__ int slot[2];
   uint8_t* smem = kw_smem_raw + ((1024u - (smem_addr(kw_smem_raw) & 1023u)) & 1023u);
   int64_t* seg_at = reinterpret_cast<int64_t*>(smem + C::SEG_OFF);
   float* seg_k = reinterpret_cast<float*>(seg_at + KW_SEGS);
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
   int seq, first = 0, count = 0;
   int64_t item0 = 0;
   if (a.b.starts) {
-    seq = kv_find_seq(a.b, item, a.group, 8, 1, a.c.status, &slot, item0);
+    seq = kv_find_seq(a.b, item, a.group, 8, 1, a.c.status, slot, item0);
   } else {
     seq = item / a.per_seq;
     item0 = (int64_t)seq * a.per_seq;

@@ -175,12 +175,12 @@ __global__ void __launch_bounds__(KV_THREADS, CH == 4 && !AHEAD ? 3 : 2) kv_writ
                                                               const T* v, const KvRows rs, int per_seq,
                                                               int units) {
   constexpr int N = 16 / sizeof(T), DPR = D / N;  // values of a piece, pieces of a row
-  __shared__ int slot;
+  __shared__ int slot[2];
   __shared__ uint32_t red[2][KV_THREADS / 32];
   PageRows pr;
   pdl_launch_dependents();
   pdl_wait();
-  if (!kv_page_rows(c, b, blockIdx.x, per_seq, &slot, pr)) return;
+  if (!kv_page_rows(c, b, blockIdx.x, per_seq, slot, pr)) return;
   const int tid = threadIdx.x, warps = blockDim.x >> 5;
   const int u0 = blockIdx.y * units, u1 = min(2 * c.kv_heads, u0 + units);
   const bool kept = pr.lo > 0;  // the page holds older tokens of the sequence
@@ -272,11 +272,11 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvCache c, co
                                                              T* v, const KvRows rs, int per_seq,
                                                              int units) {
   constexpr int N = 16 / sizeof(T), DPR = D / N;
-  __shared__ int slot;
+  __shared__ int slot[2];
   PageRows pr;
   pdl_launch_dependents();
   pdl_wait();
-  if (!kv_page_rows(c, b, blockIdx.x, per_seq, &slot, pr)) return;
+  if (!kv_page_rows(c, b, blockIdx.x, per_seq, slot, pr)) return;
   const int tid = threadIdx.x;
   const int u0 = blockIdx.y * units, u1 = min(2 * c.kv_heads, u0 + units);
   const auto load = [&](int u, Codes<N> (&q)[CH], float& scale) {

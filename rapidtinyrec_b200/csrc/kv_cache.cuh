@@ -72,21 +72,24 @@ RTR_DEVICE bool kv_len_fits(const KvCache& c, const KvBatch& b, int len, int lea
 // (Some sequences of such a call match no item, others match one another's.)
 RTR_DEVICE int kv_find_seq(const KvBatch& b, int64_t item, int num, int shift, int extra, uint32_t* status, int* slot,
                            int64_t& item0) {
-  if (threadIdx.x == 0) *slot = -1;
+  if (threadIdx.x == 0) {
+    slot[0] = -1;
+    slot[1] = 0;
+  }
   __syncthreads();
-  bool wrong = false;
   for (int s = threadIdx.x; s < b.seqs; s += blockDim.x) {
     const int first = b.starts[s], end = b.starts[s + 1];
-    wrong |= first < 0 || end < first || end > b.rows;
+    if (first < 0 || end < first || end > b.rows) slot[1] = 1;
     const int64_t lo = ((int64_t)first * num >> shift) + (int64_t)s * extra;
     const int64_t hi = ((int64_t)end * num >> shift) + (int64_t)(s + 1) * extra;
-    if (item >= lo && item < hi) *slot = s;
+    if (item >= lo && item < hi) slot[0] = s;
   }
-  if (__syncthreads_or(wrong)) {
+  __syncthreads();
+  if (slot[1]) {
     if (threadIdx.x == 0) atomicOr(status, RTR_DEV_BAD_LENGTH);
     return -2;
   }
-  const int seq = *slot;
+  const int seq = slot[0];
   if (seq >= 0) item0 = ((int64_t)b.starts[seq] * num >> shift) + (int64_t)seq * extra;
   return seq;
 }
