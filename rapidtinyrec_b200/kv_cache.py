@@ -114,10 +114,12 @@ class KvCache8:
         return KvCache8(self.k[:, cut], self.v[:, cut], self.k_scale[:, cut], self.v_scale[:, cut], self.status)
 
     def check(self):
-        """Raise for what earlier calls left undone (synchronises), and forget it."""
+        """Raise for what earlier calls, on any stream, left undone (waits for them), and forget it."""
+        torch.cuda.synchronize(self.device)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)  # before a later call on another stream can set a bit
             raise _native.NativeError(_native.RTR_ERR_DEVICE, '; '.join(t for b, t in _STATUS.items() if bits & b))
 
     # ------------------------------------------------------------ operators

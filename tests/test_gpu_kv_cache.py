@@ -964,6 +964,23 @@ def test_other_streams_and_captured_graphs():
     cache.check()
 
 
+def test_check_waits_for_calls_on_other_streams():
+    from rapidtinyrec_b200._native import NativeError
+    cache = filled(4, 2, 16, 64, seed=90)
+    q, lens = torch.randn(1, 4, 64, device='cuda'), ints([20])
+    tables_ = ints([[0, 1]]), ints([[0, 4]])
+    cache.attention(q, tables_[0], lens)
+    cache.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)  # cycles, some 50 ms
+        cache.attention(q, tables_[1], lens)
+    with pytest.raises(NativeError, match='page'):
+        cache.check()
+    cache.check()
+
+
 def test_calls_on_two_streams_at_once():
     cache = filled(80, 2, 64, 128, seed=36)
     table = tables([5000], 64, 80, seed=37)
