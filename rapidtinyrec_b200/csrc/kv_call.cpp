@@ -4,6 +4,7 @@
 // Python, as long as the smallest kernels run; here it costs under 2.
 //
 // The module links against torch only; setup() hands it the C entry points' addresses.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/cuda/EmptyTensor.h>
@@ -114,14 +115,14 @@ at::Tensor room_for(const Cache& cache, at::IntArrayRef size, at::ScalarType typ
 at::Tensor copied(const at::Tensor& x) { return x.clone(at::MemoryFormat::Contiguous); }
 
 template <typename F> PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F&& body) {
+  HANDLE_TH_ERRORS  // torch's own exceptions as torch raises them (OutOfMemoryError, say)
   try {
     if (given != wanted) refuse("%d arguments expected", (int)wanted);
     return body();
   } catch (const Raised&) {
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
   }
-  return nullptr;
+  END_HANDLE_TH_ERRORS
 }
 
 // write(cache, device, k, v, table, lens, starts)

@@ -929,6 +929,14 @@ def test_python_refuses_what_the_kernels_cannot_take():
     cache.check()
 
 
+def test_outputs_that_memory_cannot_hold():
+    """The allocator's error comes as torch raises it, and the cache serves on."""
+    cache = filled(4, 2, 16, 64, seed=91)
+    with pytest.raises(torch.OutOfMemoryError):
+        cache.read(1 << 30, ints([[0]]), ints([4]))  # 512 GiB each
+    check_attention(cache, torch.randn(1, 4, 64, device='cuda'), ints([[1]]), [9], [1], True)
+
+
 # -------------------------------------------------------- streams and graphs
 def test_other_streams_and_captured_graphs():
     """Calls on a side stream; two graphs over one cache, replayed with other inputs."""
