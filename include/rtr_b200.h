@@ -246,6 +246,9 @@ int rtr_attention_check(int32_t device, const float* q_dev, const float* k_dev, 
  * timeout bit of the session's status word, so the request fails with
  * RTR_ERR_DEVICE and the next request runs normally.  Applies to kernels
  * launched (or graph nodes replayed) after the call; wait_cycles >= 1000.
+ * The 8-bit KV cache's attention is bounded and fails the same way (its tiles of many rows
+ * then withhold the last K of a block's keys; the bit is set in the cache's status
+ * word); a captured call keeps the setting it was captured with.
  * Blocks until the setting is on the device. */
 int rtr_debug_wait_control(int32_t device, int64_t wait_cycles, int32_t withhold_activation_copies);
 

@@ -203,5 +203,5 @@ DEFAULT_WAIT_CYCLES = 2_000_000_000
 
 
 def wait_control(device, wait_cycles=DEFAULT_WAIT_CYCLES, withhold_activation_copies=False):
-    """Test control of the tensor-core GEMMs' bounded pipeline waits (``rtr_debug_wait_control``)."""
+    """Test control of the bounded waits of the tensor-core GEMMs and the KV attention (``rtr_debug_wait_control``)."""
     check(load().rtr_debug_wait_control(device, int(wait_cycles), int(bool(withhold_activation_copies))))

@@ -102,6 +102,7 @@ cudaError_t gemm_f16x2_init();
 // activation producers issue no copy (so those waits run out).
 cudaError_t gemm_f16x2_wait_control(long long wait_cycles, int withhold_x);
 cudaError_t gemm_bf16_wait_control(long long wait_cycles, int withhold_x);
+void kv_attn_wait_control(int device, long long wait_cycles, int withhold);  // kernels launched from then on
 cudaError_t gemm_f16x2(const TensorMap& tmW, const TensorMap& tmXh, const TensorMap& tmXl, float* C, float* C_big,
                        float* C_small, int ldc, const float* bias, int M, int N, int K, int epi, float* ws,
                        size_t ws_floats, int* tickets, int max_tickets, uint32_t* status, int sms, cudaStream_t stream,

@@ -130,5 +130,6 @@ extern "C" int rtr_debug_wait_control(int32_t device, int64_t wait_cycles, int32
   if (rtr::gemm_f16x2_wait_control(wait_cycles, withhold_activation_copies) != cudaSuccess ||
       rtr::gemm_bf16_wait_control(wait_cycles, withhold_activation_copies) != cudaSuccess)
     return RTR_ERR_CUDA;
+  rtr::kv_attn_wait_control(device, wait_cycles, withhold_activation_copies);
   return RTR_OK;
 }

@@ -698,6 +698,19 @@ static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   return p;
 }
 
+// What rtr_debug_wait_control has set, by device.
+constexpr int KV_DEVICES = 64;
+struct KvWait {
+  std::atomic<long long> cycles{kWaitCycles};
+  std::atomic<int> withhold{0};
+};
+static KvWait kv_wait[KV_DEVICES];
+void kv_attn_wait_control(int device, long long wait_cycles, int withhold) {
+  if (device < 0 || device >= KV_DEVICES) return;
+  kv_wait[device].cycles.store(wait_cycles, std::memory_order_relaxed);
+  kv_wait[device].withhold.store(withhold, std::memory_order_relaxed);
+}
+
 static const char* kv_attn_check(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads) {
   if (const char* e = kv_check(c, b)) return e;
   if (heads < 1 || heads % c->kv_heads) return "heads must be a multiple of kv_heads";
@@ -788,6 +801,9 @@ int rtr_kv_attention(const rtr_kv_cache* cache, const rtr_kv_batch* batch, const
   a.chunk = p.chunk;
   a.splits = p.splits;
   a.cluster = p.cluster;
+  const KvWait& w = kv_wait[device >= 0 && device < KV_DEVICES ? device : 0];
+  a.wait_cycles = w.cycles.load(std::memory_order_relaxed);
+  a.withhold = w.withhold.load(std::memory_order_relaxed);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == RTR_DTYPE_F32)

@@ -26,6 +26,8 @@ struct KvAttn {
   int per_seq;         // row tiles of a sequence without starts
   int chunk, splits;   // keys of a block, and the blocks of a row tile
   int cluster;         // the blocks of a row tile are one cluster and join among themselves
+  int withhold;        // a test's: the tile kernels do not hand over the last K of a block's keys
+  long long wait_cycles;  // the limit of the tile kernels' waits
 };
 
 // Weights enter the fp16 operands relative to 2^(maximum - lift): the lift brings the largest

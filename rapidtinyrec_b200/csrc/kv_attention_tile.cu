@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
 
       // adds the finished product of tile i, whose weights are relative to that tile's maximum
       const auto add_product = [&](int i, float keep_, float take_) {
-        mbar_wait(smem_addr(&bars.o_full[0][i & 1]), (i >> 1) & 1, abort_flag);
+        mbar_wait(smem_addr(&bars.o_full[0][i & 1]), (i >> 1) & 1, abort_flag, a.wait_cycles);
         tc_fence_after();
         const uint32_t at = tmem + lanes + O_AT + (i & 1) * 128 + half * NL;
         const uint64_t old2 = f2(keep_, keep_), new2 = f2(take_, take_);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       };
 
       for (int i = 0; i < n; ++i) {
-        mbar_wait(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1, abort_flag);
+        mbar_wait(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1, abort_flag, a.wait_cycles);
         tc_fence_after();
         const uint32_t st = tmem + lanes + (i & 1) * S_COLS + half * 64;
         const int key0 = c0 + i * KT_KEYS + half * 64, seg0 = i * 8 + half * 4;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     } else {
       const uint32_t ot = tmem + lanes + O_AT + half * 128;
       for (int i = 0; i < n; ++i) {
-        mbar_wait(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1, abort_flag);
+        mbar_wait(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1, abort_flag, a.wait_cycles);
         tc_fence_after();
         const uint32_t st = tmem + lanes + (i & 1) * S_COLS + half * 64;
         const int key0 = c0 + i * KT_KEYS + half * 64, seg0 = i * 8 + half * 4;
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
           m = top;
           l *= alpha;
           if (i > 0) {
-            mbar_wait(smem_addr(&bars.o_full[half][(i - 1) & 1]), ((i - 1) >> 1) & 1, abort_flag);
+            mbar_wait(smem_addr(&bars.o_full[half][(i - 1) & 1]), ((i - 1) >> 1) & 1, abort_flag, a.wait_cycles);
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
@@ -481,8 +481,8 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       red[half * KT_ROWS + r] = m;
       other_l[half * KT_ROWS + r] = l;
       if (n > 0) {
-        mbar_wait(smem_addr(&bars.o_full[0][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag);
-        mbar_wait(smem_addr(&bars.o_full[1][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag);
+        mbar_wait(smem_addr(&bars.o_full[0][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, a.wait_cycles);
+        mbar_wait(smem_addr(&bars.o_full[1][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, a.wait_cycles);
       }
       tc_fence_after();
       row_barrier();
@@ -540,13 +540,13 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     }
     for (int i = 0; i < n; ++i) {
       // S and O of tile i - 2 are done with the buffers
-      if (i >= 2 && !mbar_wait(smem_addr(&bars.s_full[i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      if (i >= 2 && !mbar_wait(smem_addr(&bars.s_full[i & 1]), ((i >> 1) - 1) & 1, abort_flag, a.wait_cycles)) break;
       codes.put_k(smem + C::K_OFF + (i & 1) * C::K_BYTES);
       fence_proxy_async();
-      mbar_arrive(smem_addr(&bars.k_full[i & 1]));
+      if (!a.withhold || i + 1 < n) mbar_arrive(smem_addr(&bars.k_full[i & 1]));
       if (i + 1 < n) codes.load_k(i + 1);
-      if (i >= 2 && !mbar_wait(smem_addr(&bars.o_full[0][i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
-      if (!PAIR && i >= 2 && !mbar_wait(smem_addr(&bars.o_full[1][i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      if (i >= 2 && !mbar_wait(smem_addr(&bars.o_full[0][i & 1]), ((i >> 1) - 1) & 1, abort_flag, a.wait_cycles)) break;
+      if (!PAIR && i >= 2 && !mbar_wait(smem_addr(&bars.o_full[1][i & 1]), ((i >> 1) - 1) & 1, abort_flag, a.wait_cycles)) break;
       // not every row sees every key of the tile: 0 * NaN must not reach the others
       if (c0 + (i + 1) * KT_KEYS > kmin && codes.drop_nans()) bars.nans = 1;
       codes.put_v(smem + C::V_OFF + (i & 1) * C::V_BYTES);
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     const uint64_t base = sw128_desc(smem_addr(smem));
     const uint32_t lo = (uint32_t)base, hi = (uint32_t)(base >> 32);
     int si = 0, oi[2] = {0, 0};  // products issued
-    const auto wait = [&](uint64_t& bar, int i) { return mbar_wait(smem_addr(&bar), (i >> 1) & 1, abort_flag); };
+    const auto wait = [&](uint64_t& bar, int i) { return mbar_wait(smem_addr(&bar), (i >> 1) & 1, abort_flag, a.wait_cycles); };
     const auto issue_s = [&](auto buffer) {
       constexpr int B = decltype(buffer)::value;
       tc_fence_after();
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
     };
     const std::integral_constant<int, 0> even{};
     const std::integral_constant<int, 1> odd{};
-    bool ok = n == 0 || mbar_wait(smem_addr(&bars.q_full), 0, abort_flag);
+    bool ok = n == 0 || mbar_wait(smem_addr(&bars.q_full), 0, abort_flag, a.wait_cycles);
     if (n > 0 && ok && (ok = wait(bars.k_full[0], 0))) issue_s(even);
     if (n > 1 && ok && (ok = wait(bars.k_full[1], 1))) issue_s(odd);
     for (int i = 0; i < n && ok; i += 2) {
@@ -626,7 +626,6 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
       if (ok && i + 1 < n) ok = tile(i + 1, odd);
     }
     if (!ok) {
-      if (leader) atomicOr(a.c.status, RTR_DEV_TIMEOUT);
       for (int i = si > 2 ? si - 2 : 0; i < si; ++i) mbar_drain(smem_addr(&bars.s_full[i & 1]), (i >> 1) & 1);
       for (int h = 0; h < HALVES; ++h)
         for (int i = oi[h] > 2 ? oi[h] - 2 : 0; i < oi[h]; ++i)
@@ -635,6 +634,7 @@ __global__ void __launch_bounds__(KtCfg<D, std::is_same<T, float>::value>::THREA
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(a.c.status, RTR_DEV_TIMEOUT);  // whoever's wait ran out
   if (warp == 8 + C::CODE_WARPS) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

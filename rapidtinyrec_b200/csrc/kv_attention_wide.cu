@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
     for (int i = 0; i < n && active; ++i) {
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {  // halves of the tile's keys
-        if (!ready) mbar_wait(smem_addr(&bars.s_full[g][h]), i & 1, abort_flag);
+        if (!ready) mbar_wait(smem_addr(&bars.s_full[g][h]), i & 1, abort_flag, a.wait_cycles);
         tc_fence_after();
         const uint32_t sh = st + 64 * h;
         const int key0 = c0 + i * KT_KEYS + 64 * h, seg0 = i * 8 + 4 * h;
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
           m = top;
           l *= alpha;
           if (i + h > 0) {  // the other half's product is the last that O got
-            mbar_wait(smem_addr(&bars.o_full[g][h ^ 1]), (i - 1 + h) & 1, abort_flag);
+            mbar_wait(smem_addr(&bars.o_full[g][h ^ 1]), (i - 1 + h) & 1, abort_flag, a.wait_cycles);
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
         mbar_arrive(smem_addr(&bars.p_full[g][h]));
       }
     }
-    if (n > 0 && active) mbar_wait(smem_addr(&bars.o_full[g][1]), (n - 1) & 1, abort_flag);
+    if (n > 0 && active) mbar_wait(smem_addr(&bars.o_full[g][1]), (n - 1) & 1, abort_flag, a.wait_cycles);
     tc_fence_after();
     row_barrier();  // both tiles are done with the operands
     if (!whole) l = __int_as_float(0x7fffffff);  // the sequence's length did not fit
@@ -380,12 +380,12 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
     }
     for (int i = 0; i < n; ++i) {
       // the products of tile i - 2 are done with the buffers
-      if (i >= 2 && !mbar_wait(smem_addr(&bars.k_free[i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      if (i >= 2 && !mbar_wait(smem_addr(&bars.k_free[i & 1]), ((i >> 1) - 1) & 1, abort_flag, a.wait_cycles)) break;
       codes.put_k(smem + C::K_OFF + (i & 1) * C::K_BYTES);
       fence_proxy_async();
-      mbar_arrive(smem_addr(&bars.k_full[i & 1]));
+      if (!a.withhold || i + 1 < n) mbar_arrive(smem_addr(&bars.k_full[i & 1]));
       if (i + 1 < n) codes.load_k(i + 1);
-      if (i >= 2 && !mbar_wait(smem_addr(&bars.v_free[i & 1]), ((i >> 1) - 1) & 1, abort_flag)) break;
+      if (i >= 2 && !mbar_wait(smem_addr(&bars.v_free[i & 1]), ((i >> 1) - 1) & 1, abort_flag, a.wait_cycles)) break;
       // not every row sees every key of the tile: 0 * NaN must not reach the others
       if (c0 + (i + 1) * KT_KEYS > kmin && codes.drop_nans()) bars.nans = 1;
       codes.put_v(smem + C::V_OFF + (i & 1) * C::V_BYTES);
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
     const uint64_t base = sw128_desc(smem_addr(smem));
     const uint32_t lo = (uint32_t)base, hi = (uint32_t)(base >> 32);
     int si[4] = {0, 0, 0, 0}, oi[4] = {0, 0, 0, 0};  // products issued, by chain
-    const auto wait = [&](uint64_t& bar, int phase) { return mbar_wait(smem_addr(&bar), phase & 1, abort_flag); };
+    const auto wait = [&](uint64_t& bar, int phase) { return mbar_wait(smem_addr(&bar), phase & 1, abort_flag, a.wait_cycles); };
     const auto issue_s = [&](auto buffer, auto chain) {
       constexpr int B = decltype(buffer)::value, G = decltype(chain)::value & 1, H = decltype(chain)::value >> 1;
       tc_fence_after();
@@ -465,7 +465,6 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
       if (ok && i + 1 < n) ok = keys(i + 1, c1_, c0_);
     }
     if (!ok) {
-      if (leader) atomicOr(a.c.status, RTR_DEV_TIMEOUT);
       for (int c = 0; c < 4; ++c) {
         if (si[c]) mbar_drain(smem_addr(&bars.s_full[c & 1][c >> 1]), (si[c] - 1) & 1);
         if (oi[c]) mbar_drain(smem_addr(&bars.o_full[c & 1][c >> 1]), (oi[c] - 1) & 1);
@@ -474,6 +473,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(a.c.status, RTR_DEV_TIMEOUT);  // whoever's wait ran out
   if (warp == 8 + C::CODE_WARPS) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

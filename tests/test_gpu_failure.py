@@ -1,6 +1,6 @@
 """Failure detection on the device: a bounded pipeline wait that runs out.
 
-Every mbarrier wait of the tensor-core GEMMs is bounded.  The test shortens
+Every mbarrier wait of the tensor-core GEMMs and of the KV attention's tiles is bounded.  The test shortens
 the bound and withholds the activation copies of the fp16-pair GEMM (through
 ``rtr_debug_wait_control``), so the waits run out without any fault: each CTA
 stops issuing, drains what it issued, frees its tensor memory and sets the
@@ -50,6 +50,40 @@ def test_bounded_wait_expires_and_the_session_recovers(tiny):
         for key in ('token_ids', 'beam_indices', 'sequence_logp', 'transition_logp'):
             assert a[key] == b[key], key
     eng.close()
+
+
+@pytest.mark.parametrize('dtype,heads,kv,dim,rows,tokens', [
+    (torch.float32, 12, 2, 128, 1000, 2300), (torch.float32, 14, 2, 64, 1000, 2300), (torch.bfloat16, 14, 2, 64, 1000, 2300),
+    (torch.float32, 12, 2, 128, 120, 1500), (torch.float32, 12, 2, 128, 100, 20000), (torch.bfloat16, 28, 4, 128, 50, 719),
+    (torch.bfloat16, 28, 4, 128, 1300, 2000),
+    (torch.bfloat16, 28, 4, 128, 400, 17000), (torch.float32, 12, 2, 128, 1000, 100), (torch.bfloat16, 28, 4, 128, 2000, 250)])
+def test_bounded_wait_expires_in_the_kv_attention(dtype, heads, kv, dim, rows, tokens):
+    """Tiles of 128 rows, alone, in clusters and joined by a kernel, and blocks of 256, over one tile of
+    keys and over many: products in flight are waited for, the call says so, the next one is exact."""
+    if not torch.cuda.is_available():
+        pytest.fail('CUDA device required for -m gpu tests')
+    from rapidtinyrec_b200 import _native
+    from rapidtinyrec_b200.kv_cache import KvCache8
+    page = 64
+    pages = -(-tokens // page)
+    cache = KvCache8.allocate(pages, kv, page, dim)
+    table = torch.arange(pages, dtype=torch.int32, device='cuda')[None]
+    lens = torch.tensor([tokens], dtype=torch.int32, device='cuda')
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(tokens, kv, dim, generator=g).cuda()
+    cache.write(x, x, table, lens)
+    q = torch.randn(rows, heads, dim, generator=g).to(dtype).cuda()
+    want = cache.attention(q, table, lens, causal=False)
+    cache.check()
+    _native.wait_control(0, SHORT_WAIT, withhold_activation_copies=True)
+    try:
+        cache.attention(q, table, lens, causal=False)
+        with pytest.raises(_native.NativeError, match='wait'):
+            cache.check()
+    finally:
+        _native.wait_control(0)
+    assert torch.equal(cache.attention(q, table, lens, causal=False), want)
+    cache.check()
 
 
 def test_bounded_wait_expires_in_a_clustered_split_k_gemm():
