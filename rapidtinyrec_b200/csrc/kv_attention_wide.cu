@@ -446,10 +446,9 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
       if (!wait(bars.v_full[B], i >> 1)) return false;
       if (!step(i, buffer, next, c0_) || !step(i, buffer, next, c1_)) return false;
       if (!step(i, buffer, next, c2_) || !step(i, buffer, next, c3_)) return false;
-      if (leader && i + 2 < n) {  // tile i's V, the next tile's K; nothing arrives for which no one waits
-        mma_commit(smem_addr(&bars.v_free[B]));
-        mma_commit(smem_addr(&bars.k_free[B ^ 1]));
-      }
+      // tile i's V, the next tile's K; nothing arrives for which no one waits
+      if (leader && i + 2 < n) mma_commit(smem_addr(&bars.v_free[B]));
+      if (leader && i + 3 < n) mma_commit(smem_addr(&bars.k_free[B ^ 1]));
       return true;
     };
     bool ok = n == 0 || (wait(bars.q_full, 0) && wait(bars.k_full[0], 0));
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__(KwCfg::THREADS, 1) kv_attn_wide_kernel(const K
       if (tiles > 1) issue_s(c0_, c1_);
       issue_s(c0_, c2_);
       if (tiles > 1) issue_s(c0_, c3_);
-      if (leader) mma_commit(smem_addr(&bars.k_free[0]));
+      if (leader && n > 2) mma_commit(smem_addr(&bars.k_free[0]));
     }
     for (int i = 0; i < n && ok; i += 2) {
       ok = keys(i, c0_, c1_);
