@@ -257,6 +257,7 @@ class BeamEngine:
             raise ValueError('pages must be different page numbers of the store')
         if store.device.index != self.device:
             raise ValueError('the store must lie on the engine\'s device')
+        store.check()  # what earlier calls on the store left undone is not this prefix's
         table = torch.tensor(pages, dtype=torch.int32, device=dev)
         dtype = torch.float32 if self.cfg.dtype == 'fp32' else torch.bfloat16
         hidden = torch.empty(self.cfg.hidden, dtype=dtype, device=dev)

@@ -258,6 +258,24 @@ def test_a_prefix_whose_pages_were_given_away_is_refused(tiny, engine):
             engine.generate_kept(second)
 
 
+def test_what_others_left_undone_on_the_store_is_raised_before_pages_are_taken(tiny, engine):
+    from rapidtinyrec_b200._native import NativeError
+    a, b = prompts(tiny)[:2]
+    store = engine.prefix_store(8)
+    pages = range(max(pages_for(a, 64), pages_for(b, 64)))
+    _, first = engine.generate_and_keep(a, store, pages)
+    record = engine.generate_kept(first)
+    dev = store.device
+    q = torch.zeros(1, store.kv_heads, store.head_dim, device=dev)
+    store.attention(q, torch.full((1, 1), 8, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev))
+    engine.prefill(b)
+    with pytest.raises(NativeError, match='page'):
+        engine.keep_prefix(b, store, pages)
+    assert engine.generate_kept(first) == record
+    engine.prefill(b)
+    engine.generate_kept(engine.keep_prefix(b, store, pages))
+
+
 def test_a_prompt_that_was_not_prefilled_is_not_kept(tiny, engine):
     ids = list(prompts(tiny)[0])
     store = engine.prefix_store(8)
