@@ -158,6 +158,7 @@ PyObject* call_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
       k = tensor(PyTuple_GET_ITEM(a[7], 0), "out");
       v = tensor(PyTuple_GET_ITEM(a[7], 1), "out");
       if (k.scalar_type() != v.scalar_type()) refuse("out must be two tensors of one type");
+      if (rows && k.data_ptr() == v.data_ptr()) refuse("out must be two tensors, not one twice");
       for (const at::Tensor* x : {&k, &v}) {
         bool own = dense(cache, *x, heads, "out", false) && x->size(0) == rows;
         for (int d = 0; d < 2; ++d) own = own && (x->size(d) < 2 || x->stride(d) != 0);

@@ -138,7 +138,8 @@ class KvCache8:
     def read(self, rows, table, lens, starts=None, dtype=torch.float32, out=None):
         """The last tokens of each sequence as ``(k, v)``, ``[rows, kv_heads, head_dim]`` each: the
         values that the codes stand for, rounded once to ``dtype``.  ``out``: a pair of tensors to
-        fill; rows that belong to no sequence keep what they held (new tensors: undefined there).
+        fill, of one type, which then stands for ``dtype``; rows that belong to no sequence keep what
+        they held (new tensors: undefined there).
         """
         if dtype not in _DTYPES:
             raise ValueError('dtype must be float32 or bfloat16')

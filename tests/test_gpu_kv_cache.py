@@ -937,6 +937,18 @@ def test_outputs_that_memory_cannot_hold():
     check_attention(cache, torch.randn(1, 4, 64, device='cuda'), ints([[1]]), [9], [1], True)
 
 
+def test_one_tensor_is_not_both_outputs():
+    cache = filled(4, 2, 16, 64, seed=92)
+    x = torch.full((4, 2, 64), 7.0, device='cuda')
+    with pytest.raises(ValueError, match='twice'):
+        cache.read(4, ints([[0]]), ints([9]), out=(x, x))
+    assert (x == 7).all()
+    both = torch.empty(4, 2, 2, 64, device='cuda')  # side by side is fine
+    k, v = cache.read(4, ints([[0]]), ints([9]), out=(both[:, 0], both[:, 1]))
+    want = cache.read(4, ints([[0]]), ints([9]))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
 # -------------------------------------------------------- streams and graphs
 def test_other_streams_and_captured_graphs():
     """Calls on a side stream; two graphs over one cache, replayed with other inputs."""
