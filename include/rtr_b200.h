@@ -361,7 +361,7 @@ int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_de
  * the row's sequence.  causal: a sequence's n rows stand at its last n positions and
  * see what is not behind them; otherwise each sees all lens[b] tokens.  Rows that see
  * nothing are 0.  q: row r, head h at r * q_token_stride + h * head_dim; out
- * [rows][heads][head_dim], same dtype; lse_dev (optional, float32 [rows][heads]):
+ * [rows][heads][head_dim], same dtype, q itself or apart from it; lse_dev (optional, float32 [rows][heads]):
  * log of the softmax's sum, minus infinity for rows that see nothing.  fp32 q and
  * weights enter the tensor cores as fp16 pairs: 22 bits, or for small ones half a step of 2^-38
  * of the largest q of the row, of 2^-39 of the largest weight (times V scale) among 128 keys.

@@ -105,6 +105,16 @@ bool dense(const Cache& cache, const at::Tensor& x, int64_t heads, const char* n
          reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
 }
 
+// Whether out, contiguous, shares memory with q [rows, row], rows `step` apart, without being q itself.
+// (A block has read its rows before any of them is written; other blocks' rows it must not touch.)
+bool overlaps(const at::Tensor& out, const at::Tensor& q) {
+  const int64_t size = q.element_size(), rows = q.size(0), row = q.size(1) * q.size(2) * size, step = q.stride(0) * size;
+  const int64_t from = static_cast<const char*>(out.data_ptr()) - static_cast<const char*>(q.data_ptr());
+  if (!rows || from >= (rows - 1) * step + row || from + rows * row <= 0) return false;
+  if (from == 0 && (rows == 1 || step == row)) return false;
+  return !(step > row && from > 0 && from % step >= row && from % step + rows * row <= step);  // between two rows
+}
+
 int32_t type_of(const at::Tensor& x) { return x.scalar_type() == at::kFloat ? RTR_DTYPE_F32 : RTR_DTYPE_BF16; }
 
 // A new tensor on the cache's device, by its allocator without a pass through the dispatcher.
@@ -198,6 +208,7 @@ PyObject* call_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || !cache.here(out) || !out.is_contiguous() ||
           reinterpret_cast<uintptr_t>(out.data_ptr()) % 16)
         refuse("out must be contiguous and like q");
+      if (overlaps(out, q)) refuse("out must be q itself or lie apart from it");
     }
     int64_t room = 0;
     check(kv_workspace(cache.c, &b, type_of(q), (int32_t)heads, cache.index, &room));

@@ -152,8 +152,8 @@ class KvCache8:
 
         ``causal``: a sequence's rows are its last positions, each sees what is not behind it;
         otherwise every row sees the whole sequence.  A row that sees nothing is 0.  ``scale``:
-        ``head_dim ** -0.5`` unless given.  Returns ``out`` (a new tensor, or the contiguous one given),
-        with ``return_lse`` also the float32 ``[rows, heads]`` log of the softmax's sum, by which
+        ``head_dim ** -0.5`` unless given.  Returns ``out`` (a new tensor, or the contiguous one given,
+        which may be ``q`` itself), with ``return_lse`` also the float32 ``[rows, heads]`` log of the softmax's sum, by which
         results over several stretches of keys are merged.  Rows that belong to no sequence are not
         written: a given ``out`` keeps them, new tensors are undefined there.  The work is laid out
         for sequences as long as a row of ``table``: where they are much shorter, pass a slice of it

@@ -949,6 +949,36 @@ def test_one_tensor_is_not_both_outputs():
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
 
 
+@pytest.mark.parametrize('dtype,heads,kv,dim,rows,tokens', OUTWEIGHED)
+def test_the_output_may_be_q(dtype, heads, kv, dim, rows, tokens):
+    page = 32
+    pages = -(-tokens // page)
+    cache = filled(pages, kv, page, dim, seed=93)
+    table = tables([tokens], page, pages, seed=94)
+    q = torch.randn(rows, heads, dim, generator=torch.Generator().manual_seed(95)).to(dtype).cuda()
+    for causal in (True, False):
+        want, want_lse = cache.attention(q, table, ints([tokens]), causal=causal, return_lse=True)
+        own = q.clone()
+        out, lse = cache.attention(own, table, ints([tokens]), causal=causal, return_lse=True, out=own)
+        assert out is own and torch.equal(own, want) and torch.equal(lse, want_lse)
+
+
+def test_an_output_that_overlaps_q_is_refused():
+    cache = filled(4, 2, 16, 64, seed=96)
+    table, lens = ints([[0]]), ints([9])
+    room = torch.randn(20, 4, 64, device='cuda')
+    for q, out in ((room[:8], room[1:9]), (room[1:9], room[:8]), (room[::2][:8], room[:8]), (room[::2][:8], room[7:15]),
+                   (room[:4].view(2, 8, 64)[:, :4], room[2:4]), (room[:1].expand(3, 4, 64), room[:3])):
+        before = room.clone()
+        with pytest.raises(ValueError, match='apart'):
+            cache.attention(q, table, lens, out=out)
+        assert torch.equal(room, before)
+    for q, out in ((room[:8], room[8:16]), (room[8:16], room[:8]), (room.view(2, 40, 64)[:, :4], room[2:4]),
+                   (room[:8:4], room[12:14])):
+        want = cache.attention(q, table, lens)
+        assert torch.equal(cache.attention(q, table, lens, out=out), want)
+
+
 # -------------------------------------------------------- streams and graphs
 def test_other_streams_and_captured_graphs():
     """Calls on a side stream; two graphs over one cache, replayed with other inputs."""
