@@ -373,8 +373,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32, 3) kv_attn_rows_kernel(const Kv
           if constexpr (PAIR) {
             float low[4];
             mma16816_first(low, a0, a1, a2, a3, pl[h][0], pl[h][1]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[2 * w + e][j] = fmaf(low[j], 1.0f / KA_LOW, o[2 * w + e][j]);
+            float(&to)[4] = o[2 * w + e];
+            const float2 x = f2_parts(f2_fma(f2(low[0], low[1]), f2(1.0f / KA_LOW, 1.0f / KA_LOW), f2(to[0], to[1])));
+            const float2 y = f2_parts(f2_fma(f2(low[2], low[3]), f2(1.0f / KA_LOW, 1.0f / KA_LOW), f2(to[2], to[3])));
+            to[0] = x.x; to[1] = x.y; to[2] = y.x; to[3] = y.y;
           }
         }
     }
