@@ -101,6 +101,31 @@ def test_a_prefix_that_is_exact_in_8_bits_gives_the_same_record(tiny, heads):
     e.close()
 
 
+@pytest.mark.parametrize('attn', [None, 'rows'])
+def test_a_bf16_prefix_that_is_exact_in_8_bits_gives_the_same_record(tiny, monkeypatch, attn):
+    """K = 0 and V = a bias of eighths: every weight is the same, an attention's output is V times 1 +-
+    2^-10 at most (weights of 11 bits, fp32 sums) before it is rounded to the bf16 that V is.  So nothing
+    differs between the kept and the unkept request, whatever kernel has them."""
+    from rapidtinyrec_b200 import workload
+    if attn:
+        monkeypatch.setenv('RTR_ATTN', attn)
+    weights = dict(workload.synth_weights(tiny['cfg'], seed=3, backend='numpy'))
+    g = torch.Generator().manual_seed(6)
+    for name in list(weights):
+        if '.k_proj.' in name or name.endswith('v_proj.weight'):
+            weights[name] = torch.zeros_like(weights[name])
+        if name.endswith('v_proj.bias'):
+            weights[name] = torch.randint(-7, 8, weights[name].shape, generator=g).float() / 8
+    e = make_engine(tiny, weights, dtype='bf16')
+    store = e.prefix_store(20, 16)
+    for n, ids in enumerate(prompts(tiny, 2)):
+        record, kept = e.generate_and_keep(ids, store, range(n * 10, n * 10 + pages_for(ids, 16)))
+        same(e.generate_kept(kept), record, 0)
+        if attn:
+            same(e.generate_kept(kept, in_place=False), record, 0)
+    e.close()
+
+
 def test_bf16_prefixes(tiny, monkeypatch):
     """bf16 sessions: their default decode attention reads copies of the arena, so only in place;
     with the per-head kernel both ways, within the differences of the framework's own bf16
