@@ -595,7 +595,7 @@ static KvAttnPlan kv_plan_rows(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   const int64_t most = (int64_t)b->table_width * c->page, base = p.items * c->kv_heads;
   // A stretch has at least 512 keys: below that a block is bound by the latency of
   // finding its pages, and joining costs more than it saves (61 sequences of 30 - 300
-  // keys, 14 heads: 5.4 us in one stretch, 5.8 in three); at most 1024, which a warp's lanes
+  // keys, 14 heads: 5.5 us in one stretch, 5.8 in three); at most 1024, which a warp's lanes
   // can hold the pages of and at which ragged batches spread (24 sequences of 6,000 -
   // 32,000 keys: 89.8 us, with 512 100.5); between them as many as give two blocks an SM (one
   // sequence of 128 Ki keys: 19.1 us, with three an SM 19.0, with 512 keys 23.0).
@@ -673,10 +673,10 @@ static KvAttnPlan kv_plan_wide(const rtr_kv_cache* c, const rtr_kv_batch* b, int
 }
 
 // The kernel whose expected time is less.  Measured, 28 / 4 heads of 128, bf16, tiles of
-// 128 against tiles of 8 rows: 8 sequences of 1,200 keys with 2 new tokens 12.7 : 11.0 us,
-// 4 12.9 : 12.7, 16 14.7 : 37.7; one of 300 keys with 64 11.3 : 8.4 us, with 256 11.3 : 15.6.
-// Tiles of 256 against 128: 32 sequences of 4,096 keys with 64 154 : 190 us, 4 of 512 keys with
-// 256 20.0 : 22.9, one of 4,096 with 1,024 74 : 86, with 512 57 : 47.
+// 128 against tiles of 8 rows: 8 sequences of 1,200 keys with 2 new tokens 13.2 : 10.8 us,
+// 4 13.4 : 12.3, 16 15.1 : 36.6; one of 300 keys with 64 11.5 : 8.0 us, with 256 11.3 : 15.0.
+// Tiles of 256 against 128: 32 sequences of 4,096 keys with 64 157 : 199 us, 4 of 512 keys with
+// 256 21 : 24.6, one of 4,096 with 1,024 77 : 91, with 512 52 : 49.
 static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int heads, bool f32, int sms) {
   const int group = heads / c->kv_heads;
   int64_t rows_ns, tiles_ns;
@@ -694,7 +694,7 @@ static KvAttnPlan kv_attn_plan(const rtr_kv_cache* c, const rtr_kv_batch* b, int
   }
   if (p.tile_rows == KW_ROWS)
     p.workspace = p.tails * KW_ROWS * (p.splits * (int64_t)(c->head_dim * 4 + 8) + 4);
-  else  // with starts, room for KvAttn::refused behind the sums
+  else  // with starts one row more: KvAttn::refused lies behind the sums
     p.workspace = p.splits > 1 && !p.cluster
                       ? ((int64_t)b->rows * heads * p.splits + (b->starts != nullptr)) * (c->head_dim * 4 + 8) : 0;
   return p;

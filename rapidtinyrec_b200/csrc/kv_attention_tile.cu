@@ -25,9 +25,10 @@
 // tiles hold.
 //
 // What bounds it is the chain of a tile, weights - O - S (about 2,600 cycles for 128 keys at
-// head_dim 128, of which exponentials need 1,024 and products 1,024).  2 x 1,024 rows over 6,000
-// keys: 28 / 4 heads of 128, bf16, 221 us (797 TFLOP/s; kv_attention_wide.cu 183); 12 / 2, fp32,
-// 149 us; 14 / 2 of 64 94 (bf16) and 149 us (fp32).  50 beams over 719 keys, 28 / 4, 11.5 us.
+// head_dim 128, of which exponentials need 1,024 and products 1,024).  2 x 1,024 rows at the end of
+// 6,000 keys: 28 / 4 heads of 128, bf16, 248 us (650 TFLOP/s of what the mask leaves;
+// kv_attention_wide.cu 192); 12 / 2, fp32, 154 us (448); 14 / 2 of 64 101 (399, bf16) and 153 us
+// (263, fp32).  50 beams over 719 keys, 28 / 4, 11.5 us.
 #include <cuda_runtime.h>
 
 #include <type_traits>

@@ -12,8 +12,9 @@
 //
 // 128 keys take a block some 3,200 cycles (exponentials alone 2,048, products 2,048; one row
 // tile by itself 2,600: a thread's chain of loads, exponentials and stores), its start and end
-// about seven times that.  8 x 1,024 rows over 6,000 keys, 28 / 4 heads: 597 us, 1,181 TFLOP/s,
-// tiles of 128 rows 749; 1,024 rows over 30,000 keys 425 : 600; at head_dim 64 no difference.
+// about seven times that.  8 x 1,024 rows at the end of 6,000 keys, 28 / 4 heads: 640 us,
+// 1,007 TFLOP/s of what the mask leaves, tiles of 128 rows 801; 1,024 rows at the end of 30,000 keys
+// 455 : 634; at head_dim 64 no difference.
 #include <cuda_runtime.h>
 
 #include <climits>

@@ -13,7 +13,11 @@
 // lens, table), which a block per head would repeat.  Threads take 16 bytes of
 // the dense side each, consecutive threads consecutive bytes, so the dense rows
 // move in whole lines and the codes in runs of 4 (fp32) or 8 (bf16) bytes a
-// thread.  Both are bound by HBM once a call has some thousand rows.
+// thread.  Once a call has some thousand rows, reading is bound by HBM and writing by
+// issue slots (77 % for 127,000 bf16 tokens of 4 heads, HBM 59 %): finding the maximum, scaling,
+// rounding and packing are some 45 instructions for 8 values.  The write kernels hold a page's
+// unit in registers and spill 16 - 52 bytes a thread at the limit that lets two or three blocks
+// share an SM.
 #include <cuda_runtime.h>
 
 #include <cstdio>
@@ -111,8 +115,8 @@ RTR_DEVICE float least_scale(float amax) {
   return __uint_as_float((uint32_t)(127 + max(-KV_EXP, min(KV_EXP, e))) << 23);
 }
 
-// What the common path leaves, exactly rounded: scales that are no power of two (from
-// elsewhere), values that become NaN; and older codes at a larger scale.
+// What the common path leaves: scales that are no power of two (from elsewhere; one float
+// division, rounded, before the code is), values that become NaN; and older codes at a larger scale.
 template <int N> __device__ __noinline__ Codes<N> encode_odd(uint4 raw, float s) {
   float x[N];
   values_of(raw, x);

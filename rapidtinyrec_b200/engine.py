@@ -279,7 +279,8 @@ class BeamEngine:
 
     def generate_kept(self, kept, in_place=True):
         """A request of a user whose prefix was kept: no prefill.  ``in_place``: decode attention
-        over the 8-bit pages; otherwise the pages are first read back into the arena.  The pages must
+        over the 8-bit pages; otherwise the pages are first read back into the arena (fp32, or with the
+        per-head decode kernel), which is the faster way for short prompts.  The pages must
         be as ``keep_prefix`` left them: those that a later ``keep_prefix`` took are noticed, what else is
         written to the store is not."""
         import torch

@@ -1,6 +1,6 @@
 """Failure detection on the device: a bounded pipeline wait that runs out.
 
-Every mbarrier wait of the tensor-core GEMMs and of the KV attention's tiles is bounded.  The test shortens
+Every mbarrier wait of the tensor-core GEMMs is bounded.  The test shortens
 the bound and withholds the activation copies of the fp16-pair GEMM (through
 ``rtr_debug_wait_control``), so the waits run out without any fault: each CTA
 stops issuing, drains what it issued, frees its tensor memory and sets the
