@@ -312,8 +312,9 @@ int rtr_constraint_process_static(rtr_session* s, int32_t step, const int64_t* i
  * strides of codes and their addresses are multiples of 16, and either a page's last head
  * ends before the next page or a head's last page before the next head.  `status` is a device
  * word that the kernels set bits in (never clear): 1 << 5 a length or row range
- * that does not fit, 1 << 8 a bounded wait that ran out (its call's rows are undefined), 1 << 9 a page number outside [0, pages), 1 << 10 an old scale
- * that is not positive and finite.  The work concerned is left out (attention:
+ * that does not fit, 1 << 8 a bounded wait that ran out (its call's rows are undefined),
+ * 1 << 9 a page number outside [0, pages), 1 << 10 an old scale that is not positive and
+ * finite.  The work concerned is left out (attention:
  * rows of NaN; where starts itself is at fault the whole call is left out and no row written),
  * memory outside the buffers is never touched. */
 typedef struct {
@@ -361,13 +362,13 @@ int rtr_kv_read(const rtr_kv_cache* cache, const rtr_kv_batch* batch, void* k_de
  * the row's sequence.  causal: a sequence's n rows stand at its last n positions and
  * see what is not behind them; otherwise each sees all lens[b] tokens.  Rows that see
  * nothing are 0.  q: row r, head h at r * q_token_stride + h * head_dim; out
- * [rows][heads][head_dim], same dtype, q itself or apart from it; lse_dev (optional, float32 [rows][heads]):
- * log of the softmax's sum, minus infinity for rows that see nothing.  fp32 q and
+ * [rows][heads][head_dim], same dtype, q itself or apart from it; lse_dev (optional, float32
+ * [rows][heads]): log of the softmax's sum, minus infinity for rows that see nothing.  fp32 q and
  * weights enter the tensor cores as fp16 pairs: 22 bits, or for small ones half a step of 2^-37
  * of the largest q of the row, of 2^-39 of the largest weight (times V scale) among 128 keys.
  * bf16 rows' weights are one fp16 value: 11 bits, or half a step of 2^-34 of the row's largest.
- * Sums are fp32.  A row that sees a page whose V scale is outside [2^-48, 2^48], whose K scale is negative or
- * whose number is outside the cache is NaN.  The workspace must hold
+ * Sums are fp32.  A row that sees a page whose V scale is outside [2^-48, 2^48], whose K scale
+ * is negative or NaN or whose number is outside the cache is NaN.  The workspace must hold
  * rtr_kv_attention_workspace bytes (the same batch, dtype and heads), aligned to 16, and is
  * free again when the call's kernels ran: calls that may overlap need one each.  A table row wider than the
  * sequences need costs idle blocks. */
