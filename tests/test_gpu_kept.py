@@ -101,6 +101,31 @@ def test_a_prefix_that_is_exact_in_8_bits_gives_the_same_record(tiny, heads):
     e.close()
 
 
+@pytest.mark.parametrize('attn', ['rows', 'tc', 'folded'])
+def test_kept_prefixes_beside_every_decode_attention(tiny, monkeypatch, attn):
+    """fp32 sessions of the other decode attentions: over the pages all give the same record; read back
+    where the kernel reads the arena, refused where it reads copies of it."""
+    from rapidtinyrec_b200._native import NativeError
+    ids = prompts(tiny)[2]
+    monkeypatch.setenv('RTR_ATTN', attn)
+    e = make_engine(tiny, max_users=2)
+    store = e.prefix_store(8)
+    plain = e.generate(ids)
+    record, kept = e.generate_and_keep(ids, store, range(pages_for(ids, 64)))
+    same(record, plain)
+    over_pages = e.generate_kept(kept)
+    if e.report()['decode_attention'] == 1:
+        with pytest.raises(NativeError, match='in place'):
+            e.generate_kept(kept, in_place=False)
+    else:
+        same(e.generate_kept(kept, in_place=False), over_pages)
+    two = e.generate_batch([ids, prompts(tiny)[0]])
+    same(two[0], plain)
+    same(e.generate_kept(kept), over_pages, 0)
+    same(e.generate(ids), plain, 0)
+    e.close()
+
+
 @pytest.mark.parametrize('attn', [None, 'rows'])
 def test_a_bf16_prefix_that_is_exact_in_8_bits_gives_the_same_record(tiny, monkeypatch, attn):
     """K = 0 and V = a bias of eighths: every weight is the same, an attention's output is V times 1 +-
