@@ -397,6 +397,63 @@ int rtr_keep_prefix(rtr_session* s, const rtr_kv_cache* cache, const int32_t* ta
 int rtr_prefill_kept(rtr_session* s, const rtr_kv_cache* cache, const int32_t* table_dev, int32_t table_width,
                      const int32_t* ids, int32_t L, const void* hidden_dev, int32_t in_place);
 
+/* ---- pages of sequences that grow and shrink -------------------------------
+ * The page numbers of a paged cache (the 8-bit one above or a caller's own) handed out and taken
+ * back on the GPU.  No counterpart in the reference, whose prefix arena holds one request
+ * (shared_prefix.py:67-89).  `free` [pages] is a stack of page numbers, `count` its height (device
+ * word), `marks` [pages] 1 for a page that a sequence holds and 0 for a free one, `status` a device word that the
+ * kernels set bits in, `ticket` a device word that is 0 between calls.  Calls on one pool must follow
+ * one another (one stream, or streams that wait); they may be captured into a CUDA graph.
+ * What is read from device memory is checked, and a call that does not fit as a whole changes
+ * nothing but the status word: 1 << 5 a length or row count that does not fit (negative, more
+ * tokens than a table row holds, more rows than the call has), 1 << 9 a page number outside
+ * [0, pages), 1 << 11 fewer free pages than are needed, 1 << 12 a page given back that no sequence holds. */
+typedef struct {
+  int32_t *free, *count, *marks;
+  uint32_t *status, *ticket;
+  int32_t pages, page; /* page: tokens, a power of two from 1 to 1024 */
+} rtr_page_pool;
+
+/* Sequence b holds held[b] tokens and gets fresh[b] more (fresh NULL: `each`): table row b gets the page
+ * numbers that it needs for them, the call's j-th page (sequences in order, then pages in order)
+ * free[count - 1 - j].  lens[b] = held[b] + fresh[b]; starts [seqs + 1]: running sum of the fresh tokens.  Row
+ * starts[b] + i has positions held[b] + i (its place in the sequence) and slots table[b][position / page] * page +
+ * position % page; a row whose page number is outside the pool, and rows from starts[seqs] to `rows`,
+ * have -1 in both.  A call that does not fit: lens = held, starts 0, every row -1.  At most 16384 sequences.  lens, starts,
+ * positions and slots must not overlap the inputs. */
+int rtr_pages_grow(const rtr_page_pool* pool, int32_t* table, int64_t table_stride, int32_t table_width, const int32_t* held,
+                   const int32_t* fresh, int32_t each, int32_t seqs, int32_t rows, int32_t* lens, int32_t* starts,
+                   int32_t* positions, int64_t* slots, int32_t device, void* stream);
+
+/* The reverse: of held[b] tokens the sequence keeps keep[b] (keep NULL: none), and the pages that those do not need go
+ * back: page j of m (in the same order) to free[count + m - 1 - j], so that growing again by as much takes
+ * the same pages in the same places.  The table stays as it is. */
+int rtr_pages_release(const rtr_page_pool* pool, const int32_t* table, int64_t table_stride, int32_t table_width,
+                      const int32_t* held, const int32_t* keep, int32_t seqs, int32_t device, void* stream);
+
+/* ---- rotary positions ------------------------------------------------------
+ * The rotation that the engine fuses into its q/k/v projection (Qwen2RotaryEmbedding: pairs half a
+ * head apart), for rows of a caller's own and with the other layouts: pairs (2 i, 2 i + 1) where
+ * `interleaved`, the first rotary_dim dimensions of a head alone, scaled frequencies.  Pair i of row r becomes
+ *   factor * (a cos t - b sin t, b cos t + a sin t),  t = 2 pi * fraction(positions[r] * turns[i] / 2^64)
+ * with turns [rotary_dim / 2] the frequencies in turns a position, times 2^64 (device array): the
+ * product modulo 2^64 is the angle itself, as exact at position 2^31 as at 1 (turns rounded to half a unit: off by
+ * positions * 2^-65 turns).  back: -t, which takes the rotation back and is its transpose (the
+ * gradient of a rotated row gives that of the row).  Rows may be strided; out is the input itself or apart
+ * from it, and holds all head_dim dimensions.  fp32 arithmetic, one rounding to dtype. */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t in_row, in_head, out_row, out_head; /* strides in elements; dimensions are contiguous */
+  int32_t heads;
+} rtr_rotary_rows;
+
+/* k may be NULL.  head_dim 2 to 512, rotary_dim even and at most head_dim.  positions: int32 or (wide) int64, of any
+ * sign. */
+int rtr_rotary(const rtr_rotary_rows* q, const rtr_rotary_rows* k, int64_t rows, int32_t head_dim, int32_t rotary_dim,
+               int32_t interleaved, int32_t dtype, const void* positions, int32_t wide, const uint64_t* turns, float factor,
+               int32_t back, int32_t device, void* stream);
+
 /* ---- synthetic workload --------------------------------------------------- */
 
 /* Deterministic synthetic tensor values: element i of stream (seed, tid) is

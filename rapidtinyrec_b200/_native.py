@@ -26,6 +26,7 @@ EXPORTS = (
     'rtr_session_create_batched', 'rtr_launch_batch', 'rtr_wait_batch', 'rtr_generate_batch',
     'rtr_debug_wait_control', 'rtr_attention_check', 'rtr_kv_write', 'rtr_kv_read',
     'rtr_kv_attention_workspace', 'rtr_kv_attention', 'rtr_keep_prefix', 'rtr_prefill_kept',
+    'rtr_pages_grow', 'rtr_pages_release', 'rtr_rotary',
 )
 
 
@@ -77,6 +78,17 @@ class KvBatchC(ctypes.Structure):
     _fields_ = [('table', ctypes.c_void_p), ('lens', ctypes.c_void_p), ('starts', ctypes.c_void_p),
                 ('table_stride', ctypes.c_int64), ('table_width', ctypes.c_int32), ('seqs', ctypes.c_int32),
                 ('rows', ctypes.c_int32)]
+
+
+class PagePoolC(ctypes.Structure):
+    _fields_ = [('free', ctypes.c_void_p), ('count', ctypes.c_void_p), ('marks', ctypes.c_void_p),
+                ('status', ctypes.c_void_p), ('ticket', ctypes.c_void_p), ('pages', ctypes.c_int32),
+                ('page', ctypes.c_int32)]
+
+
+class RotaryRowsC(ctypes.Structure):
+    _fields_ = [('in_', ctypes.c_void_p), ('out', ctypes.c_void_p), ('in_row', ctypes.c_int64), ('in_head', ctypes.c_int64),
+                ('out_row', ctypes.c_int64), ('out_head', ctypes.c_int64), ('heads', ctypes.c_int32)]
 
 
 class NativeError(RuntimeError):
@@ -135,6 +147,9 @@ def load():
         'rtr_kv_attention': (P, P, P, I32, I32, I64, I32, F, P, P, P, I64, I32, P),
         'rtr_keep_prefix': (P, P, P, I32, P),
         'rtr_prefill_kept': (P, P, P, I32, P, I32, P, I32),
+        'rtr_pages_grow': (P, P, I64, I32, P, P, I32, I32, I32, P, P, P, P, I32, P),
+        'rtr_pages_release': (P, P, I64, I32, P, P, I32, I32, P),
+        'rtr_rotary': (P, P, I64, I32, I32, I32, I32, P, I32, P, F, I32, I32, P),
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -144,6 +159,24 @@ def load():
     lib.rtr_last_error.restype = ctypes.c_char_p
     _lib = lib
     return lib
+
+
+_op_call = None
+
+
+def op_call():
+    """The C++ module of the decoding operators' calls (op_call.cpp), bound to the library's entry points."""
+    global _op_call
+    if _op_call is None:
+        lib = load()
+        try:
+            from . import _op_call as calls
+        except ImportError as e:
+            raise ImportError('_op_call.so is not built; run `python -m rapidtinyrec_b200.build`') from e
+        entries = (lib.rtr_pages_grow, lib.rtr_pages_release, lib.rtr_rotary, lib.rtr_last_error)
+        calls.setup(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), NativeError)
+        _op_call = calls
+    return _op_call
 
 
 def check(code, session=None):

@@ -26,6 +26,8 @@ enum : uint32_t {
   RTR_DEV_TIMEOUT = 1u << 8,        // a bounded pipeline wait expired (kernel gave up)
   RTR_DEV_BAD_PAGE = 1u << 9,       // 8-bit KV cache: page number outside the cache
   RTR_DEV_BAD_SCALE = 1u << 10,     // 8-bit KV cache: scale that is not positive and finite
+  RTR_DEV_FEW_PAGES = 1u << 11,     // page pool: fewer free pages than a call needs
+  RTR_DEV_PAGE_NOT_HELD = 1u << 12, // page pool: a page given back that no sequence holds
 };
 
 RTR_DEVICE float warp_sum(float v) {

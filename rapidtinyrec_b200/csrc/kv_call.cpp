@@ -3,18 +3,7 @@
 // call that checks six tensors and passes fourteen arguments through ctypes costs 9 - 12 us of
 // the host, longer than the smallest kernels run; here a write 2.5, an attention 3.6, a read with
 // its two outputs 4.2.
-//
-// The module links against torch only; setup() hands it the C entry points' addresses.
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAStream.h>
-
-#include <cstdarg>
-#include <cstdio>
-
-#include "rtr_b200.h"
+#include "call.h"
 
 namespace {
 
@@ -22,35 +11,6 @@ decltype(&rtr_kv_write) kv_write;
 decltype(&rtr_kv_read) kv_read;
 decltype(&rtr_kv_attention) kv_attention;
 decltype(&rtr_kv_attention_workspace) kv_workspace;
-decltype(&rtr_last_error) last_error;
-PyObject* native_error;  // _native.NativeError(code, message)
-
-// Thrown where a Python exception is set already.
-struct Raised {};
-
-[[noreturn]] void refuse(const char* format, ...) {
-  char text[256];
-  va_list args;
-  va_start(args, format);
-  vsnprintf(text, sizeof text, format, args);
-  va_end(args);
-  PyErr_SetString(PyExc_ValueError, text);
-  throw Raised{};
-}
-
-void check(int code) {
-  if (code == RTR_OK) return;
-  if (PyObject* e = PyObject_CallFunction(native_error, "is", code, last_error(nullptr))) {
-    PyErr_SetObject(native_error, e);
-    Py_DECREF(e);
-  }
-  throw Raised{};
-}
-
-const at::Tensor& tensor(PyObject* o, const char* name) {
-  if (!THPVariable_Check(o)) refuse("%s must be a tensor", name);
-  return THPVariable_Unpack(o);
-}
 
 // The cache a call works on: its C struct (kept by KvCache8) and device.
 struct Cache {
@@ -124,17 +84,6 @@ at::Tensor room_for(const Cache& cache, at::IntArrayRef size, at::ScalarType typ
 }
 
 at::Tensor copied(const at::Tensor& x) { return x.clone(at::MemoryFormat::Contiguous); }
-
-template <typename F> PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F&& body) {
-  HANDLE_TH_ERRORS  // torch's own exceptions as torch raises them (OutOfMemoryError, say)
-  try {
-    if (given != wanted) refuse("%d arguments expected", (int)wanted);
-    return body();
-  } catch (const Raised&) {
-    return nullptr;
-  }
-  END_HANDLE_TH_ERRORS
-}
 
 // write(cache, device, k, v, table, lens, starts)
 PyObject* call_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -244,7 +193,6 @@ PyObject* call_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-#define CALL(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"setup", CALL(call_setup)},
                          {"write", CALL(call_write)},
                          {"read", CALL(call_read)},
