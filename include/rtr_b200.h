@@ -454,6 +454,48 @@ int rtr_rotary(const rtr_rotary_rows* q, const rtr_rotary_rows* k, int64_t rows,
                int32_t interleaved, int32_t dtype, const void* positions, int32_t wide, const uint64_t* turns, float factor,
                int32_t back, int32_t device, void* stream);
 
+/* ---- beam search over whole vocabularies -----------------------------------
+ * One step of a beam search that no catalog constrains to a few columns (rtr_decode_step's beam update has
+ * at most 256 allowed tokens a beam and five steps; this replaces the log_softmax, top-k and
+ * bookkeeping of HF GenerationMixin._beam_search, generation/utils.py:3252-3352, for callers with a
+ * model of their own).  Item b has n beams: rows b * n .. of logits [items * n][logits_stride], scores [items][n].  The candidate
+ * (i, v) is worth logits[i][v] - log sum_u exp logits[i][u] + scores[i] where allowed (bytes [items * n][allowed_stride],
+ * NULL: everywhere; an allowed_stride of 0 is one row for all) is not 0, and minus infinity elsewhere.  all_* [items][k]: the k best, in
+ * descending order, equal ones by i * vocab + v: token v, parent i, value rounded to float32.  next_* [items][beams]: the first
+ * `beams` of those whose token is not eos (eos < 0: none is).  A row whose score is minus infinity is not read.  A row
+ * with a NaN or plus infinity among its logits, or such a score, is worth minus infinity throughout and sets 1 << 7 in `status` (a
+ * device word).  The order is that of values computed in 64 bits (log sum exps that were
+ * summed in 32 bits are summed again in 64 where two candidates are too close to tell).
+ * A value below float32's range counts as minus infinity.
+ * n 1 to 128, vocab 1 to 2^20, k 1 to 256 and at most n * vocab, beams at most k (with eos: k at least beams + n).  dtype float32 or bfloat16; the workspace (rtr_beam_select_workspace bytes, aligned to 16) is free again when the call's
+ * kernels ran. */
+typedef struct {
+  const void* logits;
+  const float* scores;
+  const uint8_t* allowed;
+  int64_t logits_stride, allowed_stride;
+  int32_t dtype, items, n, vocab, k, beams, eos;
+  int32_t *all_tokens, *all_parents, *next_tokens, *next_parents;
+  float *all_scores, *next_scores;
+  uint32_t* status;
+} rtr_beam_step;
+int rtr_beam_select_workspace(const rtr_beam_step* step, int32_t device, int64_t* bytes);
+int rtr_beam_select(const rtr_beam_step* step, void* workspace_dev, int64_t workspace_bytes, int32_t device, void* stream);
+
+/* The states of the beams in the order that a step's parents give: row b * beams + i of every state becomes what row
+ * b * beams + parents[b][i] was, in place (the reference's ReorderSuffix copies every row into new tensors,
+ * prefix_replay.py:95-117; here only rows that move are written, and their parents read once).  A state has rows at
+ * data + r * row_bytes and in each of them up to three outer dimensions of sizes[] at strides[] bytes and `inner` contiguous
+ * bytes; no two bytes of the states may be the same.  A parent outside [0, beams) sets 1 << 1 in `status`
+ * (a device word), and its row stays.  At most 128 beams. */
+typedef struct {
+  void* data;
+  int64_t row_bytes, inner, strides[3];
+  int32_t sizes[3];
+} rtr_beam_state;
+int rtr_beam_reorder(const rtr_beam_state* states, int32_t count, const int32_t* parents, int32_t items, int32_t beams,
+                     uint32_t* status, int32_t device, void* stream);
+
 /* ---- synthetic workload --------------------------------------------------- */
 
 /* Deterministic synthetic tensor values: element i of stream (seed, tid) is

@@ -26,7 +26,7 @@ EXPORTS = (
     'rtr_session_create_batched', 'rtr_launch_batch', 'rtr_wait_batch', 'rtr_generate_batch',
     'rtr_debug_wait_control', 'rtr_attention_check', 'rtr_kv_write', 'rtr_kv_read',
     'rtr_kv_attention_workspace', 'rtr_kv_attention', 'rtr_keep_prefix', 'rtr_prefill_kept',
-    'rtr_pages_grow', 'rtr_pages_release', 'rtr_rotary',
+    'rtr_pages_grow', 'rtr_pages_release', 'rtr_rotary', 'rtr_beam_select_workspace', 'rtr_beam_select', 'rtr_beam_reorder',
 )
 
 
@@ -91,6 +91,19 @@ class RotaryRowsC(ctypes.Structure):
                 ('out_row', ctypes.c_int64), ('out_head', ctypes.c_int64), ('heads', ctypes.c_int32)]
 
 
+class BeamStepC(ctypes.Structure):
+    _fields_ = ([(name, ctypes.c_void_p) for name in ('logits', 'scores', 'allowed')]
+                + [('logits_stride', ctypes.c_int64), ('allowed_stride', ctypes.c_int64)]
+                + [(name, ctypes.c_int32) for name in ('dtype', 'items', 'n', 'vocab', 'k', 'beams', 'eos')]
+                + [(name, ctypes.c_void_p) for name in ('all_tokens', 'all_parents', 'next_tokens', 'next_parents', 'all_scores',
+                                                        'next_scores', 'status')])
+
+
+class BeamStateC(ctypes.Structure):
+    _fields_ = [('data', ctypes.c_void_p), ('row_bytes', ctypes.c_int64), ('inner', ctypes.c_int64), ('strides', ctypes.c_int64 * 3),
+                ('sizes', ctypes.c_int32 * 3)]
+
+
 class NativeError(RuntimeError):
     def __init__(self, code, message):
         super().__init__(f'[rtr error {code}] {message}')
@@ -150,6 +163,9 @@ def load():
         'rtr_pages_grow': (P, P, I64, I32, P, P, I32, I32, I32, P, P, P, P, I32, P),
         'rtr_pages_release': (P, P, I64, I32, P, P, I32, I32, P),
         'rtr_rotary': (P, P, I64, I32, I32, I32, I32, P, I32, P, F, I32, I32, P),
+        'rtr_beam_select_workspace': (P, I32, ctypes.POINTER(I64)),
+        'rtr_beam_select': (P, P, I64, I32, P),
+        'rtr_beam_reorder': (P, I32, P, I32, I32, P, I32, P),
     }
     for name, args in sig.items():
         fn = getattr(lib, name)
@@ -173,7 +189,8 @@ def op_call():
             from . import _op_call as calls
         except ImportError as e:
             raise ImportError('_op_call.so is not built; run `python -m rapidtinyrec_b200.build`') from e
-        entries = (lib.rtr_pages_grow, lib.rtr_pages_release, lib.rtr_rotary, lib.rtr_last_error)
+        entries = (lib.rtr_pages_grow, lib.rtr_pages_release, lib.rtr_rotary, lib.rtr_beam_select_workspace, lib.rtr_beam_select,
+                   lib.rtr_beam_reorder, lib.rtr_last_error)
         calls.setup(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), NativeError)
         _op_call = calls
     return _op_call

@@ -11,6 +11,9 @@ namespace {
 decltype(&rtr_pages_grow) pages_grow;
 decltype(&rtr_pages_release) pages_release;
 decltype(&rtr_rotary) rotary;
+decltype(&rtr_beam_select_workspace) beam_workspace;
+decltype(&rtr_beam_select) beam_select;
+decltype(&rtr_beam_reorder) beam_reorder;
 
 int64_t whole(PyObject* o, const char* name) {
   const int64_t v = PyLong_AsLongLong(o);
@@ -41,6 +44,11 @@ PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
   Py_ssize_t i = 0;
   for (const at::Tensor& x : tensors) PyTuple_SET_ITEM(t, i++, x.defined() ? THPVariable_Wrap(x) : Py_NewRef(Py_None));
   return t;
+}
+// A tensor that is written in place: none that autograd would want back as it was.
+void written(const at::Tensor& t, const char* name) {
+  if (t.requires_grad()) refuse("%s must not require a gradient", name);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 int32_t type_of(const at::Tensor& x) { return x.scalar_type() == at::kFloat ? RTR_DTYPE_F32 : RTR_DTYPE_BF16; }
 
@@ -214,6 +222,8 @@ PyObject* call_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (two && rows && (share(out[0], out[1]) || share(out[0], in[1]) || share(out[1], in[0])))
         refuse("out of q and of k must not share memory with one another or the other's input");
     }
+    if (a[9] != Py_None)
+      for (int i = 0; i < 1 + two; ++i) written(out[i], "out");
     rtr_rotary_rows q = {}, k = {};
     fill_rows(q, in[0], out[0]);
     if (two) fill_rows(k, in[1], out[1]);
@@ -225,18 +235,188 @@ PyObject* call_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------- beam search
+// select(status address, device, beams, eos or None, candidates, logits, scores, allowed or None)
+PyObject* call_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    uint32_t* status = static_cast<uint32_t*>(PyLong_AsVoidPtr(a[0]));
+    const int index = (int)PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) throw Raised{};
+    const int64_t beams = whole(a[2], "beams"), eos = a[3] == Py_None ? -1 : whole(a[3], "eos"), k = whole(a[4], "candidates");
+    at::Tensor logits = tensor(a[5], "logits"), scores = tensor(a[6], "scores");
+    if (logits.dim() != 2 || (logits.scalar_type() != at::kFloat && logits.scalar_type() != at::kBFloat16) || !here(logits, index))
+      refuse("logits must be float32 or bfloat16 [items * beams, vocab] on the handle's device");
+    if (scores.dim() != 2 || scores.scalar_type() != at::kFloat || !scores.is_contiguous() || !here(scores, index))
+      refuse("scores must be float32 [items, beams], contiguous, on the handle's device");
+    const int64_t items = scores.size(0), width = scores.size(1), rows = logits.size(0), vocab = logits.size(1);
+    if (width < 1 || width > 128) refuse("1 to 128 beams an item");
+    if (rows != items * width) refuse("logits must have a row for each of the scores");
+    if (vocab < 1 || vocab > 1 << 20) refuse("a vocabulary of 1 to 2^20 tokens");
+    if (rows > INT32_MAX) refuse("too many rows for one call");
+    if (k > width * vocab) refuse("%lld candidates of %lld there are", (long long)k, (long long)(width * vocab));
+    if (eos >= 0 && k < beams + width)
+      refuse("with eos, %lld beams after %lld need at least %lld candidates", (long long)beams, (long long)width, (long long)(beams + width));
+    if (logits.stride(1) != 1 || (rows > 1 && logits.stride(0) < vocab)) logits = logits.clone(at::MemoryFormat::Contiguous);
+    rtr_beam_step s = {};
+    at::Tensor allowed;
+    if (a[7] != Py_None) {
+      allowed = tensor(a[7], "allowed");
+      if (allowed.scalar_type() != at::kBool || !here(allowed, index) || allowed.dim() < 1 || allowed.dim() > 2 ||
+          allowed.size(-1) != vocab || (allowed.dim() == 2 && allowed.size(0) != rows && allowed.size(0) != 1))
+        refuse("allowed must be bool [items * beams, vocab] or [vocab] on the handle's device");
+      const bool one = allowed.dim() == 1 || allowed.size(0) == 1 || allowed.stride(0) == 0;
+      if ((vocab > 1 && allowed.stride(-1) != 1) || (!one && allowed.stride(0) < vocab))
+        allowed = allowed.clone(at::MemoryFormat::Contiguous);
+      s.allowed = static_cast<const uint8_t*>(allowed.data_ptr());
+      s.allowed_stride = allowed.dim() == 1 || allowed.size(0) == 1 ? 0 : allowed.stride(0);
+    }
+    at::Tensor all_tokens = room_for(index, {items, k}, at::kInt), all_parents = room_for(index, {items, k}, at::kInt),
+               all_scores = room_for(index, {items, k}, at::kFloat), tokens = room_for(index, {items, beams}, at::kInt),
+               parents = room_for(index, {items, beams}, at::kInt), next = room_for(index, {items, beams}, at::kFloat);
+    s.logits = logits.data_ptr();
+    s.scores = static_cast<const float*>(scores.data_ptr());
+    s.logits_stride = rows > 1 ? logits.stride(0) : vocab;
+    s.dtype = type_of(logits);
+    s.items = (int32_t)items;
+    s.n = (int32_t)width;
+    s.vocab = (int32_t)vocab;
+    s.k = (int32_t)k;
+    s.beams = (int32_t)beams;
+    s.eos = eos > INT32_MAX ? -1 : (int32_t)eos;
+    s.all_tokens = static_cast<int32_t*>(all_tokens.data_ptr());
+    s.all_parents = static_cast<int32_t*>(all_parents.data_ptr());
+    s.all_scores = static_cast<float*>(all_scores.data_ptr());
+    s.next_tokens = static_cast<int32_t*>(tokens.data_ptr());
+    s.next_parents = static_cast<int32_t*>(parents.data_ptr());
+    s.next_scores = static_cast<float*>(next.data_ptr());
+    s.status = status;
+    int64_t room = 0;
+    check(beam_workspace(&s, index, &room));
+    at::Tensor work = room_for(index, {room}, at::kByte);
+    check(beam_select(&s, work.data_ptr(), room, index, stream_of(index)));
+    return tuple_of({tokens, parents, next, all_tokens, all_parents, all_scores});
+  });
+}
+
+// A state's layout: its dimensions but that of the rows, outermost first, as few as its strides allow; false where
+// it holds nothing.
+bool layout_of(const at::Tensor& t, int64_t dim, int64_t token_dim, int64_t tokens, rtr_beam_state& s) {
+  struct Dim { int64_t size, stride; };
+  Dim dims[16];
+  int n = 0;
+  const int64_t size = t.element_size();
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    const int64_t count = d == token_dim ? tokens : t.size(d);
+    if (!count) return false;
+    if (d == dim || count == 1) continue;
+    if (n == 16) refuse("a state has too many dimensions");
+    dims[n++] = Dim{count, t.stride(d)};
+  }
+  std::sort(dims, dims + n, [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
+  Dim with_rows[17];
+  std::copy(dims, dims + n, with_rows);
+  int all = n;
+  if (t.size(dim) > 1) with_rows[all++] = Dim{t.size(dim), t.stride(dim)};
+  std::sort(with_rows, with_rows + all, [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
+  int64_t reach = 0;
+  for (int i = all - 1; i >= 0; --i) {
+    if (with_rows[i].stride <= reach) refuse("the values of a state overlap in memory");
+    reach += (with_rows[i].size - 1) * with_rows[i].stride;
+  }
+  s = {};
+  s.data = t.data_ptr();
+  s.row_bytes = (t.size(dim) > 1 ? t.stride(dim) : 1) * size;
+  s.inner = size;
+  while (n && dims[n - 1].stride * size == s.inner) s.inner *= dims[--n].size;
+  int out = 0;
+  Dim outer[16];
+  for (int i = 0; i < n; ++i) {
+    if (out && outer[out - 1].stride == dims[i].stride * dims[i].size) outer[out - 1] = Dim{outer[out - 1].size * dims[i].size, dims[i].stride};
+    else outer[out++] = dims[i];
+  }
+  if (out > 3) refuse("a state's rows lie in more than three strided dimensions: reorder a contiguous one");
+  for (int d = 0; d < 3; ++d) s.sizes[d] = 1;
+  for (int i = 0; i < out; ++i) {
+    if (outer[i].size > INT32_MAX) refuse("a state's dimensions must fit 32 bits");
+    s.sizes[3 - out + i] = (int32_t)outer[i].size;
+    s.strides[3 - out + i] = outer[i].stride * size;
+  }
+  return true;
+}
+
+// reorder(status address, device, beams, states (a tensor, list or tuple), parents, dim, token_dim or None, tokens or None)
+PyObject* call_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    uint32_t* status = static_cast<uint32_t*>(PyLong_AsVoidPtr(a[0]));
+    const int index = (int)PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) throw Raised{};
+    const int64_t beams = whole(a[2], "beams"), dim_ = whole(a[5], "dim");
+    const at::Tensor& parents = tensor(a[4], "parents");
+    if (parents.scalar_type() != at::kInt || parents.dim() != 2 || parents.size(1) != beams || !parents.is_contiguous() ||
+        !here(parents, index))
+      refuse("parents must be int32 [items, %lld], contiguous, on the handle's device", (long long)beams);
+    const int64_t items = parents.size(0);
+    if (items > 65535) refuse("at most 65535 items in one call");
+    if ((a[6] == Py_None) != (a[7] == Py_None)) refuse("token_dim and tokens belong together");
+    const bool one = THPVariable_Check(a[3]);
+    if (!one && !PyList_Check(a[3]) && !PyTuple_Check(a[3])) refuse("states must be a tensor, or a list or tuple of them");
+    const Py_ssize_t count = one ? 1 : PySequence_Fast_GET_SIZE(a[3]);
+    std::vector<rtr_beam_state> states;
+    std::vector<const void*> known;
+    states.reserve(count);
+    known.reserve(count);
+    for (int pass = 0; pass < 2; ++pass) {  // all are looked at before any counts as written
+      for (Py_ssize_t i = 0; i < count; ++i) {
+        const at::Tensor& t = tensor(one ? a[3] : PySequence_Fast_GET_ITEM(a[3], i), "a state");
+        if (pass) {
+          written(t, "a state");
+          continue;
+        }
+        if (t.requires_grad()) refuse("a state must not require a gradient");
+        const int64_t rank = t.dim(), dim = dim_ < 0 ? dim_ + rank : dim_;
+        if (!here(t, index) || dim < 0 || dim >= rank || t.size(dim) != items * beams)
+          refuse("dimension dim of a state must be the %lld rows, on the handle's device", (long long)(items * beams));
+        if (t.is_complex() || t.is_quantized() || t.layout() != at::kStrided) refuse("a state must be a plain tensor");
+        int64_t token_dim = -1, tokens = 0;
+        if (a[6] != Py_None) {
+          token_dim = whole(a[6], "token_dim");
+          tokens = whole(a[7], "tokens");
+          if (token_dim < 0) token_dim += rank;
+          if (token_dim < 0 || token_dim >= rank || token_dim == dim) refuse("token_dim must be another dimension than dim");
+          if (tokens < 0 || tokens > t.size(token_dim)) refuse("a state holds %lld tokens", (long long)t.size(token_dim));
+        }
+        rtr_beam_state s;
+        if (layout_of(t, dim, token_dim, tokens, s)) {
+          states.push_back(s);
+          known.push_back(s.data);
+        }
+      }
+      if (!pass) {
+        std::sort(known.begin(), known.end());
+        if (std::adjacent_find(known.begin(), known.end()) != known.end()) refuse("a state is among the states twice");
+      }
+    }
+    check(beam_reorder(states.data(), (int32_t)states.size(), static_cast<const int32_t*>(parents.data_ptr()), (int32_t)items,
+                       (int32_t)beams, status, index, stream_of(index)));
+    Py_RETURN_NONE;
+  });
+}
+
 // setup(addresses of the entry points in the order below, last_error's, NativeError)
 PyObject* call_setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 5, [&]() -> PyObject* {
-    void* at[4];
-    for (int i = 0; i < 4; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
+  return guarded(n, 8, [&]() -> PyObject* {
+    void* at[7];
+    for (int i = 0; i < 7; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) throw Raised{};
     pages_grow = reinterpret_cast<decltype(pages_grow)>(at[0]);
     pages_release = reinterpret_cast<decltype(pages_release)>(at[1]);
     rotary = reinterpret_cast<decltype(rotary)>(at[2]);
-    last_error = reinterpret_cast<decltype(last_error)>(at[3]);
-    Py_INCREF(a[4]);
-    Py_XSETREF(native_error, a[4]);
+    beam_workspace = reinterpret_cast<decltype(beam_workspace)>(at[3]);
+    beam_select = reinterpret_cast<decltype(beam_select)>(at[4]);
+    beam_reorder = reinterpret_cast<decltype(beam_reorder)>(at[5]);
+    last_error = reinterpret_cast<decltype(last_error)>(at[6]);
+    Py_INCREF(a[7]);
+    Py_XSETREF(native_error, a[7]);
     Py_RETURN_NONE;
   });
 }
@@ -245,6 +425,8 @@ PyMethodDef methods[] = {{"setup", CALL(call_setup)},
                          {"grow", CALL(call_grow)},
                          {"release", CALL(call_release)},
                          {"rotate", CALL(call_rotate)},
+                         {"select", CALL(call_select)},
+                         {"reorder", CALL(call_reorder)},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_op_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
