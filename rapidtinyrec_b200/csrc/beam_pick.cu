@@ -19,6 +19,7 @@
 // logits arrive), the second latency: three dependent rounds of loads and the searches between them.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "engine.h"
@@ -28,10 +29,11 @@
 namespace rtr {
 
 constexpr int BP_GROUP = 256;                   // logits of a group: eight of each lane of a warp
-constexpr int BP_WARPS = 8, BP_AHEAD = 4;       // first kernel: warps of a block, groups a warp has in flight
+constexpr int BP_WARPS = 8, BP_BLOCKS = 3;      // first kernel: warps of a block, blocks of an SM
 constexpr int BP_THREADS = 1024;                // second kernel
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
 constexpr int BP_GROUPS = 512, BP_LIST = 1024;  // groups and candidates that the second kernel takes up at once
+constexpr int BP_HELD = 8;                      // quartets of groups that a thread of it holds
 constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
@@ -57,6 +59,10 @@ RTR_DEVICE float redux_max(float v) {  // NaN counts as nothing
   return r;
 }
 
+// What a sum is relative to while it grows, in units of log2.
+RTR_DEVICE bool beam_near(float base) { return fabsf(base) < 1e37f; }
+RTR_DEVICE float beam_unit(float base) { return __fmul_rn(base, BP_LOG2E); }
+
 // A warp's part of a group: each lane has eight logits, in pieces of 16 bytes.  Groups start at multiples
 // of 16 bytes: the first of a row that does not holds fewer.
 template <typename T> struct Logits {
@@ -68,6 +74,10 @@ template <typename T> struct Logits {
     const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) u[j] = make_uint4(w, w, w, w);
+  }
+  RTR_DEVICE void load_inside(const T* p) {  // p: the lane's first logit of a group whose 256 are all there
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(p + j * 32 * PER));
   }
   RTR_DEVICE void load(const T* row, int first, int lane, int vocab) {
 #pragma unroll
@@ -91,119 +101,165 @@ template <typename T> struct Logits {
       }
     }
   }
+  RTR_DEVICE float2 two(int i) const {  // logits 2 i and 2 i + 1
+    const uint4& p = u[i / (PER / 2)];
+    if constexpr (sizeof(T) == 4) {
+      return i & 1 ? make_float2(__uint_as_float(p.z), __uint_as_float(p.w)) : make_float2(__uint_as_float(p.x), __uint_as_float(p.y));
+    } else {
+      const uint32_t w = i == 0 ? p.x : i == 1 ? p.y : i == 2 ? p.z : p.w;
+      return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+  }
   RTR_DEVICE void get(float (&x)[8]) const {
 #pragma unroll
-    for (int j = 0; j < PIECES; ++j) {
-      const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = two(i);
+      x[2 * i] = t.x;
+      x[2 * i + 1] = t.y;
+    }
+  }
+  RTR_DEVICE float largest() const {
+    if constexpr (sizeof(T) == 4) {
+      float v[8];
+      get(v);
+      return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    } else {  // two at a time; NaN counts as nothing
+      const auto pair = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
+      const __nv_bfloat162 m = __hmax2(__hmax2(pair(u[0].x), pair(u[0].y)), __hmax2(pair(u[0].z), pair(u[0].w)));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
+};
+
+// The bytes that say which of a lane's eight logits are allowed: two runs of four, by aligned words that hold at least one
+// of them, since a row of bytes may start anywhere (at the same place of a word in all of a row's groups).
+template <typename T> struct Allowed {
+  uint32_t w[4];
+  RTR_DEVICE static int by(const uint8_t* row, int shift) { return 8 * (int)((reinterpret_cast<uintptr_t>(row) - shift) & 3); }
+  RTR_DEVICE void load(const uint8_t* row, int first, int lane, int vocab, int by) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          x[4 * j + i] = __uint_as_float(w[i]);
-        } else {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+    for (int j = 0; j < 2; ++j) {
+      const int e = Logits<T>::at(first, 4 * j, lane);
+      w[2 * j] = w[2 * j + 1] = 0;
+      if (e >= 0 && e + 4 <= vocab) {
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(row + e) & ~(uintptr_t)3);
+        w[2 * j] = __ldg(p);
+        if (by) w[2 * j + 1] = __ldg(p + 1);
+      } else {  // a row's ragged ends
+        uint64_t four = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (e + i >= 0 && e + i < vocab) four |= (uint64_t)row[e + i] << (8 * i);
+        four <<= by;
+        w[2 * j] = (uint32_t)four;
+        w[2 * j + 1] = (uint32_t)(four >> 32);
+      }
+    }
+  }
+  RTR_DEVICE bool operator()(int i, int by) const {
+    return __funnelshift_r(w[2 * (i >> 2)], w[2 * (i >> 2) + 1], by) >> (8 * (i & 3)) & 0xffu;
+  }
+};
+
+// The groups that a warp has in flight: g, g + BP_WARPS, ...
+template <typename T, bool MASK> struct Ahead {
+  static constexpr int N = MASK || sizeof(T) == 4 ? 2 : 4;  // 2 KB of logits (masked bf16: 1 KB, and as much of masks)
+  Logits<T> raw[N];
+  Allowed<T> ok[MASK ? N : 1];
+  RTR_DEVICE void load(const BeamPick& a, const T* x, const uint8_t* allowed, int g, int hi, int shift, int by, int lane) {
+    constexpr int LAST = (N - 1) * BP_WARPS;
+    if (!MASK && g + LAST < hi && g * BP_GROUP >= shift && (g + LAST + 1) * BP_GROUP - shift <= a.vocab) {
+      const T* p = x + (g * BP_GROUP - shift + lane * Logits<T>::PER);
+#pragma unroll
+      for (int j = 0; j < N; ++j) raw[j].load_inside(p + j * BP_WARPS * BP_GROUP);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int first = (g + j * BP_WARPS) * BP_GROUP - shift;
+      if (g + j * BP_WARPS < hi) {
+        raw[j].load(x, first, lane, a.vocab);
+        if constexpr (MASK) ok[j].load(allowed, first, lane, a.vocab, by);
+      } else {
+        raw[j].none();
       }
     }
   }
 };
 
-// Which of a lane's eight logits are allowed, as bits.  Four bytes at a time, by aligned words that hold
-// at least one of them, since a row of bytes may start anywhere.
-template <typename T> RTR_DEVICE uint32_t allowed_bits(const uint8_t* row, int first, int lane, int vocab) {
-  using L = Logits<T>;
-  uint32_t bits = 0;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int e = L::at(first, 4 * j, lane);
-    uint32_t four = 0;
-    if (e >= 0 && e + 4 <= vocab) {
-      const uintptr_t p = reinterpret_cast<uintptr_t>(row + e);
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(p & ~(uintptr_t)3);
-      const int by = (int)(p & 3);
-      four = __ldg(w);
-      if (by) four = __funnelshift_r(four, __ldg(w + 1), 8 * by);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (e + i >= 0 && e + i < vocab) four |= (uint32_t)row[e + i] << (8 * i);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bits |= (four >> (8 * i) & 0xffu ? 1u : 0u) << (4 * j + i);
-  }
-  return bits;
-}
-
-// One block: a slice of a row's groups.
+// One block: a slice of a row's groups, which its warps take in turn, the next ones on their way while some are worked on.
 template <typename T, bool MASK>
-__global__ void __launch_bounds__(BP_WARPS * 32, 4) beam_scan_kernel(const BeamPick a) {
+__global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(const BeamPick a) {
+  using A = Ahead<T, MASK>;
   __shared__ float2 sums[BP_WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
   const float score = a.scores[row];
+  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+  const uint8_t* allowed = MASK ? a.allowed + row * a.allowed_stride : nullptr;
+  const int shift = Logits<T>::shift(x), by = MASK ? Allowed<T>::by(allowed, shift) : 0;
+  const int lo = (int)((int64_t)a.groups * slice / a.slices), hi = (int)((int64_t)a.groups * (slice + 1) / a.slices);
+  float* best = a.best + (int64_t)row * a.padded;
   if (!(score > -INFINITY)) {  // minus infinity: nothing to offer; NaN: the second kernel reports it
     if (tid == 0) a.part[blockIdx.x] = make_float2(-INFINITY, 0.f);
     return;
   }
-  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-  const uint8_t* allowed = MASK ? a.allowed + row * a.allowed_stride : nullptr;
-  const int shift = Logits<T>::shift(x);
-  const int lo = (int)((int64_t)a.groups * slice / a.slices), hi = (int)((int64_t)a.groups * (slice + 1) / a.slices);
-  if (slice == a.slices - 1 && tid < a.padded - a.groups) a.best[(int64_t)row * a.padded + a.groups + tid] = -INFINITY;
+  if (slice == a.slices - 1 && tid < a.padded - a.groups) best[a.groups + tid] = -INFINITY;
   float base = -INFINITY;
-  uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-  const uint64_t log2e = f2(BP_LOG2E, BP_LOG2E);
-  for (int g = lo + warp * BP_AHEAD; g < hi; g += BP_WARPS * BP_AHEAD) {
-    Logits<T> raw[BP_AHEAD];
-    uint32_t bits[BP_AHEAD];
-#pragma unroll
-    for (int j = 0; j < BP_AHEAD; ++j) {
-      const int first = (g + j) * BP_GROUP - shift;
-      if (g + j < hi) raw[j].load(x, first, lane, a.vocab);
-      else raw[j].none();
-      if constexpr (MASK) bits[j] = g + j < hi ? allowed_bits<T>(allowed, first, lane, a.vocab) : 0u;
-    }
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 log2e = make_float2(BP_LOG2E, BP_LOG2E);
+  A now, next;
+  now.load(a, x, allowed, lo + warp, hi, shift, by, lane);
+  for (int g = lo + warp; g < hi; g += A::N * BP_WARPS) {
+    next.load(a, x, allowed, g + A::N * BP_WARPS, hi, shift, by, lane);
     float top = -INFINITY, mine = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < BP_AHEAD; ++j) {
-      float v[8], m = -INFINITY;
-      raw[j].get(v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, v[i]);
-      m = redux_max(m);
+    for (int j = 0; j < A::N; ++j) {
+      float m = redux_max(now.raw[j].largest());
       top = fmaxf(top, m);
       if constexpr (MASK) {
+        float v[8];
+        now.raw[j].get(v);
         m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, bits[j] >> i & 1 ? v[i] : -INFINITY);
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, now.ok[j](i, by) ? v[i] : -INFINITY);
         m = redux_max(m);
       }
       if (lane == j) mine = m;
     }
-    if (lane < BP_AHEAD && g + lane < hi) a.best[(int64_t)row * a.padded + g + lane] = mine;
+    if (lane < A::N && g + lane * BP_WARPS < hi) best[g + lane * BP_WARPS] = mine;
     if (top > base) {  // the same in all lanes
-      const float f = ex2((base - top) * BP_LOG2E);
+      const float f = ex2(beam_near(base) && beam_near(top) ? beam_unit(base) - beam_unit(top) : (base - top) * BP_LOG2E);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sum[i] = f2_mul(sum[i], f2(f, f));
+      for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * f, sum[i].y * f);
       base = top;
     }
-    const float zero = base == -INFINITY ? 0.f : -base;
-    const uint64_t minus = f2(zero, zero);
+    // 2^(x log2(e) - unit), unit = base log2(e) rounded (made up for at the end); near the ends of float's range,
+    // where that product is infinite, the difference comes first
+    if (beam_near(base)) {
+      const float unit = beam_unit(base);
+      const float2 minus = make_float2(-unit, -unit);
 #pragma unroll
-    for (int j = 0; j < BP_AHEAD; ++j) {
-      float v[8];
-      raw[j].get(v);
+      for (int j = 0; j < A::N; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 y = f2_parts(f2_mul(f2_add(f2(v[2 * i], v[2 * i + 1]), minus), log2e));
-        sum[i & 1] = f2_add(sum[i & 1], f2(ex2(y.x), ex2(y.y)));
+        for (int i = 0; i < 4; ++i) {
+          const float2 y = __ffma2_rn(now.raw[j].two(i), log2e, minus);
+          sum[i & 1] = __fadd2_rn(sum[i & 1], make_float2(ex2(y.x), ex2(y.y)));
+        }
+    } else {
+      const float zero = base == -INFINITY ? 0.f : base;
+      for (int j = 0; j < A::N; ++j) {
+        float v[8];
+        now.raw[j].get(v);
+        for (int i = 0; i < 8; ++i) sum[0].x += ex2((v[i] - zero) * BP_LOG2E);
       }
     }
+    now = next;
   }
-  const float2 s = f2_parts(f2_add(sum[0], sum[1]));
-  const float total = warp_sum(s.x + s.y);
+  float total = warp_sum((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y));
+  if (beam_near(base)) total *= ex2(-fmaf(base, BP_LOG2E, -beam_unit(base)));
   if (lane == 0) sums[warp] = make_float2(base, total);
   __syncthreads();
   if (tid == 0) {
@@ -234,10 +290,11 @@ struct PickShared {
   uint64_t key[BP_LIST];
   float x[BP_LIST];
   uint32_t at[BP_LIST];
+  uint8_t row[BP_LIST];
   uint16_t order[BP_LIST];
   double red[BP_THREADS / 32];
   int n_groups, n_list, doubts;
-  float most;
+  int most;  // the largest |off32|, as bits
 };
 
 // A value that at least k threads reach with what they have, or minus infinity where fewer have a finite one:
@@ -257,6 +314,7 @@ RTR_DEVICE float reached_by(float mine, int k) {
 }
 
 template <typename T, bool MASK> struct Picker {
+  static constexpr int TAKE = MASK ? 2 : 4;  // groups that a warp reads again at a time
   const BeamPick& a;
   PickShared& s;
   const int item, tid, warp, lane;
@@ -270,61 +328,107 @@ template <typename T, bool MASK> struct Picker {
   RTR_DEVICE double worth(int r, float x) const { return ((double)x - (double)s.top[r]) + s.off[r]; }
   RTR_DEVICE float near(int r, float x) const { return (x - s.top[r]) + s.off32[r]; }
 
-  // f(group index row * padded + g, best logit) for the thread's groups, of rows that are alive
+  // The thread's quartets of groups: the first ones are held in registers, from the start of the kernel.
+  float4 held[BP_HELD];
+  RTR_DEVICE void hold() {
+    const int all = a.n * (a.padded >> 2);
+#pragma unroll
+    for (int j = 0; j < BP_HELD; ++j) {
+      const int q = tid + j * BP_THREADS;
+      if (q < all) held[j] = __ldcg(reinterpret_cast<const float4*>(best) + q);
+    }
+  }
+  // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer
   template <typename F> RTR_DEVICE void each_group(F&& f) const {
     const int quartets = a.padded >> 2, all = a.n * quartets;
-    for (int q = tid; q < all; q += BP_THREADS) {
+    const auto one = [&](int q, const float4& v) {
       const int r = a.n == 1 ? 0 : row_of((uint32_t)q);
-      if (!(s.off32[r] > -INFINITY)) continue;
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(best) + q);
-      const int g0 = 4 * (q - r * quartets);
-      f(r, g0, v);
+      if (s.off32[r] > -INFINITY) f(r, 4 * (q - r * quartets), v);
+    };
+#pragma unroll
+    for (int j = 0; j < BP_HELD; ++j)
+      if (tid + j * BP_THREADS < all) one(tid + j * BP_THREADS, held[j]);
+    for (int q = tid + BP_HELD * BP_THREADS; q < all; q += BP_THREADS) one(q, __ldcg(reinterpret_cast<const float4*>(best) + q));
+  }
+
+  // f(row, place in the vocabulary, logit) for the lane's finite, allowed logits of all groups of the list
+  template <typename F> RTR_DEVICE void each_logit(int ng, F&& f) const {
+    for (int j0 = warp; j0 < ng; j0 += TAKE * (BP_THREADS / 32)) {
+      Logits<T> raw[TAKE];
+      Allowed<T> ok[MASK ? TAKE : 1];
+      int rows[TAKE], first[TAKE];
+#pragma unroll
+      for (int t = 0; t < TAKE; ++t) {
+        const int j = j0 + t * (BP_THREADS / 32);
+        if (j >= ng) break;
+        const int id = s.groups[j], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
+        rows[t] = r;
+        first[t] = (id - r * a.padded) * BP_GROUP - Logits<T>::shift(row(r));
+        raw[t].load(row(r), first[t], lane, a.vocab);
+        if constexpr (MASK) ok[t].load(mask(r), first[t], lane, a.vocab, Allowed<T>::by(mask(r), Logits<T>::shift(row(r))));
+      }
+#pragma unroll
+      for (int t = 0; t < TAKE; ++t) {
+        if (j0 + t * (BP_THREADS / 32) >= ng) break;
+        float v[8];
+        raw[t].get(v);
+        int by = 0;
+        if constexpr (MASK) by = Allowed<T>::by(mask(rows[t]), Logits<T>::shift(row(rows[t])));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (MASK)
+            if (!ok[t](i, by)) continue;
+          if (v[i] > -INFINITY) f(rows[t], Logits<T>::at(first[t], i, lane), v[i]);
+        }
+      }
     }
   }
-
-  // f(row, place in the vocabulary, logit) for a lane's allowed logits of group r, g
-  template <typename F> RTR_DEVICE void each_logit(int r, int g, const Logits<T>& raw, uint32_t bits, F&& f) const {
-    float v[8];
-    raw.get(v);
-    const int first = g * BP_GROUP - Logits<T>::shift(row(r));
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (v[i] > -INFINITY && (!MASK || (bits >> i & 1))) f(r, Logits<T>::at(first, i, lane), v[i]);
+  RTR_DEVICE const uint8_t* mask(int r) const { return allowed0 + r * a.allowed_stride; }
+  RTR_DEVICE void add(int r, int v, float x) {
+    const int to = atomicAdd(&s.n_list, 1);
+    if (to >= BP_LIST) return;
+    s.x[to] = x;
+    s.row[to] = (uint8_t)r;
+    s.at[to] = (uint32_t)r * a.vocab + v;
   }
 
-  // Each row's sum from its slices, and what its candidates are offset by
+  // Each row's sum from its slices, and what its candidates are offset by: eight lanes a row.
   RTR_DEVICE void offsets() {
-    for (int r = warp; r < a.n; r += BP_THREADS / 32) {
-      const float2* p = a.part + ((int64_t)item * a.n + r) * a.slices;
-      float m = -INFINITY;
-      for (int i = lane; i < a.slices; i += 32) m = fmaxf(m, __ldcg(&p[i].x));
-      m = redux_max(m);
-      double t = 0.0;
-      for (int i = lane; i < a.slices; i += 32) {
-        const float2 v = __ldcg(p + i);
-        t += v.x == m ? (double)v.y : (double)v.y * exp((double)v.x - (double)m);
-      }
+    static_assert(BP_MAX_N * 8 == BP_THREADS, "a row for every eight threads");
+    const int r = tid >> 3, part = tid & 7;
+    const bool there = r < a.n;
+    const float score = there && part == 0 ? a.scores[item * a.n + r] : -INFINITY;
+    const float2* p = a.part + ((int64_t)item * a.n + (there ? r : 0)) * a.slices;
+    float m = -INFINITY;
+    double t = 0.0;
+    for (int i0 = part; there && i0 < a.slices; i0 += 32) {
+      float2 v[4];
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-      if (lane == 0) {
-        const float score = a.scores[item * a.n + r];
-        const bool wrong = !(score < INFINITY) || (score > -INFINITY && !(t >= 0.0 && m < INFINITY));
-        if (wrong) atomicOr(a.status, RTR_DEV_NAN_SCORE);
-        const bool alive = !wrong && score > -INFINITY && m > -INFINITY;
-        s.sum[r] = alive ? log(t) : 0.0;
-        s.top[r] = m;
-        s.off[r] = alive ? (double)score - s.sum[r] : -INFINITY;
-        s.off32[r] = (float)s.off[r];
-        s.again[r] = s.done[r] = 0;
-      }
+      for (int i = 0; i < 4; ++i) v[i] = i0 + 8 * i < a.slices ? __ldcg(p + i0 + 8 * i) : make_float2(-INFINITY, 0.f);
+      const float top = fmaxf(m, fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)));
+      if (m != top) t *= ex2((m - top) * BP_LOG2E);
+      m = top;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t += v[i].x == m ? v[i].y : v[i].y * ex2((v[i].x - m) * BP_LOG2E);
     }
+    float all = m;
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
+    if (m != all) t *= ex2((m - all) * BP_LOG2E);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    if (tid == 0) s.most = 0;
     __syncthreads();
-    if (warp == 0) {
-      float most = 0.f;
-      for (int r = lane; r < a.n; r += 32)
-        if (s.off32[r] > -INFINITY) most = fmaxf(most, fabsf(s.off32[r]));
-      most = redux_max(most);
-      if (lane == 0) s.most = most;
+    if (there && part == 0) {
+      const bool wrong = !(score < INFINITY) || (score > -INFINITY && !(t >= 0.0 && all < INFINITY));
+      if (wrong) atomicOr(a.status, RTR_DEV_NAN_SCORE);
+      const bool alive = !wrong && score > -INFINITY && all > -INFINITY;
+      s.sum[r] = alive ? log(t) : 0.0;
+      s.top[r] = all;
+      s.off[r] = alive ? (double)score - s.sum[r] : -INFINITY;
+      s.off32[r] = (float)s.off[r];
+      s.again[r] = s.done[r] = 0;
+      if (alive) atomicMax(&s.most, __float_as_int(fabsf(s.off32[r])));
     }
     __syncthreads();
   }
@@ -364,7 +468,7 @@ template <typename T, bool MASK> struct Picker {
   }
 
   // What `near` may be off by (three roundings of 2^-24), with room, and what two sums may be.
-  RTR_DEVICE float slack(float t) const { return (float)BP_DOUBT + 4.77e-7f * (s.most + fabsf(t)); }
+  RTR_DEVICE float slack(float t) const { return (float)BP_DOUBT + 4.77e-7f * (__int_as_float(s.most) + fabsf(t)); }
 
   // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too
   // many (ties).
@@ -396,33 +500,16 @@ template <typename T, bool MASK> struct Picker {
     if (!(t > -INFINITY) && ng > BP_LIST / BP_GROUP) {
       // too few threads have groups for a bound: their lanes' best may give one
       mine = -INFINITY;
-      for (int j = warp; j < ng; j += BP_THREADS / 32)
-        take(j, [&](int r, int, float v) { mine = fmaxf(mine, near(r, v)); });
+      each_logit(ng, [&](int r, int, float x) { mine = fmaxf(mine, near(r, x)); });
       t = reached_by(mine, a.k);
       floor_ = t - slack(t);
     }
-    for (int j = warp; j < ng; j += BP_THREADS / 32)
-      take(j, [&](int r, int v, float x) {
-        const float u = near(r, x);
-        if (u > -INFINITY && u >= floor_) {
-          const int to = atomicAdd(&s.n_list, 1);
-          if (to < BP_LIST) {
-            s.x[to] = x;
-            s.at[to] = (uint32_t)r * a.vocab + v;
-          }
-        }
-      });
+    each_logit(ng, [&](int r, int v, float x) {
+      const float u = near(r, x);
+      if (u > -INFINITY && u >= floor_) add(r, v, x);
+    });
     __syncthreads();
     return s.n_list <= BP_LIST;
-  }
-  template <typename F> RTR_DEVICE void take(int j, F&& f) const {
-    const int id = s.groups[j], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2), g = id - r * a.padded;
-    const int first = g * BP_GROUP - Logits<T>::shift(row(r));
-    Logits<T> raw;
-    raw.load(row(r), first, lane, a.vocab);
-    uint32_t bits = 0;
-    if constexpr (MASK) bits = allowed_bits<T>(allowed0 + r * a.allowed_stride, first, lane, a.vocab);
-    each_logit(r, g, raw, bits, f);
   }
 
   RTR_DEVICE int block_count(int mine) {
@@ -458,7 +545,8 @@ template <typename T, bool MASK> struct Picker {
       if (block_count(c) <= wanted) last = t;
     }
   }
-  __device__ __noinline__ void gather_exactly() {
+  RTR_DEVICE void gather_exactly() {
+    hold();
     for (int r = tid; r < a.n; r += BP_THREADS) {
       bool differs = false;
       for (int q = 0; q < a.n; ++q) differs |= s.off[q] > -INFINITY && s.sum[q] != s.sum[r];
@@ -487,18 +575,13 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
     const int ng = min(s.n_groups, BP_GROUPS);
     const auto logits = [&](auto&& f) {
-      for (int j = warp; j < ng; j += BP_THREADS / 32)
-        take(j, [&](int r, int v, float x) { f(double_key(worth(r, x)), (uint32_t)r * a.vocab + v, x); });
+      each_logit(ng, [&](int r, int v, float x) { f(double_key(worth(r, x)), (uint32_t)r * a.vocab + v); });
     };
-    bisect([&](auto&& f) { logits([&](uint64_t key, uint32_t at, float) { f(key, at); }); }, a.k, least, last);
-    logits([&](uint64_t key, uint32_t at, float x) {
-      if (key > least || (key == least && at < last)) {
-        const int to = atomicAdd(&s.n_list, 1);
-        if (to < BP_LIST) {
-          s.x[to] = x;
-          s.at[to] = at;
-        }
-      }
+    bisect(logits, a.k, least, last);
+    each_logit(ng, [&](int r, int v, float x) {
+      const uint64_t key = double_key(worth(r, x));
+      const uint32_t at = (uint32_t)r * a.vocab + v;
+      if (key > least || (key == least && at < last)) add(r, v, x);
     });
     __syncthreads();
   }
@@ -506,7 +589,7 @@ template <typename T, bool MASK> struct Picker {
   // Candidates by value, then place: each one's rank is the number of those before it.
   RTR_DEVICE void put_in_order() {
     const int n = s.n_list;
-    for (int i = tid; i < n; i += BP_THREADS) s.key[i] = double_key(worth(s.at[i] / a.vocab, s.x[i]));
+    for (int i = tid; i < n; i += BP_THREADS) s.key[i] = double_key(worth(s.row[i], s.x[i]));
     __syncthreads();
     for (int i = warp; i < n; i += BP_THREADS / 32) {
       const uint64_t key = s.key[i];
@@ -528,7 +611,7 @@ template <typename T, bool MASK> struct Picker {
     for (int i = tid; i + 1 < n; i += BP_THREADS) {
       // behind the k-th everything is compared with that one
       const int p = s.order[min(i, a.k - 1)], q = s.order[i + 1];
-      const int rp = s.at[p] / a.vocab, rq = s.at[q] / a.vocab;
+      const int rp = s.row[p], rq = s.row[q];
       if (rp == rq || s.sum[rp] == s.sum[rq] || (s.done[rp] && s.done[rq])) continue;
       if (key_double(s.key[p]) - key_double(s.key[q]) >= BP_DOUBT) continue;
       s.again[rp] = s.again[rq] = 1;
@@ -546,17 +629,27 @@ template <typename T, bool MASK> struct Picker {
   }
 };
 
+template <typename T, bool MASK> RTR_DEVICE Picker<T, MASK> picker(const BeamPick& a, PickShared& s) {
+  const int tid = threadIdx.x;
+  const int64_t row0 = (int64_t)blockIdx.x * a.n;
+  return Picker<T, MASK>{a, s, (int)blockIdx.x, tid, tid >> 5, tid & 31, static_cast<const T*>(a.logits) + row0 * a.stride,
+                         MASK ? a.allowed + row0 * a.allowed_stride : nullptr, a.best + row0 * a.padded, {}};
+}
+// Apart, so that what it needs costs the usual path no registers.
+template <typename T, bool MASK> __device__ __noinline__ void gather_exactly(const BeamPick& a, PickShared& s) {
+  picker<T, MASK>(a, s).gather_exactly();
+}
+
 template <typename T, bool MASK>
-__global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const BeamPick a) {
+__global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_constant__ BeamPick a) {
   __shared__ PickShared s;
   pdl_launch_dependents();
   pdl_wait();
   const int item = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t row0 = (int64_t)item * a.n;
-  Picker<T, MASK> p{a, s, item, tid, warp, lane, static_cast<const T*>(a.logits) + row0 * a.stride,
-                    MASK ? a.allowed + row0 * a.allowed_stride : nullptr, a.best + row0 * a.padded};
+  Picker<T, MASK> p = picker<T, MASK>(a, s);
+  p.hold();
   p.offsets();
-  if (!p.gather()) p.gather_exactly();
+  if (!p.gather()) gather_exactly<T, MASK>(a, s);
   p.put_in_order();
   if (p.doubtful()) {
     p.sum_again();
@@ -575,6 +668,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const BeamPick a)
     for (int w = 0; w < warp; ++w) before += (int)s.red[w];
     if (free_ && n + before < a.k) {
       s.at[n + before] = (uint32_t)tid;
+      s.row[n + before] = (uint8_t)(tid / a.vocab);
       s.key[n + before] = double_key(-INFINITY);
       s.order[n + before] = (uint16_t)(n + before);
     }
@@ -583,22 +677,22 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const BeamPick a)
   if (tid < a.k) {
     const int i = s.order[tid];
     const int64_t to = (int64_t)item * a.k + tid;
-    a.all_tokens[to] = s.at[i] % a.vocab;
-    a.all_parents[to] = s.at[i] / a.vocab;
+    a.all_tokens[to] = (int32_t)s.at[i] - s.row[i] * a.vocab;
+    a.all_parents[to] = s.row[i];
     a.all_scores[to] = (float)key_double(s.key[i]);
   }
   if (warp == 0) {
     int taken = 0;
     for (int j0 = 0; j0 < a.k && taken < a.beams; j0 += 32) {
       const int j = j0 + lane;
-      const int i = j < a.k ? s.order[j] : 0, token = s.at[i] % a.vocab;
+      const int i = j < a.k ? s.order[j] : 0, token = (int32_t)s.at[i] - s.row[i] * a.vocab;
       const bool on = j < a.k && token != a.eos;
       const unsigned mask = __ballot_sync(0xffffffffu, on);
       const int place = taken + __popc(mask & ((1u << lane) - 1));
       if (on && place < a.beams) {
         const int64_t to = (int64_t)item * a.beams + place;
         a.next_tokens[to] = token;
-        a.next_parents[to] = s.at[i] / a.vocab;
+        a.next_parents[to] = s.row[i];
         a.next_scores[to] = (float)key_double(s.key[i]);
       }
       taken += __popc(mask);
@@ -631,11 +725,11 @@ static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& bes
   p.groups = (int)(((int64_t)b->vocab + per - 1 + BP_GROUP - 1) / BP_GROUP);
   p.padded = (p.groups + 3) & ~3;
   p.quarter_inv = (uint32_t)((0x100000000ull + p.padded / 4 - 1) / (p.padded / 4));
-  // A slice is two rounds of a block's warps where the rows alone fill the GPU, and one where they do not
-  const int64_t rows = (int64_t)b->items * b->n;
-  const int round = BP_WARPS * BP_AHEAD;
-  int64_t slices = (p.groups + 2 * round - 1) / (2 * round);
-  if (rows * slices < 4 * (int64_t)sms) slices = (p.groups + round - 1) / round;
+  // Slices of a row: as many blocks as the SMs hold at once while the rows are few (a warp takes a group at least), eight times as many
+  // blocks as that where they are many, so that the last ones to finish cost little.
+  const int64_t rows = (int64_t)b->items * b->n, room = BP_BLOCKS * (int64_t)sms;
+  const int64_t want = rows <= room ? room / std::max<int64_t>(rows, 1) : (8 * room + rows - 1) / rows;
+  const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(want, (p.groups + BP_WARPS - 1) / BP_WARPS));
   p.slices = (int)slices;
   best_bytes = rows * p.padded * (int64_t)sizeof(float);
   best_bytes = (best_bytes + 15) & ~(int64_t)15;
