@@ -4,9 +4,9 @@
 // of exponentials of row i.  Within a row the order is that of the logits; across rows it
 // needs lse, which is known only when a row has been read.  So the first kernel
 // reads each logit once and leaves, beside the row's running maximum and sum, the largest logit of every
-// group of 256.  The k-th largest of the groups' best is a lower bound T of the k-th largest candidate, and only
+// group of 512.  The k-th largest of the groups' best is a lower bound T of the k-th largest candidate, and only
 // groups whose best reaches T can hold one of the k: k of them but for ties.  The second kernel
-// (a block an item) finds T, reads those groups again (25,600 of 7.6 million logits for 100 candidates of 50 beams), takes what
+// (a block an item) finds T, reads those groups again (51,200 of 7.6 million logits for 100 candidates of 50 beams), takes what
 // reaches T and puts it in order.
 //
 // Order.  The sums are fp32 (an error of some 2e-7 in lse), the 100 best of 7.6 million candidates lie 1e-3 apart, and a batch
@@ -28,12 +28,13 @@
 
 namespace rtr {
 
-constexpr int BP_GROUP = 256;                   // logits of a group: eight of each lane of a warp
-constexpr int BP_WARPS = 8, BP_BLOCKS = 3;      // first kernel: warps of a block, blocks of an SM
+constexpr int BP_GROUP = 512, BP_EACH = 16;     // logits of a group, and of each lane of the warp that has it
+constexpr int BP_WARPS = 8, BP_BLOCKS = 4;      // first kernel: warps of a block, blocks of an SM
+constexpr int BP_RING = 6144;                   // bytes of logits that a warp of it has on their way
 constexpr int BP_THREADS = 1024;                // second kernel
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
 constexpr int BP_GROUPS = 512, BP_LIST = 1024;  // groups and candidates that the second kernel takes up at once
-constexpr int BP_HELD = 8;                      // quartets of groups that a thread of it holds
+constexpr int BP_HELD = 4;                      // quartets of groups that a thread of it holds
 constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
@@ -63,10 +64,10 @@ RTR_DEVICE float redux_max(float v) {  // NaN counts as nothing
 RTR_DEVICE bool beam_near(float base) { return fabsf(base) < 1e37f; }
 RTR_DEVICE float beam_unit(float base) { return __fmul_rn(base, BP_LOG2E); }
 
-// A warp's part of a group: each lane has eight logits, in pieces of 16 bytes.  Groups start at multiples
+// A warp's part of a group: each lane has sixteen logits, in pieces of 16 bytes.  Groups start at multiples
 // of 16 bytes: the first of a row that does not holds fewer.
 template <typename T> struct Logits {
-  static constexpr int PER = 16 / sizeof(T), PIECES = 8 / PER;
+  static constexpr int PER = 16 / sizeof(T), PIECES = BP_EACH / PER;
   uint4 u[PIECES];
   RTR_DEVICE static int shift(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
   RTR_DEVICE static int at(int first, int i, int lane) { return first + (i / PER) * 32 * PER + lane * PER + i % PER; }
@@ -75,7 +76,7 @@ template <typename T> struct Logits {
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) u[j] = make_uint4(w, w, w, w);
   }
-  RTR_DEVICE void load_inside(const T* p) {  // p: the lane's first logit of a group whose 256 are all there
+  RTR_DEVICE void load_inside(const T* p) {  // p: the lane's first logit of a group that is all there
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) u[j] = __ldg(reinterpret_cast<const uint4*>(p + j * 32 * PER));
   }
@@ -106,92 +107,65 @@ template <typename T> struct Logits {
     if constexpr (sizeof(T) == 4) {
       return i & 1 ? make_float2(__uint_as_float(p.z), __uint_as_float(p.w)) : make_float2(__uint_as_float(p.x), __uint_as_float(p.y));
     } else {
-      const uint32_t w = i == 0 ? p.x : i == 1 ? p.y : i == 2 ? p.z : p.w;
+      const uint32_t w = (i & 3) == 0 ? p.x : (i & 3) == 1 ? p.y : (i & 3) == 2 ? p.z : p.w;
       return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     }
   }
-  RTR_DEVICE void get(float (&x)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = two(i);
-      x[2 * i] = t.x;
-      x[2 * i + 1] = t.y;
-    }
-  }
+  RTR_DEVICE float one(int i) const { return i & 1 ? two(i >> 1).y : two(i >> 1).x; }
   RTR_DEVICE float largest() const {
     if constexpr (sizeof(T) == 4) {
-      float v[8];
-      get(v);
-      return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+      float m[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(one(4 * j), one(4 * j + 1)), fmaxf(one(4 * j + 2), one(4 * j + 3)));
+      return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     } else {  // two at a time; NaN counts as nothing
       const auto pair = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
-      const __nv_bfloat162 m = __hmax2(__hmax2(pair(u[0].x), pair(u[0].y)), __hmax2(pair(u[0].z), pair(u[0].w)));
+      const auto four = [&](const uint4& x) { return __hmax2(__hmax2(pair(x.x), pair(x.y)), __hmax2(pair(x.z), pair(x.w))); };
+      const __nv_bfloat162 m = __hmax2(four(u[0]), four(u[1]));
       return fmaxf(__low2float(m), __high2float(m));
     }
   }
 };
 
-// The bytes that say which of a lane's eight logits are allowed: two runs of four, by aligned words that hold at least one
+// The bytes that say which of a lane's logits are allowed: runs of four, by aligned words that hold at least one
 // of them, since a row of bytes may start anywhere (at the same place of a word in all of a row's groups).
 template <typename T> struct Allowed {
-  uint32_t w[4];
+  static constexpr int RUNS = BP_EACH / 4;
+  uint32_t w[RUNS][2];
   RTR_DEVICE static int by(const uint8_t* row, int shift) { return 8 * (int)((reinterpret_cast<uintptr_t>(row) - shift) & 3); }
   RTR_DEVICE void load(const uint8_t* row, int first, int lane, int vocab, int by) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < RUNS; ++j) {
       const int e = Logits<T>::at(first, 4 * j, lane);
-      w[2 * j] = w[2 * j + 1] = 0;
+      w[j][0] = w[j][1] = 0;
       if (e >= 0 && e + 4 <= vocab) {
         const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(row + e) & ~(uintptr_t)3);
-        w[2 * j] = __ldg(p);
-        if (by) w[2 * j + 1] = __ldg(p + 1);
+        w[j][0] = __ldg(p);
+        if (by) w[j][1] = __ldg(p + 1);
       } else {  // a row's ragged ends
         uint64_t four = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (e + i >= 0 && e + i < vocab) four |= (uint64_t)row[e + i] << (8 * i);
         four <<= by;
-        w[2 * j] = (uint32_t)four;
-        w[2 * j + 1] = (uint32_t)(four >> 32);
+        w[j][0] = (uint32_t)four;
+        w[j][1] = (uint32_t)(four >> 32);
       }
     }
   }
   RTR_DEVICE bool operator()(int i, int by) const {
-    return __funnelshift_r(w[2 * (i >> 2)], w[2 * (i >> 2) + 1], by) >> (8 * (i & 3)) & 0xffu;
+    return __funnelshift_r(w[i >> 2][0], w[i >> 2][1], by) >> (8 * (i & 3)) & 0xffu;
   }
 };
 
-// The groups that a warp has in flight: g, g + BP_WARPS, ...
-template <typename T, bool MASK> struct Ahead {
-  static constexpr int N = MASK || sizeof(T) == 4 ? 2 : 4;  // 2 KB of logits (masked bf16: 1 KB, and as much of masks)
-  Logits<T> raw[N];
-  Allowed<T> ok[MASK ? N : 1];
-  RTR_DEVICE void load(const BeamPick& a, const T* x, const uint8_t* allowed, int g, int hi, int shift, int by, int lane) {
-    constexpr int LAST = (N - 1) * BP_WARPS;
-    if (!MASK && g + LAST < hi && g * BP_GROUP >= shift && (g + LAST + 1) * BP_GROUP - shift <= a.vocab) {
-      const T* p = x + (g * BP_GROUP - shift + lane * Logits<T>::PER);
-#pragma unroll
-      for (int j = 0; j < N; ++j) raw[j].load_inside(p + j * BP_WARPS * BP_GROUP);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int first = (g + j * BP_WARPS) * BP_GROUP - shift;
-      if (g + j * BP_WARPS < hi) {
-        raw[j].load(x, first, lane, a.vocab);
-        if constexpr (MASK) ok[j].load(allowed, first, lane, a.vocab, by);
-      } else {
-        raw[j].none();
-      }
-    }
-  }
-};
-
-// One block: a slice of a row's groups, which its warps take in turn, the next ones on their way while some are worked on.
+// One block: a slice of a row's groups, which its warps take in turn.  The groups that are all there come through a ring in shared
+// memory of each warp's own, every lane's pieces copied by the lane that reads them: 6 KB a warp keep 192 KB an SM on their way without
+// a register (two groups in registers of their own, the one read while the other comes, 24 warps: 110 us instead of NN for 32 x 50 rows of bf16).
 template <typename T, bool MASK>
 __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(const BeamPick a) {
-  using A = Ahead<T, MASK>;
-  __shared__ float2 sums[BP_WARPS];
+  using L = Logits<T>;
+  constexpr int BYTES = BP_GROUP * (int)sizeof(T), STAGES = BP_RING / BYTES;
+  __shared__ __align__(16) uint8_t ring[BP_WARPS][BP_RING];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -199,7 +173,7 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
   const float score = a.scores[row];
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   const uint8_t* allowed = MASK ? a.allowed + row * a.allowed_stride : nullptr;
-  const int shift = Logits<T>::shift(x), by = MASK ? Allowed<T>::by(allowed, shift) : 0;
+  const int shift = L::shift(x), by = MASK ? Allowed<T>::by(allowed, shift) : 0;
   const int lo = (int)((int64_t)a.groups * slice / a.slices), hi = (int)((int64_t)a.groups * (slice + 1) / a.slices);
   float* best = a.best + (int64_t)row * a.padded;
   if (!(score > -INFINITY)) {  // minus infinity: nothing to offer; NaN: the second kernel reports it
@@ -210,26 +184,16 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
   float base = -INFINITY;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   const float2 log2e = make_float2(BP_LOG2E, BP_LOG2E);
-  A now, next;
-  now.load(a, x, allowed, lo + warp, hi, shift, by, lane);
-  for (int g = lo + warp; g < hi; g += A::N * BP_WARPS) {
-    next.load(a, x, allowed, g + A::N * BP_WARPS, hi, shift, by, lane);
-    float top = -INFINITY, mine = -INFINITY;
+  const auto take = [&](const L& raw, const Allowed<T>& ok, int g) {
+    const float top = redux_max(raw.largest());
+    float mine = top;
+    if constexpr (MASK) {
+      mine = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < A::N; ++j) {
-      float m = redux_max(now.raw[j].largest());
-      top = fmaxf(top, m);
-      if constexpr (MASK) {
-        float v[8];
-        now.raw[j].get(v);
-        m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, now.ok[j](i, by) ? v[i] : -INFINITY);
-        m = redux_max(m);
-      }
-      if (lane == j) mine = m;
+      for (int i = 0; i < BP_EACH; ++i) mine = fmaxf(mine, ok(i, by) ? raw.one(i) : -INFINITY);
+      mine = redux_max(mine);
     }
-    if (lane < A::N && g + lane * BP_WARPS < hi) best[g + lane * BP_WARPS] = mine;
+    if (lane == 0) best[g] = mine;
     if (top > base) {  // the same in all lanes
       const float f = ex2(beam_near(base) && beam_near(top) ? beam_unit(base) - beam_unit(top) : (base - top) * BP_LOG2E);
 #pragma unroll
@@ -242,32 +206,67 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
       const float unit = beam_unit(base);
       const float2 minus = make_float2(-unit, -unit);
 #pragma unroll
-      for (int j = 0; j < A::N; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 y = __ffma2_rn(now.raw[j].two(i), log2e, minus);
-          sum[i & 1] = __fadd2_rn(sum[i & 1], make_float2(ex2(y.x), ex2(y.y)));
-        }
+      for (int i = 0; i < BP_EACH / 2; ++i) {
+        const float2 y = __ffma2_rn(raw.two(i), log2e, minus);
+        sum[i & 1] = __fadd2_rn(sum[i & 1], make_float2(ex2(y.x), ex2(y.y)));
+      }
     } else {
       const float zero = base == -INFINITY ? 0.f : base;
-      for (int j = 0; j < A::N; ++j) {
-        float v[8];
-        now.raw[j].get(v);
-        for (int i = 0; i < 8; ++i) sum[0].x += ex2((v[i] - zero) * BP_LOG2E);
-      }
+#pragma unroll
+      for (int i = 0; i < BP_EACH; ++i) sum[0].x += ex2((raw.one(i) - zero) * BP_LOG2E);
     }
-    now = next;
+  };
+  // the warp's groups that are all there, and before and behind them those at the row's ends
+  const int end = min(hi, (int)(((int64_t)a.vocab + shift) / BP_GROUP));
+  int g = lo + warp;
+  L raw;
+  Allowed<T> ok;
+  if (g == 0 && shift && hi > 0) {
+    raw.load(x, -shift, lane, a.vocab);
+    if constexpr (MASK) ok.load(allowed, -shift, lane, a.vocab, by);
+    take(raw, ok, 0);
+    g = BP_WARPS;
+  }
+  const int n = g < end ? (end - g + BP_WARPS - 1) / BP_WARPS : 0;
+  const T* from = x + ((int64_t)g * BP_GROUP - shift + lane * L::PER);
+  uint8_t* mine = ring[warp] + lane * 16;
+  const auto issue = [&](int i, int stage) {
+    if (i < n) {
+#pragma unroll
+      for (int j = 0; j < L::PIECES; ++j)
+        cp_async16(mine + stage * BYTES + j * 512, from + (int64_t)i * (BP_WARPS * BP_GROUP) + j * 32 * L::PER, true);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
+  for (int i = 0, stage = 0; i < n; ++i) {
+    if constexpr (MASK) ok.load(allowed, (g + i * BP_WARPS) * BP_GROUP - shift, lane, a.vocab, by);
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < L::PIECES; ++j) raw.u[j] = *reinterpret_cast<const uint4*>(mine + stage * BYTES + j * 512);
+    __syncwarp();
+    issue(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);  // where the last one was
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    take(raw, ok, g + i * BP_WARPS);
+  }
+  for (g += n * BP_WARPS; g < hi; g += BP_WARPS) {
+    raw.load(x, g * BP_GROUP - shift, lane, a.vocab);
+    if constexpr (MASK) ok.load(allowed, g * BP_GROUP - shift, lane, a.vocab, by);
+    take(raw, ok, g);
   }
   float total = warp_sum((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y));
   if (beam_near(base)) total *= ex2(-fmaf(base, BP_LOG2E, -beam_unit(base)));
-  if (lane == 0) sums[warp] = make_float2(base, total);
+  const auto sums = [&](int w) -> float2& { return *reinterpret_cast<float2*>(ring[w]); };  // nothing is under way any more
+  if (lane == 0) sums(warp) = make_float2(base, total);
   __syncthreads();
   if (tid == 0) {
     float m = -INFINITY, t = 0.f;
 #pragma unroll
-    for (int w = 0; w < BP_WARPS; ++w) m = fmaxf(m, sums[w].x);
+    for (int w = 0; w < BP_WARPS; ++w) m = fmaxf(m, sums(w).x);
 #pragma unroll
-    for (int w = 0; w < BP_WARPS; ++w) t += sums[w].x == m ? sums[w].y : sums[w].y * ex2((sums[w].x - m) * BP_LOG2E);
+    for (int w = 0; w < BP_WARPS; ++w) t += sums(w).x == m ? sums(w).y : sums(w).y * ex2((sums(w).x - m) * BP_LOG2E);
     a.part[blockIdx.x] = make_float2(m, t);
   }
 }
@@ -314,7 +313,7 @@ RTR_DEVICE float reached_by(float mine, int k) {
 }
 
 template <typename T, bool MASK> struct Picker {
-  static constexpr int TAKE = MASK ? 2 : 4;  // groups that a warp reads again at a time
+  static constexpr int TAKE = MASK ? 1 : sizeof(T) == 4 ? 2 : 4;  // groups that a warp reads again at a time
   const BeamPick& a;
   PickShared& s;
   const int item, tid, warp, lane;
@@ -370,15 +369,14 @@ template <typename T, bool MASK> struct Picker {
 #pragma unroll
       for (int t = 0; t < TAKE; ++t) {
         if (j0 + t * (BP_THREADS / 32) >= ng) break;
-        float v[8];
-        raw[t].get(v);
         int by = 0;
         if constexpr (MASK) by = Allowed<T>::by(mask(rows[t]), Logits<T>::shift(row(rows[t])));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < BP_EACH; ++i) {
           if constexpr (MASK)
             if (!ok[t](i, by)) continue;
-          if (v[i] > -INFINITY) f(rows[t], Logits<T>::at(first[t], i, lane), v[i]);
+          const float v = raw[t].one(i);
+          if (v > -INFINITY) f(rows[t], Logits<T>::at(first[t], i, lane), v);
         }
       }
     }
