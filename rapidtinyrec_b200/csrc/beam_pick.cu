@@ -28,13 +28,13 @@
 
 namespace rtr {
 
-constexpr int BP_GROUP = 512, BP_EACH = 16;     // logits of a group, and of each lane of the warp that has it
+constexpr int BP_BYTES = 1024;                  // of a group: two pieces of 16 of each lane of a warp
 constexpr int BP_WARPS = 8, BP_BLOCKS = 4;      // first kernel: warps of a block, blocks of an SM
 constexpr int BP_RING = 6144;                   // bytes of logits that a warp of it has on their way
 constexpr int BP_THREADS = 1024;                // second kernel
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
 constexpr int BP_GROUPS = 512, BP_LIST = 1024;  // groups and candidates that the second kernel takes up at once
-constexpr int BP_HELD = 4;                      // quartets of groups that a thread of it holds
+constexpr int BP_HELD = 8;                      // quartets of groups that a thread of it holds
 constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
@@ -64,10 +64,10 @@ RTR_DEVICE float redux_max(float v) {  // NaN counts as nothing
 RTR_DEVICE bool beam_near(float base) { return fabsf(base) < 1e37f; }
 RTR_DEVICE float beam_unit(float base) { return __fmul_rn(base, BP_LOG2E); }
 
-// A warp's part of a group: each lane has sixteen logits, in pieces of 16 bytes.  Groups start at multiples
+// A warp's part of a group (512 logits in bf16, 256 in fp32), two pieces of 16 bytes each lane.  Groups start at multiples
 // of 16 bytes: the first of a row that does not holds fewer.
 template <typename T> struct Logits {
-  static constexpr int PER = 16 / sizeof(T), PIECES = BP_EACH / PER;
+  static constexpr int PER = 16 / sizeof(T), PIECES = 2, EACH = PIECES * PER, GROUP = 32 * EACH;
   uint4 u[PIECES];
   RTR_DEVICE static int shift(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
   RTR_DEVICE static int at(int first, int i, int lane) { return first + (i / PER) * 32 * PER + lane * PER + i % PER; }
@@ -114,10 +114,7 @@ template <typename T> struct Logits {
   RTR_DEVICE float one(int i) const { return i & 1 ? two(i >> 1).y : two(i >> 1).x; }
   RTR_DEVICE float largest() const {
     if constexpr (sizeof(T) == 4) {
-      float m[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = fmaxf(fmaxf(one(4 * j), one(4 * j + 1)), fmaxf(one(4 * j + 2), one(4 * j + 3)));
-      return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      return fmaxf(fmaxf(fmaxf(one(0), one(1)), fmaxf(one(2), one(3))), fmaxf(fmaxf(one(4), one(5)), fmaxf(one(6), one(7))));
     } else {  // two at a time; NaN counts as nothing
       const auto pair = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
       const auto four = [&](const uint4& x) { return __hmax2(__hmax2(pair(x.x), pair(x.y)), __hmax2(pair(x.z), pair(x.w))); };
@@ -130,7 +127,7 @@ template <typename T> struct Logits {
 // The bytes that say which of a lane's logits are allowed: runs of four, by aligned words that hold at least one
 // of them, since a row of bytes may start anywhere (at the same place of a word in all of a row's groups).
 template <typename T> struct Allowed {
-  static constexpr int RUNS = BP_EACH / 4;
+  static constexpr int RUNS = Logits<T>::EACH / 4;
   uint32_t w[RUNS][2];
   RTR_DEVICE static int by(const uint8_t* row, int shift) { return 8 * (int)((reinterpret_cast<uintptr_t>(row) - shift) & 3); }
   RTR_DEVICE void load(const uint8_t* row, int first, int lane, int vocab, int by) {
@@ -164,7 +161,7 @@ template <typename T> struct Allowed {
 template <typename T, bool MASK>
 __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(const BeamPick a) {
   using L = Logits<T>;
-  constexpr int BYTES = BP_GROUP * (int)sizeof(T), STAGES = BP_RING / BYTES;
+  constexpr int BYTES = BP_BYTES, STAGES = BP_RING / BYTES, GROUP = L::GROUP;
   __shared__ __align__(16) uint8_t ring[BP_WARPS][BP_RING];
   pdl_launch_dependents();
   pdl_wait();
@@ -190,7 +187,7 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
     if constexpr (MASK) {
       mine = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < BP_EACH; ++i) mine = fmaxf(mine, ok(i, by) ? raw.one(i) : -INFINITY);
+      for (int i = 0; i < L::EACH; ++i) mine = fmaxf(mine, ok(i, by) ? raw.one(i) : -INFINITY);
       mine = redux_max(mine);
     }
     if (lane == 0) best[g] = mine;
@@ -206,18 +203,18 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
       const float unit = beam_unit(base);
       const float2 minus = make_float2(-unit, -unit);
 #pragma unroll
-      for (int i = 0; i < BP_EACH / 2; ++i) {
+      for (int i = 0; i < L::EACH / 2; ++i) {
         const float2 y = __ffma2_rn(raw.two(i), log2e, minus);
         sum[i & 1] = __fadd2_rn(sum[i & 1], make_float2(ex2(y.x), ex2(y.y)));
       }
     } else {
       const float zero = base == -INFINITY ? 0.f : base;
 #pragma unroll
-      for (int i = 0; i < BP_EACH; ++i) sum[0].x += ex2((raw.one(i) - zero) * BP_LOG2E);
+      for (int i = 0; i < L::EACH; ++i) sum[0].x += ex2((raw.one(i) - zero) * BP_LOG2E);
     }
   };
   // the warp's groups that are all there, and before and behind them those at the row's ends
-  const int end = min(hi, (int)(((int64_t)a.vocab + shift) / BP_GROUP));
+  const int end = min(hi, (int)(((int64_t)a.vocab + shift) / GROUP));
   int g = lo + warp;
   L raw;
   Allowed<T> ok;
@@ -228,20 +225,20 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
     g = BP_WARPS;
   }
   const int n = g < end ? (end - g + BP_WARPS - 1) / BP_WARPS : 0;
-  const T* from = x + ((int64_t)g * BP_GROUP - shift + lane * L::PER);
+  const T* from = x + ((int64_t)g * GROUP - shift + lane * L::PER);
   uint8_t* mine = ring[warp] + lane * 16;
   const auto issue = [&](int i, int stage) {
     if (i < n) {
 #pragma unroll
       for (int j = 0; j < L::PIECES; ++j)
-        cp_async16(mine + stage * BYTES + j * 512, from + (int64_t)i * (BP_WARPS * BP_GROUP) + j * 32 * L::PER, true);
+        cp_async16(mine + stage * BYTES + j * 512, from + (int64_t)i * (BP_WARPS * GROUP) + j * 32 * L::PER, true);
     }
     cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
   for (int i = 0, stage = 0; i < n; ++i) {
-    if constexpr (MASK) ok.load(allowed, (g + i * BP_WARPS) * BP_GROUP - shift, lane, a.vocab, by);
+    if constexpr (MASK) ok.load(allowed, (g + i * BP_WARPS) * GROUP - shift, lane, a.vocab, by);
     cp_async_wait<STAGES - 2>();
     __syncwarp();
 #pragma unroll
@@ -252,8 +249,8 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
     take(raw, ok, g + i * BP_WARPS);
   }
   for (g += n * BP_WARPS; g < hi; g += BP_WARPS) {
-    raw.load(x, g * BP_GROUP - shift, lane, a.vocab);
-    if constexpr (MASK) ok.load(allowed, g * BP_GROUP - shift, lane, a.vocab, by);
+    raw.load(x, g * GROUP - shift, lane, a.vocab);
+    if constexpr (MASK) ok.load(allowed, g * GROUP - shift, lane, a.vocab, by);
     take(raw, ok, g);
   }
   float total = warp_sum((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y));
@@ -281,39 +278,66 @@ RTR_DEVICE double key_double(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
+struct PickEntry {  // a candidate in order: larger keys first, then lower places
+  uint64_t key;
+  uint32_t at, row;
+};
 struct PickShared {
   double sum[BP_MAX_N], off[BP_MAX_N];  // log of the sum of exponentials relative to the maximum, score - that
-  float off32[BP_MAX_N], top[BP_MAX_N];  // off rounded (minus infinity: nothing to offer), the row's maximum
+  float2 near[BP_MAX_N];                // the row's maximum, and off rounded (minus infinity: nothing to offer)
+  float need[BP_MAX_N];                 // what its logits have to reach
   uint8_t again[BP_MAX_N], done[BP_MAX_N];  // rows to sum in 64 bits, and those that are
   int32_t groups[BP_GROUPS];
-  uint64_t key[BP_LIST];
+  PickEntry list[BP_LIST];
   float x[BP_LIST];
-  uint32_t at[BP_LIST];
-  uint8_t row[BP_LIST];
   uint16_t order[BP_LIST];
   double red[BP_THREADS / 32];
-  int n_groups, n_list, doubts;
+  int n_groups, n_list;
+  int bins[BP_THREADS], word2[BP_THREADS / 32];
+  uint32_t word[BP_THREADS / 32], reached;
   int most;  // the largest |off32|, as bits
 };
 
-// A value that at least k threads reach with what they have, or minus infinity where fewer have a finite one:
-// bit by bit from the top of the keys, until the count is near k.
-RTR_DEVICE float reached_by(float mine, int k) {
+// A value that at least k threads reach with what they have, and few more, or minus infinity where fewer have a finite one.  The
+// threads are counted by how far their keys lie behind the largest, in bins of 1/32 of that distance: one pass
+// and one scan (600 cycles; finding the value bit by bit, with a barrier each, 2,600).
+RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t key = mine > -INFINITY ? float_key(mine) : 0u;
-  uint32_t low = 0;
-  const int near = k + (k >> 3) + 4;
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t t = low | 1u << b;
-    const int c = __syncthreads_count(key >= t);
-    if (c < k) continue;
-    low = t;
-    if (c <= near) break;
+  const uint32_t warp_most = __reduce_max_sync(0xffffffffu, key);
+  s.bins[tid] = 0;
+  if (lane == 0) s.word[warp] = warp_most;
+  __syncthreads();
+  const uint32_t most = __reduce_max_sync(0xffffffffu, s.word[lane]);
+  if (key) {
+    const uint32_t bits = __float_as_uint((float)(most - key));
+    atomicAdd(&s.bins[bits ? min(BP_THREADS - 1, (int)(bits >> 18) - (127 << 5) + 1) : 0], 1);
   }
-  return low ? key_float(low) : -INFINITY;
+  __syncthreads();
+  const int c = s.bins[tid];
+  int sum = c;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += u;
+  }
+  if (lane == 31) s.word2[warp] = sum;
+  if (tid == 0) s.reached = 0;
+  __syncthreads();
+  int before = lane < warp ? s.word2[lane] : 0;
+  sum += __reduce_add_sync(0xffffffffu, before);
+  // the last bin holds whatever is further away than it starts: no bound
+  if (tid < BP_THREADS - 1 && sum >= k && sum - c < k) {
+    const float edge = __uint_as_float((uint32_t)(tid + (127 << 5)) << 18);  // where the next bin starts
+    s.reached = max(0x00800000u, most - min(most, tid ? (uint32_t)ceilf(edge) : 0u));  // no further than the least float
+  }
+  __syncthreads();
+  return s.reached ? key_float(s.reached) : -INFINITY;
 }
 
 template <typename T, bool MASK> struct Picker {
-  static constexpr int TAKE = MASK ? 1 : sizeof(T) == 4 ? 2 : 4;  // groups that a warp reads again at a time
+  using L = Logits<T>;
+  static constexpr int TAKE = MASK ? 2 : 4;  // groups that a warp reads again at a time
   const BeamPick& a;
   PickShared& s;
   const int item, tid, warp, lane;
@@ -324,8 +348,9 @@ template <typename T, bool MASK> struct Picker {
   RTR_DEVICE int row_of(uint32_t quartet) const { return (int)(a.quarter_inv ? __umulhi(quartet, a.quarter_inv) : quartet); }
   RTR_DEVICE const T* row(int r) const { return x0 + r * a.stride; }
   // what a candidate is worth, and nearly so
-  RTR_DEVICE double worth(int r, float x) const { return ((double)x - (double)s.top[r]) + s.off[r]; }
-  RTR_DEVICE float near(int r, float x) const { return (x - s.top[r]) + s.off32[r]; }
+  RTR_DEVICE double worth(int r, float x) const { return ((double)x - (double)s.near[r].x) + s.off[r]; }
+  RTR_DEVICE float near(int r, float x) const { return (x - s.near[r].x) + s.near[r].y; }
+  RTR_DEVICE bool alive(int r) const { return s.near[r].y > -INFINITY; }
 
   // The thread's quartets of groups: the first ones are held in registers, from the start of the kernel.
   float4 held[BP_HELD];
@@ -342,7 +367,7 @@ template <typename T, bool MASK> struct Picker {
     const int quartets = a.padded >> 2, all = a.n * quartets;
     const auto one = [&](int q, const float4& v) {
       const int r = a.n == 1 ? 0 : row_of((uint32_t)q);
-      if (s.off32[r] > -INFINITY) f(r, 4 * (q - r * quartets), v);
+      if (alive(r)) f(r, 4 * (q - r * quartets), v);
     };
 #pragma unroll
     for (int j = 0; j < BP_HELD; ++j)
@@ -350,8 +375,8 @@ template <typename T, bool MASK> struct Picker {
     for (int q = tid + BP_HELD * BP_THREADS; q < all; q += BP_THREADS) one(q, __ldcg(reinterpret_cast<const float4*>(best) + q));
   }
 
-  // f(row, place in the vocabulary, logit) for the lane's finite, allowed logits of all groups of the list
-  template <typename F> RTR_DEVICE void each_logit(int ng, F&& f) const {
+  // f(row, first place, logits, mask) for the warp's groups of the list
+  template <typename F> RTR_DEVICE void each_read(int ng, F&& f) const {
     for (int j0 = warp; j0 < ng; j0 += TAKE * (BP_THREADS / 32)) {
       Logits<T> raw[TAKE];
       Allowed<T> ok[MASK ? TAKE : 1];
@@ -362,7 +387,7 @@ template <typename T, bool MASK> struct Picker {
         if (j >= ng) break;
         const int id = s.groups[j], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
         rows[t] = r;
-        first[t] = (id - r * a.padded) * BP_GROUP - Logits<T>::shift(row(r));
+        first[t] = (id - r * a.padded) * L::GROUP - L::shift(row(r));
         raw[t].load(row(r), first[t], lane, a.vocab);
         if constexpr (MASK) ok[t].load(mask(r), first[t], lane, a.vocab, Allowed<T>::by(mask(r), Logits<T>::shift(row(r))));
       }
@@ -371,23 +396,27 @@ template <typename T, bool MASK> struct Picker {
         if (j0 + t * (BP_THREADS / 32) >= ng) break;
         int by = 0;
         if constexpr (MASK) by = Allowed<T>::by(mask(rows[t]), Logits<T>::shift(row(rows[t])));
-#pragma unroll
-        for (int i = 0; i < BP_EACH; ++i) {
-          if constexpr (MASK)
-            if (!ok[t](i, by)) continue;
-          const float v = raw[t].one(i);
-          if (v > -INFINITY) f(rows[t], Logits<T>::at(first[t], i, lane), v);
-        }
+        f(rows[t], first[t], raw[t], ok[MASK ? t : 0], by);
       }
     }
+  }
+  // f(row, place in the vocabulary, logit) for the lane's finite, allowed logits of these groups
+  template <typename F> RTR_DEVICE void each_logit(int ng, F&& f) const {
+    each_read(ng, [&](int r, int first, const Logits<T>& raw, const Allowed<T>& ok, int by) {
+#pragma unroll
+      for (int i = 0; i < L::EACH; ++i) {
+        const float v = raw.one(i);
+        if (v > -INFINITY && (!MASK || ok(i, by))) f(r, Logits<T>::at(first, i, lane), v);
+      }
+    });
   }
   RTR_DEVICE const uint8_t* mask(int r) const { return allowed0 + r * a.allowed_stride; }
   RTR_DEVICE void add(int r, int v, float x) {
     const int to = atomicAdd(&s.n_list, 1);
     if (to >= BP_LIST) return;
     s.x[to] = x;
-    s.row[to] = (uint8_t)r;
-    s.at[to] = (uint32_t)r * a.vocab + v;
+    s.list[to].row = r;
+    s.list[to].at = (uint32_t)r * a.vocab + v;
   }
 
   // Each row's sum from its slices, and what its candidates are offset by: eight lanes a row.
@@ -421,12 +450,15 @@ template <typename T, bool MASK> struct Picker {
       const bool wrong = !(score < INFINITY) || (score > -INFINITY && !(t >= 0.0 && all < INFINITY));
       if (wrong) atomicOr(a.status, RTR_DEV_NAN_SCORE);
       const bool alive = !wrong && score > -INFINITY && all > -INFINITY;
-      s.sum[r] = alive ? log(t) : 0.0;
-      s.top[r] = all;
+      // log t = exponent log 2 + log of the rest, which is 0.75 to 1.5: a float has that to 2^-25 or so
+      const float rounded = (float)t;
+      const int e = alive ? (int)(__float_as_uint(rounded) - 0x3f400000u) >> 23 : 0;
+      const float rest = alive ? __uint_as_float(__float_as_uint(rounded) - ((uint32_t)e << 23)) : 1.f;
+      s.sum[r] = alive ? e * 0.69314718055994530942 + (double)(logf(rest) + (float)(t - (double)rounded) / rounded) : 0.0;
       s.off[r] = alive ? (double)score - s.sum[r] : -INFINITY;
-      s.off32[r] = (float)s.off[r];
+      s.near[r] = make_float2(all, (float)s.off[r]);
       s.again[r] = s.done[r] = 0;
-      if (alive) atomicMax(&s.most, __float_as_int(fabsf(s.off32[r])));
+      if (alive) atomicMax(&s.most, __float_as_int(fabsf((float)s.off[r])));
     }
     __syncthreads();
   }
@@ -437,7 +469,7 @@ template <typename T, bool MASK> struct Picker {
     for (int r = 0; r < a.n; ++r) {
       if (!s.again[r] || s.done[r]) continue;  // the same for all threads
       const T* p = row(r);
-      const double m = s.top[r];
+      const double m = s.near[r].x;
       double t = 0.0;
       for (int i0 = tid; i0 < a.vocab; i0 += 8 * BP_THREADS) {
         float v[8];
@@ -458,7 +490,7 @@ template <typename T, bool MASK> struct Picker {
         for (int w = 0; w < BP_THREADS / 32; ++w) t += s.red[w];
         s.sum[r] = log(t);
         s.off[r] = (double)a.scores[item * a.n + r] - s.sum[r];
-        s.off32[r] = (float)s.off[r];
+        s.near[r].y = (float)s.off[r];
         s.done[r] = 1;
       }
       __syncthreads();
@@ -468,6 +500,15 @@ template <typename T, bool MASK> struct Picker {
   // What `near` may be off by (three roundings of 2^-24), with room, and what two sums may be.
   RTR_DEVICE float slack(float t) const { return (float)BP_DOUBT + 4.77e-7f * (__int_as_float(s.most) + fabsf(t)); }
 
+  // What the rows' logits have to reach for `near` to reach t, with room for its roundings.
+  RTR_DEVICE void needs(float t) {
+    for (int r = tid; r < a.n; r += BP_THREADS) {
+      const float2 v = s.near[r];
+      s.need[r] = v.y > -INFINITY ? (t - v.y) + v.x - 4.77e-7f * (fabsf(t) + fabsf(v.y) + fabsf(v.x)) : INFINITY;
+    }
+    __syncthreads();
+  }
+
   // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too
   // many (ties).
   RTR_DEVICE bool gather() {
@@ -476,35 +517,40 @@ template <typename T, bool MASK> struct Picker {
     each_group([&](int r, int, const float4& v) {
       mine = fmaxf(mine, near(r, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
     });
-    float t = reached_by(mine, a.k);
-    float floor_ = t - slack(t);
-    __syncthreads();
+    float t = reached_by(mine, a.k, s);
+    const float floor_ = t - slack(t);
+    needs(floor_);
     if (mine > -INFINITY && mine >= floor_) {
       each_group([&](int r, int g0, const float4& v) {
-        const float w[4] = {v.x, v.y, v.z, v.w};
+        const float x = s.need[r], w[4] = {v.x, v.y, v.z, v.w};
+        if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x)) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = near(r, w[i]);
-          if (u > -INFINITY && u >= floor_) {
+        for (int i = 0; i < 4; ++i)
+          if (w[i] >= x && w[i] > -INFINITY) {
             const int to = atomicAdd(&s.n_groups, 1);
             if (to < BP_GROUPS) s.groups[to] = r * a.padded + g0 + i;
           }
-        }
       });
     }
     __syncthreads();
     const int ng = s.n_groups;
     if (ng > BP_GROUPS) return false;
-    if (!(t > -INFINITY) && ng > BP_LIST / BP_GROUP) {
+    if (!(t > -INFINITY) && ng > 2) {
       // too few threads have groups for a bound: their lanes' best may give one
       mine = -INFINITY;
       each_logit(ng, [&](int r, int, float x) { mine = fmaxf(mine, near(r, x)); });
-      t = reached_by(mine, a.k);
-      floor_ = t - slack(t);
+      t = reached_by(mine, a.k, s);
+      needs(t - slack(t));
     }
-    each_logit(ng, [&](int r, int v, float x) {
-      const float u = near(r, x);
-      if (u > -INFINITY && u >= floor_) add(r, v, x);
+    each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>&, int) {
+      // hardly ever more than one lane of a group has any: the others look at its logits one each
+      const float x = s.need[r];
+      for (unsigned who = __ballot_sync(0xffffffffu, raw.largest() >= x); who; who &= who - 1) {
+        const int e = L::at(first, lane % L::EACH, __ffs(who) - 1);
+        if (lane >= L::EACH || e < 0 || e >= a.vocab) continue;
+        const float v = to_f32(row(r)[e]);
+        if (v >= x && v > -INFINITY && (!MASK || mask(r)[e])) add(r, e, v);
+      }
     });
     __syncthreads();
     return s.n_list <= BP_LIST;
@@ -584,18 +630,25 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
   }
 
-  // Candidates by value, then place: each one's rank is the number of those before it.
+  // Candidates by value, then place: each one's rank is the number of those before it, counted by eight threads.
   RTR_DEVICE void put_in_order() {
     const int n = s.n_list;
-    for (int i = tid; i < n; i += BP_THREADS) s.key[i] = double_key(worth(s.row[i], s.x[i]));
+    for (int i = tid; i < n; i += BP_THREADS) s.list[i].key = double_key(worth(s.list[i].row, s.x[i]));
     __syncthreads();
-    for (int i = warp; i < n; i += BP_THREADS / 32) {
-      const uint64_t key = s.key[i];
-      const uint32_t at = s.at[i];
+    for (int i0 = 0; i0 < n; i0 += BP_THREADS / 8) {
+      const int i = i0 + (tid >> 3);
       int before = 0;
-      for (int j = lane; j < n; j += 32) before += s.key[j] > key || (s.key[j] == key && s.at[j] < at);
-      before = __reduce_add_sync(0xffffffffu, before);
-      if (lane == 0) s.order[before] = (uint16_t)i;
+      if (i < n) {
+        const PickEntry me = s.list[i];
+#pragma unroll 4
+        for (int j = tid & 7; j < n; j += 8) {
+          const PickEntry it = s.list[j];
+          before += (it.key > me.key) | ((it.key == me.key) & (it.at < me.at));
+        }
+      }
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+      if (i < n && (tid & 7) == 0) s.order[before] = (uint16_t)i;
     }
     __syncthreads();
   }
@@ -603,20 +656,18 @@ template <typename T, bool MASK> struct Picker {
   // Marks the rows of candidates among (or just behind) the first k that are too close to those of another row.  Rows whose
   // sums are equal have exact differences, as long as either all of them are summed again or none.
   RTR_DEVICE bool doubtful() {
-    if (tid == 0) s.doubts = 0;
-    __syncthreads();
     const int n = s.n_list;
+    bool doubt = false;
     for (int i = tid; i + 1 < n; i += BP_THREADS) {
       // behind the k-th everything is compared with that one
-      const int p = s.order[min(i, a.k - 1)], q = s.order[i + 1];
-      const int rp = s.row[p], rq = s.row[q];
+      const PickEntry p = s.list[s.order[min(i, a.k - 1)]], q = s.list[s.order[i + 1]];
+      const int rp = p.row, rq = q.row;
       if (rp == rq || s.sum[rp] == s.sum[rq] || (s.done[rp] && s.done[rq])) continue;
-      if (key_double(s.key[p]) - key_double(s.key[q]) >= BP_DOUBT) continue;
+      if (key_double(p.key) - key_double(q.key) >= BP_DOUBT) continue;
       s.again[rp] = s.again[rq] = 1;
-      s.doubts = 1;
+      doubt = true;
     }
-    __syncthreads();
-    if (!s.doubts) return false;
+    if (!__syncthreads_or(doubt)) return false;
     bool equal = false;
     if (tid < a.n && s.off[tid] > -INFINITY)
       for (int q = 0; q < a.n; ++q) equal |= s.again[q] && s.sum[q] == s.sum[tid];
@@ -658,40 +709,39 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
   if (n < a.k) {
     const int64_t all = (int64_t)a.n * a.vocab;
     bool free_ = tid < 2 * a.k && tid < all;
-    for (int j = 0; j < n && free_; ++j) free_ = s.at[j] != (uint32_t)tid;
+    for (int j = 0; j < n && free_; ++j) free_ = s.list[j].at != (uint32_t)tid;
     const unsigned mask = __ballot_sync(0xffffffffu, free_);
     if (lane == 0) s.red[warp] = __popc(mask);
     __syncthreads();
     int before = __popc(mask & ((1u << lane) - 1));
     for (int w = 0; w < warp; ++w) before += (int)s.red[w];
     if (free_ && n + before < a.k) {
-      s.at[n + before] = (uint32_t)tid;
-      s.row[n + before] = (uint8_t)(tid / a.vocab);
-      s.key[n + before] = double_key(-INFINITY);
+      s.list[n + before] = PickEntry{double_key(-INFINITY), (uint32_t)tid, (uint32_t)(tid / a.vocab)};
       s.order[n + before] = (uint16_t)(n + before);
     }
     __syncthreads();
   }
   if (tid < a.k) {
-    const int i = s.order[tid];
+    const PickEntry c = s.list[s.order[tid]];
     const int64_t to = (int64_t)item * a.k + tid;
-    a.all_tokens[to] = (int32_t)s.at[i] - s.row[i] * a.vocab;
-    a.all_parents[to] = s.row[i];
-    a.all_scores[to] = (float)key_double(s.key[i]);
+    a.all_tokens[to] = (int32_t)(c.at - c.row * a.vocab);
+    a.all_parents[to] = (int32_t)c.row;
+    a.all_scores[to] = (float)key_double(c.key);
   }
   if (warp == 0) {
     int taken = 0;
     for (int j0 = 0; j0 < a.k && taken < a.beams; j0 += 32) {
       const int j = j0 + lane;
-      const int i = j < a.k ? s.order[j] : 0, token = (int32_t)s.at[i] - s.row[i] * a.vocab;
+      const PickEntry c = s.list[j < a.k ? s.order[j] : 0];
+      const int token = (int32_t)(c.at - c.row * a.vocab);
       const bool on = j < a.k && token != a.eos;
       const unsigned mask = __ballot_sync(0xffffffffu, on);
       const int place = taken + __popc(mask & ((1u << lane) - 1));
       if (on && place < a.beams) {
         const int64_t to = (int64_t)item * a.beams + place;
         a.next_tokens[to] = token;
-        a.next_parents[to] = s.row[i];
-        a.next_scores[to] = (float)key_double(s.key[i]);
+        a.next_parents[to] = (int32_t)c.row;
+        a.next_scores[to] = (float)key_double(c.key);
       }
       taken += __popc(mask);
     }
@@ -720,7 +770,8 @@ static const char* beam_check(const rtr_beam_step* b) {
 // Groups of a row (one more where it starts in the middle of one), slices, and the workspace they need.
 static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& best_bytes, int64_t& bytes) {
   const int per = b->dtype == RTR_DTYPE_F32 ? 4 : 8;
-  p.groups = (int)(((int64_t)b->vocab + per - 1 + BP_GROUP - 1) / BP_GROUP);
+  const int group = BP_BYTES * per / 16;
+  p.groups = (int)(((int64_t)b->vocab + per - 1 + group - 1) / group);
   p.padded = (p.groups + 3) & ~3;
   p.quarter_inv = (uint32_t)((0x100000000ull + p.padded / 4 - 1) / (p.padded / 4));
   // Slices of a row: as many blocks as the SMs hold at once while the rows are few (a warp takes a group at least), eight times as many
