@@ -31,9 +31,9 @@ namespace rtr {
 constexpr int BP_BYTES = 1024;                  // of a group: two pieces of 16 of each lane of a warp
 constexpr int BP_WARPS = 8, BP_BLOCKS = 4;      // first kernel: warps of a block, blocks of an SM
 constexpr int BP_RING = 6144;                   // bytes of logits that a warp of it has on their way
-constexpr int BP_THREADS = 1024;                // second kernel
+constexpr int BP_THREADS = 1024;                // second kernel: threads of a block
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
-constexpr int BP_GROUPS = 512, BP_LIST = 1024;  // groups and candidates that the second kernel takes up at once
+constexpr int BP_GROUPS = 512, BP_LANES = 384, BP_LIST = 1024;  // groups, lanes' parts of them and candidates that it takes up at once
 constexpr int BP_HELD = 8;                      // quartets of groups that a thread of it holds
 constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
@@ -292,7 +292,10 @@ struct PickShared {
   float x[BP_LIST];
   uint16_t order[BP_LIST];
   double red[BP_THREADS / 32];
-  int n_groups, n_list;
+  uint4 lane_raw[BP_LANES][2];          // what lanes read whose largest logit reaches its row's need
+  int32_t lane_first[BP_LANES];         // the place of its first logit's lane in the group, and the row
+  uint8_t lane_row[BP_LANES], lane_at[BP_LANES];
+  int n_groups, n_lanes, n_list;
   int bins[BP_THREADS], word2[BP_THREADS / 32];
   uint32_t word[BP_THREADS / 32], reached;
   int most;  // the largest |off32|, as bits
@@ -362,17 +365,23 @@ template <typename T, bool MASK> struct Picker {
       if (q < all) held[j] = __ldcg(reinterpret_cast<const float4*>(best) + q);
     }
   }
-  // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer
+  // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer: those that are not held,
+  // and all
+  template <typename F> RTR_DEVICE void each_later_group(F&& f) const {
+    const int quartets = a.padded >> 2, all = a.n * quartets;
+    for (int q = tid + BP_HELD * BP_THREADS; q < all; q += BP_THREADS) {
+      const int r = a.n == 1 ? 0 : row_of((uint32_t)q);
+      if (alive(r)) f(r, 4 * (q - r * quartets), __ldcg(reinterpret_cast<const float4*>(best) + q));
+    }
+  }
   template <typename F> RTR_DEVICE void each_group(F&& f) const {
     const int quartets = a.padded >> 2, all = a.n * quartets;
-    const auto one = [&](int q, const float4& v) {
-      const int r = a.n == 1 ? 0 : row_of((uint32_t)q);
-      if (alive(r)) f(r, 4 * (q - r * quartets), v);
-    };
 #pragma unroll
-    for (int j = 0; j < BP_HELD; ++j)
-      if (tid + j * BP_THREADS < all) one(tid + j * BP_THREADS, held[j]);
-    for (int q = tid + BP_HELD * BP_THREADS; q < all; q += BP_THREADS) one(q, __ldcg(reinterpret_cast<const float4*>(best) + q));
+    for (int j = 0; j < BP_HELD; ++j) {
+      const int q = tid + j * BP_THREADS, r = q >= all || a.n == 1 ? 0 : row_of((uint32_t)q);
+      if (q < all && alive(r)) f(r, 4 * (q - r * quartets), held[j]);
+    }
+    each_later_group(f);
   }
 
   // f(row, first place, logits, mask) for the warp's groups of the list
@@ -512,25 +521,39 @@ template <typename T, bool MASK> struct Picker {
   // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too
   // many (ties).
   RTR_DEVICE bool gather() {
-    if (tid == 0) s.n_groups = s.n_list = 0;
-    float mine = -INFINITY;
-    each_group([&](int r, int, const float4& v) {
+    if (tid == 0) s.n_groups = s.n_lanes = s.n_list = 0;
+    float mine = -INFINITY, of[BP_HELD];  // of: the held quartets' best
+    const int quartets = a.padded >> 2, all = a.n * quartets;
+#pragma unroll
+    for (int j = 0; j < BP_HELD; ++j) {
+      const int q = tid + j * BP_THREADS, r = q >= all || a.n == 1 ? 0 : row_of((uint32_t)q);
+      const float x = fmaxf(fmaxf(held[j].x, held[j].y), fmaxf(held[j].z, held[j].w));
+      of[j] = q < all && alive(r) ? near(r, x) : -INFINITY;
+      mine = fmaxf(mine, of[j]);
+    }
+    each_later_group([&](int r, int, const float4& v) {
       mine = fmaxf(mine, near(r, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
     });
     float t = reached_by(mine, a.k, s);
     const float floor_ = t - slack(t);
     needs(floor_);
-    if (mine > -INFINITY && mine >= floor_) {
-      each_group([&](int r, int g0, const float4& v) {
-        const float x = s.need[r], w[4] = {v.x, v.y, v.z, v.w};
-        if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= x)) return;
+    const auto look = [&](int r, int g0, const float4& v) {
+      const float x = s.need[r], w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (w[i] >= x && w[i] > -INFINITY) {
-            const int to = atomicAdd(&s.n_groups, 1);
-            if (to < BP_GROUPS) s.groups[to] = r * a.padded + g0 + i;
-          }
-      });
+      for (int i = 0; i < 4; ++i)
+        if (w[i] >= x && w[i] > -INFINITY) {
+          const int to = atomicAdd(&s.n_groups, 1);
+          if (to < BP_GROUPS) s.groups[to] = r * a.padded + g0 + i;
+        }
+    };
+    if (mine > -INFINITY && mine >= floor_) {
+#pragma unroll
+      for (int j = 0; j < BP_HELD; ++j)
+        if (of[j] > -INFINITY && of[j] >= floor_) {
+          const int q = tid + j * BP_THREADS, r = a.n == 1 ? 0 : row_of((uint32_t)q);
+          look(r, 4 * (q - r * quartets), held[j]);
+        }
+      each_later_group(look);
     }
     __syncthreads();
     const int ng = s.n_groups;
@@ -542,16 +565,25 @@ template <typename T, bool MASK> struct Picker {
       t = reached_by(mine, a.k, s);
       needs(t - slack(t));
     }
+    // Hardly ever more than one lane of a group has any: its logits are put aside, for all threads to look at one each.
     each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>&, int) {
-      // hardly ever more than one lane of a group has any: the others look at its logits one each
-      const float x = s.need[r];
-      for (unsigned who = __ballot_sync(0xffffffffu, raw.largest() >= x); who; who &= who - 1) {
-        const int e = L::at(first, lane % L::EACH, __ffs(who) - 1);
-        if (lane >= L::EACH || e < 0 || e >= a.vocab) continue;
-        const float v = to_f32(row(r)[e]);
-        if (v >= x && v > -INFINITY && (!MASK || mask(r)[e])) add(r, e, v);
-      }
+      if (!(raw.largest() >= s.need[r])) return;
+      const int to = atomicAdd(&s.n_lanes, 1);
+      if (to >= BP_LANES) return;
+      s.lane_raw[to][0] = raw.u[0];
+      s.lane_raw[to][1] = raw.u[1];
+      s.lane_first[to] = first;
+      s.lane_row[to] = (uint8_t)r;
+      s.lane_at[to] = (uint8_t)lane;
     });
+    __syncthreads();
+    const int nl = s.n_lanes;
+    if (nl > BP_LANES) return false;
+    for (int i = tid; i < nl * L::EACH; i += BP_THREADS) {
+      const int l = i / L::EACH, j = i % L::EACH, r = s.lane_row[l], e = L::at(s.lane_first[l], j, s.lane_at[l]);
+      const float v = to_f32(reinterpret_cast<const T*>(s.lane_raw[l])[j]);
+      if (v >= s.need[r] && v > -INFINITY && (!MASK || mask(r)[e])) add(r, e, v);
+    }
     __syncthreads();
     return s.n_list <= BP_LIST;
   }
