@@ -64,6 +64,23 @@ RTR_DEVICE float redux_max(float v) {  // NaN counts as nothing
 RTR_DEVICE bool beam_near(float base) { return fabsf(base) < 1e37f; }
 RTR_DEVICE float beam_unit(float base) { return __fmul_rn(base, BP_LOG2E); }
 
+// A piece of 16 bytes at a row's ragged ends, of which some logits are not there.  Out of line: the code that a
+// kernel goes through once comes from L2 at some 500 cycles a line.
+template <typename T> __device__ __noinline__ uint4 beam_ragged(const T* row, int e, int vocab) {
+  constexpr int PER = 16 / sizeof(T);
+  uint32_t v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    v[i] = sizeof(T) == 4 ? 0xff800000u : 0xff80u;
+    if (e + i >= 0 && e + i < vocab) {
+      if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(row[e + i]);
+      else v[i] = __bfloat16_as_ushort(row[e + i]);
+    }
+  }
+  if constexpr (sizeof(T) == 4) return make_uint4(v[0], v[1], v[2], v[3]);
+  else return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+}
+
 // A warp's part of a group (512 logits in bf16, 256 in fp32), two pieces of 16 bytes each lane.  Groups start at multiples
 // of 16 bytes: the first of a row that does not holds fewer.
 template <typename T> struct Logits {
@@ -86,19 +103,8 @@ template <typename T> struct Logits {
       const int e = at(first, j * PER, lane);
       if (e >= 0 && e + PER <= vocab) {
         u[j] = __ldg(reinterpret_cast<const uint4*>(row + e));
-      } else {  // a row's ragged ends
-        const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xff80u;
-        uint32_t v[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          v[i] = w;
-          if (e + i >= 0 && e + i < vocab) {
-            if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(row[e + i]);
-            else v[i] = __bfloat16_as_ushort(row[e + i]);
-          }
-        }
-        if constexpr (sizeof(T) == 4) u[j] = make_uint4(v[0], v[1], v[2], v[3]);
-        else u[j] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+      } else {
+        u[j] = beam_ragged(row, e, vocab);
       }
     }
   }
@@ -287,16 +293,22 @@ struct PickShared {
   float2 near[BP_MAX_N];                // the row's maximum, and off rounded (minus infinity: nothing to offer)
   float need[BP_MAX_N];                 // what its logits have to reach
   uint8_t again[BP_MAX_N], done[BP_MAX_N];  // rows to sum in 64 bits, and those that are
-  int32_t groups[BP_GROUPS];
+  int32_t quartet_at[BP_GROUPS], groups[BP_GROUPS];
   PickEntry list[BP_LIST];
   float x[BP_LIST];
-  uint16_t order[BP_LIST];
+  union {
+    int bins[BP_THREADS];               // of the search for the k-th best
+    uint16_t order[BP_LIST];            // and then the candidates' places in the list
+  };
   double red[BP_THREADS / 32];
-  uint4 lane_raw[BP_LANES][2];          // what lanes read whose largest logit reaches its row's need
-  int32_t lane_first[BP_LANES];         // the place of its first logit's lane in the group, and the row
+  union {
+    float4 quartet[BP_GROUPS];          // quartets of groups one of which reaches the row's need
+    uint4 lane_raw[BP_LANES][2];        // and then what lanes read whose largest logit does
+  };
+  int32_t lane_first[BP_LANES];         // first place of its group, the row, the lane
   uint8_t lane_row[BP_LANES], lane_at[BP_LANES];
-  int n_groups, n_lanes, n_list;
-  int bins[BP_THREADS], word2[BP_THREADS / 32];
+  int n_quartets, n_groups, n_lanes, n_list;
+  int word2[BP_THREADS / 32];
   uint32_t word[BP_THREADS / 32], reached;
   int most;  // the largest |off32|, as bits
 };
@@ -337,6 +349,12 @@ RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
   __syncthreads();
   return s.reached ? key_float(s.reached) : -INFINITY;
 }
+
+// What the usual path does not come by, out of line.
+template <typename T, bool MASK> __device__ __noinline__ void pick_exactly(const BeamPick& a, PickShared& s);
+template <typename T, bool MASK> __device__ __noinline__ void pick_needs(const BeamPick& a, PickShared& s, int ng);
+template <typename T, bool MASK> __device__ __noinline__ void pick_again(const BeamPick& a, PickShared& s);
+__device__ __noinline__ void pick_fill(const BeamPick& a, PickShared& s);
 
 template <typename T, bool MASK> struct Picker {
   using L = Logits<T>;
@@ -428,6 +446,10 @@ template <typename T, bool MASK> struct Picker {
     s.list[to].at = (uint32_t)r * a.vocab + v;
   }
 
+  // A sum relative to its maximum as one relative to a larger one.
+  RTR_DEVICE static float relative(const float2& part, float top) {
+    return part.x == top ? part.y : part.y * ex2((part.x - top) * BP_LOG2E);
+  }
   // Each row's sum from its slices, and what its candidates are offset by: eight lanes a row.
   RTR_DEVICE void offsets() {
     static_assert(BP_MAX_N * 8 == BP_THREADS, "a row for every eight threads");
@@ -435,22 +457,19 @@ template <typename T, bool MASK> struct Picker {
     const bool there = r < a.n;
     const float score = there && part == 0 ? a.scores[item * a.n + r] : -INFINITY;
     const float2* p = a.part + ((int64_t)item * a.n + (there ? r : 0)) * a.slices;
-    float m = -INFINITY;
-    double t = 0.0;
-    for (int i0 = part; there && i0 < a.slices; i0 += 32) {
-      float2 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = i0 + 8 * i < a.slices ? __ldcg(p + i0 + 8 * i) : make_float2(-INFINITY, 0.f);
-      const float top = fmaxf(m, fmaxf(fmaxf(v[0].x, v[1].x), fmaxf(v[2].x, v[3].x)));
-      if (m != top) t *= ex2((m - top) * BP_LOG2E);
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2 u = there && part < a.slices ? __ldcg(p + part) : none, v = there && part + 8 < a.slices ? __ldcg(p + part + 8) : none;
+    float m = fmaxf(u.x, v.x), sum = relative(u, m) + relative(v, m);
+    for (int i = part + 16; there && i < a.slices; i += 8) {
+      const float2 w = __ldcg(p + i);
+      const float top = fmaxf(m, w.x);
+      sum = relative(make_float2(m, sum), top) + relative(w, top);
       m = top;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t += v[i].x == m ? v[i].y : v[i].y * ex2((v[i].x - m) * BP_LOG2E);
     }
     float all = m;
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
-    if (m != all) t *= ex2((m - all) * BP_LOG2E);
+    double t = relative(make_float2(m, sum), all);
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
     if (tid == 0) s.most = 0;
@@ -518,10 +537,18 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
   }
 
+  // Too few threads have groups for a bound: their lanes' best may give one.
+  RTR_DEVICE void needs_by_lanes(int ng) {
+    float mine = -INFINITY;
+    each_logit(ng, [&](int r, int, float x) { mine = fmaxf(mine, near(r, x)); });
+    const float t = reached_by(mine, a.k, s);
+    needs(t - slack(t));
+  }
+
   // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too
   // many (ties).
   RTR_DEVICE bool gather() {
-    if (tid == 0) s.n_groups = s.n_lanes = s.n_list = 0;
+    if (tid == 0) s.n_quartets = s.n_groups = s.n_lanes = s.n_list = 0;
     float mine = -INFINITY, of[BP_HELD];  // of: the held quartets' best
     const int quartets = a.padded >> 2, all = a.n * quartets;
 #pragma unroll
@@ -534,37 +561,37 @@ template <typename T, bool MASK> struct Picker {
     each_later_group([&](int r, int, const float4& v) {
       mine = fmaxf(mine, near(r, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))));
     });
-    float t = reached_by(mine, a.k, s);
-    const float floor_ = t - slack(t);
+    const float t = reached_by(mine, a.k, s), floor_ = t - slack(t);
     needs(floor_);
-    const auto look = [&](int r, int g0, const float4& v) {
-      const float x = s.need[r], w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (w[i] >= x && w[i] > -INFINITY) {
-          const int to = atomicAdd(&s.n_groups, 1);
-          if (to < BP_GROUPS) s.groups[to] = r * a.padded + g0 + i;
-        }
+    const auto put = [&](int q, const float4& v) {
+      const int to = atomicAdd(&s.n_quartets, 1);
+      if (to >= BP_GROUPS) return;
+      s.quartet[to] = v;
+      s.quartet_at[to] = q;
     };
     if (mine > -INFINITY && mine >= floor_) {
 #pragma unroll
       for (int j = 0; j < BP_HELD; ++j)
-        if (of[j] > -INFINITY && of[j] >= floor_) {
-          const int q = tid + j * BP_THREADS, r = a.n == 1 ? 0 : row_of((uint32_t)q);
-          look(r, 4 * (q - r * quartets), held[j]);
-        }
-      each_later_group(look);
+        if (of[j] > -INFINITY && of[j] >= floor_) put(tid + j * BP_THREADS, held[j]);
+      each_later_group([&](int r, int g0, const float4& v) {
+        if (near(r, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))) >= floor_) put((r * a.padded + g0) >> 2, v);
+      });
+    }
+    __syncthreads();
+    const int nq = s.n_quartets;
+    if (nq > BP_GROUPS) return false;
+    for (int i = tid; i < 4 * nq; i += BP_THREADS) {
+      const int q = s.quartet_at[i >> 2], r = a.n == 1 ? 0 : row_of((uint32_t)q);
+      const float v = (&s.quartet[i >> 2].x)[i & 3];
+      if (v >= s.need[r] && v > -INFINITY) {
+        const int to = atomicAdd(&s.n_groups, 1);
+        if (to < BP_GROUPS) s.groups[to] = 4 * q + (i & 3);
+      }
     }
     __syncthreads();
     const int ng = s.n_groups;
     if (ng > BP_GROUPS) return false;
-    if (!(t > -INFINITY) && ng > 2) {
-      // too few threads have groups for a bound: their lanes' best may give one
-      mine = -INFINITY;
-      each_logit(ng, [&](int r, int, float x) { mine = fmaxf(mine, near(r, x)); });
-      t = reached_by(mine, a.k, s);
-      needs(t - slack(t));
-    }
+    if (!(t > -INFINITY) && ng > 2) pick_needs<T, MASK>(a, s, ng);
     // Hardly ever more than one lane of a group has any: its logits are put aside, for all threads to look at one each.
     each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>&, int) {
       if (!(raw.largest() >= s.need[r])) return;
@@ -699,14 +726,17 @@ template <typename T, bool MASK> struct Picker {
       s.again[rp] = s.again[rq] = 1;
       doubt = true;
     }
-    if (!__syncthreads_or(doubt)) return false;
+    return __syncthreads_or(doubt);
+  }
+  RTR_DEVICE void settle() {
     bool equal = false;
     if (tid < a.n && s.off[tid] > -INFINITY)
       for (int q = 0; q < a.n; ++q) equal |= s.again[q] && s.sum[q] == s.sum[tid];
     __syncthreads();
     if (equal) s.again[tid] = 1;
     __syncthreads();
-    return true;
+    sum_again();
+    put_in_order();
   }
 };
 
@@ -716,9 +746,31 @@ template <typename T, bool MASK> RTR_DEVICE Picker<T, MASK> picker(const BeamPic
   return Picker<T, MASK>{a, s, (int)blockIdx.x, tid, tid >> 5, tid & 31, static_cast<const T*>(a.logits) + row0 * a.stride,
                          MASK ? a.allowed + row0 * a.allowed_stride : nullptr, a.best + row0 * a.padded, {}};
 }
-// Apart, so that what it needs costs the usual path no registers.
-template <typename T, bool MASK> __device__ __noinline__ void gather_exactly(const BeamPick& a, PickShared& s) {
+template <typename T, bool MASK> __device__ __noinline__ void pick_exactly(const BeamPick& a, PickShared& s) {
   picker<T, MASK>(a, s).gather_exactly();
+}
+template <typename T, bool MASK> __device__ __noinline__ void pick_needs(const BeamPick& a, PickShared& s, int ng) {
+  picker<T, MASK>(a, s).needs_by_lanes(ng);
+}
+template <typename T, bool MASK> __device__ __noinline__ void pick_again(const BeamPick& a, PickShared& s) {
+  picker<T, MASK>(a, s).settle();
+}
+// Fewer finite candidates than k: the first places that have none.
+__device__ __noinline__ void pick_fill(const BeamPick& a, PickShared& s) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = s.n_list;
+  const int64_t all = (int64_t)a.n * a.vocab;
+  bool free_ = tid < 2 * a.k && tid < all;
+  for (int j = 0; j < n && free_; ++j) free_ = s.list[j].at != (uint32_t)tid;
+  const unsigned mask = __ballot_sync(0xffffffffu, free_);
+  if (lane == 0) s.red[warp] = __popc(mask);
+  __syncthreads();
+  int before = __popc(mask & ((1u << lane) - 1));
+  for (int w = 0; w < warp; ++w) before += (int)s.red[w];
+  if (free_ && n + before < a.k) {
+    s.list[n + before] = PickEntry{double_key(-INFINITY), (uint32_t)tid, (uint32_t)(tid / a.vocab)};
+    s.order[n + before] = (uint16_t)(n + before);
+  }
+  __syncthreads();
 }
 
 template <typename T, bool MASK>
@@ -730,29 +782,10 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
   Picker<T, MASK> p = picker<T, MASK>(a, s);
   p.hold();
   p.offsets();
-  if (!p.gather()) gather_exactly<T, MASK>(a, s);
+  if (!p.gather()) pick_exactly<T, MASK>(a, s);
   p.put_in_order();
-  if (p.doubtful()) {
-    p.sum_again();
-    p.put_in_order();
-  }
-  // fewer finite candidates than k: the first places that have none
-  const int n = min(s.n_list, a.k);
-  if (n < a.k) {
-    const int64_t all = (int64_t)a.n * a.vocab;
-    bool free_ = tid < 2 * a.k && tid < all;
-    for (int j = 0; j < n && free_; ++j) free_ = s.list[j].at != (uint32_t)tid;
-    const unsigned mask = __ballot_sync(0xffffffffu, free_);
-    if (lane == 0) s.red[warp] = __popc(mask);
-    __syncthreads();
-    int before = __popc(mask & ((1u << lane) - 1));
-    for (int w = 0; w < warp; ++w) before += (int)s.red[w];
-    if (free_ && n + before < a.k) {
-      s.list[n + before] = PickEntry{double_key(-INFINITY), (uint32_t)tid, (uint32_t)(tid / a.vocab)};
-      s.order[n + before] = (uint16_t)(n + before);
-    }
-    __syncthreads();
-  }
+  if (p.doubtful()) pick_again<T, MASK>(a, s);
+  if (s.n_list < a.k) pick_fill(a, s);
   if (tid < a.k) {
     const PickEntry c = s.list[s.order[tid]];
     const int64_t to = (int64_t)item * a.k + tid;
