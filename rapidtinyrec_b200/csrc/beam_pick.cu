@@ -28,13 +28,13 @@
 
 namespace rtr {
 
-constexpr int BP_BYTES = 1024;                  // of a group: two pieces of 16 of each lane of a warp
+constexpr int BP_BYTES = 2048;                  // of a group: four pieces of 16 of each lane of a warp
 constexpr int BP_WARPS = 8, BP_BLOCKS = 4;      // first kernel: warps of a block, blocks of an SM
 constexpr int BP_RING = 6144;                   // bytes of logits that a warp of it has on their way
 constexpr int BP_THREADS = 1024;                // second kernel: threads of a block
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
-constexpr int BP_GROUPS = 512, BP_LANES = 384, BP_LIST = 1024;  // groups, lanes' parts of them and candidates that it takes up at once
-constexpr int BP_HELD = 8;                      // quartets of groups that a thread of it holds
+constexpr int BP_GROUPS = 512, BP_LANES = 1024, BP_LIST = 1024;  // groups, lanes of them and candidates that it takes up at once
+constexpr int BP_HELD = 4;                      // quartets of groups that a thread of it holds
 constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
@@ -48,6 +48,7 @@ struct BeamPick {
   uint32_t quarter_inv;    // ceil(2^32 / (padded / 4)): a group quartet's row by one multiplication (0: 2^32, the quartet itself)
   int slices;              // blocks of a row
   float* best;             // [items * n][padded]: a group's largest allowed logit
+  uint32_t* second;        // likewise: the largest of the other lanes' (rounded up) and, in the last five bits, whose the first is
   float2* part;            // [items * n][slices]: maximum, sum of exponentials relative to it
   int32_t *all_tokens, *all_parents, *next_tokens, *next_parents;
   float *all_scores, *next_scores;
@@ -81,10 +82,10 @@ template <typename T> __device__ __noinline__ uint4 beam_ragged(const T* row, in
   else return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
 }
 
-// A warp's part of a group (512 logits in bf16, 256 in fp32), two pieces of 16 bytes each lane.  Groups start at multiples
+// A warp's part of a group (1,024 logits in bf16, 512 in fp32), four pieces of 16 bytes each lane.  Groups start at multiples
 // of 16 bytes: the first of a row that does not holds fewer.
 template <typename T> struct Logits {
-  static constexpr int PER = 16 / sizeof(T), PIECES = 2, EACH = PIECES * PER, GROUP = 32 * EACH;
+  static constexpr int PER = 16 / sizeof(T), PIECES = 4, EACH = PIECES * PER, GROUP = 32 * EACH;
   uint4 u[PIECES];
   RTR_DEVICE static int shift(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
   RTR_DEVICE static int at(int first, int i, int lane) { return first + (i / PER) * 32 * PER + lane * PER + i % PER; }
@@ -120,15 +121,21 @@ template <typename T> struct Logits {
   RTR_DEVICE float one(int i) const { return i & 1 ? two(i >> 1).y : two(i >> 1).x; }
   RTR_DEVICE float largest() const {
     if constexpr (sizeof(T) == 4) {
-      return fmaxf(fmaxf(fmaxf(one(0), one(1)), fmaxf(one(2), one(3))), fmaxf(fmaxf(one(4), one(5)), fmaxf(one(6), one(7))));
+      float m[PIECES];
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) m[j] = fmaxf(fmaxf(one(4 * j), one(4 * j + 1)), fmaxf(one(4 * j + 2), one(4 * j + 3)));
+      return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     } else {  // two at a time; NaN counts as nothing
       const auto pair = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
       const auto four = [&](const uint4& x) { return __hmax2(__hmax2(pair(x.x), pair(x.y)), __hmax2(pair(x.z), pair(x.w))); };
-      const __nv_bfloat162 m = __hmax2(four(u[0]), four(u[1]));
+      const __nv_bfloat162 m = __hmax2(__hmax2(four(u[0]), four(u[1])), __hmax2(four(u[2]), four(u[3])));
       return fmaxf(__low2float(m), __high2float(m));
     }
   }
 };
+// The word of BeamPick::second, and the value that its largest is at most.
+RTR_DEVICE uint32_t beam_second(float value, int lane) { return (__float_as_uint(value) & ~31u) | (uint32_t)lane; }
+RTR_DEVICE float beam_second_value(uint32_t w) { return __uint_as_float(w >> 31 ? w & ~31u : w | 31u); }
 
 // The bytes that say which of a lane's logits are allowed: runs of four, by aligned words that hold at least one
 // of them, since a row of bytes may start anywhere (at the same place of a word in all of a row's groups).
@@ -188,15 +195,21 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   const float2 log2e = make_float2(BP_LOG2E, BP_LOG2E);
   const auto take = [&](const L& raw, const Allowed<T>& ok, int g) {
-    const float top = redux_max(raw.largest());
-    float mine = top;
+    float mine = raw.largest();
+    const float top = redux_max(mine);
+    float most = top;
     if constexpr (MASK) {
       mine = -INFINITY;
 #pragma unroll
       for (int i = 0; i < L::EACH; ++i) mine = fmaxf(mine, ok(i, by) ? raw.one(i) : -INFINITY);
-      mine = redux_max(mine);
+      most = redux_max(mine);
     }
-    if (lane == 0) best[g] = mine;
+    const int whose = __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1;
+    const float other = redux_max(lane == whose ? -INFINITY : mine);
+    if (lane == 0) {
+      best[g] = most;
+      a.second[(int64_t)row * a.padded + g] = beam_second(other, whose & 31);
+    }
     if (top > base) {  // the same in all lanes
       const float f = ex2(beam_near(base) && beam_near(top) ? beam_unit(base) - beam_unit(top) : (base - top) * BP_LOG2E);
 #pragma unroll
@@ -295,19 +308,17 @@ struct PickShared {
   uint8_t again[BP_MAX_N], done[BP_MAX_N];  // rows to sum in 64 bits, and those that are
   int32_t quartet_at[BP_GROUPS], groups[BP_GROUPS];
   PickEntry list[BP_LIST];
-  float x[BP_LIST];
+  uint16_t order[BP_LIST];              // and their places in the list
   union {
     int bins[BP_THREADS];               // of the search for the k-th best
-    uint16_t order[BP_LIST];            // and then the candidates' places in the list
+    float x[BP_LIST];                   // and then the candidates' logits
   };
   double red[BP_THREADS / 32];
   union {
     float4 quartet[BP_GROUPS];          // quartets of groups one of which reaches the row's need
-    uint4 lane_raw[BP_LANES][2];        // and then what lanes read whose largest logit does
+    int2 lane[BP_LANES];                // and then the lanes whose largest logit does: 32 row + lane, first place of the group
   };
-  int32_t lane_first[BP_LANES];         // first place of its group, the row, the lane
-  uint8_t lane_row[BP_LANES], lane_at[BP_LANES];
-  int n_quartets, n_groups, n_lanes, n_list;
+  int n_quartets, n_groups, n_whole, n_lanes, n_list;
   int word2[BP_THREADS / 32];
   uint32_t word[BP_THREADS / 32], reached;
   int most;  // the largest |off32|, as bits
@@ -353,12 +364,12 @@ RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
 // What the usual path does not come by, out of line.
 template <typename T, bool MASK> __device__ __noinline__ void pick_exactly(const BeamPick& a, PickShared& s);
 template <typename T, bool MASK> __device__ __noinline__ void pick_needs(const BeamPick& a, PickShared& s, int ng);
+template <typename T, bool MASK> __device__ __noinline__ void pick_whole(const BeamPick& a, PickShared& s);
 template <typename T, bool MASK> __device__ __noinline__ void pick_again(const BeamPick& a, PickShared& s);
 __device__ __noinline__ void pick_fill(const BeamPick& a, PickShared& s);
 
 template <typename T, bool MASK> struct Picker {
   using L = Logits<T>;
-  static constexpr int TAKE = MASK ? 2 : 4;  // groups that a warp reads again at a time
   const BeamPick& a;
   PickShared& s;
   const int item, tid, warp, lane;
@@ -404,36 +415,23 @@ template <typename T, bool MASK> struct Picker {
 
   // f(row, first place, logits, mask) for the warp's groups of the list
   template <typename F> RTR_DEVICE void each_read(int ng, F&& f) const {
-    for (int j0 = warp; j0 < ng; j0 += TAKE * (BP_THREADS / 32)) {
-      Logits<T> raw[TAKE];
-      Allowed<T> ok[MASK ? TAKE : 1];
-      int rows[TAKE], first[TAKE];
-#pragma unroll
-      for (int t = 0; t < TAKE; ++t) {
-        const int j = j0 + t * (BP_THREADS / 32);
-        if (j >= ng) break;
-        const int id = s.groups[j], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
-        rows[t] = r;
-        first[t] = (id - r * a.padded) * L::GROUP - L::shift(row(r));
-        raw[t].load(row(r), first[t], lane, a.vocab);
-        if constexpr (MASK) ok[t].load(mask(r), first[t], lane, a.vocab, Allowed<T>::by(mask(r), Logits<T>::shift(row(r))));
-      }
-#pragma unroll
-      for (int t = 0; t < TAKE; ++t) {
-        if (j0 + t * (BP_THREADS / 32) >= ng) break;
-        int by = 0;
-        if constexpr (MASK) by = Allowed<T>::by(mask(rows[t]), Logits<T>::shift(row(rows[t])));
-        f(rows[t], first[t], raw[t], ok[MASK ? t : 0], by);
-      }
+    for (int j = warp; j < ng; j += BP_THREADS / 32) {
+      const int id = s.groups[j], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2), shift = L::shift(row(r));
+      const int first = (id - r * a.padded) * L::GROUP - shift, by = MASK ? Allowed<T>::by(mask(r), shift) : 0;
+      L raw;
+      Allowed<T> ok;
+      raw.load(row(r), first, lane, a.vocab);
+      if constexpr (MASK) ok.load(mask(r), first, lane, a.vocab, by);
+      f(r, first, raw, ok, by);
     }
   }
   // f(row, place in the vocabulary, logit) for the lane's finite, allowed logits of these groups
   template <typename F> RTR_DEVICE void each_logit(int ng, F&& f) const {
-    each_read(ng, [&](int r, int first, const Logits<T>& raw, const Allowed<T>& ok, int by) {
+    each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>& ok, int by) {
 #pragma unroll
       for (int i = 0; i < L::EACH; ++i) {
         const float v = raw.one(i);
-        if (v > -INFINITY && (!MASK || ok(i, by))) f(r, Logits<T>::at(first, i, lane), v);
+        if (v > -INFINITY && (!MASK || ok(i, by))) f(r, L::at(first, i, lane), v);
       }
     });
   }
@@ -548,7 +546,7 @@ template <typename T, bool MASK> struct Picker {
   // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too
   // many (ties).
   RTR_DEVICE bool gather() {
-    if (tid == 0) s.n_quartets = s.n_groups = s.n_lanes = s.n_list = 0;
+    if (tid == 0) s.n_quartets = s.n_groups = s.n_whole = s.n_lanes = s.n_list = 0;
     float mine = -INFINITY, of[BP_HELD];  // of: the held quartets' best
     const int quartets = a.padded >> 2, all = a.n * quartets;
 #pragma unroll
@@ -591,28 +589,56 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
     const int ng = s.n_groups;
     if (ng > BP_GROUPS) return false;
-    if (!(t > -INFINITY) && ng > 2) pick_needs<T, MASK>(a, s, ng);
-    // Hardly ever more than one lane of a group has any: its logits are put aside, for all threads to look at one each.
-    each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>&, int) {
-      if (!(raw.largest() >= s.need[r])) return;
-      const int to = atomicAdd(&s.n_lanes, 1);
-      if (to >= BP_LANES) return;
-      s.lane_raw[to][0] = raw.u[0];
-      s.lane_raw[to][1] = raw.u[1];
-      s.lane_first[to] = first;
-      s.lane_row[to] = (uint8_t)r;
-      s.lane_at[to] = (uint8_t)lane;
-    });
+    if (!(t > -INFINITY) && ng > 1) pick_needs<T, MASK>(a, s, ng);
+    // Hardly ever more than one lane of a group has any, and the first kernel has said which.  Of other groups all lanes are
+    // looked at, or, where there are many, those whose largest logit says so.
+    int whole = -1, r = 0, first = 0;
+    if (tid < ng) {
+      const int id = s.groups[tid];
+      r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
+      first = (id - r * a.padded) * L::GROUP - L::shift(row(r));
+      const uint32_t w = __ldcg(a.second + ((int64_t)item * a.n * a.padded + id));
+      if (beam_second_value(w) < s.need[r]) add_lane(r, first, (int)(w & 31));
+      else whole = id;
+    }
+    const int wholes = __syncthreads_count(whole >= 0);
+    if (ng + 31 * wholes <= BP_LANES) {
+      if (whole >= 0) {
+        const int to = atomicAdd(&s.n_lanes, 32);
+        for (int l = 0; l < 32; ++l) s.lane[to + l] = make_int2(32 * r + l, first);
+      }
+    } else {
+      if (whole >= 0) s.groups[atomicAdd(&s.n_whole, 1)] = whole;
+      __syncthreads();
+      pick_whole<T, MASK>(a, s);
+    }
     __syncthreads();
     const int nl = s.n_lanes;
     if (nl > BP_LANES) return false;
-    for (int i = tid; i < nl * L::EACH; i += BP_THREADS) {
-      const int l = i / L::EACH, j = i % L::EACH, r = s.lane_row[l], e = L::at(s.lane_first[l], j, s.lane_at[l]);
-      const float v = to_f32(reinterpret_cast<const T*>(s.lane_raw[l])[j]);
-      if (v >= s.need[r] && v > -INFINITY && (!MASK || mask(r)[e])) add(r, e, v);
+    for (int i = tid; i < nl * L::PIECES; i += BP_THREADS) {
+      const int2 l = s.lane[i / L::PIECES];
+      r = l.x >> 5;
+      const int e = L::at(l.y, i % L::PIECES * L::PER, l.x & 31);
+      const uint4 u = e >= 0 && e + L::PER <= a.vocab ? __ldg(reinterpret_cast<const uint4*>(row(r) + e)) : beam_ragged(row(r), e, a.vocab);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      const float x = s.need[r];
+#pragma unroll
+      for (int j = 0; j < L::PER; ++j) {
+        const float v = __uint_as_float(sizeof(T) == 4 ? w[j % 4] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+        if (v >= x && v > -INFINITY && (!MASK || mask(r)[e + j])) add(r, e + j, v);
+      }
     }
     __syncthreads();
     return s.n_list <= BP_LIST;
+  }
+  RTR_DEVICE void add_lane(int r, int first, int lane_) {
+    const int to = atomicAdd(&s.n_lanes, 1);
+    if (to < BP_LANES) s.lane[to] = make_int2(32 * r + lane_, first);
+  }
+  RTR_DEVICE void take_whole() {
+    each_read(s.n_whole, [&](int r, int first, const L& raw, const Allowed<T>&, int) {
+      if (raw.largest() >= s.need[r]) add_lane(r, first, lane);
+    });
   }
 
   RTR_DEVICE int block_count(int mine) {
@@ -689,7 +715,8 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
   }
 
-  // Candidates by value, then place: each one's rank is the number of those before it, counted by eight threads.
+  // Candidates by value, then place: each one's rank is the number of those before it, counted by eight threads.  (110 candidates
+  // 2,500 cycles; a bitonic sort by shuffles 7,500.)
   RTR_DEVICE void put_in_order() {
     const int n = s.n_list;
     for (int i = tid; i < n; i += BP_THREADS) s.list[i].key = double_key(worth(s.list[i].row, s.x[i]));
@@ -699,7 +726,6 @@ template <typename T, bool MASK> struct Picker {
       int before = 0;
       if (i < n) {
         const PickEntry me = s.list[i];
-#pragma unroll 4
         for (int j = tid & 7; j < n; j += 8) {
           const PickEntry it = s.list[j];
           before += (it.key > me.key) | ((it.key == me.key) & (it.at < me.at));
@@ -752,6 +778,9 @@ template <typename T, bool MASK> __device__ __noinline__ void pick_exactly(const
 template <typename T, bool MASK> __device__ __noinline__ void pick_needs(const BeamPick& a, PickShared& s, int ng) {
   picker<T, MASK>(a, s).needs_by_lanes(ng);
 }
+template <typename T, bool MASK> __device__ __noinline__ void pick_whole(const BeamPick& a, PickShared& s) {
+  picker<T, MASK>(a, s).take_whole();
+}
 template <typename T, bool MASK> __device__ __noinline__ void pick_again(const BeamPick& a, PickShared& s) {
   picker<T, MASK>(a, s).settle();
 }
@@ -797,7 +826,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
     int taken = 0;
     for (int j0 = 0; j0 < a.k && taken < a.beams; j0 += 32) {
       const int j = j0 + lane;
-      const PickEntry c = s.list[j < a.k ? s.order[j] : 0];
+      const PickEntry c = s.list[s.order[min(j, a.k - 1)]];
       const int token = (int32_t)(c.at - c.row * a.vocab);
       const bool on = j < a.k && token != a.eos;
       const unsigned mask = __ballot_sync(0xffffffffu, on);
@@ -833,7 +862,7 @@ static const char* beam_check(const rtr_beam_step* b) {
 }
 
 // Groups of a row (one more where it starts in the middle of one), slices, and the workspace they need.
-static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& best_bytes, int64_t& bytes) {
+static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& groups_bytes, int64_t& bytes) {
   const int per = b->dtype == RTR_DTYPE_F32 ? 4 : 8;
   const int group = BP_BYTES * per / 16;
   p.groups = (int)(((int64_t)b->vocab + per - 1 + group - 1) / group);
@@ -845,9 +874,8 @@ static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& bes
   const int64_t want = rows <= room ? room / std::max<int64_t>(rows, 1) : (8 * room + rows - 1) / rows;
   const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(want, (p.groups + BP_WARPS - 1) / BP_WARPS));
   p.slices = (int)slices;
-  best_bytes = rows * p.padded * (int64_t)sizeof(float);
-  best_bytes = (best_bytes + 15) & ~(int64_t)15;
-  bytes = best_bytes + rows * p.slices * (int64_t)sizeof(float2);
+  groups_bytes = rows * p.padded * (int64_t)sizeof(float);  // a multiple of 16
+  bytes = 2 * groups_bytes + rows * p.slices * (int64_t)sizeof(float2);
 }
 
 }  // namespace rtr
@@ -892,7 +920,8 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.beams = step->beams;
   p.eos = step->eos < 0 ? -1 : step->eos;
   p.best = static_cast<float*>(workspace);
-  p.part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + best);
+  p.second = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + best);
+  p.part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 2 * best);
   p.all_tokens = step->all_tokens;
   p.all_parents = step->all_parents;
   p.all_scores = step->all_scores;
