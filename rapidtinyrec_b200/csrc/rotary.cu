@@ -12,6 +12,8 @@
 // over four heads that is 1.9 of the 5.5 instructions a byte that the SMs issue while HBM delivers it.
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "engine.h"
 #include "kv_host.h"
 
@@ -38,14 +40,15 @@ struct Rotary {
   bool wide;
 };
 
-// N values of a thread's piece: 16 bytes, or one value where rows do not lie at multiples of 16.
+// N values of a thread's piece, as they lie in memory: 16 bytes, or one value where rows do not lie at multiples of 16.
 template <typename T, int N> struct Piece {
-  float x[N];
-  RTR_DEVICE void load(const T* p) {
+  using Raw = typename std::conditional<N == 1, T, uint4>::type;
+  Raw u;
+  RTR_DEVICE void load(const T* p) { u = *reinterpret_cast<const Raw*>(p); }
+  RTR_DEVICE void get(float (&x)[N]) const {
     if constexpr (N == 1) {
-      x[0] = to_f32(*p);
+      x[0] = to_f32(u);
     } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -58,9 +61,9 @@ template <typename T, int N> struct Piece {
       }
     }
   }
-  RTR_DEVICE void store(T* p) const {
+  RTR_DEVICE void set(const float (&x)[N]) {
     if constexpr (N == 1) {
-      *p = from_f32<T>(x[0]);
+      u = from_f32<T>(x[0]);
     } else {
       uint32_t w[4];
 #pragma unroll
@@ -72,10 +75,17 @@ template <typename T, int N> struct Piece {
           w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
       }
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      u = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+  RTR_DEVICE void store(T* p) const { *reinterpret_cast<Raw*>(p) = u; }
 };
+
+RTR_DEVICE void turn(float& a, float& b, float cosine, float sine) {
+  const float u = a;
+  a = fmaf(u, cosine, -b * sine);
+  b = fmaf(b, cosine, u * sine);
+}
 
 template <typename T, int N, bool INTERLEAVED>
 __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const Rotary a) {
@@ -128,23 +138,21 @@ __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(const Rotary a) {
       const int h = h0 + j * a.split;
       if (h >= a.heads) continue;
       if (turns) {
+        float u[N], v[N];
+        x[j].get(u);
+        y[j].get(v);
         if constexpr (INTERLEAVED && N > 1) {
 #pragma unroll
           for (int i = 0; i < N / 2; ++i) {
-            const float u = x[j].x[2 * i], v = x[j].x[2 * i + 1], s = y[j].x[2 * i], w = y[j].x[2 * i + 1];
-            x[j].x[2 * i] = fmaf(u, cosine[i], -v * sine[i]);
-            x[j].x[2 * i + 1] = fmaf(v, cosine[i], u * sine[i]);
-            y[j].x[2 * i] = fmaf(s, cosine[N / 2 + i], -w * sine[N / 2 + i]);
-            y[j].x[2 * i + 1] = fmaf(w, cosine[N / 2 + i], s * sine[N / 2 + i]);
+            turn(u[2 * i], u[2 * i + 1], cosine[i], sine[i]);
+            turn(v[2 * i], v[2 * i + 1], cosine[N / 2 + i], sine[N / 2 + i]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float u = x[j].x[i], v = y[j].x[i];
-            x[j].x[i] = fmaf(u, cosine[i], -v * sine[i]);
-            y[j].x[i] = fmaf(v, cosine[i], u * sine[i]);
-          }
+          for (int i = 0; i < N; ++i) turn(u[i], v[i], cosine[i], sine[i]);
         }
+        x[j].set(u);
+        y[j].set(v);
       }
       const RotaryRows& r = h < a.q_heads ? a.q : a.k;
       T* p = static_cast<T*>(r.out) + row * r.out_row + (int64_t)(h < a.q_heads ? h : h - a.q_heads) * r.out_head;
