@@ -38,6 +38,24 @@ bool here(const at::Tensor& t, int index) { return t.is_cuda() && t.get_device()
 at::Tensor room_for(int index, at::IntArrayRef size, at::ScalarType type) {
   return at::Tensor(at::detail::empty_cuda(size, type, at::Device(at::kCUDA, (c10::DeviceIndex)index), std::nullopt));
 }
+// Several new tensors in one piece of memory, 16 bytes apart at least: a call to the allocator costs a microsecond, a tensor of
+// memory that is there a quarter of one.
+struct Room {
+  at::Tensor all;
+  int64_t used = 0;
+  Room(int index, int64_t bytes) : all(room_for(index, {bytes}, at::kByte)) {}
+  static int64_t of(int64_t values, int64_t size) { return (values * size + 15) & ~(int64_t)15; }
+  at::Tensor take(at::IntArrayRef size, at::ScalarType type) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                            c10::scalarTypeToTypeMeta(type));
+    c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+    impl->set_sizes_contiguous(size);
+    const int64_t each = c10::elementSize(type);
+    impl->set_storage_offset(used / each);
+    used += of(impl->numel(), each);
+    return t;
+  }
+};
 PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
   PyObject* t = PyTuple_New((Py_ssize_t)tensors.size());
   if (!t) throw Raised{};
@@ -97,8 +115,9 @@ PyObject* call_grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (a[5] != Py_None) rows = whole(a[5], "rows");
     if (rows < 0 || rows > INT32_MAX) refuse("rows must not be negative and must fit 32 bits");
-    at::Tensor lens = room_for(pool.index, {s.seqs}, at::kInt), starts = room_for(pool.index, {s.seqs + 1}, at::kInt),
-               positions = room_for(pool.index, {rows}, at::kInt), slots = room_for(pool.index, {rows}, at::kLong);
+    Room out(pool.index, Room::of(s.seqs, 4) + Room::of(s.seqs + 1, 4) + Room::of(rows, 4) + Room::of(rows, 8));
+    const at::Tensor lens = out.take({s.seqs}, at::kInt), starts = out.take({s.seqs + 1}, at::kInt),
+                     positions = out.take({rows}, at::kInt), slots = out.take({rows}, at::kLong);
     check(pages_grow(pool.c, static_cast<int32_t*>(s.table.data_ptr()), s.stride, (int32_t)s.width,
                      static_cast<const int32_t*>(s.held.data_ptr()), fresh, (int32_t)each, (int32_t)s.seqs, (int32_t)rows,
                      static_cast<int32_t*>(lens.data_ptr()), static_cast<int32_t*>(starts.data_ptr()),
@@ -270,9 +289,11 @@ PyObject* call_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
       s.allowed = static_cast<const uint8_t*>(allowed.data_ptr());
       s.allowed_stride = allowed.dim() == 1 || allowed.size(0) == 1 ? 0 : allowed.stride(0);
     }
-    at::Tensor all_tokens = room_for(index, {items, k}, at::kInt), all_parents = room_for(index, {items, k}, at::kInt),
-               all_scores = room_for(index, {items, k}, at::kFloat), tokens = room_for(index, {items, beams}, at::kInt),
-               parents = room_for(index, {items, beams}, at::kInt), next = room_for(index, {items, beams}, at::kFloat);
+    if (items > INT32_MAX / 256) refuse("too many items for one call");
+    Room out(index, 3 * (Room::of(items * k, 4) + Room::of(items * beams, 4)));
+    const at::Tensor all_tokens = out.take({items, k}, at::kInt), all_parents = out.take({items, k}, at::kInt),
+                     all_scores = out.take({items, k}, at::kFloat), tokens = out.take({items, beams}, at::kInt),
+                     parents = out.take({items, beams}, at::kInt), next = out.take({items, beams}, at::kFloat);
     s.logits = logits.data_ptr();
     s.scores = static_cast<const float*>(scores.data_ptr());
     s.logits_stride = rows > 1 ? logits.stride(0) : vocab;

@@ -27,8 +27,9 @@
 
 namespace rtr {
 
-constexpr int PG_THREADS = 256, PG_MAX_SEQS = 16384, PG_ROWS = 4;  // rows a thread: one 16-byte store of positions
-constexpr int PG_BACK_THREADS = 512, PG_BACK_CLUSTER = 8;
+constexpr int PG_FEW = 256, PG_MANY = 1024;  // threads of a block, up to so many sequences and beyond
+constexpr int PG_MAX_SEQS = 16384, PG_BACK_CLUSTER = 8;
+constexpr int PG_HELD = 8;                   // pages given back that a thread remembers
 
 struct PagePool {
   int32_t* free;
@@ -46,67 +47,67 @@ struct PageSeqs {
   const int32_t* held;
 };
 
-RTR_DEVICE int pages_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
+RTR_DEVICE int pages_of(int tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }  // lengths leave room for a page
 
 // The running sums of two numbers a sequence, by all threads of the block: a[0 .. seqs], b[0 .. seqs]
 // (b null: one number).  value(s, x, y) gives sequence s's two numbers and false where it does not fit; the
-// result is false where any sequence does not fit or a sum is above its limit.  Each thread takes consecutive sequences.
+// result is false where any sequence does not fit or a sum is above its limit (what a and b hold then means nothing).
+// A round takes as many sequences as the block has threads.
 template <typename F>
-RTR_DEVICE bool page_sums(int seqs, int32_t* a, int32_t* b, int64_t* red, int64_t limit_a, int64_t limit_b, F&& value) {
-  const int tid = threadIdx.x, warps = blockDim.x >> 5, lane = tid & 31, warp = tid >> 5;
-  const int per = (seqs + blockDim.x - 1) / blockDim.x, lo = min(seqs, tid * per), hi = min(seqs, lo + per);
-  int64_t x = 0, y = 0;
-  int fits = 1;
-  for (int s = lo; s < hi; ++s) {
-    int p = 0, q = 0;
-    if (!value(s, p, q)) fits = p = q = 0;
-    a[s + 1] = p;
-    if (b) b[s + 1] = q;
-    x += p;
-    y += q;
-  }
-  int64_t xs = x, ys = y;  // inclusive over the warp
+RTR_DEVICE bool page_sums(int seqs, int32_t* a, int32_t* b, int64_t limit_a, int64_t limit_b, F&& value) {
+  __shared__ longlong2 red[PG_MANY / 32 + 1];  // warps' sums, then what lies before each warp; behind them all that was seen
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  int fits = 1, p = 0, q = 0;
+  const auto load = [&](int s) {
+    p = q = 0;
+    if (s < seqs && !value(s, p, q)) fits = p = q = 0;
+  };
+  load(tid);
+  for (int s0 = 0; s0 < seqs; s0 += blockDim.x) {
+    const int s = s0 + tid;
+    // a warp's sums in 64 bits, by halves of the numbers; the running ones in 32, which are right where the call fits
+    const auto whole = [](int n) {
+      return ((int64_t)__reduce_add_sync(0xffffffffu, (unsigned)n >> 16) << 16) + __reduce_add_sync(0xffffffffu, (unsigned)n & 0xffffu);
+    };
+    const int64_t all_x = whole(p), all_y = b ? whole(q) : 0;
+    uint32_t x = p, y = q;
+    load(s + blockDim.x);
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, xs, d), v = __shfl_up_sync(0xffffffffu, ys, d);
-    if (lane >= d) {
-      xs += u;
-      ys += v;
-    }
-  }
-  if (lane == 31) {
-    red[2 * warp] = xs;
-    red[2 * warp + 1] = ys;
-  }
-  fits = __syncthreads_and(fits);
-  int64_t all_x = 0, all_y = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w == warp) {
-      xs += all_x;
-      ys += all_y;
-    }
-    all_x += red[2 * w];
-    all_y += red[2 * w + 1];
-  }
-  const bool good = fits && all_x <= limit_a && all_y <= limit_b;
-  if (good) {  // the sums fit 32 bits: limits do
-    xs -= x;
-    ys -= y;
-    if (tid == 0) {
-      a[0] = 0;
-      if (b) b[0] = 0;
-    }
-    for (int s = lo; s < hi; ++s) {
-      xs += a[s + 1];
-      a[s + 1] = (int32_t)xs;
-      if (b) {
-        ys += b[s + 1];
-        b[s + 1] = (int32_t)ys;
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, x, d), v = b ? __shfl_up_sync(0xffffffffu, y, d) : 0u;
+      if (lane >= d) {
+        x += u;
+        y += v;
       }
     }
+    if (lane == 31) red[warp] = make_longlong2(all_x, all_y);
+    __syncthreads();
+    if (warp == 0) {
+      longlong2 m = lane < warps ? red[lane] : make_longlong2(0, 0), sum = m;
+      const longlong2 seen = s0 ? red[PG_MANY / 32] : make_longlong2(0, 0);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, sum.x, d), v = __shfl_up_sync(0xffffffffu, sum.y, d);
+        if (lane >= d) {
+          sum.x += u;
+          sum.y += v;
+        }
+      }
+      __syncwarp();
+      if (lane < warps) red[lane] = make_longlong2(seen.x + sum.x - m.x, seen.y + sum.y - m.y);
+      if (lane == 31) red[PG_MANY / 32] = make_longlong2(seen.x + sum.x, seen.y + sum.y);
+    }
+    __syncthreads();
+    if (s < seqs) {
+      a[s + 1] = (int32_t)(x + (uint32_t)red[warp].x);
+      if (b) b[s + 1] = (int32_t)(y + (uint32_t)red[warp].y);
+    }
   }
-  __syncthreads();
-  return good;
+  if (tid == 0) {
+    a[0] = 0;
+    if (b) b[0] = 0;
+  }
+  return __syncthreads_and(fits && (!seqs || (red[PG_MANY / 32].x <= limit_a && red[PG_MANY / 32].y <= limit_b)));
 }
 
 // The sequence s with sums[s] <= item < sums[s + 1].
@@ -120,11 +121,12 @@ RTR_DEVICE int page_seq(const int32_t* sums, int seqs, int item) {
   return lo;
 }
 
-__global__ void __launch_bounds__(PG_THREADS) pages_grow_kernel(const PagePool p, const PageSeqs q, const int32_t* fresh,
+// ROWS: rows a thread; with four, positions are one 16-byte store.
+template <int ROWS>
+__global__ void __launch_bounds__(PG_MANY) pages_grow_kernel(const PagePool p, const PageSeqs q, const int32_t* fresh,
                                                                 int each, int rows, int32_t* lens, int32_t* starts_out,
                                                                 int32_t* positions, int64_t* slots) {
   extern __shared__ int32_t pg_sums[];
-  __shared__ int64_t red[2 * PG_THREADS / 32];
   int32_t *starts = pg_sums, *items = pg_sums + q.seqs + 1;
   pdl_launch_dependents();
   pdl_wait();
@@ -138,10 +140,10 @@ __global__ void __launch_bounds__(PG_THREADS) pages_grow_kernel(const PagePool p
     need = pages_of(h + n, shift) - pages_of(h, shift);
     return true;
   };
-  const bool fits = page_sums(q.seqs, starts, items, red, rows, INT32_MAX, value);
+  const bool fits = page_sums(q.seqs, starts, items, rows, INT32_MAX, value);
   const int all = fits ? items[q.seqs] : 0;
   const bool enough = counted && all <= count;
-  const int64_t at = (int64_t)blockIdx.x * PG_THREADS + tid, step = (int64_t)gridDim.x * PG_THREADS;
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + tid, step = (int64_t)gridDim.x * blockDim.x;
   if (!fits || !enough) {
     if (at == 0) atomicOr(p.status, fits ? RTR_DEV_FEW_PAGES : RTR_DEV_BAD_LENGTH);
     for (int64_t s = at; s <= q.seqs; s += step) {
@@ -166,74 +168,72 @@ __global__ void __launch_bounds__(PG_THREADS) pages_grow_kernel(const PagePool p
     else atomicOr(p.status, RTR_DEV_BAD_PAGE);
   }
   const int end = starts[q.seqs];
-  for (int64_t r0 = at * PG_ROWS; r0 < rows; r0 += step * PG_ROWS) {
-    int32_t pos[PG_ROWS];
-    int64_t slot[PG_ROWS];
-    int s = r0 < end ? page_seq(starts, q.seqs, (int)r0) : 0, had = -1, of = -1, nth = -1, page = -1;
+  for (int64_t r0 = at * ROWS; r0 < rows; r0 += step * ROWS) {
+    // the rows' sequences, then all their loads at a time
+    int32_t pos[ROWS], page[ROWS];
+    int64_t slot[ROWS];
+    int s = r0 < end ? page_seq(starts, q.seqs, (int)r0) : 0;
+    const int32_t* from[ROWS];
 #pragma unroll
-    for (int j = 0; j < PG_ROWS; ++j) {
-      const int r = (int)min(r0 + j, (int64_t)INT32_MAX);
+    for (int j = 0; j < ROWS; ++j) {
+      from[j] = nullptr;
       pos[j] = -1;
-      slot[j] = -1;
-      if (r >= end) continue;
+      if (r0 + j >= end) continue;
+      const int r = (int)r0 + j;
       while (starts[s + 1] <= r) ++s;
-      if (s != of) {
-        had = q.held[s];
-        of = s;
-        nth = -1;
-      }
-      const int t = had + r - starts[s];
-      if (t >> shift != nth) {
-        nth = t >> shift;
-        const int old = pages_of(had, shift);
-        page = nth < old ? q.table[s * q.stride + nth] : top[-(int64_t)(items[s] + nth - old)];
-        if (page < 0 || page >= p.pages) {
-          atomicOr(p.status, RTR_DEV_BAD_PAGE);
-          page = -1;
-        }
-      }
-      if (page >= 0) {
-        pos[j] = t;
-        slot[j] = ((int64_t)page << shift) + (t & ((1 << shift) - 1));
+      const int had = q.held[s], t = had + r - starts[s], nth = t >> shift, old = pages_of(had, shift);
+      pos[j] = t;
+      from[j] = nth < old ? q.table + s * q.stride + nth : top - (int64_t)(items[s] + nth - old);
+    }
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) page[j] = from[j] ? *from[j] : -1;
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      slot[j] = -1;
+      if (page[j] >= 0 && page[j] < p.pages) {
+        slot[j] = ((int64_t)page[j] << shift) + (pos[j] & ((1 << shift) - 1));
+      } else {
+        if (from[j]) atomicOr(p.status, RTR_DEV_BAD_PAGE);
+        pos[j] = -1;
       }
     }
-    if (r0 + PG_ROWS <= rows) {
-      *reinterpret_cast<int4*>(positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-      *reinterpret_cast<longlong2*>(slots + r0) = make_longlong2(slot[0], slot[1]);
-      *reinterpret_cast<longlong2*>(slots + r0 + 2) = make_longlong2(slot[2], slot[3]);
+    if (ROWS == 4 && r0 + ROWS <= rows) {
+      *reinterpret_cast<int4*>(positions + r0) = make_int4(pos[0], pos[1 % ROWS], pos[2 % ROWS], pos[3 % ROWS]);
+      *reinterpret_cast<longlong2*>(slots + r0) = make_longlong2(slot[0], slot[1 % ROWS]);
+      *reinterpret_cast<longlong2*>(slots + r0 + 2) = make_longlong2(slot[2 % ROWS], slot[3 % ROWS]);
     } else {
 #pragma unroll
-      for (int j = 0; j < PG_ROWS; ++j)
+      for (int j = 0; j < ROWS; ++j)
         if (r0 + j < rows) {
           positions[r0 + j] = pos[j];
           slots[r0 + j] = slot[j];
         }
     }
   }
-  // The stack's height changes when every block has read it (and what lies below it).
+  // The stack's height changes when every block has read it.  (Nothing else of one block is read by another: no fence.)
   __syncthreads();
   if (tid == 0) {
-    __threadfence();
-    if (atomicAdd(p.ticket, 1u) == gridDim.x - 1) {
+    if (gridDim.x == 1) {
+      *p.count = count - all;
+    } else if (atomicAdd(p.ticket, 1u) == gridDim.x - 1) {
       *p.ticket = 0;
       *p.count = count - all;
     }
   }
 }
 
-__global__ void __launch_bounds__(PG_BACK_THREADS) pages_release_kernel(const PagePool p, const PageSeqs q,
+__global__ void __launch_bounds__(PG_MANY) pages_release_kernel(const PagePool p, const PageSeqs q,
                                                                         const int32_t* keep) {
   extern __shared__ int32_t pg_sums[];
-  __shared__ int64_t red[2 * PG_BACK_THREADS / 32];
   __shared__ uint32_t wrong;
   pdl_launch_dependents();
   pdl_wait();
   const auto cluster = cooperative_groups::this_cluster();
   const int tid = threadIdx.x, shift = p.shift, count = *p.count;
-  const int at = (int)cluster.block_rank() * PG_BACK_THREADS + tid, step = (int)cluster.num_blocks() * PG_BACK_THREADS;
+  const int at = (int)cluster.block_rank() * blockDim.x + tid, step = (int)cluster.num_blocks() * blockDim.x;
   const int64_t room = (int64_t)q.width << shift;
   if (tid == 0) wrong = 0;
-  const bool fits = page_sums(q.seqs, pg_sums, nullptr, red, INT32_MAX, INT32_MAX, [&](int s, int& n, int&) {
+  const bool fits = page_sums(q.seqs, pg_sums, nullptr, INT32_MAX, INT32_MAX, [&](int s, int& n, int&) {
     const int h = q.held[s], k = keep ? keep[s] : 0;
     if (k < 0 || k > h || h > room) return false;
     n = pages_of(h, shift) - pages_of(k, shift);
@@ -249,26 +249,39 @@ __global__ void __launch_bounds__(PG_BACK_THREADS) pages_release_kernel(const Pa
     return q.table[s * q.stride + pages_of(k, shift) + (i - pg_sums[s])];
   };
   uint32_t bad = count < 0 || count > p.pages || all > p.pages - count ? RTR_DEV_PAGE_NOT_HELD : 0u;
-  if (!bad) {
-    for (int64_t i = at; i < all; i += step) {
-      const int page = page_at((int)i);
-      if (page < 0 || page >= p.pages) bad |= RTR_DEV_BAD_PAGE;
-      else if (atomicCAS(p.marks + page, 1, 2) != 1) bad |= RTR_DEV_PAGE_NOT_HELD;
-    }
+  int held[PG_HELD];  // the thread's first pages
+  const auto mark = [&](int page) {
+    if (page < 0 || page >= p.pages) bad |= RTR_DEV_BAD_PAGE;
+    else if (atomicCAS(p.marks + page, 1, 2) != 1) bad |= RTR_DEV_PAGE_NOT_HELD;
+  };
+  const bool look = !bad;
+#pragma unroll
+  for (int j = 0; j < PG_HELD; ++j) {
+    const int64_t i = at + (int64_t)j * step;
+    if (i < all) held[j] = page_at((int)i);
+  }
+  if (look) {
+#pragma unroll
+    for (int j = 0; j < PG_HELD; ++j)
+      if (at + (int64_t)j * step < all) mark(held[j]);
+    for (int64_t i = at + (int64_t)PG_HELD * step; i < all; i += step) mark(page_at((int)i));
   }
   if (bad) atomicOr(&wrong, bad);
   cluster.sync();
   bad = 0;
   for (unsigned r = 0; r < cluster.num_blocks(); ++r) bad |= *cluster.map_shared_rank(&wrong, r);
-  for (int64_t i = at; i < all; i += step) {
-    const int page = page_at((int)i);
+  const auto settle = [&](int64_t i, int page) {
     if (!bad) {
       p.marks[page] = 0;
       p.free[(int64_t)count + all - 1 - i] = page;
     } else if (page >= 0 && page < p.pages && p.marks[page] == 2) {
       p.marks[page] = 1;
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < PG_HELD; ++j)
+    if (at + (int64_t)j * step < all) settle(at + (int64_t)j * step, held[j]);
+  for (int64_t i = at + (int64_t)PG_HELD * step; i < all; i += step) settle(i, page_at((int)i));
   if (at == 0) {
     if (bad) atomicOr(p.status, bad);
     else *p.count = count + all;
@@ -310,18 +323,22 @@ int rtr_pages_grow(const rtr_page_pool* pool, int32_t* table, int64_t table_stri
     return set_error(RTR_ERR_ARG, "positions and slots must lie at multiples of 16 bytes");
   KvDevice on(device);
   if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
-  // A block for every 1,024 rows, every 256 sequences, and no more than fill the GPU four times: a
-  // block's own scan of the lengths is then a small part of what it does.
-  const int64_t want = std::max<int64_t>((rows + PG_THREADS * PG_ROWS - 1) / (PG_THREADS * PG_ROWS), (seqs + PG_THREADS) / PG_THREADS);
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 4 * (int64_t)on.sms);
-  const int smem = 2 * (seqs + 1) * (int)sizeof(int32_t);
-  static std::atomic<uint64_t> allowed;
-  cudaError_t e = smem > 32 << 10 ? kv_allow_smem(pages_grow_kernel, 2 * (PG_MAX_SEQS + 1) * (int)sizeof(int32_t), allowed, device)
-                                  : cudaSuccess;
-  if (e == cudaSuccess)
-    e = kv_launch(pages_grow_kernel, dim3(grid), PG_THREADS, smem, 1, static_cast<cudaStream_t>(stream), device_pool(pool),
+  // A block for as many rows (four a thread where one each would be more blocks than fill the GPU) and sequences as it has threads, and
+  // no more than fill the GPU four times: a block's own scan of the lengths is then a small part of what it does.
+  const int threads = seqs <= PG_FEW ? PG_FEW : PG_MANY, room = on.sms * (2048 / threads);
+  const bool four = rows > (int64_t)room * threads / 4;
+  const int64_t each_block = (int64_t)threads * (four ? 4 : 1);
+  const int64_t want = std::max<int64_t>((rows + each_block - 1) / each_block, (seqs + threads) / threads);
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 4 * (int64_t)room);
+  const int smem = 2 * (seqs + 1) * (int)sizeof(int32_t), most = 2 * (PG_MAX_SEQS + 1) * (int)sizeof(int32_t);
+  static std::atomic<uint64_t> allowed[2];
+  const auto run = [&](auto kernel) {
+    const cudaError_t e = smem > 32 << 10 ? kv_allow_smem(kernel, most, allowed[four], device) : cudaSuccess;
+    return e != cudaSuccess ? e : kv_launch(kernel, dim3(grid), threads, smem, 1, static_cast<cudaStream_t>(stream), device_pool(pool),
                   PageSeqs{table, table_stride, table_width, seqs, held}, fresh, (int)each, (int)rows, lens, starts, positions,
                   slots);
+  };
+  const cudaError_t e = four ? run(pages_grow_kernel<4>) : run(pages_grow_kernel<1>);
   return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -331,14 +348,15 @@ int rtr_pages_release(const rtr_page_pool* pool, const int32_t* table, int64_t t
   if (!seqs) return RTR_OK;
   KvDevice on(device);
   if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
-  // One block while every page that the tables can name is a round of its threads or two.
-  const int cluster = (int64_t)seqs * table_width <= 2 * PG_BACK_THREADS ? 1 : PG_BACK_CLUSTER;
+  // One block while it remembers every page that the tables can name.
+  const int threads = (int64_t)seqs * table_width <= PG_FEW * PG_HELD ? PG_FEW : PG_MANY;
+  const int cluster = (int64_t)seqs * table_width <= PG_HELD * (int64_t)threads ? 1 : PG_BACK_CLUSTER;
   const int smem = (seqs + 1) * (int)sizeof(int32_t);
   static std::atomic<uint64_t> allowed;
   cudaError_t e = smem > 32 << 10 ? kv_allow_smem(pages_release_kernel, (PG_MAX_SEQS + 1) * (int)sizeof(int32_t), allowed, device)
                                   : cudaSuccess;
   if (e == cudaSuccess)
-    e = kv_launch(pages_release_kernel, dim3(1, 1, cluster), PG_BACK_THREADS, smem, cluster, static_cast<cudaStream_t>(stream),
+    e = kv_launch(pages_release_kernel, dim3(1, 1, cluster), threads, smem, cluster, static_cast<cudaStream_t>(stream),
                   device_pool(pool), PageSeqs{const_cast<int32_t*>(table), table_stride, table_width, seqs, held}, keep);
   return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
 }
