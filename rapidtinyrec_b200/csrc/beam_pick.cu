@@ -29,7 +29,8 @@
 namespace rtr {
 
 constexpr int BP_BYTES = 2048;                  // of a group: four pieces of 16 of each lane of a warp
-constexpr int BP_WARPS = 8, BP_BLOCKS = 4;      // first kernel: warps of a block, blocks of an SM
+constexpr int BP_WARPS = 8;                     // first kernel: warps of a block
+constexpr int beam_blocks(bool mask) { return mask ? 3 : 4; }  // blocks of an SM
 constexpr int BP_RING = 6144;                   // bytes of logits that a warp of it has on their way
 constexpr int BP_THREADS = 1024;                // second kernel: threads of a block
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
@@ -143,6 +144,24 @@ template <typename T> struct Allowed {
   static constexpr int RUNS = Logits<T>::EACH / 4;
   uint32_t w[RUNS][2];
   RTR_DEVICE static int by(const uint8_t* row, int shift) { return 8 * (int)((reinterpret_cast<uintptr_t>(row) - shift) & 3); }
+  RTR_DEVICE void load_inside(const uint8_t* row, int first, int lane, int by) {  // a group that is all there
+    if (Logits<T>::PER == 8 && (reinterpret_cast<uintptr_t>(row + first) & 7) == 0) {
+#pragma unroll
+      for (int j = 0; j < RUNS; j += 2) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(row + Logits<T>::at(first, 4 * j, lane)));
+        w[j][0] = u.x;
+        w[(j + 1) % RUNS][0] = u.y;
+      }
+      return;
+    }
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row + Logits<T>::at(first, 0, lane)) & ~(uintptr_t)3;
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j) {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p + (Logits<T>::at(0, 4 * j, lane) - Logits<T>::at(0, 0, lane)));
+      w[j][0] = __ldg(q);
+      if (by) w[j][1] = __ldg(q + 1);
+    }
+  }
   RTR_DEVICE void load(const uint8_t* row, int first, int lane, int vocab, int by) {
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
@@ -166,13 +185,25 @@ template <typename T> struct Allowed {
   RTR_DEVICE bool operator()(int i, int by) const {
     return __funnelshift_r(w[i >> 2][0], w[i >> 2][1], by) >> (8 * (i & 3)) & 0xffu;
   }
+  // The largest allowed one of the lane's logits: the others become NaN, which counts as nothing.
+  RTR_DEVICE float largest(const Logits<T>& raw, int by) const {
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j) {
+      const uint32_t none = __vcmpeq4(__funnelshift_r(w[j][0], w[j][1], by), 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        m = fmaxf(m, __uint_as_float(__float_as_uint(raw.one(4 * j + i)) | __byte_perm(none, 0u, 0x1111 * i)));
+    }
+    return m;
+  }
 };
 
 // One block: a slice of a row's groups, which its warps take in turn.  The groups that are all there come through a ring in shared
 // memory of each warp's own, every lane's pieces copied by the lane that reads them: 6 KB a warp keep 192 KB an SM on their way without
 // a register (two groups in registers of their own, the one read while the other comes, 24 warps: 110 us instead of NN for 32 x 50 rows of bf16).
 template <typename T, bool MASK>
-__global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(const BeamPick a) {
+__global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_kernel(const BeamPick a) {
   using L = Logits<T>;
   constexpr int BYTES = BP_BYTES, STAGES = BP_RING / BYTES, GROUP = L::GROUP;
   __shared__ __align__(16) uint8_t ring[BP_WARPS][BP_RING];
@@ -199,9 +230,7 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
     const float top = redux_max(mine);
     float most = top;
     if constexpr (MASK) {
-      mine = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < L::EACH; ++i) mine = fmaxf(mine, ok(i, by) ? raw.one(i) : -INFINITY);
+      mine = ok.largest(raw, by);
       most = redux_max(mine);
     }
     const int whose = __ffs(__ballot_sync(0xffffffffu, mine == most)) - 1;
@@ -256,8 +285,14 @@ __global__ void __launch_bounds__(BP_WARPS * 32, BP_BLOCKS) beam_scan_kernel(con
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) issue(i, i);
+  Allowed<T> next;  // masks come a group ahead, in registers
+  if constexpr (MASK)
+    if (n > 0) next.load_inside(allowed, g * GROUP - shift, lane, by);
   for (int i = 0, stage = 0; i < n; ++i) {
-    if constexpr (MASK) ok.load(allowed, (g + i * BP_WARPS) * GROUP - shift, lane, a.vocab, by);
+    if constexpr (MASK) {
+      ok = next;
+      if (i + 1 < n) next.load_inside(allowed, (g + (i + 1) * BP_WARPS) * GROUP - shift, lane, by);
+    }
     cp_async_wait<STAGES - 2>();
     __syncwarp();
 #pragma unroll
@@ -620,12 +655,17 @@ template <typename T, bool MASK> struct Picker {
       r = l.x >> 5;
       const int e = L::at(l.y, i % L::PIECES * L::PER, l.x & 31);
       const uint4 u = e >= 0 && e + L::PER <= a.vocab ? __ldg(reinterpret_cast<const uint4*>(row(r) + e)) : beam_ragged(row(r), e, a.vocab);
+      bool ok[L::PER];
+      if constexpr (MASK) {
+#pragma unroll
+        for (int j = 0; j < L::PER; ++j) ok[j] = e + j >= 0 && e + j < a.vocab && mask(r)[e + j];
+      }
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
       const float x = s.need[r];
 #pragma unroll
       for (int j = 0; j < L::PER; ++j) {
         const float v = __uint_as_float(sizeof(T) == 4 ? w[j % 4] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-        if (v >= x && v > -INFINITY && (!MASK || mask(r)[e + j])) add(r, e + j, v);
+        if (v >= x && v > -INFINITY && (!MASK || ok[j])) add(r, e + j, v);
       }
     }
     __syncthreads();
@@ -868,10 +908,11 @@ static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& gro
   p.groups = (int)(((int64_t)b->vocab + per - 1 + group - 1) / group);
   p.padded = (p.groups + 3) & ~3;
   p.quarter_inv = (uint32_t)((0x100000000ull + p.padded / 4 - 1) / (p.padded / 4));
-  // Slices of a row: as many blocks as the SMs hold at once while the rows are few (a warp takes a group at least), eight times as many
-  // blocks as that where they are many, so that the last ones to finish cost little.
-  const int64_t rows = (int64_t)b->items * b->n, room = BP_BLOCKS * (int64_t)sms;
-  const int64_t want = rows <= room ? room / std::max<int64_t>(rows, 1) : (8 * room + rows - 1) / rows;
+  // Slices of a row: enough for as many blocks as the SMs hold at once where the rows are few (a warp takes a group at least), and eight
+  // times as many blocks as that where they are many.  200 rows of 152,832 in bf16: 2, 3, 4 slices 24.9, 21.5, 22.4 us; 50 of 152,704 in
+  // fp32: 8, 11, 16 slices 14.9, 14.3, 15.0; 1,600 rows: 1 to 4 slices the same.
+  const int64_t rows = (int64_t)b->items * b->n, room = beam_blocks(b->allowed != nullptr) * (int64_t)sms;
+  const int64_t want = ((rows <= room ? room : 8 * room) + rows - 1) / std::max<int64_t>(rows, 1);
   const int64_t slices = std::max<int64_t>(1, std::min<int64_t>(want, (p.groups + BP_WARPS - 1) / BP_WARPS));
   p.slices = (int)slices;
   groups_bytes = rows * p.padded * (int64_t)sizeof(float);  // a multiple of 16
