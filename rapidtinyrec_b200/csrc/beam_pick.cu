@@ -419,15 +419,26 @@ template <typename T, bool MASK> struct Picker {
   RTR_DEVICE float near(int r, float x) const { return (x - s.near[r].x) + s.near[r].y; }
   RTR_DEVICE bool alive(int r) const { return s.near[r].y > -INFINITY; }
 
-  // The thread's quartets of groups: the first ones are held in registers, from the start of the kernel.
+  // The thread's quartets of groups: the first ones are held in registers, from the start of the kernel.  Where there is not one for
+  // every thread, groups are dealt one by one, as quartets whose others are minus infinity: the fewer a thread has, the nearer
+  // to the k-th best candidate is the k-th best thread's.
   float4 held[BP_HELD];
+  RTR_DEVICE bool single() const { return a.n * a.padded <= BP_HELD * BP_THREADS; }
+  RTR_DEVICE int held_at(int j) const { return single() ? (tid + j * BP_THREADS) >> 2 : tid + j * BP_THREADS; }
+  RTR_DEVICE bool holds(int j) const { return held_at(j) < a.n * (a.padded >> 2); }
   RTR_DEVICE void hold() {
-    const int all = a.n * (a.padded >> 2);
+    if (single()) {
 #pragma unroll
-    for (int j = 0; j < BP_HELD; ++j) {
-      const int q = tid + j * BP_THREADS;
-      if (q < all) held[j] = __ldcg(reinterpret_cast<const float4*>(best) + q);
+      for (int j = 0; j < BP_HELD; ++j) {
+        const float v = holds(j) ? __ldcg(best + tid + j * BP_THREADS) : -INFINITY;
+        held[j] = make_float4(tid & 3 ? -INFINITY : v, (tid & 3) == 1 ? v : -INFINITY, (tid & 3) == 2 ? v : -INFINITY,
+                              (tid & 3) == 3 ? v : -INFINITY);
+      }
+      return;
     }
+#pragma unroll
+    for (int j = 0; j < BP_HELD; ++j)
+      if (holds(j)) held[j] = __ldcg(reinterpret_cast<const float4*>(best) + held_at(j));
   }
   // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer: those that are not held,
   // and all
@@ -439,11 +450,11 @@ template <typename T, bool MASK> struct Picker {
     }
   }
   template <typename F> RTR_DEVICE void each_group(F&& f) const {
-    const int quartets = a.padded >> 2, all = a.n * quartets;
+    const int quartets = a.padded >> 2;
 #pragma unroll
     for (int j = 0; j < BP_HELD; ++j) {
-      const int q = tid + j * BP_THREADS, r = q >= all || a.n == 1 ? 0 : row_of((uint32_t)q);
-      if (q < all && alive(r)) f(r, 4 * (q - r * quartets), held[j]);
+      const int q = held_at(j), r = !holds(j) || a.n == 1 ? 0 : row_of((uint32_t)q);
+      if (holds(j) && alive(r)) f(r, 4 * (q - r * quartets), held[j]);
     }
     each_later_group(f);
   }
@@ -583,12 +594,11 @@ template <typename T, bool MASK> struct Picker {
   RTR_DEVICE bool gather() {
     if (tid == 0) s.n_quartets = s.n_groups = s.n_whole = s.n_lanes = s.n_list = 0;
     float mine = -INFINITY, of[BP_HELD];  // of: the held quartets' best
-    const int quartets = a.padded >> 2, all = a.n * quartets;
 #pragma unroll
     for (int j = 0; j < BP_HELD; ++j) {
-      const int q = tid + j * BP_THREADS, r = q >= all || a.n == 1 ? 0 : row_of((uint32_t)q);
+      const int r = !holds(j) || a.n == 1 ? 0 : row_of((uint32_t)held_at(j));
       const float x = fmaxf(fmaxf(held[j].x, held[j].y), fmaxf(held[j].z, held[j].w));
-      of[j] = q < all && alive(r) ? near(r, x) : -INFINITY;
+      of[j] = holds(j) && alive(r) ? near(r, x) : -INFINITY;
       mine = fmaxf(mine, of[j]);
     }
     each_later_group([&](int r, int, const float4& v) {
@@ -605,7 +615,7 @@ template <typename T, bool MASK> struct Picker {
     if (mine > -INFINITY && mine >= floor_) {
 #pragma unroll
       for (int j = 0; j < BP_HELD; ++j)
-        if (of[j] > -INFINITY && of[j] >= floor_) put(tid + j * BP_THREADS, held[j]);
+        if (of[j] > -INFINITY && of[j] >= floor_) put(held_at(j), held[j]);
       each_later_group([&](int r, int g0, const float4& v) {
         if (near(r, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w))) >= floor_) put((r * a.padded + g0) >> 2, v);
       });
