@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from rapidtinyrec_b200 import _native
+from rapidtinyrec_b200.beam_search import BeamSearch
 from rapidtinyrec_b200.page_pool import PagePool
 from rapidtinyrec_b200.rotary import Rotary, frequencies
 
@@ -133,3 +134,69 @@ def test_frequencies_that_are_refused(kw):
 def test_rotary_handles_that_are_refused(kw):
     with pytest.raises(ValueError):
         Rotary(**kw)
+
+
+# ---------------------------------------------------------------- beam search
+def step(**change):
+    args = dict(logits=A, scores=A, allowed=None, logits_stride=1000, allowed_stride=0, dtype=0, items=2, n=4, vocab=1000, k=8, beams=4,
+                eos=-1, all_tokens=A, all_parents=A, next_tokens=A, next_parents=A, all_scores=A, next_scores=A, status=A)
+    args.update(change)
+    return _native.BeamStepC(**args)
+
+
+@pytest.mark.parametrize('change,says', [
+    (dict(dtype=2), 'dtype'), (dict(items=-1), '1 to 128'), (dict(n=0), '1 to 128'), (dict(n=129), '1 to 128'), (dict(vocab=0), 'vocabulary'),
+    (dict(vocab=(1 << 20) + 1), 'vocabulary'), (dict(k=0), '1 to 256'), (dict(k=257), '1 to 256'), (dict(n=1, vocab=7, k=8), 'there are'),
+    (dict(beams=0), 'next beams'), (dict(beams=9), 'next beams'), (dict(eos=3, k=7), 'eos'), (dict(eos=3, beams=5), 'eos'),
+    (dict(logits_stride=999), 'logits overlap'), (dict(allowed=A, allowed_stride=999), 'allowed overlap'), (dict(logits=A + 2), 'multiples'),
+    (dict(dtype=1, logits=A + 1), 'multiples')] + [(dict([(name, None)]), 'null buffer') for name in (
+        'logits', 'scores', 'all_tokens', 'all_parents', 'all_scores', 'next_tokens', 'next_parents', 'next_scores', 'status')])
+def test_steps_that_are_refused(change, says):
+    lib, room = _native.load(), ctypes.c_int64()
+    s = step(**change)
+    assert lib.rtr_beam_select_workspace(ctypes.byref(s), 0, ctypes.byref(room)) == _native.RTR_ERR_ARG
+    assert says in message()
+    assert lib.rtr_beam_select(ctypes.byref(s), A, 1 << 30, 0, None) == _native.RTR_ERR_ARG
+    assert says in message()
+
+
+def test_steps_without_items_are_no_work():
+    s = step(items=0, logits=None, scores=None)
+    assert _native.load().rtr_beam_select(ctypes.byref(s), None, 0, 0, None) == _native.RTR_OK
+
+
+def state(**change):
+    args = dict(data=A, row_bytes=4096, inner=256, strides=(ctypes.c_int64 * 3)(0, 0, 256), sizes=(ctypes.c_int32 * 3)(1, 1, 2))
+    args.update(change)
+    return _native.BeamStateC(**args)
+
+
+def reorder(states, parents=A, items=2, beams=4, status=A):
+    many = (_native.BeamStateC * max(1, len(states)))(*states)
+    return _native.load().rtr_beam_reorder(many, len(states), parents, items, beams, status, 0, None)
+
+
+@pytest.mark.parametrize('change,says', [
+    (dict(data=None), 'null state'), (dict(inner=0), 'positive'), (dict(sizes=(ctypes.c_int32 * 3)(1, 0, 2)), 'positive'),
+    (dict(row_bytes=0), 'rows of a state'), (dict(strides=(ctypes.c_int64 * 3)(0, 0, 0)), 'dimensions overlap')])
+def test_states_that_are_refused(change, says):
+    assert reorder([state(), state(**change)]) == _native.RTR_ERR_ARG
+    assert says in message()
+
+
+@pytest.mark.parametrize('kw,says', [(dict(beams=0), '128 beams'), (dict(beams=129), '128 beams'), (dict(items=-1), 'items'),
+                                     (dict(items=65536), '65535'), (dict(parents=None), 'null'), (dict(status=None), 'null')])
+def test_reorderings_that_are_refused(kw, says):
+    assert reorder([state()], **kw) == _native.RTR_ERR_ARG
+    assert says in message()
+
+
+def test_nothing_to_reorder():
+    assert reorder([]) == _native.RTR_OK and reorder([state()], items=0) == _native.RTR_OK
+
+
+@pytest.mark.parametrize('kw', [dict(beams=0), dict(beams=129), dict(beams=4, candidates=3), dict(beams=4, candidates=257), dict(beams=4, eos=-1),
+                                dict(beams=4, device='cpu')])
+def test_searches_that_are_refused(kw):
+    with pytest.raises(ValueError):
+        BeamSearch(**kw)
