@@ -332,6 +332,25 @@ RTR_DEVICE double key_double(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
+// e^d for d from -100 to 0: e^(n log 2 + f) with n the nearest whole number, f at most 0.347 and e^f its Taylor series up to f^10 / 10!
+// (off by 2.2e-13 at most).  Sixteen fp64 operations with the subtraction and the sum; exp() made two rows of 152,704 take 95 us.
+RTR_DEVICE double exp_of(double d) {
+  const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to whole numbers, in the low bits
+  const double z = fma(d, 1.4426950408889634, whole), n = z - whole, f = fma(n, -0.69314718055994531, d);
+  double e = 1.0 / 3628800.0;
+  e = fma(e, f, 1.0 / 362880.0);
+  e = fma(e, f, 1.0 / 40320.0);
+  e = fma(e, f, 1.0 / 5040.0);
+  e = fma(e, f, 1.0 / 720.0);
+  e = fma(e, f, 1.0 / 120.0);
+  e = fma(e, f, 1.0 / 24.0);
+  e = fma(e, f, 1.0 / 6.0);
+  e = fma(e, f, 0.5);
+  e = fma(e, f, 1.0);
+  e = fma(e, f, 1.0);
+  return __hiloint2double(__double2hiint(e) + (__double2loint(z) << 20), __double2loint(e));
+}
+
 struct PickEntry {  // a candidate in order: larger keys first, then lower places
   uint64_t key;
   uint32_t at, row;
@@ -541,18 +560,18 @@ template <typename T, bool MASK> struct Picker {
     for (int r = 0; r < a.n; ++r) {
       if (!s.again[r] || s.done[r]) continue;  // the same for all threads
       const T* p = row(r);
-      const double m = s.near[r].x;
-      double t = 0.0;
+      const float top = s.near[r].x;
+      const double m = top;
+      double part[4] = {0.0, 0.0, 0.0, 0.0};
       for (int i0 = tid; i0 < a.vocab; i0 += 8 * BP_THREADS) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i0 + i * BP_THREADS < a.vocab ? to_f32(p[i0 + i * BP_THREADS]) : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const double d = (double)v[i] - m;
-          if (d > -100.0) t += exp(d);  // a vocabulary of what is left out is below 2^-124 of the sum
-        }
+        for (int i = 0; i < 8; ++i)  // below e^-100 nothing counts: 2^20 of them are 2^-124 of the sum
+          part[i & 3] += exp_of(v[i] - top > -100.f ? (double)v[i] - m : -100.0);
       }
+      double t = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
       if (lane == 0) s.red[warp] = t;

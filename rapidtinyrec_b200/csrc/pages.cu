@@ -29,6 +29,7 @@ namespace rtr {
 
 constexpr int PG_FEW = 256, PG_MANY = 1024;  // threads of a block, up to so many sequences and beyond
 constexpr int PG_MAX_SEQS = 16384, PG_BACK_CLUSTER = 8;
+constexpr int PG_PER = 2;                    // entries of a table a thread, by which pages given back get blocks
 constexpr int PG_HELD = 8;                   // pages given back that a thread remembers
 
 struct PagePool {
@@ -244,33 +245,46 @@ __global__ void __launch_bounds__(PG_MANY) pages_release_kernel(const PagePool p
     return;
   }
   const int all = pg_sums[q.seqs];
-  const auto page_at = [&](int i) {
-    const int s = page_seq(pg_sums, q.seqs, i), k = keep ? keep[s] : 0;
-    return q.table[s * q.stride + pages_of(k, shift) + (i - pg_sums[s])];
+  // each thread has neighbouring items: one search, then from sequence to sequence
+  const int share = (all - 1) / step + 1, lo = (int)min((int64_t)at * share, (int64_t)all), hi = (int)min((int64_t)lo + share, (int64_t)all);
+  const auto each = [&](int from, auto&& f) {
+    int s = from < hi ? page_seq(pg_sums, q.seqs, from) : 0;
+    for (int i = from; i < hi; ++i) {
+      while (pg_sums[s + 1] <= i) ++s;
+      f(i, q.table + s * q.stride + pages_of(keep ? keep[s] : 0, shift) + (i - pg_sums[s]));
+    }
   };
   uint32_t bad = count < 0 || count > p.pages || all > p.pages - count ? RTR_DEV_PAGE_NOT_HELD : 0u;
   int held[PG_HELD];  // the thread's first pages
+#pragma unroll
+  for (int j = 0; j < PG_HELD; ++j) held[j] = -1;
   const auto mark = [&](int page) {
     if (page < 0 || page >= p.pages) bad |= RTR_DEV_BAD_PAGE;
     else if (atomicCAS(p.marks + page, 1, 2) != 1) bad |= RTR_DEV_PAGE_NOT_HELD;
   };
-  const bool look = !bad;
+  if (!bad) {
+    const int32_t* where[PG_HELD];
+    int s = lo < hi ? page_seq(pg_sums, q.seqs, lo) : 0;
 #pragma unroll
-  for (int j = 0; j < PG_HELD; ++j) {
-    const int64_t i = at + (int64_t)j * step;
-    if (i < all) held[j] = page_at((int)i);
-  }
-  if (look) {
+    for (int j = 0; j < PG_HELD; ++j) {
+      const int i = lo + j;
+      if (i >= hi) break;
+      while (pg_sums[s + 1] <= i) ++s;
+      where[j] = q.table + s * q.stride + pages_of(keep ? keep[s] : 0, shift) + (i - pg_sums[s]);
+    }
 #pragma unroll
     for (int j = 0; j < PG_HELD; ++j)
-      if (at + (int64_t)j * step < all) mark(held[j]);
-    for (int64_t i = at + (int64_t)PG_HELD * step; i < all; i += step) mark(page_at((int)i));
+      if (lo + j < hi) held[j] = *where[j];
+#pragma unroll
+    for (int j = 0; j < PG_HELD; ++j)
+      if (lo + j < hi) mark(held[j]);
+    each(lo + PG_HELD, [&](int, const int32_t* at_) { mark(*at_); });
   }
   if (bad) atomicOr(&wrong, bad);
   cluster.sync();
   bad = 0;
   for (unsigned r = 0; r < cluster.num_blocks(); ++r) bad |= *cluster.map_shared_rank(&wrong, r);
-  const auto settle = [&](int64_t i, int page) {
+  const auto settle = [&](int i, int page) {
     if (!bad) {
       p.marks[page] = 0;
       p.free[(int64_t)count + all - 1 - i] = page;
@@ -280,8 +294,8 @@ __global__ void __launch_bounds__(PG_MANY) pages_release_kernel(const PagePool p
   };
 #pragma unroll
   for (int j = 0; j < PG_HELD; ++j)
-    if (at + (int64_t)j * step < all) settle(at + (int64_t)j * step, held[j]);
-  for (int64_t i = at + (int64_t)PG_HELD * step; i < all; i += step) settle(i, page_at((int)i));
+    if (lo + j < hi) settle(lo + j, held[j]);
+  each(lo + PG_HELD, [&](int i, const int32_t* at_) { settle(i, *at_); });
   if (at == 0) {
     if (bad) atomicOr(p.status, bad);
     else *p.count = count + all;
@@ -348,9 +362,13 @@ int rtr_pages_release(const rtr_page_pool* pool, const int32_t* table, int64_t t
   if (!seqs) return RTR_OK;
   KvDevice on(device);
   if (on.error) return set_error(RTR_ERR_CUDA, cudaGetErrorString(on.error));
-  // One block while it remembers every page that the tables can name.
-  const int threads = (int64_t)seqs * table_width <= PG_FEW * PG_HELD ? PG_FEW : PG_MANY;
-  const int cluster = (int64_t)seqs * table_width <= PG_HELD * (int64_t)threads ? 1 : PG_BACK_CLUSTER;
+  // How many pages come back is not known here, only the tables' entries: one block for two entries a thread, a cluster of up to eight
+  // for more.  (64 x 66 entries, 64 pages at most given back and taken: one block 7.8 us, four 8.4, eight 9.4; 96 x 66, 4,000 pages: 14.9,
+  // 10.5 and 10.5.)
+  const int64_t entries = (int64_t)seqs * table_width;
+  const int threads = entries <= 2 * PG_FEW ? PG_FEW : PG_MANY;
+  int cluster = 1;
+  while (cluster < PG_BACK_CLUSTER && entries > (int64_t)PG_PER * cluster * threads) cluster *= 2;
   const int smem = (seqs + 1) * (int)sizeof(int32_t);
   static std::atomic<uint64_t> allowed;
   cudaError_t e = smem > 32 << 10 ? kv_allow_smem(pages_release_kernel, (PG_MAX_SEQS + 1) * (int)sizeof(int32_t), allowed, device)
