@@ -62,12 +62,24 @@ def inputs(items, n, vocab, dtype, seed, gain=2.5):
 @pytest.mark.parametrize('items,n,beams,vocab,k,eos', [
     (1, 1, 1, 1000, 1, None), (1, 4, 4, 8192, 8, 17), (3, 50, 50, 32003, 100, 5), (2, 1, 50, 151, 100, None),
     (1, 128, 128, 4096, 256, 0), (5, 10, 5, 1, 10, None), (2, 3, 3, 7, 6, 6), (1, 2, 64, 152704, 128, 152703), (70, 3, 3, 2047, 9, None),
-    (1, 1, 128, 2000, 256, None), (2, 60, 5, 513, 65, 44), (1, 50, 50, 152832, 100, None), (1, 1, 3, 1 << 20, 6, None)])
+    (1, 1, 128, 2000, 256, None), (2, 60, 5, 513, 65, 44), (1, 50, 50, 152832, 100, None), (1, 1, 3, 1 << 20, 6, None),
+    (1, 128, 128, 152704, 256, 7), (1, 1, 128, 152704, 256, None), (3, 1, 50, 152704, 100, 1), (2, 33, 33, 32000, 66, None)])
 def test_sizes_and_types(items, n, beams, vocab, k, eos, dtype):
     from rapidtinyrec_b200.beam_search import BeamSearch
     logits, scores = inputs(items, n, vocab, dtype, items + vocab)
     search = BeamSearch(beams, eos=eos, candidates=k)
     check_step(search.select(logits, scores), logits, scores, k, beams, eos)
+    search.check()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('items,n,vocab,share', [(2, 20, 152704, 0.5), (1, 128, 40001, 0.01), (3, 1, 152832, 0.9), (40, 10, 5008, 0.2)])
+def test_lists_of_allowed_tokens(items, n, vocab, share, dtype):
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    logits, scores = inputs(items, n, vocab, dtype, vocab)
+    allowed = torch.rand(items * n, vocab, generator=generator(n), device='cuda') < share
+    search = BeamSearch(n, eos=3)
+    check_step(search.select(logits, scores, allowed=allowed), logits, scores, 2 * n, n, eos=3, allowed=allowed)
     search.check()
 
 
@@ -230,6 +242,47 @@ def test_every_call_the_same_and_captured():
         other = search.select(logits, scores)
     stream.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(step, other))
+    search.check()
+
+
+def test_rows_and_states_beyond_32_bits():
+    """Rows and states more than 2^31 values apart."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    far = (1 << 30) + 7
+    room = torch.empty(2 * far + 60000, dtype=torch.bfloat16, device='cuda')
+    logits = room.as_strided((3, 50021), (far, 1))
+    made, scores = inputs(1, 3, 50021, torch.bfloat16, 5)
+    logits.copy_(made)
+    check_step(BeamSearch(3).select(logits, scores), made, scores, 6, 3)
+    state = room.as_strided((3, 2, 1009), (far, 2048, 1))
+    made = values((3, 2, 1009), torch.bfloat16, 6)
+    state.copy_(made)
+    parents = torch.tensor([[2, 0, 0]], dtype=torch.int32, device='cuda')
+    BeamSearch(3).reorder(state, parents)
+    assert torch.equal(state, moved(made, parents, 0))
+
+
+def test_two_calls_at_once():
+    """Two streams, each with calls of its own; the handle is one."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    search = BeamSearch(30)
+    sets = [inputs(2, 30, 60000 + 5 * i, torch.float32, i) for i in range(2)]
+    states = [values((60, 40000), torch.float32, i) for i in range(2)]
+    want = [x.clone() for x in states]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    steps = [[], []]
+    for _ in range(5):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                steps[i].append(search.select(*sets[i]))
+                search.reorder(states[i], steps[i][-1].parents)
+    torch.cuda.synchronize()
+    for i in range(2):
+        for step in steps[i]:
+            check_step(step, *sets[i], 60, 30)
+            want[i] = moved(want[i], step.parents, 0)
+        assert torch.equal(states[i], want[i])
     search.check()
 
 

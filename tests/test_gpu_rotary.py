@@ -189,6 +189,19 @@ def test_nothing_to_do_and_values_that_are_not_finite():
     assert torch.equal(bad, want)
 
 
+def test_rows_beyond_32_bits():
+    from rapidtinyrec_b200.rotary import Rotary
+    rotary = Rotary(64)
+    far = (1 << 30) + 64
+    room = torch.empty(2 * far + 256, dtype=torch.bfloat16, device='cuda')
+    q = room.as_strided((3, 2, 64), (far, 64, 1))
+    made = rows_of(3, 2, 64, torch.bfloat16, 20)
+    q.copy_(made)
+    positions = torch.tensor([3, 50, 700], device='cuda')
+    rotary.rotate(q, None, positions, out=q)
+    check_rows(q, plain(made, positions, rotary.frequencies, 64, False))
+
+
 def test_captured_and_on_another_stream():
     from rapidtinyrec_b200.rotary import Rotary
     rotary = Rotary(64)
