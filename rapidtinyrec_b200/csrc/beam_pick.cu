@@ -15,14 +15,16 @@
 // off by at most 5.2e-7, those of two rows of a kind by 6.1e-7 from one another.  The 100 best of 7.6 million
 // candidates lie 1e-4 to 1e-3 apart, so now and then two are too close to tell.  Differences of logits and scores are exact enough in
 // fp64; what is not known well is the sum.  Where two neighbours of different rows are closer than BP_DOUBT, 1e-6, both rows' sums are
-// taken again in fp64 and the list is put in order again (two rows of 152,832: 63 us more, for one item in 100 or so): the
-// order is that of 64-bit arithmetic, however the rows were split.
+// taken again in fp64 and the list is put in order again (two rows of 152,832: 63 us more by one block, some 25 by the four that are
+// there in a batch; for one item in 100 or so): the order is that of 64-bit arithmetic, however the rows were split.
 //
-// What bounds it.  The first kernel: exponentials (one of the 16 a clock that an SM has for each logit; XU 81 %, issue slots 62 %) and HBM
-// (5.96 TB/s) alike, 1,600 rows of 152,832 in bf16 in 81 us.  The second: latency, some 17,000 cycles, 8.5 us, for 50 beams: dependent
+// What bounds it.  The first kernel: exponentials (XU 81 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 81 us, 5.96 TB/s;
+// without its exponentials it reads at 7.3 TB/s.  An eighth or a quarter of them on the FMA pipe instead: no change, and 3 us slower.  The second: latency, some 17,000 cycles, 8.5 us, for 50 beams: dependent
 // loads (slices and groups, second bests, lanes' logits; 700 to 2,500 cycles each), code that comes from L2 as it is
 // gone through once, and a dozen barriers of 1,024 threads (512 threads: 0.4 us less for 4 beams, 0.9 more for 50).
 #include <cuda_runtime.h>
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -41,6 +43,7 @@ constexpr int BP_THREADS = 1024;                // second kernel: threads of a b
 constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
 constexpr int BP_GROUPS = 512, BP_LANES = 1024, BP_LIST = 1024;  // groups, lanes of them and candidates that it takes up at once
 constexpr int BP_HELD = 4;                      // quartets of groups that a thread of it holds
+constexpr int BP_RANKS = 4;                     // blocks that sum an item's doubtful rows together
 constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
@@ -53,6 +56,7 @@ struct BeamPick {
   int groups, padded;      // groups of a row, and their number rounded up to 4
   uint32_t quarter_inv;    // ceil(2^32 / (padded / 4)): a group quartet's row by one multiplication (0: 2^32, the quartet itself)
   int slices;              // blocks of a row
+  int ranks;               // blocks of the second kernel's clusters
   float* best;             // [items * n][padded]: a group's largest allowed logit
   uint32_t* second;        // likewise: the largest of the other lanes' (rounded up) and, in the last five bits, whose the first is
   float2* part;            // [items * n][slices]: maximum, sum of exponentials relative to it
@@ -366,6 +370,8 @@ struct PickShared {
   float2 near[BP_MAX_N];                // the row's maximum, and off rounded (minus infinity: nothing to offer)
   float need[BP_MAX_N];                 // what its logits have to reach
   uint8_t again[BP_MAX_N], done[BP_MAX_N];  // rows to sum in 64 bits, and those that are
+  double share[BP_RANKS][BP_MAX_N];         // and what the blocks of the cluster have of their sums
+  int doubt;                                // whether there are any
   int32_t quartet_at[BP_GROUPS], groups[BP_GROUPS];
   PickEntry list[BP_LIST];
   uint16_t order[BP_LIST];              // and their places in the list
@@ -560,16 +566,16 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
   }
 
-  // The sums of the rows marked `again`, in 64 bits: one row after the other, all threads.  The order of
-  // a sum goes by places in the vocabulary, not by the row's place in memory, so that equal rows have equal sums.
-  RTR_DEVICE void sum_again() {
+  // A block's share of the sums of the rows marked `again`, in 64 bits: one row after the other, all threads.  The order of a
+  // sum goes by places in the vocabulary, not by the row's place in memory, so that equal rows have equal sums.
+  RTR_DEVICE void share_again(int rank, int ranks, double (&share)[BP_MAX_N]) {
     for (int r = 0; r < a.n; ++r) {
       if (!s.again[r] || s.done[r]) continue;  // the same for all threads
       const T* p = row(r);
       const float top = s.near[r].x;
       const double m = top;
       double part[4] = {0.0, 0.0, 0.0, 0.0};
-      for (int i0 = tid; i0 < a.vocab; i0 += 8 * BP_THREADS) {
+      for (int i0 = tid + rank * 8 * BP_THREADS; i0 < a.vocab; i0 += ranks * 8 * BP_THREADS) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i0 + i * BP_THREADS < a.vocab ? to_f32(p[i0 + i * BP_THREADS]) : -INFINITY;
@@ -585,13 +591,23 @@ template <typename T, bool MASK> struct Picker {
       if (tid == 0) {
         t = 0.0;
         for (int w = 0; w < BP_THREADS / 32; ++w) t += s.red[w];
-        s.sum[r] = log(t);
-        s.off[r] = (double)a.scores[item * a.n + r] - s.sum[r];
-        s.near[r].y = (float)s.off[r];
-        s.done[r] = 1;
+        share[r] = t;
       }
       __syncthreads();
     }
+  }
+  RTR_DEVICE void sum_again(int ranks) {
+    share_again(0, ranks, s.share[0]);
+    if (ranks > 1) cooperative_groups::this_cluster().sync();  // the others' shares are there
+    if (tid < a.n && s.again[tid] && !s.done[tid]) {
+      double t = 0.0;
+      for (int r = 0; r < ranks; ++r) t += s.share[r][tid];
+      s.sum[tid] = log(t);
+      s.off[tid] = (double)a.scores[item * a.n + tid] - s.sum[tid];
+      s.near[tid].y = (float)s.off[tid];
+      s.done[tid] = 1;
+    }
+    __syncthreads();
   }
 
   // What `near` may be off by (three roundings of 2^-24), with room, and what two sums may be.
@@ -757,7 +773,7 @@ template <typename T, bool MASK> struct Picker {
       s.again[r] = differs && s.off[r] > -INFINITY;
     }
     __syncthreads();
-    sum_again();
+    sum_again(1);
     uint64_t least;
     uint32_t last;
     const auto groups = [&](auto&& f) {
@@ -835,8 +851,10 @@ template <typename T, bool MASK> struct Picker {
       for (int q = 0; q < a.n; ++q) equal |= s.again[q] && s.sum[q] == s.sum[tid];
     __syncthreads();
     if (equal) s.again[tid] = 1;
+    if (tid == 0) s.doubt = 1;
     __syncthreads();
-    sum_again();
+    if (a.ranks > 1) cooperative_groups::this_cluster().sync();  // the others may look
+    sum_again(a.ranks);
     put_in_order();
   }
 };
@@ -858,6 +876,24 @@ template <typename T, bool MASK> __device__ __noinline__ void pick_whole(const B
 }
 template <typename T, bool MASK> __device__ __noinline__ void pick_again(const BeamPick& a, PickShared& s) {
   picker<T, MASK>(a, s).settle();
+}
+// The other blocks of an item's cluster: they wait for the first one's doubts, and take their shares of the sums.
+template <typename T, bool MASK> RTR_DEVICE void pick_help(const BeamPick& a, PickShared& s) {
+  const auto cluster = cooperative_groups::this_cluster();
+  const int tid = threadIdx.x, rank = (int)cluster.block_rank();
+  cluster.sync();
+  PickShared* lead = cluster.map_shared_rank(&s, 0);
+  if (lead->doubt) {
+    if (tid < a.n) {
+      s.again[tid] = lead->again[tid];
+      s.done[tid] = lead->done[tid];
+      s.near[tid].x = lead->near[tid].x;
+    }
+    __syncthreads();
+    picker<T, MASK>(a, s).share_again(rank, a.ranks, lead->share[rank]);
+    cluster.sync();
+  }
+  cluster.sync();  // the first block does not leave before its flag is read
 }
 // Fewer finite candidates than k: the first places that have none.
 __device__ __noinline__ void pick_fill(const BeamPick& a, PickShared& s) {
@@ -883,12 +919,21 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
   pdl_launch_dependents();
   pdl_wait();
   const int item = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (blockIdx.z) {
+    pick_help<T, MASK>(a, s);
+    return;
+  }
   Picker<T, MASK> p = picker<T, MASK>(a, s);
   p.hold();
   p.offsets();
   if (!p.gather()) pick_exactly<T, MASK>(a, s);
   p.put_in_order();
-  if (p.doubtful()) pick_again<T, MASK>(a, s);
+  if (p.doubtful()) {
+    pick_again<T, MASK>(a, s);
+  } else if (a.ranks > 1) {
+    if (tid == 0) s.doubt = 0;
+    cooperative_groups::this_cluster().sync();
+  }
   if (s.n_list < a.k) pick_fill(a, s);
   if (tid < a.k) {
     const PickEntry c = s.list[s.order[tid]];
@@ -915,6 +960,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
       taken += __popc(mask);
     }
   }
+  if (a.ranks > 1) cooperative_groups::this_cluster().sync();
 }
 
 // --------------------------------------------------------------------- host
@@ -1005,10 +1051,14 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.next_parents = step->next_parents;
   p.next_scores = step->next_scores;
   p.status = step->status;
+  // Where there are eight items or more one is in doubt now and then (an item in 100 or so): their blocks have others of a cluster beside
+  // them, on SMs that have no item, for those sums.
+  p.ranks = 1;
+  while (step->items >= 8 && p.ranks < BP_RANKS && 2 * p.ranks * (int64_t)step->items <= on.sms) p.ranks *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto run = [&](auto scan, auto pick) {
     const cudaError_t e = kv_launch(scan, dim3((unsigned)blocks), BP_WARPS * 32, 0, 1, st, p);
-    return e == cudaSuccess ? kv_launch(pick, dim3((unsigned)p.items), BP_THREADS, 0, 1, st, p) : e;
+    return e == cudaSuccess ? kv_launch(pick, dim3((unsigned)p.items, 1, (unsigned)p.ranks), BP_THREADS, 0, p.ranks, st, p) : e;
   };
   cudaError_t e;
   if (step->dtype == RTR_DTYPE_F32)

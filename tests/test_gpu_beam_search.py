@@ -211,8 +211,11 @@ def test_candidates_too_close_for_32_bits(vocab):
     gaps = value[0, :-1] - value[0, 1:]
     assert (gaps < 1e-6).sum() >= 15 and (gaps[gaps > 0] > 1e-12).all()
     check_step(BeamSearch(12).select(logits, scores), logits, scores, 24, 12)
-    more = logits.repeat(3, 1)
-    check_step(BeamSearch(12).select(more, scores.repeat(3, 1)), more, scores.repeat(3, 1), 24, 12)
+    for items in (3, 8, 40, 100):  # one block an item, clusters of four, of two, one again
+        more, same = logits.repeat(items, 1), scores.repeat(items, 1)
+        if items > 3:
+            more[6:12] = 1.3 * torch.randn(n, vocab, generator=g, device='cuda')  # an item without doubts
+        check_step(BeamSearch(12).select(more, same), more, same, 24, 12)
 
 
 def test_every_call_the_same_and_captured():
