@@ -19,9 +19,10 @@
 // there in a batch; for one item in 100 or so): the order is that of 64-bit arithmetic, however the rows were split.
 //
 // What bounds it.  The first kernel: exponentials (XU 81 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 81 us, 5.96 TB/s;
-// without its exponentials it reads at 7.3 TB/s.  An eighth or a quarter of them on the FMA pipe instead: no change, and 3 us slower.  The second: latency, some 17,000 cycles, 8.5 us, for 50 beams: dependent
-// loads (slices and groups, second bests, lanes' logits; 700 to 2,500 cycles each), code that comes from L2 as it is
-// gone through once, and a dozen barriers of 1,024 threads (512 threads: 0.4 us less for 4 beams, 0.9 more for 50).
+// without its exponentials it reads at 7.3 TB/s.  An eighth or a quarter of them on the FMA pipe instead: no change, and 3 us slower.
+// The second: latency, some 17,000 cycles, 8.5 us, for 50 beams: dependent loads (slices and groups, second bests, lanes' logits; 700
+// to 2,500 cycles each), code that comes from L2 as it is gone through once, and a dozen barriers of 1,024 threads (512 threads: 0.4 us
+// less for 4 beams, 0.9 more for 50).
 #include <cuda_runtime.h>
 
 #include <cooperative_groups.h>
@@ -913,16 +914,18 @@ __device__ __noinline__ void pick_fill(const BeamPick& a, PickShared& s) {
   __syncthreads();
 }
 
-template <typename T, bool MASK>
+// HELP: a cluster of a.ranks blocks an item, else one block.
+template <typename T, bool MASK, bool HELP>
 __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_constant__ BeamPick a) {
   __shared__ PickShared s;
   pdl_launch_dependents();
   pdl_wait();
   const int item = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (blockIdx.z) {
-    pick_help<T, MASK>(a, s);
-    return;
-  }
+  if constexpr (HELP)
+    if (blockIdx.z) {
+      pick_help<T, MASK>(a, s);
+      return;
+    }
   Picker<T, MASK> p = picker<T, MASK>(a, s);
   p.hold();
   p.offsets();
@@ -930,7 +933,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
   p.put_in_order();
   if (p.doubtful()) {
     pick_again<T, MASK>(a, s);
-  } else if (a.ranks > 1) {
+  } else if constexpr (HELP) {
     if (tid == 0) s.doubt = 0;
     cooperative_groups::this_cluster().sync();
   }
@@ -960,7 +963,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
       taken += __popc(mask);
     }
   }
-  if (a.ranks > 1) cooperative_groups::this_cluster().sync();
+  if constexpr (HELP) cooperative_groups::this_cluster().sync();
 }
 
 // --------------------------------------------------------------------- host
@@ -1051,22 +1054,27 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.next_parents = step->next_parents;
   p.next_scores = step->next_scores;
   p.status = step->status;
-  // Where there are eight items or more one is in doubt now and then (an item in 100 or so): their blocks have others of a cluster beside
-  // them, on SMs that have no item, for those sums.
+  // Where there are eight items or more, of two rows at least (one row is never in doubt), an item is in doubt now and then (one in 100
+  // or so), and summing its rows takes one block long where they are long (65,536 logits 14 us each): its block has others of a
+  // cluster beside it, on SMs that have no item.  (16 items of 10 rows of 32,003 without doubts: 14.7 us with one block each, 15.7
+  // with four.)
   p.ranks = 1;
-  while (step->items >= 8 && p.ranks < BP_RANKS && 2 * p.ranks * (int64_t)step->items <= on.sms) p.ranks *= 2;
+  if (step->items >= 8 && step->n > 1 && step->vocab >= 1 << 16)
+    while (p.ranks < BP_RANKS && 2 * p.ranks * (int64_t)step->items <= on.sms) p.ranks *= 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto run = [&](auto scan, auto pick) {
     const cudaError_t e = kv_launch(scan, dim3((unsigned)blocks), BP_WARPS * 32, 0, 1, st, p);
     return e == cudaSuccess ? kv_launch(pick, dim3((unsigned)p.items, 1, (unsigned)p.ranks), BP_THREADS, 0, p.ranks, st, p) : e;
   };
+  const auto run_type = [&](auto type, auto mask) {
+    using T = decltype(type);
+    constexpr bool MASK = decltype(mask)::value;
+    return p.ranks > 1 ? run(beam_scan_kernel<T, MASK>, beam_pick_kernel<T, MASK, true>)
+                       : run(beam_scan_kernel<T, MASK>, beam_pick_kernel<T, MASK, false>);
+  };
   cudaError_t e;
-  if (step->dtype == RTR_DTYPE_F32)
-    e = p.allowed ? run(beam_scan_kernel<float, true>, beam_pick_kernel<float, true>)
-                  : run(beam_scan_kernel<float, false>, beam_pick_kernel<float, false>);
-  else
-    e = p.allowed ? run(beam_scan_kernel<__nv_bfloat16, true>, beam_pick_kernel<__nv_bfloat16, true>)
-                  : run(beam_scan_kernel<__nv_bfloat16, false>, beam_pick_kernel<__nv_bfloat16, false>);
+  if (step->dtype == RTR_DTYPE_F32) e = p.allowed ? run_type(float{}, std::true_type{}) : run_type(float{}, std::false_type{});
+  else e = p.allowed ? run_type(__nv_bfloat16{}, std::true_type{}) : run_type(__nv_bfloat16{}, std::false_type{});
   return e == cudaSuccess ? RTR_OK : set_error(RTR_ERR_CUDA, cudaGetErrorString(e));
 }
 

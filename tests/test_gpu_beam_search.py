@@ -193,7 +193,7 @@ def test_values_that_are_not_finite():
                 search.check()
 
 
-@pytest.mark.parametrize('vocab', [1500, 60001])
+@pytest.mark.parametrize('vocab', [1500, 60001, 70001])
 def test_candidates_too_close_for_32_bits(vocab):
     """Candidates of different beams 1e-9 to 3e-7 apart, both ways, closer than fp32 sums tell: the order is float64's."""
     from rapidtinyrec_b200.beam_search import BeamSearch
@@ -211,7 +211,7 @@ def test_candidates_too_close_for_32_bits(vocab):
     gaps = value[0, :-1] - value[0, 1:]
     assert (gaps < 1e-6).sum() >= 15 and (gaps[gaps > 0] > 1e-12).all()
     check_step(BeamSearch(12).select(logits, scores), logits, scores, 24, 12)
-    for items in (3, 8, 40, 100):  # one block an item, clusters of four, of two, one again
+    for items in (3, 8, 40, 100):  # of 70,001: one block an item, clusters of four, of two, one again
         more, same = logits.repeat(items, 1), scores.repeat(items, 1)
         if items > 3:
             more[6:12] = 1.3 * torch.randn(n, vocab, generator=g, device='cuda')  # an item without doubts
