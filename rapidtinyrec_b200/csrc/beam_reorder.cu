@@ -129,13 +129,22 @@ __global__ void __launch_bounds__(BR_THREADS) beam_reorder_kernel(const __grid_c
   }
 }
 
+// Bytes of a column: 16 or 4 where all of a state lies at multiples of them, else 1.
+static int state_column(const rtr_beam_state& s) {
+  uint64_t bits = reinterpret_cast<uintptr_t>(s.data) | (uint64_t)s.row_bytes | (uint64_t)s.inner;
+  for (int d = 0; d < 3; ++d)
+    if (s.sizes[d] > 1) bits |= (uint64_t)s.strides[d];
+  return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+}
 static const char* state_check(const rtr_beam_state& s) {
   if (!s.data) return "null state";
   if (s.inner < 1 || s.sizes[0] < 1 || s.sizes[1] < 1 || s.sizes[2] < 1) return "a state's dimensions must be positive";
   if (s.row_bytes == 0) return "the rows of a state overlap";
   for (int d = 0; d < 3; ++d)
     if (s.sizes[d] > 1 && s.strides[d] == 0) return "a state's dimensions overlap";
-  return nullptr;
+  uint64_t columns = (uint64_t)s.inner / state_column(s);
+  for (int d = 0; d < 3 && columns <= INT32_MAX; ++d) columns *= (uint64_t)s.sizes[d];
+  return columns > INT32_MAX ? "a state's rows are too long" : nullptr;
 }
 
 }  // namespace rtr
@@ -186,14 +195,9 @@ int rtr_beam_reorder(const rtr_beam_state* states, int32_t count, const int32_t*
     cudaError_t e = cudaSuccess;
     for (int i = 0; i < count && e == cudaSuccess; ++i) {
       const rtr_beam_state& s = states[i];
-      uint64_t bits = reinterpret_cast<uintptr_t>(s.data) | (uint64_t)s.row_bytes | (uint64_t)s.inner;
-      for (int d = 0; d < 3; ++d)
-        if (s.sizes[d] > 1) bits |= (uint64_t)s.strides[d];
-      const int fits = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
-      if (fits != vec) continue;
+      if (state_column(s) != vec) continue;
       const uint64_t inner = (uint64_t)s.inner / vec;
       const uint64_t columns = inner * s.sizes[0] * s.sizes[1] * s.sizes[2];
-      if (inner > INT32_MAX || columns > INT32_MAX) return set_error(RTR_ERR_ARG, "a state's rows are too long");
       const uint64_t more = (columns + tile - 1) / tile;
       if (m.count == BR_STATES || tiles + more > INT32_MAX) e = launch();
       MoveState& to = m.states[m.count++];

@@ -115,6 +115,7 @@ PyObject* call_grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (a[5] != Py_None) rows = whole(a[5], "rows");
     if (rows < 0 || rows > INT32_MAX) refuse("rows must not be negative and must fit 32 bits");
+    written(s.table, "table");
     Room out(pool.index, Room::of(s.seqs, 4) + Room::of(s.seqs + 1, 4) + Room::of(rows, 4) + Room::of(rows, 8));
     const at::Tensor lens = out.take({s.seqs}, at::kInt), starts = out.take({s.seqs + 1}, at::kInt),
                      positions = out.take({rows}, at::kInt), slots = out.take({rows}, at::kLong);

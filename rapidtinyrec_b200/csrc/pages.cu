@@ -104,6 +104,7 @@ RTR_DEVICE bool page_sums(int seqs, int32_t* a, int32_t* b, int64_t limit_a, int
       a[s + 1] = (int32_t)(x + (uint32_t)red[warp].x);
       if (b) b[s + 1] = (int32_t)(y + (uint32_t)red[warp].y);
     }
+    __syncwarp();  // the next round writes the warp's place
   }
   if (tid == 0) {
     a[0] = 0;

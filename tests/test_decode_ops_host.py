@@ -178,7 +178,8 @@ def reorder(states, parents=A, items=2, beams=4, status=A):
 
 @pytest.mark.parametrize('change,says', [
     (dict(data=None), 'null state'), (dict(inner=0), 'positive'), (dict(sizes=(ctypes.c_int32 * 3)(1, 0, 2)), 'positive'),
-    (dict(row_bytes=0), 'rows of a state'), (dict(strides=(ctypes.c_int64 * 3)(0, 0, 0)), 'dimensions overlap')])
+    (dict(row_bytes=0), 'rows of a state'), (dict(strides=(ctypes.c_int64 * 3)(0, 0, 0)), 'dimensions overlap'),
+    (dict(inner=(1 << 31) + 1), 'too long'), (dict(inner=17, sizes=(ctypes.c_int32 * 3)(1 << 30, 1 << 30, 2), strides=(ctypes.c_int64 * 3)(1, 1, 1)), 'too long')])
 def test_states_that_are_refused(change, says):
     assert reorder([state(), state(**change)]) == _native.RTR_ERR_ARG
     assert says in message()

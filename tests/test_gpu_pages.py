@@ -99,10 +99,11 @@ def test_growing_again_takes_the_same_pages():
     assert table[0, :3].tolist() == [0, 1, 2] and table[2, :7].tolist() == [3, 4, 5, 6, 7, 8, 9]
     assert first.starts.tolist() == [0, 40, 40, 140]
     more = pool.grow(table, first.lens, ints([20, 1, 0]), rows=21)
-    kept = table.clone()
+    kept, version = table.clone(), table._version
     pool.release(table, more.lens, first.lens)
+    assert table._version == version
     again = pool.grow(table, first.lens, ints([20, 1, 0]), rows=21)
-    assert torch.equal(table, kept) and torch.equal(again.slots, more.slots)
+    assert torch.equal(table, kept) and torch.equal(again.slots, more.slots) and table._version > version
     pool.check()
 
 
