@@ -15,7 +15,7 @@
 // off by at most 5.2e-7, those of two rows of a kind by 6.1e-7 from one another.  The 100 best of 7.6 million
 // candidates lie 1e-4 to 1e-3 apart, so now and then two are too close to tell.  Differences of logits and scores are exact enough in
 // fp64; what is not known well is the sum.  Where two neighbours of different rows are closer than BP_DOUBT, 1e-6, both rows' sums are
-// taken again in fp64 and the list is put in order again (two rows of 152,832: 63 us more by one block, some 25 by the four that are
+// taken again in fp64 (rows whose fp32 sums are the same among them) and the list is put in order again (two rows of 152,832: 63 us more by one block, some 25 by the four that are
 // there in a batch; for one item in 100 or so): the order is that of 64-bit arithmetic, however the rows were split.
 //
 // What bounds it.  The first kernel: exponentials (XU 81 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 81 us, 5.96 TB/s;
@@ -568,12 +568,34 @@ template <typename T, bool MASK> struct Picker {
   }
 
   // A block's share of the sums of the rows marked `again`, in 64 bits: one row after the other, all threads.  The order of a
-  // sum goes by places in the vocabulary, not by the row's place in memory, so that equal rows have equal sums.
+  // sum goes by places in the vocabulary, not by the row's place in memory, so that equal rows have equal sums.  Of rows that are the
+  // same in all places (beams that have not parted yet) one is summed: comparing takes 12 us of
+  // 152,704 logits, summing 31.
   RTR_DEVICE void share_again(int rank, int ranks, double (&share)[BP_MAX_N]) {
     for (int r = 0; r < a.n; ++r) {
       if (!s.again[r] || s.done[r]) continue;  // the same for all threads
       const T* p = row(r);
       const float top = s.near[r].x;
+      int like = 0;  // the first row of this sum and maximum
+      while (like < r && !(s.again[like] && !s.done[like] && s.sum[like] == s.sum[r] && s.near[like].x == top)) ++like;
+      if (like < r) {
+        const T* q = row(like);
+        bool same = true;
+        for (int i0 = tid + rank * 8 * BP_THREADS; i0 < a.vocab && same; i0 += ranks * 8 * BP_THREADS) {
+          float v[8], w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = i0 + i * BP_THREADS < a.vocab ? to_f32(p[i0 + i * BP_THREADS]) : 0.f;
+            w[i] = i0 + i * BP_THREADS < a.vocab ? to_f32(q[i0 + i * BP_THREADS]) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) same &= v[i] == w[i];
+        }
+        if (__syncthreads_and(same)) {
+          if (tid == 0) share[r] = share[like];
+          continue;
+        }
+      }
       const double m = top;
       double part[4] = {0.0, 0.0, 0.0, 0.0};
       for (int i0 = tid + rank * 8 * BP_THREADS; i0 < a.vocab; i0 += ranks * 8 * BP_THREADS) {
@@ -745,7 +767,7 @@ template <typename T, bool MASK> struct Picker {
 
   // The same where ties make the lists too long (rows of equal logits, most of them masked by the type's lowest value): the exact
   // k best groups, by value and place, and of those the exact k best candidates; each by bisection of the
-  // value's 64 bits and, among equal ones, of the place.  Rows whose sums differ are summed in 64 bits first.
+  // value's 64 bits and, among equal ones, of the place.  Rows are summed in 64 bits first.
   template <typename Each> RTR_DEVICE void bisect(Each&& each, int k, uint64_t& least, uint32_t& last) {
     least = 0;  // the largest key that at least k reach (every finite candidate's is above 0)
     for (int b = 63; b >= 0; --b) {
@@ -768,11 +790,7 @@ template <typename T, bool MASK> struct Picker {
   }
   RTR_DEVICE void gather_exactly() {
     hold();
-    for (int r = tid; r < a.n; r += BP_THREADS) {
-      bool differs = false;
-      for (int q = 0; q < a.n; ++q) differs |= s.off[q] > -INFINITY && s.sum[q] != s.sum[r];
-      s.again[r] = differs && s.off[r] > -INFINITY;
-    }
+    for (int r = tid; r < a.n; r += BP_THREADS) s.again[r] = a.n > 1 && s.off[r] > -INFINITY;
     __syncthreads();
     sum_again(1);
     uint64_t least;
@@ -830,8 +848,8 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
   }
 
-  // Marks the rows of candidates among (or just behind) the first k that are too close to those of another row.  Rows whose
-  // sums are equal have exact differences, as long as either all of them are summed again or none.
+  // Marks the rows of candidates among (or just behind) the first k that are too close to those of another row, rows
+  // of one 32-bit sum among them: what tells them apart may be too small for it.
   RTR_DEVICE bool doubtful() {
     const int n = s.n_list;
     bool doubt = false;
@@ -839,7 +857,7 @@ template <typename T, bool MASK> struct Picker {
       // behind the k-th everything is compared with that one
       const PickEntry p = s.list[s.order[min(i, a.k - 1)]], q = s.list[s.order[i + 1]];
       const int rp = p.row, rq = q.row;
-      if (rp == rq || s.sum[rp] == s.sum[rq] || (s.done[rp] && s.done[rq])) continue;
+      if (rp == rq || (s.done[rp] && s.done[rq])) continue;
       if (key_double(p.key) - key_double(q.key) >= BP_DOUBT) continue;
       s.again[rp] = s.again[rq] = 1;
       doubt = true;
@@ -847,13 +865,7 @@ template <typename T, bool MASK> struct Picker {
     return __syncthreads_or(doubt);
   }
   RTR_DEVICE void settle() {
-    bool equal = false;
-    if (tid < a.n && s.off[tid] > -INFINITY)
-      for (int q = 0; q < a.n; ++q) equal |= s.again[q] && s.sum[q] == s.sum[tid];
-    __syncthreads();
-    if (equal) s.again[tid] = 1;
     if (tid == 0) s.doubt = 1;
-    __syncthreads();
     if (a.ranks > 1) cooperative_groups::this_cluster().sync();  // the others may look
     sum_again(a.ranks);
     put_in_order();
@@ -888,6 +900,7 @@ template <typename T, bool MASK> RTR_DEVICE void pick_help(const BeamPick& a, Pi
     if (tid < a.n) {
       s.again[tid] = lead->again[tid];
       s.done[tid] = lead->done[tid];
+      s.sum[tid] = lead->sum[tid];
       s.near[tid].x = lead->near[tid].x;
     }
     __syncthreads();

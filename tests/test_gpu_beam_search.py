@@ -218,6 +218,31 @@ def test_candidates_too_close_for_32_bits(vocab):
         check_step(BeamSearch(12).select(more, same), more, same, 24, 12)
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('items,vocab', [(1, 1500), (2, 60001), (9, 70001)])
+def test_rows_that_differ_less_than_32_bits_tell(items, vocab, dtype):
+    """Beams with one score whose logits are the same but for a token that adds 3e-10 to 2e-9 to their sums: the smaller sums come
+    first, and only two that are the same in all places rank by beam."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    logits, scores = inputs(items, 5, vocab, dtype, vocab)
+    rows = logits.view(items, 5, vocab)
+    rows[:] = rows[:, :1].clone()
+    scores[:] = scores[:, :1].clone()
+    rows[:, :, 7] = -math.inf
+    lse = rows[:, 0].double().logsumexp(1)
+    for j, away in enumerate((20, 21, 22, 21, 20.5)):
+        rows[:, j, 7] = (lse - away).to(dtype)
+    sums = rows.double().logsumexp(2)
+    gaps = (sums[:, :, None] - sums[:, None]).abs()
+    assert (gaps[gaps > 1e-14] > 1e-10).all() and (gaps < 3e-9).all()
+    sums[:, 3] = sums[:, 1]  # rows that are the same, however the library adds them
+    value = rows.double() - sums[:, :, None] + scores.double()[:, :, None]
+    value, place = value.view(items, -1).sort(dim=1, descending=True, stable=True)
+    step = BeamSearch(16).select(logits, scores)
+    assert torch.equal(step.all_parents.long() * vocab + step.all_tokens.long(), place[:, :32])
+    assert ((step.all_scores.double() - value[:, :32]).abs() <= LSE + 2.0 ** -24 * value[:, :32].abs()).all()
+
+
 def test_every_call_the_same_and_captured():
     from rapidtinyrec_b200.beam_search import BeamSearch
     logits, scores = inputs(4, 20, 30011, torch.bfloat16, 8)
