@@ -11,12 +11,13 @@
 // have more); and puts what reaches the bound in order: for 100 candidates of 50 beams some 7 KB of
 // 30 MB are read again.
 //
-// Order.  Sums are fp32: in 30,720 rows of 1,000 to 2^20 logits (normal, spreads from 0 to 20, some rounded to halves) their logs were
-// off by at most 5.2e-7, those of two rows of a kind by 6.1e-7 from one another.  The 100 best of 7.6 million
-// candidates lie 1e-4 to 1e-3 apart, so now and then two are too close to tell.  Differences of logits and scores are exact enough in
-// fp64; what is not known well is the sum.  Where two neighbours of different rows are closer than BP_DOUBT, 1e-6, both rows' sums are
-// taken again in fp64 (rows whose fp32 sums are the same among them) and the list is put in order again (two rows of 152,832: 63 us more by one block, some 25 by the four that are
-// there in a batch; for one item in 100 or so): the order is that of 64-bit arithmetic, however the rows were split.
+// Order.  Sums are fp32: in 1.2 million rows of 1,000 to 2^20 logits (normal ones, and rows of one or two values or a ramp, where
+// roundings do not cancel) their logs were off by -7.2e-7 to 6.4e-7.  The 100 best of 7.6 million candidates lie 1e-4 to 1e-3 apart,
+// so now and then two are too close to tell.  Differences of logits and scores are exact enough in fp64; what is not known
+// well is the sum.  Where two neighbours of different rows are closer than BP_DOUBT, 1.5e-6, both rows' sums are taken again in fp64
+// (rows whose fp32 sums are the same among them) and the list is put in order again (two rows of 152,832: 63 us more by
+// one block, some 25 by the four that are there in a batch; for one item in 70 or so): the order is that of 64-bit arithmetic, however the
+// rows were split.
 //
 // What bounds it.  The first kernel: exponentials (XU 81 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 81 us, 5.96 TB/s;
 // without its exponentials it reads at 7.3 TB/s.  An eighth or a quarter of them on the FMA pipe instead: no change, and 3 us slower.
@@ -45,7 +46,7 @@ constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
 constexpr int BP_GROUPS = 512, BP_LANES = 1024, BP_LIST = 1024;  // groups, lanes of them and candidates that it takes up at once
 constexpr int BP_HELD = 4;                      // quartets of groups that a thread of it holds
 constexpr int BP_RANKS = 4;                     // blocks that sum an item's doubtful rows together
-constexpr double BP_DOUBT = 1e-6;               // candidates of different rows that are closer are looked at again
+constexpr double BP_DOUBT = 1.5e-6;             // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
 struct BeamPick {
@@ -234,7 +235,9 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
   }
   if (slice == a.slices - 1 && tid < a.padded - a.groups) best[a.groups + tid] = -INFINITY;
   float base = -INFINITY;
-  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  // A group's exponentials are added to one another, and that to the running sum with what the last such addition lost (all in one
+  // running sum: rows of 152,832 of one value off by up to 1.3e-6; no faster).
+  float2 sum = make_float2(0.f, 0.f), lost = sum;
   const float2 log2e = make_float2(BP_LOG2E, BP_LOG2E);
   const auto take = [&](const L& raw, const Allowed<T>& ok, int g) {
     float mine = raw.largest();
@@ -252,8 +255,8 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
     }
     if (top > base) {  // the same in all lanes
       const float f = ex2(beam_near(base) && beam_near(top) ? beam_unit(base) - beam_unit(top) : (base - top) * BP_LOG2E);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * f, sum[i].y * f);
+      sum = make_float2(sum.x * f, sum.y * f);
+      lost = make_float2(lost.x * f, lost.y * f);
       base = top;
     }
     // 2^(x log2(e) - unit), unit = base log2(e) rounded (made up for at the end); near the ends of float's range,
@@ -261,15 +264,20 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
     if (beam_near(base)) {
       const float unit = beam_unit(base);
       const float2 minus = make_float2(-unit, -unit);
+      const float2 less = make_float2(-1.f, -1.f);
+      float2 part[2];
 #pragma unroll
       for (int i = 0; i < L::EACH / 2; ++i) {
-        const float2 y = __ffma2_rn(raw.two(i), log2e, minus);
-        sum[i & 1] = __fadd2_rn(sum[i & 1], make_float2(ex2(y.x), ex2(y.y)));
+        const float2 y = __ffma2_rn(raw.two(i), log2e, minus), e = make_float2(ex2(y.x), ex2(y.y));
+        part[i & 1] = i < 2 ? e : __fadd2_rn(part[i & 1], e);
       }
+      const float2 more = __fadd2_rn(__fadd2_rn(part[0], part[1]), lost), now = __fadd2_rn(sum, more);
+      lost = __ffma2_rn(__ffma2_rn(sum, less, now), less, more);
+      sum = now;
     } else {
       const float zero = base == -INFINITY ? 0.f : base;
 #pragma unroll
-      for (int i = 0; i < L::EACH; ++i) sum[0].x += ex2((raw.one(i) - zero) * BP_LOG2E);
+      for (int i = 0; i < L::EACH; ++i) sum.x += ex2((raw.one(i) - zero) * BP_LOG2E);
     }
   };
   // the warp's groups that are all there, and before and behind them those at the row's ends
@@ -318,7 +326,7 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
     if constexpr (MASK) ok.load(allowed, g * GROUP - shift, lane, a.vocab, by);
     take(raw, ok, g);
   }
-  float total = warp_sum((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y));
+  float total = warp_sum((sum.x + sum.y) + (lost.x + lost.y));
   if (beam_near(base)) total *= ex2(-fmaf(base, BP_LOG2E, -beam_unit(base)));
   const auto sums = [&](int w) -> float2& { return *reinterpret_cast<float2*>(ring[w]); };  // nothing is under way any more
   if (lane == 0) sums(warp) = make_float2(base, total);
@@ -1067,7 +1075,7 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.next_parents = step->next_parents;
   p.next_scores = step->next_scores;
   p.status = step->status;
-  // Where there are eight items or more, of two rows at least (one row is never in doubt), an item is in doubt now and then (one in 100
+  // Where there are eight items or more, of two rows at least (one row is never in doubt), an item is in doubt now and then (one in 70
   // or so), and summing its rows takes one block long where they are long (65,536 logits 14 us each): its block has others of a
   // cluster beside it, on SMs that have no item.  (16 items of 10 rows of 32,003 without doubts: 14.7 us with one block each, 15.7
   // with four.)

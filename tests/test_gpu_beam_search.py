@@ -218,6 +218,27 @@ def test_candidates_too_close_for_32_bits(vocab):
         check_step(BeamSearch(12).select(more, same), more, same, 24, 12)
 
 
+@pytest.mark.parametrize('seed', range(4))
+@pytest.mark.parametrize('vocab', [5003, 152833, 1 << 20])
+def test_candidates_too_close_in_rows_of_few_values(vocab, seed):
+    """The same where a row's other logits have one value, so that the roundings of its sum do not cancel."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    g = generator(vocab + seed)
+    n = 6
+    logits = (-6 - torch.rand(n, 1, generator=g, device='cuda')).expand(n, vocab).clone()
+    at = torch.randperm(vocab, generator=g, device='cuda')[:12]
+    best = 0.3 * torch.rand(12, generator=g, device='cuda').double()
+    apart = (torch.rand(n, 12, generator=g, device='cuda').double() - 0.5) * 6e-7
+    scores = (-0.01 * torch.arange(n, device='cuda').float())[None]
+    for _ in range(40):
+        lse = torch.logsumexp(logits.double(), 1, keepdim=True)
+        logits[:, at] = (best + apart + lse - lse[:1] - scores.double().t()).float()
+    value = plain_select(logits, scores, 24, 12)[2]
+    gaps = value[0, :-1] - value[0, 1:]
+    assert (gaps < 1e-6).sum() >= 15 and (gaps[gaps > 0] > 1e-12).all()
+    check_step(BeamSearch(12).select(logits, scores), logits, scores, 24, 12)
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('items,vocab', [(1, 1500), (2, 60001), (9, 70001)])
 def test_rows_that_differ_less_than_32_bits_tell(items, vocab, dtype):
