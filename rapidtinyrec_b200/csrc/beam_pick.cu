@@ -61,7 +61,7 @@ struct BeamPick {
   int ranks;               // blocks of the second kernel's clusters
   float* best;             // [items * n][padded]: a group's largest allowed logit
   uint32_t* second;        // likewise: the largest of the other lanes' (rounded up) and, in the last five bits, whose the first is
-  float2* part;            // [items * n][slices]: maximum, sum of exponentials relative to it
+  float2* part;            // [items * n][slices]: maximum, sum of exponentials relative to beam_reference of it
   int32_t *all_tokens, *all_parents, *next_tokens, *next_parents;
   float *all_scores, *next_scores;
   uint32_t* status;
@@ -73,9 +73,28 @@ RTR_DEVICE float redux_max(float v) {  // NaN counts as nothing
   return r;
 }
 
-// What a sum is relative to while it grows, in units of log2.
-RTR_DEVICE bool beam_near(float base) { return fabsf(base) < 1e37f; }
-RTR_DEVICE float beam_unit(float base) { return __fmul_rn(base, BP_LOG2E); }
+// What a sum of exponentials with the largest logit `base` is relative to, as a power of two.  Where base is within 2^21 that is
+// a whole number near base log2(e): exponents are x log2(e) less it, by one rounding of what is left, and sums change from one
+// to another by exact powers of two.  Beyond (all of a slice masked by -1e10, say) the rounding of base log2(e) itself would be what is
+// left, so there the difference x - base comes first, which is exact wherever it counts: such logits are a quarter apart at least.
+constexpr float BP_NEAR = 0x1p21f;
+RTR_DEVICE bool beam_near(float base) { return fabsf(base) < BP_NEAR; }
+RTR_DEVICE float beam_unit(float base) {
+  const float whole = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers
+  return __fadd_rn(__fmaf_rn(fmaxf(base, -BP_NEAR), BP_LOG2E, whole), -whole);
+}
+RTR_DEVICE double beam_reference(float base) { return beam_near(base) ? beam_unit(base) : (double)base * BP_LOG2E; }
+// A sum of `base` times this is one of `top`, another and larger base: of two that are near (a base below -2^21 as if it were that),
+// and of any.
+RTR_DEVICE float beam_power(float d) { return d < -126.f ? 0.f : __int_as_float((127 + (int)d) << 23); }  // 2^d, d a whole number
+RTR_DEVICE float beam_near_scale(float base, float top) { return beam_power(beam_unit(base) - beam_unit(top)); }
+__device__ __noinline__ float beam_far_scale(float base, float top) {
+  return base == -INFINITY ? 0.f : ex2((float)(beam_reference(base) - beam_reference(top)));
+}
+RTR_DEVICE float beam_relative(const float2& part, float top) {  // part: a base and its sum
+  if (part.x == top || part.y == 0.f) return part.y;
+  return part.y * (beam_near(part.x) && beam_near(top) ? beam_near_scale(part.x, top) : beam_far_scale(part.x, top));
+}
 
 // A piece of 16 bytes at a row's ragged ends, of which some logits are not there.  Out of line: the code that a
 // kernel goes through once comes from L2 at some 500 cycles a line.
@@ -210,6 +229,21 @@ template <typename T> struct Allowed {
   }
 };
 
+// The sum of the exponentials of a warp's groups relative to m, the slice's largest logit, where that is beyond 2^21.
+template <typename T> __device__ __noinline__ float beam_far_sum(const T* row, float m, int g, int hi, int vocab) {
+  using L = Logits<T>;
+  float sum = 0.f;
+  for (; g < hi; g += BP_WARPS) {
+    L raw;
+    raw.load(row, g * L::GROUP - L::shift(row), threadIdx.x & 31, vocab);
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < L::EACH; ++i) part[i % 4] += ex2((raw.one(i) - m) * BP_LOG2E);
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
+  }
+  return warp_sum(sum);
+}
+
 // One block: a slice of a row's groups, which its warps take in turn.  The groups that are all there come through a ring in shared
 // memory of each warp's own, every lane's pieces copied by the lane that reads them: 6 KB a warp keep 192 KB an SM on their way without
 // a register (two groups in registers, one read while the other comes, 24 warps an SM: 110 us instead of 96 for 32 x 50 rows of bf16 and
@@ -234,7 +268,7 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
     return;
   }
   if (slice == a.slices - 1 && tid < a.padded - a.groups) best[a.groups + tid] = -INFINITY;
-  float base = -INFINITY;
+  float base = -INFINITY, unit = beam_unit(base);
   // A group's exponentials are added to one another, and that to the running sum with what the last such addition lost (all in one
   // running sum: rows of 152,832 of one value off by up to 1.3e-6; no faster).
   float2 sum = make_float2(0.f, 0.f), lost = sum;
@@ -253,32 +287,23 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
       best[g] = most;
       a.second[(int64_t)row * a.padded + g] = beam_second(other, whose & 31);
     }
-    if (top > base) {  // the same in all lanes
-      const float f = ex2(beam_near(base) && beam_near(top) ? beam_unit(base) - beam_unit(top) : (base - top) * BP_LOG2E);
+    if (top > base) {  // the same in all lanes.  (Beyond 2^21 what is summed means nothing: see the end.)
+      base = top;
+      const float to = beam_unit(base), f = beam_power(unit - to);
+      unit = to;
       sum = make_float2(sum.x * f, sum.y * f);
       lost = make_float2(lost.x * f, lost.y * f);
-      base = top;
     }
-    // 2^(x log2(e) - unit), unit = base log2(e) rounded (made up for at the end); near the ends of float's range,
-    // where that product is infinite, the difference comes first
-    if (beam_near(base)) {
-      const float unit = beam_unit(base);
-      const float2 minus = make_float2(-unit, -unit);
-      const float2 less = make_float2(-1.f, -1.f);
-      float2 part[2];
+    const float2 minus = make_float2(-unit, -unit), less = make_float2(-1.f, -1.f);
+    float2 part[2];
 #pragma unroll
-      for (int i = 0; i < L::EACH / 2; ++i) {
-        const float2 y = __ffma2_rn(raw.two(i), log2e, minus), e = make_float2(ex2(y.x), ex2(y.y));
-        part[i & 1] = i < 2 ? e : __fadd2_rn(part[i & 1], e);
-      }
-      const float2 more = __fadd2_rn(__fadd2_rn(part[0], part[1]), lost), now = __fadd2_rn(sum, more);
-      lost = __ffma2_rn(__ffma2_rn(sum, less, now), less, more);
-      sum = now;
-    } else {
-      const float zero = base == -INFINITY ? 0.f : base;
-#pragma unroll
-      for (int i = 0; i < L::EACH; ++i) sum.x += ex2((raw.one(i) - zero) * BP_LOG2E);
+    for (int i = 0; i < L::EACH / 2; ++i) {
+      const float2 y = __ffma2_rn(raw.two(i), log2e, minus), e = make_float2(ex2(y.x), ex2(y.y));
+      part[i & 1] = i < 2 ? e : __fadd2_rn(part[i & 1], e);
     }
+    const float2 more = __fadd2_rn(__fadd2_rn(part[0], part[1]), lost), now = __fadd2_rn(sum, more);
+    lost = __ffma2_rn(__ffma2_rn(sum, less, now), less, more);
+    sum = now;
   };
   // the warp's groups that are all there, and before and behind them those at the row's ends
   const int end = min(hi, (int)(((int64_t)a.vocab + shift) / GROUP));
@@ -326,18 +351,22 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
     if constexpr (MASK) ok.load(allowed, g * GROUP - shift, lane, a.vocab, by);
     take(raw, ok, g);
   }
-  float total = warp_sum((sum.x + sum.y) + (lost.x + lost.y));
-  if (beam_near(base)) total *= ex2(-fmaf(base, BP_LOG2E, -beam_unit(base)));
+  const float total = warp_sum((sum.x + sum.y) + (lost.x + lost.y));
   const auto sums = [&](int w) -> float2& { return *reinterpret_cast<float2*>(ring[w]); };  // nothing is under way any more
   if (lane == 0) sums(warp) = make_float2(base, total);
   __syncthreads();
-  if (tid == 0) {
-    float m = -INFINITY, t = 0.f;
-#pragma unroll
-    for (int w = 0; w < BP_WARPS; ++w) m = fmaxf(m, sums(w).x);
-#pragma unroll
-    for (int w = 0; w < BP_WARPS; ++w) t += sums(w).x == m ? sums(w).y : sums(w).y * ex2((sums(w).x - m) * BP_LOG2E);
-    a.part[blockIdx.x] = make_float2(m, t);
+  // a slice whose largest logit is beyond 2^21 is read once more
+  const float m = redux_max(lane < BP_WARPS ? sums(lane).x : -INFINITY);
+  if (!beam_near(m) && m > -INFINITY) {
+    __syncthreads();
+    const float far = beam_far_sum(x, m, lo + warp, hi, a.vocab);
+    if (lane == 0) sums(warp) = make_float2(m, far);
+    __syncthreads();
+  }
+  if (warp == 0) {
+    const float2 u = lane < BP_WARPS ? sums(lane) : make_float2(-INFINITY, 0.f);
+    const float t = warp_sum(u.x == m ? u.y : u.y * beam_near_scale(u.x, m));
+    if (lane == 0) a.part[blockIdx.x] = make_float2(m, t);
   }
 }
 
@@ -530,43 +559,36 @@ template <typename T, bool MASK> struct Picker {
     s.list[to].at = (uint32_t)r * a.vocab + v;
   }
 
-  // A sum relative to its maximum as one relative to a larger one.
-  RTR_DEVICE static float relative(const float2& part, float top) {
-    return part.x == top ? part.y : part.y * ex2((part.x - top) * BP_LOG2E);
-  }
-  // Each row's sum from its slices, and what its candidates are offset by: eight lanes a row.
+  // Each row's sum from its slices, and what its candidates are offset by: 8 to 32 lanes a row.
   RTR_DEVICE void offsets() {
     static_assert(BP_MAX_N * 8 == BP_THREADS, "a row for every eight threads");
-    const int r = tid >> 3, part = tid & 7;
+    const int bits = a.n > 64 ? 3 : a.n > 32 ? 4 : 5, lanes = 1 << bits, r = tid >> bits, part = tid & (lanes - 1);
     const bool there = r < a.n;
     const float score = there && part == 0 ? a.scores[item * a.n + r] : -INFINITY;
     const float2* p = a.part + ((int64_t)item * a.n + (there ? r : 0)) * a.slices;
-    const float2 none = make_float2(-INFINITY, 0.f);
-    const float2 u = there && part < a.slices ? __ldcg(p + part) : none, v = there && part + 8 < a.slices ? __ldcg(p + part + 8) : none;
-    float m = fmaxf(u.x, v.x), sum = relative(u, m) + relative(v, m);
-    for (int i = part + 16; there && i < a.slices; i += 8) {
-      const float2 w = __ldcg(p + i);
-      const float top = fmaxf(m, w.x);
-      sum = relative(make_float2(m, sum), top) + relative(w, top);
-      m = top;
-    }
-    float all = m;
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
-    double t = relative(make_float2(m, sum), all);
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    const float2 u = there && part < a.slices ? __ldcg(p + part) : make_float2(-INFINITY, 0.f);
+    float all = u.x;
+    for (int i = part + lanes; there && i < a.slices; i += lanes) all = fmaxf(all, __ldcg(&p[i].x));
+#pragma unroll 1
+    for (int d = 1; d < lanes; d <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
+    double t = beam_relative(u, all);
+#pragma unroll 1
+    for (int i = part + lanes; there && i < a.slices; i += lanes) t += beam_relative(__ldcg(p + i), all);
+#pragma unroll 1
+    for (int d = 1; d < lanes; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
     if (tid == 0) s.most = 0;
     __syncthreads();
     if (there && part == 0) {
       const bool wrong = !(score < INFINITY) || (score > -INFINITY && !(t >= 0.0 && all < INFINITY));
       if (wrong) atomicOr(a.status, RTR_DEV_NAN_SCORE);
       const bool alive = !wrong && score > -INFINITY && all > -INFINITY;
-      // log t = exponent log 2 + log of the rest, which is 0.75 to 1.5: a float has that to 2^-25 or so
+      // log t = exponent log 2 + log of the rest, which is 0.75 to 1.5: a float has that to 2^-25 or so.  (t is relative to a power
+      // of two; the sum to the maximum.)
       const float rounded = (float)t;
       const int e = alive ? (int)(__float_as_uint(rounded) - 0x3f400000u) >> 23 : 0;
+      const double unit = alive ? beam_reference(all) - (double)all * BP_LOG2E : 0.0;
       const float rest = alive ? __uint_as_float(__float_as_uint(rounded) - ((uint32_t)e << 23)) : 1.f;
-      s.sum[r] = alive ? e * 0.69314718055994530942 + (double)(logf(rest) + (float)(t - (double)rounded) / rounded) : 0.0;
+      s.sum[r] = alive ? (e + unit) * 0.69314718055994530942 + (double)(logf(rest) + (float)(t - (double)rounded) / rounded) : 0.0;
       s.off[r] = alive ? (double)score - s.sum[r] : -INFINITY;
       s.near[r] = make_float2(all, (float)s.off[r]);
       s.again[r] = s.done[r] = 0;
