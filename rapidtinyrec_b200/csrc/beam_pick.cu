@@ -11,14 +11,13 @@
 // have more); and puts what reaches the bound in order: for 100 candidates of 50 beams some 7 KB of
 // 30 MB are read again.
 //
-// Order.  Sums are fp32: in 1.2 million rows of 1,000 to 2^20 logits (normal ones, and rows of one or two values or a ramp, where
-// roundings do not cancel) their logs were off by -7.2e-7 to 6.4e-7.  The 100 best of 7.6 million candidates lie 1e-4 to 1e-3 apart,
-// so now and then two are too close to tell.  Differences of logits and scores are exact enough in fp64; what is not known
-// well is the sum.  Where two neighbours of different rows are closer than BP_DOUBT, 1.5e-6, both rows' sums are taken again in fp64
-// (rows whose fp32 sums are the same among them) and the list is put in order again (two rows of 152,832: 63 us more by
-// one block, some 25 by the four that are there in a batch; for one item in 70 or so): the order is that of 64-bit arithmetic, however the
-// rows were split.
-//
+// Order.  Sums are fp32, their logs off by some 1e-6 at most (beam_close has the bound; in 27,648 rows of 1,000 to 2^20 logits, normal ones,
+// ramps and rows of one or two values among them, by -5.2e-7 to 3.1e-7).  The 100 best of
+// 7.6 million candidates lie 1e-4 to 1e-3 apart, so now and then two are too close to tell.  Differences of logits and scores are exact
+// enough in fp64; what is not known well is the sum.  Where two neighbours of different rows are closer than BeamPick::close, twice that
+// bound, both rows' sums are taken again in fp64 (rows whose fp32 sums are the same among them) and the list is put in order
+// again (two rows of 152,832: 63 us more by one block, some 25 by the four that are there in a batch; for one item in 80 or so): the
+// order is that of 64-bit arithmetic, however the rows were split.
 // What bounds it.  The first kernel: exponentials (XU 81 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 81 us, 5.96 TB/s;
 // without its exponentials it reads at 7.3 TB/s.  An eighth or a quarter of them on the FMA pipe instead: no change, and 3 us slower.
 // The second: latency, some 17,000 cycles, 8.5 us, for 50 beams: dependent loads (slices and groups, second bests, lanes' logits; 700
@@ -29,6 +28,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "engine.h"
@@ -46,7 +46,6 @@ constexpr int BP_MAX_N = 128, BP_MAX_K = 256;
 constexpr int BP_GROUPS = 512, BP_LANES = 1024, BP_LIST = 1024;  // groups, lanes of them and candidates that it takes up at once
 constexpr int BP_HELD = 4;                      // quartets of groups that a thread of it holds
 constexpr int BP_RANKS = 4;                     // blocks that sum an item's doubtful rows together
-constexpr double BP_DOUBT = 1.5e-6;             // candidates of different rows that are closer are looked at again
 constexpr float BP_LOG2E = 1.4426950408889634f;
 
 struct BeamPick {
@@ -58,10 +57,11 @@ struct BeamPick {
   int groups, padded;      // groups of a row, and their number rounded up to 4
   uint32_t quarter_inv;    // ceil(2^32 / (padded / 4)): a group quartet's row by one multiplication (0: 2^32, the quartet itself)
   int slices;              // blocks of a row
+  float close;             // see beam_close
   int ranks;               // blocks of the second kernel's clusters
   float* best;             // [items * n][padded]: a group's largest allowed logit
   uint32_t* second;        // likewise: the largest of the other lanes' (rounded up) and, in the last five bits, whose the first is
-  float2* part;            // [items * n][slices]: maximum, sum of exponentials relative to beam_reference of it
+  float2* part;            // [items * n][slices]: maximum, sum of exponentials relative to 2^beam_unit of it, or to it
   int32_t *all_tokens, *all_parents, *next_tokens, *next_parents;
   float *all_scores, *next_scores;
   uint32_t* status;
@@ -74,26 +74,55 @@ RTR_DEVICE float redux_max(float v) {  // NaN counts as nothing
 }
 
 // What a sum of exponentials with the largest logit `base` is relative to, as a power of two.  Where base is within 2^21 that is
-// a whole number near base log2(e): exponents are x log2(e) less it, by one rounding of what is left, and sums change from one
-// to another by exact powers of two.  Beyond (all of a slice masked by -1e10, say) the rounding of base log2(e) itself would be what is
-// left, so there the difference x - base comes first, which is exact wherever it counts: such logits are a quarter apart at least.
+// the whole number nearest to base log2(e), less 8: exponents are x log2(e) less it, rounded once as what is left (which is least
+// about 0, so that is put where the many are and not at the best), and sums change from one to another by exact powers of two.
+// Beyond (all of a slice masked by -1e10, say) the rounding of base log2(e) itself would be what is left, so there the difference x - base
+// comes first, which is exact wherever it counts: such logits are a quarter apart at least.
 constexpr float BP_NEAR = 0x1p21f;
 RTR_DEVICE bool beam_near(float base) { return fabsf(base) < BP_NEAR; }
 RTR_DEVICE float beam_unit(float base) {
   const float whole = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers
-  return __fadd_rn(__fmaf_rn(fmaxf(base, -BP_NEAR), BP_LOG2E, whole), -whole);
+  return __fadd_rn(__fmaf_rn(fmaxf(base, -BP_NEAR), BP_LOG2E, whole), -whole - 8.f);
 }
-RTR_DEVICE double beam_reference(float base) { return beam_near(base) ? beam_unit(base) : (double)base * BP_LOG2E; }
+RTR_DEVICE double beam_offset(float base) { return beam_near(base) ? beam_unit(base) - (double)base * BP_LOG2E : 0.0; }
 // A sum of `base` times this is one of `top`, another and larger base: of two that are near (a base below -2^21 as if it were that),
 // and of any.
 RTR_DEVICE float beam_power(float d) { return d < -126.f ? 0.f : __int_as_float((127 + (int)d) << 23); }  // 2^d, d a whole number
 RTR_DEVICE float beam_near_scale(float base, float top) { return beam_power(beam_unit(base) - beam_unit(top)); }
 __device__ __noinline__ float beam_far_scale(float base, float top) {
-  return base == -INFINITY ? 0.f : ex2((float)(beam_reference(base) - beam_reference(top)));
+  return (float)exp2(((double)base - top) * 1.4426950408889634 + beam_offset(base) - beam_offset(top));
 }
 RTR_DEVICE float beam_relative(const float2& part, float top) {  // part: a base and its sum
   if (part.x == top || part.y == 0.f) return part.y;
   return part.y * (beam_near(part.x) && beam_near(top) ? beam_near_scale(part.x, top) : beam_far_scale(part.x, top));
+}
+// e^d for d from -100 to 0: e^(n log 2 + f) with n the nearest whole number, f at most 0.347 and e^f its Taylor series up to f^10 / 10!
+// (off by 2.2e-13 at most).  Sixteen fp64 operations with the subtraction and the sum; exp() made two rows of 152,704 take 95 us.
+RTR_DEVICE double exp_of(double d) {
+  const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to whole numbers, in the low bits
+  const double z = fma(d, 1.4426950408889634, whole), n = z - whole, f = fma(n, -0.69314718055994531, d);
+  double e = 1.0 / 3628800.0;
+  e = fma(e, f, 1.0 / 362880.0);
+  e = fma(e, f, 1.0 / 40320.0);
+  e = fma(e, f, 1.0 / 5040.0);
+  e = fma(e, f, 1.0 / 720.0);
+  e = fma(e, f, 1.0 / 120.0);
+  e = fma(e, f, 1.0 / 24.0);
+  e = fma(e, f, 1.0 / 6.0);
+  e = fma(e, f, 0.5);
+  e = fma(e, f, 1.0);
+  e = fma(e, f, 1.0);
+  return __hiloint2double(__double2hiint(e) + (__double2loint(z) << 20), __double2loint(e));
+}
+
+struct BeamSum {
+  double sum;
+  float base;
+};
+RTR_DEVICE double beam_warp_sum(double v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
 }
 
 // A piece of 16 bytes at a row's ragged ends, of which some logits are not there.  Out of line: the code that a
@@ -230,18 +259,19 @@ template <typename T> struct Allowed {
 };
 
 // The sum of the exponentials of a warp's groups relative to m, the slice's largest logit, where that is beyond 2^21.
-template <typename T> __device__ __noinline__ float beam_far_sum(const T* row, float m, int g, int hi, int vocab) {
+template <typename T> __device__ __noinline__ double beam_far_sum(const T* row, float m, int g, int hi, int vocab) {
   using L = Logits<T>;
-  float sum = 0.f;
+  double sum = 0.0;
   for (; g < hi; g += BP_WARPS) {
     L raw;
     raw.load(row, g * L::GROUP - L::shift(row), threadIdx.x & 31, vocab);
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < L::EACH; ++i) part[i % 4] += ex2((raw.one(i) - m) * BP_LOG2E);
-    sum += (part[0] + part[1]) + (part[2] + part[3]);
+    for (int i = 0; i < L::EACH; ++i) {
+      const float d = raw.one(i) - m;
+      sum += d == d ? exp_of(fmax((double)d, -100.0)) : (double)d;  // below e^-100 nothing counts: 2^20 of them are 2^-124 of the sum
+    }
   }
-  return warp_sum(sum);
+  return beam_warp_sum(sum);
 }
 
 // One block: a slice of a row's groups, which its warps take in turn.  The groups that are all there come through a ring in shared
@@ -269,8 +299,8 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
   }
   if (slice == a.slices - 1 && tid < a.padded - a.groups) best[a.groups + tid] = -INFINITY;
   float base = -INFINITY, unit = beam_unit(base);
-  // A group's exponentials are added to one another, and that to the running sum with what the last such addition lost (all in one
-  // running sum: rows of 152,832 of one value off by up to 1.3e-6; no faster).
+  // A group's exponentials are added to one another, and that to the running sum; what these additions lose is a sum of its
+  // own (all in one running sum: rows of 152,832 of one value off by up to 1.3e-6; no faster).
   float2 sum = make_float2(0.f, 0.f), lost = sum;
   const float2 log2e = make_float2(BP_LOG2E, BP_LOG2E);
   const auto take = [&](const L& raw, const Allowed<T>& ok, int g) {
@@ -295,14 +325,14 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
       lost = make_float2(lost.x * f, lost.y * f);
     }
     const float2 minus = make_float2(-unit, -unit), less = make_float2(-1.f, -1.f);
-    float2 part[2];
+    float2 part[4];
 #pragma unroll
     for (int i = 0; i < L::EACH / 2; ++i) {
       const float2 y = __ffma2_rn(raw.two(i), log2e, minus), e = make_float2(ex2(y.x), ex2(y.y));
-      part[i & 1] = i < 2 ? e : __fadd2_rn(part[i & 1], e);
+      part[i & 3] = i < 4 ? e : __fadd2_rn(part[i & 3], e);
     }
-    const float2 more = __fadd2_rn(__fadd2_rn(part[0], part[1]), lost), now = __fadd2_rn(sum, more);
-    lost = __ffma2_rn(__ffma2_rn(sum, less, now), less, more);
+    const float2 more = __fadd2_rn(__fadd2_rn(part[0], part[1]), __fadd2_rn(part[2], part[3])), now = __fadd2_rn(sum, more);
+    lost = __fadd2_rn(lost, __ffma2_rn(__ffma2_rn(sum, less, now), less, more));
     sum = now;
   };
   // the warp's groups that are all there, and before and behind them those at the row's ends
@@ -351,22 +381,22 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
     if constexpr (MASK) ok.load(allowed, g * GROUP - shift, lane, a.vocab, by);
     take(raw, ok, g);
   }
-  const float total = warp_sum((sum.x + sum.y) + (lost.x + lost.y));
-  const auto sums = [&](int w) -> float2& { return *reinterpret_cast<float2*>(ring[w]); };  // nothing is under way any more
-  if (lane == 0) sums(warp) = make_float2(base, total);
+  const double total = beam_warp_sum(((double)sum.x + sum.y) + ((double)lost.x + lost.y));
+  const auto sums = [&](int w) -> BeamSum& { return *reinterpret_cast<BeamSum*>(ring[w]); };  // nothing is under way any more
+  if (lane == 0) sums(warp) = BeamSum{total, base};
   __syncthreads();
   // a slice whose largest logit is beyond 2^21 is read once more
-  const float m = redux_max(lane < BP_WARPS ? sums(lane).x : -INFINITY);
+  const float m = redux_max(lane < BP_WARPS ? sums(lane).base : -INFINITY);
   if (!beam_near(m) && m > -INFINITY) {
     __syncthreads();
-    const float far = beam_far_sum(x, m, lo + warp, hi, a.vocab);
-    if (lane == 0) sums(warp) = make_float2(m, far);
+    const double far = beam_far_sum(x, m, lo + warp, hi, a.vocab);
+    if (lane == 0) sums(warp) = BeamSum{far, m};
     __syncthreads();
   }
   if (warp == 0) {
-    const float2 u = lane < BP_WARPS ? sums(lane) : make_float2(-INFINITY, 0.f);
-    const float t = warp_sum(u.x == m ? u.y : u.y * beam_near_scale(u.x, m));
-    if (lane == 0) a.part[blockIdx.x] = make_float2(m, t);
+    const BeamSum u = lane < BP_WARPS ? sums(lane) : BeamSum{0.0, -INFINITY};
+    const double t = beam_warp_sum(u.base == m ? u.sum : u.sum * beam_near_scale(u.base, m));
+    if (lane == 0) a.part[blockIdx.x] = make_float2(m, (float)t);
   }
 }
 
@@ -378,25 +408,6 @@ RTR_DEVICE uint64_t double_key(double d) {
 }
 RTR_DEVICE double key_double(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
-}
-
-// e^d for d from -100 to 0: e^(n log 2 + f) with n the nearest whole number, f at most 0.347 and e^f its Taylor series up to f^10 / 10!
-// (off by 2.2e-13 at most).  Sixteen fp64 operations with the subtraction and the sum; exp() made two rows of 152,704 take 95 us.
-RTR_DEVICE double exp_of(double d) {
-  const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to whole numbers, in the low bits
-  const double z = fma(d, 1.4426950408889634, whole), n = z - whole, f = fma(n, -0.69314718055994531, d);
-  double e = 1.0 / 3628800.0;
-  e = fma(e, f, 1.0 / 362880.0);
-  e = fma(e, f, 1.0 / 40320.0);
-  e = fma(e, f, 1.0 / 5040.0);
-  e = fma(e, f, 1.0 / 720.0);
-  e = fma(e, f, 1.0 / 120.0);
-  e = fma(e, f, 1.0 / 24.0);
-  e = fma(e, f, 1.0 / 6.0);
-  e = fma(e, f, 0.5);
-  e = fma(e, f, 1.0);
-  e = fma(e, f, 1.0);
-  return __hiloint2double(__double2hiint(e) + (__double2loint(z) << 20), __double2loint(e));
 }
 
 struct PickEntry {  // a candidate in order: larger keys first, then lower places
@@ -586,7 +597,7 @@ template <typename T, bool MASK> struct Picker {
       // of two; the sum to the maximum.)
       const float rounded = (float)t;
       const int e = alive ? (int)(__float_as_uint(rounded) - 0x3f400000u) >> 23 : 0;
-      const double unit = alive ? beam_reference(all) - (double)all * BP_LOG2E : 0.0;
+      const double unit = alive ? beam_offset(all) : 0.0;
       const float rest = alive ? __uint_as_float(__float_as_uint(rounded) - ((uint32_t)e << 23)) : 1.f;
       s.sum[r] = alive ? (e + unit) * 0.69314718055994530942 + (double)(logf(rest) + (float)(t - (double)rounded) / rounded) : 0.0;
       s.off[r] = alive ? (double)score - s.sum[r] : -INFINITY;
@@ -664,7 +675,7 @@ template <typename T, bool MASK> struct Picker {
   }
 
   // What `near` may be off by (three roundings of 2^-24), with room, and what two sums may be.
-  RTR_DEVICE float slack(float t) const { return (float)BP_DOUBT + 4.77e-7f * (__int_as_float(s.most) + fabsf(t)); }
+  RTR_DEVICE float slack(float t) const { return a.close + 4.77e-7f * (__int_as_float(s.most) + fabsf(t)); }
 
   // What the rows' logits have to reach for `near` to reach t, with room for its roundings.
   RTR_DEVICE void needs(float t) {
@@ -888,7 +899,7 @@ template <typename T, bool MASK> struct Picker {
       const PickEntry p = s.list[s.order[min(i, a.k - 1)]], q = s.list[s.order[i + 1]];
       const int rp = p.row, rq = q.row;
       if (rp == rq || (s.done[rp] && s.done[rq])) continue;
-      if (key_double(p.key) - key_double(q.key) >= BP_DOUBT) continue;
+      if (key_double(p.key) - key_double(q.key) >= a.close) continue;
       s.again[rp] = s.again[rq] = 1;
       doubt = true;
     }
@@ -1028,6 +1039,21 @@ static const char* beam_check(const rtr_beam_step* b) {
   return nullptr;
 }
 
+// Values of different rows may be told wrong by their sums of 32 bits where they are closer than this: twice what the log of one
+// such sum may be off by, whatever the logits.  In units of 2^-24:
+//  - exponents y round by |y| at most, and |y| <= 8.5 + max(0, D - 16) with D the distance from the row's maximum in units of log2.  The
+//    mean of that over a row, whose weights are 2^-D / sum, is at most 9.95 + max(0, log2(vocab) - 17.44): where w of the weight lies beyond
+//    16, the mean of D there is at most log2(vocab) - log2(w), since nothing over vocab places has an entropy above log(vocab).  Times log 2;
+//  - a group's additions: 3 + 2 in bf16, 1 + 2 in fp32, and twice one where a group is more than all before it;
+//  - a slice's sum rounded to a float: 1; the logarithm of the rest: 0.75.
+// And what errs to one side, once: ex2.approx is off by -1.45e-7 to 1.46e-7 (all floats from -40 to 40 measured), log2(e) as a float by
+// 1.34e-8 of the exponent.  (Slices beyond 2^21 are summed in 64 bits.)  For 152,832 logits 2.3e-6 in bf16, 2.1e-6 in fp32.
+static float beam_close(int vocab, bool fp32) {
+  const float spread = std::log((float)vocab);
+  const float one = 6.9f + std::max(0.f, spread - 12.08f) + (fp32 ? 3.f : 5.f) + 2.f + 1.75f;
+  return 2.f * 5.97e-8f * one + 2.92e-7f + 1.34e-8f * spread;
+}
+
 // Groups of a row (one more where it starts in the middle of one), slices, and the workspace they need.
 static void beam_plan(const rtr_beam_step* b, int sms, BeamPick& p, int64_t& groups_bytes, int64_t& bytes) {
   const int per = b->dtype == RTR_DTYPE_F32 ? 4 : 8;
@@ -1087,6 +1113,7 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.k = step->k;
   p.beams = step->beams;
   p.eos = step->eos < 0 ? -1 : step->eos;
+  p.close = beam_close(step->vocab, step->dtype == RTR_DTYPE_F32);
   p.best = static_cast<float*>(workspace);
   p.second = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + best);
   p.part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 2 * best);
@@ -1097,7 +1124,7 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.next_parents = step->next_parents;
   p.next_scores = step->next_scores;
   p.status = step->status;
-  // Where there are eight items or more, of two rows at least (one row is never in doubt), an item is in doubt now and then (one in 70
+  // Where there are eight items or more, of two rows at least (one row is never in doubt), an item is in doubt now and then (one in 80
   // or so), and summing its rows takes one block long where they are long (65,536 logits 14 us each): its block has others of a
   // cluster beside it, on SMs that have no item.  (16 items of 10 rows of 32,003 without doubts: 14.7 us with one block each, 15.7
   // with four.)

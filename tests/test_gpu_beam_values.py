@@ -1,4 +1,8 @@
-"""Beam selection at logits of any size against float64 on the GPU: what masks by -1e10 and the like leave."""
+"""Beam selection at logits of any size against float64 on the GPU: what masks by -1e10 and the like leave, and sums whose
+terms are all rounded the same way."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
@@ -64,3 +68,56 @@ def test_rows_about_a_large_value(middle):
     search = BeamSearch(6)
     check_step(search.select(logits, scores), shifted(logits), scores, 12, 6)
     search.check()
+
+
+# --------------------------------------------- sums rounded the same way in all terms
+def exponents(top, tail):
+    """What float32 makes of the exponents of tail under top, in two forms, less what they are (units of log2)."""
+    one = np.float32(1.4426950408889634)
+    exact = (tail.astype(np.float64) - top.astype(np.float64)) * 1.4426950408889634
+    apart = ((tail - top) * one).astype(np.float64)
+    unit = np.ceil(top * one) - np.float32(6)
+    fused = (tail.astype(np.float64) * np.float64(one) - unit).astype(np.float32).astype(np.float64)
+    return apart - exact, fused - (tail.astype(np.float64) * 1.4426950408889634 - unit)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [20000, 152704, 262144, 1 << 20])
+@pytest.mark.parametrize('form', [0, 1])
+@pytest.mark.parametrize('each', [0, 1024, 8192, 65536])
+def test_rows_whose_terms_are_rounded_alike(each, form, vocab, dtype):
+    """Two beams, each with one value (at one place, or every so many) above a tail of one other value, 6 to 14 below: all terms of
+    a sum have the same error.  The values are those of 4,000 pairs whose exponent is rounded up and down the most; the best
+    candidates of the two are 1e-8 to 6e-7 apart, both ways, and come in float64's order."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    rng = np.random.default_rng(vocab + form)
+    top = rng.uniform(0.5, 2.0, 4000).astype(np.float32)
+    tail = (top - rng.uniform(6.0, 14.0, 4000)).astype(np.float32)
+    if dtype == torch.bfloat16:
+        top, tail = (torch.tensor(x).to(dtype).float().numpy() for x in (top, tail))
+    count = vocab // each if each else 1
+    share = 1 / (1 + count / (vocab - count) * np.exp(top - tail))  # how much of the sum is the tail
+    order = np.argsort(exponents(top, tail)[form] * share)
+    gaps = [s * x for x in (1e-8, 3e-8, 1e-7, 2e-7, 4e-7, 6e-7) for s in (1, -1)]
+    pick = [(order[-1 - i % 3], order[i % 4]) for i in range(len(gaps))]
+    pick = [p if i % 4 < 2 else p[::-1] for i, p in enumerate(pick)]
+    logits = torch.empty(2 * len(gaps), vocab, dtype=dtype, device='cuda')
+    scores = torch.zeros(len(gaps), 2, device='cuda')
+    sums = []
+    for i, pair in enumerate(pick):
+        for j, p in enumerate(pair):
+            logits[2 * i + j] = float(tail[p])
+            logits[2 * i + j, 5::each or vocab] = float(top[p])
+            n = len(range(5, vocab, each or vocab))
+            sums.append(math.log(n + (vocab - n) * math.exp(float(tail[p]) - float(top[p]))))
+        scores[i, 1] = sums[-1] - sums[-2] - gaps[i]
+    value = -torch.tensor(sums, dtype=torch.float64).view(-1, 2) + scores.double().cpu()
+    first = (value[:, 1] > value[:, 0]).int()
+    away = value[:, 0] - value[:, 1]
+    rounded = 2.0 ** -24 * scores[:, 1].double().abs().cpu() + 1e-12  # of the second score
+    assert ((away - torch.tensor(gaps, dtype=torch.float64)).abs() <= rounded).all() and away.abs().min() > 1e-10
+    for items in (1, 3, len(gaps)):
+        for i in range(0, len(gaps), items):
+            step = BeamSearch(1).select(logits[2 * i:2 * (i + items)], scores[i:i + items].contiguous())
+            assert torch.equal(step.parents.cpu()[:, 0], first[i:i + items])
+            assert (step.tokens == 5).all()
