@@ -435,25 +435,28 @@ struct PickShared {
   };
   int n_quartets, n_groups, n_whole, n_lanes, n_list;
   int word2[BP_THREADS / 32];
-  uint32_t word[BP_THREADS / 32], reached;
+  uint32_t word[BP_THREADS / 32], reached, above;
   int most;  // the largest |off32|, as bits
 };
 
-// A value that at least k threads reach with what they have, and few more, or minus infinity where fewer have a finite one.  The
-// threads are counted by how far their keys lie behind the largest, in bins of 1/32 of that distance: one pass
-// and one scan (600 cycles; finding the value bit by bit, with a barrier each, 2,600).
-RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
+// A value that at least k of many reach, and few more, or minus infinity where fewer are finite; each(f) calls f with a thread's
+// values.  They are counted by how far their keys lie behind the largest, in bins of 1/32 of that distance: one pass
+// and one scan (with one value a thread 600 cycles; finding the value bit by bit, with a barrier each, 2,600).  FINER: by how far they
+// lie behind s.above, which a call leaves where its bin ends above.
+template <bool FINER, typename Each> RTR_DEVICE float reached_among(Each&& each, int k, PickShared& s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t key = mine > -INFINITY ? float_key(mine) : 0u;
+  const auto key_of = [](float v) { return v > -INFINITY ? float_key(v) : 0u; };
+  uint32_t key = 0;
+  if constexpr (!FINER) each([&](float v) { key = max(key, key_of(v)); });
   const uint32_t warp_most = __reduce_max_sync(0xffffffffu, key);
   s.bins[tid] = 0;
   if (lane == 0) s.word[warp] = warp_most;
   __syncthreads();
-  const uint32_t most = __reduce_max_sync(0xffffffffu, s.word[lane]);
-  if (key) {
-    const uint32_t bits = __float_as_uint((float)(most - key));
-    atomicAdd(&s.bins[bits ? min(BP_THREADS - 1, (int)(bits >> 18) - (127 << 5) + 1) : 0], 1);
-  }
+  const uint32_t most = FINER ? s.above : __reduce_max_sync(0xffffffffu, s.word[lane]);
+  each([&](float v) {
+    const uint32_t u = key_of(v), bits = __float_as_uint((float)(most - min(u, most)));
+    if (u) atomicAdd(&s.bins[bits ? min(BP_THREADS - 1, (int)(bits >> 18) - (127 << 5) + 1) : 0], 1);
+  });
   __syncthreads();
   const int c = s.bins[tid];
   int sum = c;
@@ -469,14 +472,21 @@ RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
   sum += __reduce_add_sync(0xffffffffu, before);
   // the last bin holds whatever is further away than it starts: no bound
   if (tid < BP_THREADS - 1 && sum >= k && sum - c < k) {
-    const float edge = __uint_as_float((uint32_t)(tid + (127 << 5)) << 18);  // where the next bin starts
-    s.reached = max(0x00800000u, most - min(most, tid ? (uint32_t)ceilf(edge) : 0u));  // no further than the least float
+    const auto behind = [&](int bin) {  // the key where a bin starts
+      return most - min(most, bin > 0 ? (uint32_t)ceilf(__uint_as_float((uint32_t)(bin - 1 + (127 << 5)) << 18)) : 0u);
+    };
+    s.reached = max(0x00800000u, tid ? behind(tid + 1) : most);  // no further than the least float
+    s.above = behind(tid);
   }
   __syncthreads();
   return s.reached ? key_float(s.reached) : -INFINITY;
 }
-
+// The same of one value a thread.
+RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
+  return reached_among<false>([&](auto&& f) { f(mine); }, k, s);
+}
 // What the usual path does not come by, out of line.
+template <typename T, bool MASK> __device__ __noinline__ void pick_closely(const BeamPick& a, PickShared& s);
 template <typename T, bool MASK> __device__ __noinline__ void pick_exactly(const BeamPick& a, PickShared& s);
 template <typename T, bool MASK> __device__ __noinline__ void pick_needs(const BeamPick& a, PickShared& s, int ng);
 template <typename T, bool MASK> __device__ __noinline__ void pick_whole(const BeamPick& a, PickShared& s);
@@ -522,9 +532,9 @@ template <typename T, bool MASK> struct Picker {
   }
   // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer: those that are not held,
   // and all
-  template <typename F> RTR_DEVICE void each_later_group(F&& f) const {
+  template <typename F> RTR_DEVICE void each_later_group(F&& f, int from = BP_HELD * BP_THREADS) const {
     const int quartets = a.padded >> 2, all = a.n * quartets;
-    for (int q = tid + BP_HELD * BP_THREADS; q < all; q += BP_THREADS) {
+    for (int q = tid + from; q < all; q += BP_THREADS) {
       const int r = a.n == 1 ? 0 : row_of((uint32_t)q);
       if (alive(r)) f(r, 4 * (q - r * quartets), __ldcg(reinterpret_cast<const float4*>(best) + q));
     }
@@ -674,8 +684,20 @@ template <typename T, bool MASK> struct Picker {
     __syncthreads();
   }
 
-  // What `near` may be off by (three roundings of 2^-24), with room, and what two sums may be.
-  RTR_DEVICE float slack(float t) const { return a.close + 4.77e-7f * (__int_as_float(s.most) + fabsf(t)); }
+  // How far below t, which k candidates reach by `near`, others may lie that have to be looked at: what two sums may be off by, and
+  // what `near` may (three roundings of 2^-24, with room).
+  RTR_DEVICE float slack_of(float t, float most) const { return a.close + 4.77e-7f * (most + fabsf(t)); }
+  RTR_DEVICE float slack(float t) const { return slack_of(t, __int_as_float(s.most)); }
+  // The same by the rows alone that can have a candidate there (none is worth more than its row's offset): one of a beam
+  // at -1e9 leaves no logit of the others out.  Whole warps.
+  RTR_DEVICE float least_slack(float t) const {
+    float most = 0.f;
+    for (int r = lane; r < a.n; r += 32) {
+      const float off = s.near[r].y;
+      if (off > -INFINITY && off + 4.77e-7f * (fabsf(off) + fabsf(t)) >= t) most = fmaxf(most, fabsf(off));
+    }
+    return slack_of(t, redux_max(most));
+  }
 
   // What the rows' logits have to reach for `near` to reach t, with room for its roundings.
   RTR_DEVICE void needs(float t) {
@@ -694,8 +716,7 @@ template <typename T, bool MASK> struct Picker {
     needs(t - slack(t));
   }
 
-  // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too
-  // many (ties).
+  // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too many.
   RTR_DEVICE bool gather() {
     if (tid == 0) s.n_quartets = s.n_groups = s.n_whole = s.n_lanes = s.n_list = 0;
     float mine = -INFINITY, of[BP_HELD];  // of: the held quartets' best
@@ -769,22 +790,28 @@ template <typename T, bool MASK> struct Picker {
       const int2 l = s.lane[i / L::PIECES];
       r = l.x >> 5;
       const int e = L::at(l.y, i % L::PIECES * L::PER, l.x & 31);
-      const uint4 u = e >= 0 && e + L::PER <= a.vocab ? __ldg(reinterpret_cast<const uint4*>(row(r) + e)) : beam_ragged(row(r), e, a.vocab);
-      bool ok[L::PER];
-      if constexpr (MASK) {
-#pragma unroll
-        for (int j = 0; j < L::PER; ++j) ok[j] = e + j >= 0 && e + j < a.vocab && mask(r)[e + j];
-      }
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
       const float x = s.need[r];
-#pragma unroll
-      for (int j = 0; j < L::PER; ++j) {
-        const float v = __uint_as_float(sizeof(T) == 4 ? w[j % 4] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-        if (v >= x && v > -INFINITY && (!MASK || ok[j])) add(r, e + j, v);
-      }
+      each_of_piece(r, e, [&](int j, float v) {
+        if (v >= x) add(r, e + j, v);
+      });
     }
     __syncthreads();
     return s.n_list <= BP_LIST;
+  }
+  // f(j, logit) for the finite, allowed logits of row r's piece at place e of the vocabulary
+  template <typename F> RTR_DEVICE void each_of_piece(int r, int e, F&& f) const {
+    const uint4 u = e >= 0 && e + L::PER <= a.vocab ? __ldg(reinterpret_cast<const uint4*>(row(r) + e)) : beam_ragged(row(r), e, a.vocab);
+    bool ok[L::PER];
+    if constexpr (MASK) {
+#pragma unroll
+      for (int j = 0; j < L::PER; ++j) ok[j] = e + j >= 0 && e + j < a.vocab && mask(r)[e + j];
+    }
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < L::PER; ++j) {
+      const float v = __uint_as_float(sizeof(T) == 4 ? w[j % 4] : j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+      if (v > -INFINITY && (!MASK || ok[j])) f(j, v);
+    }
   }
   RTR_DEVICE void add_lane(int r, int first, int lane_) {
     const int to = atomicAdd(&s.n_lanes, 1);
@@ -794,6 +821,70 @@ template <typename T, bool MASK> struct Picker {
     each_read(s.n_whole, [&](int r, int first, const L& raw, const Allowed<T>&, int) {
       if (raw.largest() >= s.need[r]) add_lane(r, first, lane);
     });
+  }
+
+  // Where these are too many the bound was too low: threads stand for several groups, so where most of the k best are
+  // candidates of few rows (the other beams are far behind), a row of another has the k-th best thread.  Here every group counts, and then
+  // every logit of the groups that reach the bound; false where there are too many still (ties).  (50 beams of 152,704, one 6 or more
+  // ahead of the others: 49 - 52 us a call; with each row's sum in 64 bits and the exact search below 2,680.)
+  RTR_DEVICE bool gather_closely() {
+    const auto groups = [&](auto&& f) {
+      each_later_group([&](int r, int g0, const float4& v) {
+        f(near(r, v.x), r, g0);
+        f(near(r, v.y), r, g0 + 1);
+        f(near(r, v.z), r, g0 + 2);
+        f(near(r, v.w), r, g0 + 3);
+      }, 0);
+    };
+    const auto by_groups = [&](auto&& f) { groups([&](float v, int, int) { f(v); }); };
+    const auto too_many = [&](float least) {  // or the list of those that reach it
+      if (tid == 0) s.n_groups = 0;
+      __syncthreads();
+      groups([&](float v, int r, int g) {
+        if (!(v > -INFINITY) || v < least) return;
+        const int to = atomicAdd(&s.n_groups, 1);
+        if (to < BP_GROUPS) s.groups[to] = r * a.padded + g;
+      });
+      __syncthreads();
+      return s.n_groups > BP_GROUPS;
+    };
+    const auto logits = [&](float least, auto&& f) {  // a piece at a time: registers that are taken here are saved on the usual path
+      for (int i = warp; i < s.n_groups * L::PIECES; i += BP_THREADS / 32) {
+        const int id = s.groups[i / L::PIECES], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
+        const int e = L::at((id - r * a.padded) * L::GROUP - L::shift(row(r)), i % L::PIECES * L::PER, lane);
+        each_of_piece(r, e, [&](int j, float x) {
+          if (near(r, x) >= least) f(r, e + j, x);
+        });
+      }
+    };
+    const auto by_logits = [&](float least) {
+      return [&, least](auto&& f) { logits(least, [&](int r, int, float x) { f(near(r, x)); }); };
+    };
+    float t = reached_among<false>(by_groups, a.k, s);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, s.word[lane]);  // the largest of all, of groups or logits
+    bool many = too_many(t - least_slack(t));
+    for (int i = 0; i < 2 && many; ++i) {
+      t = fmaxf(t, reached_among<true>(by_groups, a.k, s));
+      many = too_many(t - least_slack(t));
+    }
+    if (many) {  // the groups above those (fewer than k) may have k better logits
+      too_many(nextafterf(key_float(s.above), INFINITY));
+      if (tid == 0) s.above = top;
+      t = fmaxf(t, reached_among<true>(by_logits(-INFINITY), a.k, s));
+      if (too_many(t - least_slack(t))) return false;
+    }
+    const float least = t - least_slack(t);
+    if (tid == 0) s.above = top;
+    for (int i = 0; i < 2; ++i) {
+      t = fmaxf(t, reached_among<true>(by_logits(least), a.k, s));
+      if (tid == 0) s.n_list = 0;
+      __syncthreads();
+      logits(t - least_slack(t), [&](int r, int at, float x) { add(r, at, x); });
+      __syncthreads();
+      if (s.n_list <= BP_LIST) return true;
+      __syncthreads();
+    }
+    return false;
   }
 
   RTR_DEVICE int block_count(int mine) {
@@ -919,6 +1010,9 @@ template <typename T, bool MASK> RTR_DEVICE Picker<T, MASK> picker(const BeamPic
   return Picker<T, MASK>{a, s, (int)blockIdx.x, tid, tid >> 5, tid & 31, static_cast<const T*>(a.logits) + row0 * a.stride,
                          MASK ? a.allowed + row0 * a.allowed_stride : nullptr, a.best + row0 * a.padded, {}};
 }
+template <typename T, bool MASK> __device__ __noinline__ void pick_closely(const BeamPick& a, PickShared& s) {
+  if (!picker<T, MASK>(a, s).gather_closely()) pick_exactly<T, MASK>(a, s);
+}
 template <typename T, bool MASK> __device__ __noinline__ void pick_exactly(const BeamPick& a, PickShared& s) {
   picker<T, MASK>(a, s).gather_exactly();
 }
@@ -983,7 +1077,7 @@ __global__ void __launch_bounds__(BP_THREADS) beam_pick_kernel(const __grid_cons
   Picker<T, MASK> p = picker<T, MASK>(a, s);
   p.hold();
   p.offsets();
-  if (!p.gather()) pick_exactly<T, MASK>(a, s);
+  if (!p.gather()) pick_closely<T, MASK>(a, s);
   p.put_in_order();
   if (p.doubtful()) {
     pick_again<T, MASK>(a, s);

@@ -1,5 +1,5 @@
-"""Beam selection at logits of any size against float64 on the GPU: what masks by -1e10 and the like leave, and sums whose
-terms are all rounded the same way."""
+"""Beam selection at logits and scores of any size, against float64 on the GPU: what masks by -1e10 and the like leave, sums whose
+terms are all rounded the same way, beams far behind the best."""
 import math
 
 import numpy as np
@@ -121,3 +121,62 @@ def test_rows_whose_terms_are_rounded_alike(each, form, vocab, dtype):
             step = BeamSearch(1).select(logits[2 * i:2 * (i + items)], scores[i:i + items].contiguous())
             assert torch.equal(step.parents.cpu()[:, 0], first[i:i + items])
             assert (step.tokens == 5).all()
+
+
+# ------------------------------------------------------ scores of any size
+def spread_scores(items, n, far, seed):
+    """Beams most of which are far behind: the first of an item alone, or two of them, as a search starts."""
+    s = far - torch.rand(items, n, generator=generator(seed), device='cuda')
+    s[:, 0] = -0.5
+    if n > 3:
+        s[::2, 3] = -1.25
+    return s
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('far', [-6.0, -20.0, -100.0, -1e4, -1e9, -1e30])
+@pytest.mark.parametrize('items,n,vocab,k', [(1, 50, 152704, 100), (3, 50, 32003, 100), (2, 128, 4000, 256), (2, 128, 32000, 256), (9, 10, 70001, 20), (4, 12, 900, 256),
+                                             (2, 4, 152833, 256)])
+def test_beams_far_behind(items, n, vocab, k, far, dtype):
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    logits, _ = inputs(items, n, vocab, dtype, 41)
+    scores = spread_scores(items, n, far, 42)
+    search = BeamSearch(n, candidates=k)
+    check_step(search.select(logits, scores), logits, scores, k, n)
+    logits.view(items, n, -1)[:] = logits.view(items, n, -1)[:, :1].clone()  # and the same logits for all of them
+    check_step(search.select(logits, scores), logits, scores, k, n)
+    search.check()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_a_far_score_above(dtype):
+    """A beam far above the others takes all places that it has candidates for."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    for far in (30.0, 1e4, 1e9):
+        logits, scores = inputs(2, 8, 20011, dtype, 43)
+        scores[:, 5] += far
+        check_step(BeamSearch(8).select(logits, scores), logits, scores, 16, 8)
+
+
+@pytest.mark.parametrize('far', [-20.0, -100.0, -1e9])
+def test_beams_far_behind_take_no_longer(far):
+    """At most six times what beams of a kind take (summing every row again, and finding the best bit by bit, is more than a hundred)."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    logits, near = inputs(1, 50, 152704, torch.float32, 44)
+    scores = spread_scores(1, 50, far, 45)
+    search = BeamSearch(50)
+
+    def took(s):
+        best = math.inf
+        for _ in range(5):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            search.select(logits, s)
+            start.record()
+            for _ in range(10):
+                search.select(logits, s)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best
+
+    assert took(scores) <= 6 * took(near)
