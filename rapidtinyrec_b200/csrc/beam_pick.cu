@@ -437,6 +437,7 @@ struct PickShared {
   int word2[BP_THREADS / 32];
   uint32_t word[BP_THREADS / 32], reached, above;
   int most;  // the largest |off32|, as bits
+  int wild;  // whether a row's largest logit or its offset is above 1e30
 };
 
 // A value that at least k of many reach, and few more, or minus infinity where fewer are finite; each(f) calls f with a thread's
@@ -508,6 +509,9 @@ template <typename T, bool MASK> struct Picker {
   RTR_DEVICE double worth(int r, float x) const { return ((double)x - (double)s.near[r].x) + s.off[r]; }
   RTR_DEVICE float near(int r, float x) const { return (x - s.near[r].x) + s.near[r].y; }
   RTR_DEVICE bool alive(int r) const { return s.near[r].y > -INFINITY; }
+  // A value below float32's range counts as minus infinity.  Where none of an item's rows reaches 1e30 by a logit or its offset, those
+  // are the ones that `near` has as minus infinity.
+  RTR_DEVICE static bool counts(double value) { return (float)value > -INFINITY; }
 
   // The thread's quartets of groups: the first ones are held in registers, from the start of the kernel.  Where there is not one for
   // every thread, groups are dealt one by one, as quartets whose others are minus infinity: the fewer a thread has, the nearer
@@ -530,24 +534,15 @@ template <typename T, bool MASK> struct Picker {
     for (int j = 0; j < BP_HELD; ++j)
       if (holds(j)) held[j] = __ldcg(reinterpret_cast<const float4*>(best) + held_at(j));
   }
-  // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer: those that are not held,
-  // and all
-  template <typename F> RTR_DEVICE void each_later_group(F&& f, int from = BP_HELD * BP_THREADS) const {
+  // f(row, first group, best logits) for the thread's quartets, of rows that have something to offer: all, or those that are not held
+  template <typename F> RTR_DEVICE void each_group(F&& f, int from = 0) const {
     const int quartets = a.padded >> 2, all = a.n * quartets;
     for (int q = tid + from; q < all; q += BP_THREADS) {
       const int r = a.n == 1 ? 0 : row_of((uint32_t)q);
       if (alive(r)) f(r, 4 * (q - r * quartets), __ldcg(reinterpret_cast<const float4*>(best) + q));
     }
   }
-  template <typename F> RTR_DEVICE void each_group(F&& f) const {
-    const int quartets = a.padded >> 2;
-#pragma unroll
-    for (int j = 0; j < BP_HELD; ++j) {
-      const int q = held_at(j), r = !holds(j) || a.n == 1 ? 0 : row_of((uint32_t)q);
-      if (holds(j) && alive(r)) f(r, 4 * (q - r * quartets), held[j]);
-    }
-    each_later_group(f);
-  }
+  template <typename F> RTR_DEVICE void each_later_group(F&& f) const { each_group(f, BP_HELD * BP_THREADS); }
 
   // f(row, first place, logits, mask) for the warp's groups of the list
   template <typename F> RTR_DEVICE void each_read(int ng, F&& f) const {
@@ -561,18 +556,20 @@ template <typename T, bool MASK> struct Picker {
       f(r, first, raw, ok, by);
     }
   }
-  // f(row, place in the vocabulary, logit) for the lane's finite, allowed logits of these groups
+  // f(row, place in the vocabulary, logit) for the finite, allowed logits of the groups of the list, a piece a lane at a time
+  // (registers that are taken here are saved on the usual path)
   template <typename F> RTR_DEVICE void each_logit(int ng, F&& f) const {
-    each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>& ok, int by) {
-#pragma unroll
-      for (int i = 0; i < L::EACH; ++i) {
-        const float v = raw.one(i);
-        if (v > -INFINITY && (!MASK || ok(i, by))) f(r, L::at(first, i, lane), v);
-      }
-    });
+    for (int i = warp; i < ng * L::PIECES; i += BP_THREADS / 32) {
+      const int id = s.groups[i / L::PIECES], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
+      const int e = L::at((id - r * a.padded) * L::GROUP - L::shift(row(r)), i % L::PIECES * L::PER, lane);
+      each_of_piece(r, e, [&](int j, float x) { f(r, e + j, x); });
+    }
   }
   RTR_DEVICE const uint8_t* mask(int r) const { return allowed0 + r * a.allowed_stride; }
   RTR_DEVICE void add(int r, int v, float x) {
+    if (near(r, x) > -INFINITY) put(r, v, x);
+  }
+  RTR_DEVICE void put(int r, int v, float x) {
     const int to = atomicAdd(&s.n_list, 1);
     if (to >= BP_LIST) return;
     s.x[to] = x;
@@ -597,7 +594,7 @@ template <typename T, bool MASK> struct Picker {
     for (int i = part + lanes; there && i < a.slices; i += lanes) t += beam_relative(__ldcg(p + i), all);
 #pragma unroll 1
     for (int d = 1; d < lanes; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-    if (tid == 0) s.most = 0;
+    if (tid == 0) s.most = s.wild = 0;
     __syncthreads();
     if (there && part == 0) {
       const bool wrong = !(score < INFINITY) || (score > -INFINITY && !(t >= 0.0 && all < INFINITY));
@@ -614,6 +611,7 @@ template <typename T, bool MASK> struct Picker {
       s.near[r] = make_float2(all, (float)s.off[r]);
       s.again[r] = s.done[r] = 0;
       if (alive) atomicMax(&s.most, __float_as_int(fabsf((float)s.off[r])));
+      if (alive && fmaxf(all, (float)s.off[r]) > 1e30f) s.wild = 1;
     }
     __syncthreads();
   }
@@ -711,13 +709,18 @@ template <typename T, bool MASK> struct Picker {
   // Too few threads have groups for a bound: their lanes' best may give one.
   RTR_DEVICE void needs_by_lanes(int ng) {
     float mine = -INFINITY;
-    each_logit(ng, [&](int r, int, float x) { mine = fmaxf(mine, near(r, x)); });
+    each_read(ng, [&](int r, int, const L& raw, const Allowed<T>& ok, int by) {
+      float x = raw.largest();
+      if constexpr (MASK) x = ok.largest(raw, by);
+      mine = fmaxf(mine, near(r, x));
+    });
     const float t = reached_by(mine, a.k, s);
     needs(t - slack(t));
   }
 
   // The groups and then the candidates that reach the k-th best of what stands for them: false where there are too many.
   RTR_DEVICE bool gather() {
+    if (s.wild) return false;
     if (tid == 0) s.n_quartets = s.n_groups = s.n_whole = s.n_lanes = s.n_list = 0;
     float mine = -INFINITY, of[BP_HELD];  // of: the held quartets' best
 #pragma unroll
@@ -828,13 +831,14 @@ template <typename T, bool MASK> struct Picker {
   // every logit of the groups that reach the bound; false where there are too many still (ties).  (50 beams of 152,704, one 6 or more
   // ahead of the others: 49 - 52 us a call; with each row's sum in 64 bits and the exact search below 2,680.)
   RTR_DEVICE bool gather_closely() {
+    if (s.wild) return false;
     const auto groups = [&](auto&& f) {
-      each_later_group([&](int r, int g0, const float4& v) {
+      each_group([&](int r, int g0, const float4& v) {
         f(near(r, v.x), r, g0);
         f(near(r, v.y), r, g0 + 1);
         f(near(r, v.z), r, g0 + 2);
         f(near(r, v.w), r, g0 + 3);
-      }, 0);
+      });
     };
     const auto by_groups = [&](auto&& f) { groups([&](float v, int, int) { f(v); }); };
     const auto too_many = [&](float least) {  // or the list of those that reach it
@@ -848,14 +852,10 @@ template <typename T, bool MASK> struct Picker {
       __syncthreads();
       return s.n_groups > BP_GROUPS;
     };
-    const auto logits = [&](float least, auto&& f) {  // a piece at a time: registers that are taken here are saved on the usual path
-      for (int i = warp; i < s.n_groups * L::PIECES; i += BP_THREADS / 32) {
-        const int id = s.groups[i / L::PIECES], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
-        const int e = L::at((id - r * a.padded) * L::GROUP - L::shift(row(r)), i % L::PIECES * L::PER, lane);
-        each_of_piece(r, e, [&](int j, float x) {
-          if (near(r, x) >= least) f(r, e + j, x);
-        });
-      }
+    const auto logits = [&](float least, auto&& f) {
+      each_logit(s.n_groups, [&](int r, int at, float x) {
+        if (near(r, x) >= least) f(r, at, x);
+      });
     };
     const auto by_logits = [&](float least) {
       return [&, least](auto&& f) { logits(least, [&](int r, int, float x) { f(near(r, x)); }); };
@@ -921,7 +921,6 @@ template <typename T, bool MASK> struct Picker {
     }
   }
   RTR_DEVICE void gather_exactly() {
-    hold();
     for (int r = tid; r < a.n; r += BP_THREADS) s.again[r] = a.n > 1 && s.off[r] > -INFINITY;
     __syncthreads();
     sum_again(1);
@@ -931,7 +930,7 @@ template <typename T, bool MASK> struct Picker {
       each_group([&](int r, int g0, const float4& v) {
         const float w[4] = {v.x, v.y, v.z, v.w};
         for (int i = 0; i < 4; ++i)
-          if (w[i] > -INFINITY && g0 + i < a.groups) f(double_key(worth(r, w[i])), (uint32_t)(r * a.padded + g0 + i));
+          if (w[i] > -INFINITY && g0 + i < a.groups && counts(worth(r, w[i]))) f(double_key(worth(r, w[i])), (uint32_t)(r * a.padded + g0 + i));
       });
     };
     bisect(groups, a.k, least, last);
@@ -945,14 +944,15 @@ template <typename T, bool MASK> struct Picker {
     });
     __syncthreads();
     const int ng = min(s.n_groups, BP_GROUPS);
-    const auto logits = [&](auto&& f) {
-      each_logit(ng, [&](int r, int v, float x) { f(double_key(worth(r, x)), (uint32_t)r * a.vocab + v); });
+    const auto logits = [&](auto&& f) {  // the same ones in every pass: so no more than k are added
+      each_logit(ng, [&](int r, int v, float x) {
+        const double value = worth(r, x);
+        if (counts(value)) f(double_key(value), (uint32_t)r * a.vocab + v, r, v, x);
+      });
     };
-    bisect(logits, a.k, least, last);
-    each_logit(ng, [&](int r, int v, float x) {
-      const uint64_t key = double_key(worth(r, x));
-      const uint32_t at = (uint32_t)r * a.vocab + v;
-      if (key > least || (key == least && at < last)) add(r, v, x);
+    bisect([&](auto&& f) { logits([&](uint64_t key, uint32_t at, int, int, float) { f(key, at); }); }, a.k, least, last);
+    logits([&](uint64_t key, uint32_t at, int r, int v, float x) {
+      if (key > least || (key == least && at < last)) put(r, v, x);
     });
     __syncthreads();
   }

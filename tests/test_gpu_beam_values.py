@@ -1,5 +1,5 @@
 """Beam selection at logits and scores of any size, against float64 on the GPU: what masks by -1e10 and the like leave, sums whose
-terms are all rounded the same way, beams far behind the best."""
+terms are all rounded the same way, beams far behind the best, values below float32's range."""
 import math
 
 import numpy as np
@@ -180,3 +180,44 @@ def test_beams_far_behind_take_no_longer(far):
         return best
 
     assert took(scores) <= 6 * took(near)
+
+
+def check_range(logits, scores, beams):
+    """The order is that of the values rounded to float32 where these are below its range, by beam and token."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    items, k, vocab = scores.shape[0], 2 * beams, logits.shape[1]
+    search = BeamSearch(beams)
+    step = search.select(logits, scores)
+    value = shifted(logits)
+    value = value - value.logsumexp(1, keepdim=True) + scores.double().view(-1, 1)
+    value = torch.where(value.float() == -math.inf, -math.inf, value)
+    value, place = value.view(items, -1).sort(dim=1, descending=True, stable=True)
+    assert torch.equal(step.all_parents.long() * vocab + step.all_tokens.long(), place[:, :k])
+    assert torch.equal(step.all_scores == -math.inf, value[:, :k] == -math.inf)
+    search.check()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('top', [1e30, 1e32, 1e37])
+def test_values_below_the_range_of_float32(top, dtype):
+    """A candidate whose value is below float32's range counts as minus infinity: it ranks by beam and token with the others."""
+    logits = torch.full((4, 9001), torch.finfo(dtype).min, dtype=dtype, device='cuda')
+    logits[0, 5000] = top
+    logits[0, 5001:5005] = -top
+    logits[1, 4000] = top
+    logits[2:, 8000] = 0
+    check_range(logits, torch.tensor([[-1.0, -2.0], [-1.0, -math.inf]], device='cuda'), 8)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('few', [3, 40])
+def test_scores_and_logits_at_the_lowest_value(few, dtype):
+    """Beams set aside by float32's lowest value, logits masked by their type's: both together are below the range."""
+    logits, scores = inputs(3, 4, 9001, dtype, 51)
+    keep = torch.zeros(9001, dtype=torch.bool, device='cuda')
+    keep[torch.randperm(9001, generator=generator(few), device='cuda')[:few]] = True
+    logits = torch.where(keep, logits, torch.finfo(dtype).min)
+    scores[:, 1:] = torch.finfo(torch.float32).min
+    scores[2] = torch.finfo(torch.float32).min
+    check_range(logits, scores, 8)
+    check_range(logits, scores, 128)
