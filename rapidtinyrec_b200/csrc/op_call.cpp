@@ -221,9 +221,9 @@ PyObject* call_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
     } else {
       if (two) {
-        if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != 2) refuse("out must be a pair of tensors");
-        out[0] = tensor(PyTuple_GET_ITEM(a[9], 0), "out");
-        out[1] = tensor(PyTuple_GET_ITEM(a[9], 1), "out");
+        if ((!PyTuple_Check(a[9]) && !PyList_Check(a[9])) || PySequence_Fast_GET_SIZE(a[9]) != 2) refuse("out must be a pair of tensors");
+        out[0] = tensor(PySequence_Fast_GET_ITEM(a[9], 0), "out");
+        out[1] = tensor(PySequence_Fast_GET_ITEM(a[9], 1), "out");
       } else {
         out[0] = tensor(a[9], "out");
       }

@@ -240,3 +240,20 @@ def test_refusals():
             ((q, 3, at), {}, 'k must be a tensor'), (('q', k, at), {}, 'q must be a tensor')]:
         with pytest.raises(ValueError, match=says):
             rotary.rotate(*args, **kw)
+
+
+def test_a_pair_is_a_tuple_or_a_list():
+    from rapidtinyrec_b200.rotary import Rotary
+    rotary = Rotary(64)
+    q, k = rows_of(6, 4, 64, torch.float32, 1), rows_of(6, 2, 64, torch.float32, 2)
+    at = torch.arange(6, dtype=torch.int32, device='cuda')
+    want = rotary.rotate(q, k, at)
+    room = [torch.empty_like(q), torch.empty_like(k)]
+    got = rotary.rotate(q, k, at, out=room)
+    assert got[0].data_ptr() == room[0].data_ptr() and got[1].data_ptr() == room[1].data_ptr()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    rotary.rotate(q, k, at, out=[q, k])
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    for out in ([q], [q, k, k], (q,), [q, 'k']):
+        with pytest.raises(ValueError, match='pair|tensor'):
+            rotary.rotate(q, k, at, out=out)
