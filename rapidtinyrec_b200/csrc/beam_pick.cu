@@ -96,25 +96,6 @@ RTR_DEVICE float beam_relative(const float2& part, float top) {  // part: a base
   if (part.x == top || part.y == 0.f) return part.y;
   return part.y * (beam_near(part.x) && beam_near(top) ? beam_near_scale(part.x, top) : beam_far_scale(part.x, top));
 }
-// e^d for d from -100 to 0: e^(n log 2 + f) with n the nearest whole number, f at most 0.347 and e^f its Taylor series up to f^10 / 10!
-// (off by 2.2e-13 at most).  Sixteen fp64 operations with the subtraction and the sum; exp() made two rows of 152,704 take 95 us.
-RTR_DEVICE double exp_of(double d) {
-  const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to whole numbers, in the low bits
-  const double z = fma(d, 1.4426950408889634, whole), n = z - whole, f = fma(n, -0.69314718055994531, d);
-  double e = 1.0 / 3628800.0;
-  e = fma(e, f, 1.0 / 362880.0);
-  e = fma(e, f, 1.0 / 40320.0);
-  e = fma(e, f, 1.0 / 5040.0);
-  e = fma(e, f, 1.0 / 720.0);
-  e = fma(e, f, 1.0 / 120.0);
-  e = fma(e, f, 1.0 / 24.0);
-  e = fma(e, f, 1.0 / 6.0);
-  e = fma(e, f, 0.5);
-  e = fma(e, f, 1.0);
-  e = fma(e, f, 1.0);
-  return __hiloint2double(__double2hiint(e) + (__double2loint(z) << 20), __double2loint(e));
-}
-
 struct BeamSum {
   double sum;
   float base;
@@ -258,20 +239,29 @@ template <typename T> struct Allowed {
   }
 };
 
-// The sum of the exponentials of a warp's groups relative to m, the slice's largest logit, where that is beyond 2^21.
+// The sum of the exponentials of a warp's groups relative to m, the slice's largest logit, where that is beyond 2^21: exponents are
+// rounded about 8 as above.  (50 rows of 152,704 of which all but 1,000 are masked by -1e10: 46 us, by -1e4 42, by minus
+// infinity 22; with exponentials in 64 bits 57.)
 template <typename T> __device__ __noinline__ double beam_far_sum(const T* row, float m, int g, int hi, int vocab) {
   using L = Logits<T>;
+  const int lane = threadIdx.x & 31, shift = L::shift(row);
+  const float2 less = make_float2(-m, -m), log2e = make_float2(BP_LOG2E, BP_LOG2E), eight = make_float2(8.f, 8.f);
   double sum = 0.0;
+  L next;
+  if (g < hi) next.load(row, g * L::GROUP - shift, lane, vocab);
   for (; g < hi; g += BP_WARPS) {
-    L raw;
-    raw.load(row, g * L::GROUP - L::shift(row), threadIdx.x & 31, vocab);
+    const L raw = next;
+    if (g + BP_WARPS < hi) next.load(row, (g + BP_WARPS) * L::GROUP - shift, lane, vocab);
+    float2 part[4];
 #pragma unroll
-    for (int i = 0; i < L::EACH; ++i) {
-      const float d = raw.one(i) - m;
-      sum += d == d ? exp_of(fmax((double)d, -100.0)) : (double)d;  // below e^-100 nothing counts: 2^20 of them are 2^-124 of the sum
+    for (int i = 0; i < L::EACH / 2; ++i) {
+      const float2 y = __ffma2_rn(__fadd2_rn(raw.two(i), less), log2e, eight), e = make_float2(ex2(y.x), ex2(y.y));
+      part[i & 3] = i < 4 ? e : __fadd2_rn(part[i & 3], e);
     }
+    const float2 more = __fadd2_rn(__fadd2_rn(part[0], part[1]), __fadd2_rn(part[2], part[3]));
+    sum += (double)more.x + more.y;
   }
-  return beam_warp_sum(sum);
+  return beam_warp_sum(sum) * 0x1p-8;
 }
 
 // One block: a slice of a row's groups, which its warps take in turn.  The groups that are all there come through a ring in shared
@@ -408,6 +398,25 @@ RTR_DEVICE uint64_t double_key(double d) {
 }
 RTR_DEVICE double key_double(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
+}
+
+// e^d for d from -100 to 0: e^(n log 2 + f) with n the nearest whole number, f at most 0.347 and e^f its Taylor series up to f^10 / 10!
+// (off by 2.2e-13 at most).  Sixteen fp64 operations with the subtraction and the sum; exp() made two rows of 152,704 take 95 us.
+RTR_DEVICE double exp_of(double d) {
+  const double whole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to whole numbers, in the low bits
+  const double z = fma(d, 1.4426950408889634, whole), n = z - whole, f = fma(n, -0.69314718055994531, d);
+  double e = 1.0 / 3628800.0;
+  e = fma(e, f, 1.0 / 362880.0);
+  e = fma(e, f, 1.0 / 40320.0);
+  e = fma(e, f, 1.0 / 5040.0);
+  e = fma(e, f, 1.0 / 720.0);
+  e = fma(e, f, 1.0 / 120.0);
+  e = fma(e, f, 1.0 / 24.0);
+  e = fma(e, f, 1.0 / 6.0);
+  e = fma(e, f, 0.5);
+  e = fma(e, f, 1.0);
+  e = fma(e, f, 1.0);
+  return __hiloint2double(__double2hiint(e) + (__double2loint(z) << 20), __double2loint(e));
 }
 
 struct PickEntry {  // a candidate in order: larger keys first, then lower places
@@ -845,7 +854,7 @@ template <typename T, bool MASK> struct Picker {
       if (tid == 0) s.n_groups = 0;
       __syncthreads();
       groups([&](float v, int r, int g) {
-        if (!(v > -INFINITY) || v < least) return;
+        if (!(v > -INFINITY) || v < least || *const_cast<volatile int*>(&s.n_groups) > BP_GROUPS) return;
         const int to = atomicAdd(&s.n_groups, 1);
         if (to < BP_GROUPS) s.groups[to] = r * a.padded + g;
       });
@@ -862,16 +871,19 @@ template <typename T, bool MASK> struct Picker {
     };
     float t = reached_among<false>(by_groups, a.k, s);
     const uint32_t top = __reduce_max_sync(0xffffffffu, s.word[lane]);  // the largest of all, of groups or logits
-    bool many = too_many(t - least_slack(t));
-    for (int i = 0; i < 2 && many; ++i) {
-      t = fmaxf(t, reached_among<true>(by_groups, a.k, s));
-      many = too_many(t - least_slack(t));
-    }
-    if (many) {  // the groups above those (fewer than k) may have k better logits
-      too_many(nextafterf(key_float(s.above), INFINITY));
+    if (too_many(t - least_slack(t))) {
+      // the groups above the k-th one's bin, fewer than k, may have k logits; or a closer look at the groups shows that fewer will do
+      const uint32_t above = s.above;
+      too_many(nextafterf(key_float(above), INFINITY));
       if (tid == 0) s.above = top;
       t = fmaxf(t, reached_among<true>(by_logits(-INFINITY), a.k, s));
-      if (too_many(t - least_slack(t))) return false;
+      bool many = too_many(t - least_slack(t));
+      if (many && tid == 0) s.above = above;
+      for (int i = 0; i < 2 && many; ++i) {
+        t = fmaxf(t, reached_among<true>(by_groups, a.k, s));
+        many = too_many(t - least_slack(t));
+      }
+      if (many) return false;
     }
     const float least = t - least_slack(t);
     if (tid == 0) s.above = top;
@@ -1141,7 +1153,7 @@ static const char* beam_check(const rtr_beam_step* b) {
 //  - a group's additions: 3 + 2 in bf16, 1 + 2 in fp32, and twice one where a group is more than all before it;
 //  - a slice's sum rounded to a float: 1; the logarithm of the rest: 0.75.
 // And what errs to one side, once: ex2.approx is off by -1.45e-7 to 1.46e-7 (all floats from -40 to 40 measured), log2(e) as a float by
-// 1.34e-8 of the exponent.  (Slices beyond 2^21 are summed in 64 bits.)  For 152,832 logits 2.3e-6 in bf16, 2.1e-6 in fp32.
+// 1.34e-8 of the exponent.  For 152,832 logits 2.3e-6 in bf16, 2.1e-6 in fp32.
 static float beam_close(int vocab, bool fp32) {
   const float spread = std::log((float)vocab);
   const float one = 6.9f + std::max(0.f, spread - 12.08f) + (fp32 ? 3.f : 5.f) + 2.f + 1.75f;

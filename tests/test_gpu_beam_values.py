@@ -158,6 +158,21 @@ def test_a_far_score_above(dtype):
         check_step(BeamSearch(8).select(logits, scores), logits, scores, 16, 8)
 
 
+def took(search, logits, scores):
+    """Of ten calls."""
+    best = math.inf
+    for _ in range(5):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        search.select(logits, scores)
+        start.record()
+        for _ in range(10):
+            search.select(logits, scores)
+        end.record()
+        end.synchronize()
+        best = min(best, start.elapsed_time(end))
+    return best
+
+
 @pytest.mark.parametrize('far', [-20.0, -100.0, -1e9])
 def test_beams_far_behind_take_no_longer(far):
     """At most six times what beams of a kind take (summing every row again, and finding the best bit by bit, is more than a hundred)."""
@@ -166,20 +181,31 @@ def test_beams_far_behind_take_no_longer(far):
     scores = spread_scores(1, 50, far, 45)
     search = BeamSearch(50)
 
-    def took(s):
-        best = math.inf
-        for _ in range(5):
-            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
-            search.select(logits, s)
-            start.record()
-            for _ in range(10):
-                search.select(logits, s)
-            end.record()
-            end.synchronize()
-            best = min(best, start.elapsed_time(end))
-        return best
+    assert took(search, logits, scores) <= 6 * took(search, logits, near)
 
-    assert took(scores) <= 6 * took(near)
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('value', [-1e4, -1e9, -math.inf, 'lowest'])
+@pytest.mark.parametrize('items,n,vocab,live', [(1, 50, 152704, 1000), (3, 50, 32003, 5), (9, 12, 70001, 300), (1, 128, 5003, 700)])
+def test_rows_of_which_a_mask_leaves_few_groups(items, n, vocab, live, value, dtype):
+    """Fewer groups of logits than candidates, whose best are asked for, and more that the mask has made equal."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    logits, scores = inputs(items, n, vocab, dtype, 61)
+    logits[:, live:] = torch.finfo(dtype).min if value == 'lowest' else value
+    search = BeamSearch(n)
+    check_step(search.select(logits, scores), shifted(logits), scores, 2 * n, n)
+    search.check()
+
+
+def test_masks_take_no_longer():
+    """At most six times what rows that are not masked take."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    logits, scores = inputs(1, 50, 152704, torch.float32, 62)
+    search = BeamSearch(50)
+    plain = took(search, logits, scores)
+    for value in (-1e4, -1e9, -math.inf, torch.finfo(torch.float32).min):
+        logits[:, 1000:] = value
+        assert took(search, logits, scores) <= 6 * plain
 
 
 def check_range(logits, scores, beams):
