@@ -385,7 +385,9 @@ __global__ void __launch_bounds__(BP_WARPS * 32, beam_blocks(MASK)) beam_scan_ke
   }
   if (warp == 0) {
     const BeamSum u = lane < BP_WARPS ? sums(lane) : BeamSum{0.0, -INFINITY};
-    const double t = beam_warp_sum(u.base == m ? u.sum : u.sum * beam_near_scale(u.base, m));
+    double t = u.base == m ? u.sum : u.sum * beam_near_scale(u.base, m);
+#pragma unroll
+    for (int d = BP_WARPS / 2; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
     if (lane == 0) a.part[blockIdx.x] = make_float2(m, (float)t);
   }
 }
@@ -449,11 +451,14 @@ struct PickShared {
   int wild;  // whether a row's largest logit or its offset is above 1e30
 };
 
+// A count in shared memory that other threads are adding to.
+RTR_DEVICE int so_far(const int& count) { return *const_cast<const volatile int*>(&count); }
+
 // A value that at least k of many reach, and few more, or minus infinity where fewer are finite; each(f) calls f with a thread's
 // values.  They are counted by how far their keys lie behind the largest, in bins of 1/32 of that distance: one pass
 // and one scan (with one value a thread 600 cycles; finding the value bit by bit, with a barrier each, 2,600).  FINER: by how far they
-// lie behind s.above, which a call leaves where its bin ends above.
-template <bool FINER, typename Each> RTR_DEVICE float reached_among(Each&& each, int k, PickShared& s) {
+// lie behind s.above, which a call leaves where its bin ends above.  MANY: values may be the same, and a bin that has k counts no more.
+template <bool FINER, bool MANY = true, typename Each> RTR_DEVICE float reached_among(Each&& each, int k, PickShared& s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const auto key_of = [](float v) { return v > -INFINITY ? float_key(v) : 0u; };
   uint32_t key = 0;
@@ -465,7 +470,8 @@ template <bool FINER, typename Each> RTR_DEVICE float reached_among(Each&& each,
   const uint32_t most = FINER ? s.above : __reduce_max_sync(0xffffffffu, s.word[lane]);
   each([&](float v) {
     const uint32_t u = key_of(v), bits = __float_as_uint((float)(most - min(u, most)));
-    if (u) atomicAdd(&s.bins[bits ? min(BP_THREADS - 1, (int)(bits >> 18) - (127 << 5) + 1) : 0], 1);
+    int* bin = &s.bins[bits ? min(BP_THREADS - 1, (int)(bits >> 18) - (127 << 5) + 1) : 0];
+    if (u && (!MANY || so_far(*bin) < k)) atomicAdd(bin, 1);
   });
   __syncthreads();
   const int c = s.bins[tid];
@@ -493,7 +499,7 @@ template <bool FINER, typename Each> RTR_DEVICE float reached_among(Each&& each,
 }
 // The same of one value a thread.
 RTR_DEVICE float reached_by(float mine, int k, PickShared& s) {
-  return reached_among<false>([&](auto&& f) { f(mine); }, k, s);
+  return reached_among<false, false>([&](auto&& f) { f(mine); }, k, s);
 }
 // What the usual path does not come by, out of line.
 template <typename T, bool MASK> __device__ __noinline__ void pick_closely(const BeamPick& a, PickShared& s);
@@ -518,9 +524,9 @@ template <typename T, bool MASK> struct Picker {
   RTR_DEVICE double worth(int r, float x) const { return ((double)x - (double)s.near[r].x) + s.off[r]; }
   RTR_DEVICE float near(int r, float x) const { return (x - s.near[r].x) + s.near[r].y; }
   RTR_DEVICE bool alive(int r) const { return s.near[r].y > -INFINITY; }
-  // A value below float32's range counts as minus infinity.  Where none of an item's rows reaches 1e30 by a logit or its offset, those
-  // are the ones that `near` has as minus infinity.
-  RTR_DEVICE static bool counts(double value) { return (float)value > -INFINITY; }
+  // A value below float32's range, which rounds to minus infinity, counts as that.  Where none of an item's rows reaches 1e30 by a
+  // logit or its offset, those are the ones that `near` has as minus infinity.
+  RTR_DEVICE static bool counts(double value) { return value > -0x1.ffffffp127; }
 
   // The thread's quartets of groups: the first ones are held in registers, from the start of the kernel.  Where there is not one for
   // every thread, groups are dealt one by one, as quartets whose others are minus infinity: the fewer a thread has, the nearer
@@ -565,9 +571,18 @@ template <typename T, bool MASK> struct Picker {
       f(r, first, raw, ok, by);
     }
   }
-  // f(row, place in the vocabulary, logit) for the finite, allowed logits of the groups of the list, a piece a lane at a time
-  // (registers that are taken here are saved on the usual path)
+  // f(row, place in the vocabulary, logit) for the finite, allowed logits of the groups of the list: a group a warp, or a piece a lane at
+  // a time (registers that are taken off the usual path are saved on it)
   template <typename F> RTR_DEVICE void each_logit(int ng, F&& f) const {
+    each_read(ng, [&](int r, int first, const L& raw, const Allowed<T>& ok, int by) {
+#pragma unroll
+      for (int i = 0; i < L::EACH; ++i) {
+        const float v = raw.one(i);
+        if (v > -INFINITY && (!MASK || ok(i, by))) f(r, L::at(first, i, lane), v);
+      }
+    });
+  }
+  template <typename F> RTR_DEVICE void each_logit_of_pieces(int ng, F&& f) const {
     for (int i = warp; i < ng * L::PIECES; i += BP_THREADS / 32) {
       const int id = s.groups[i / L::PIECES], r = a.n == 1 ? 0 : row_of((uint32_t)id >> 2);
       const int e = L::at((id - r * a.padded) * L::GROUP - L::shift(row(r)), i % L::PIECES * L::PER, lane);
@@ -589,7 +604,7 @@ template <typename T, bool MASK> struct Picker {
   // Each row's sum from its slices, and what its candidates are offset by: 8 to 32 lanes a row.
   RTR_DEVICE void offsets() {
     static_assert(BP_MAX_N * 8 == BP_THREADS, "a row for every eight threads");
-    const int bits = a.n > 64 ? 3 : a.n > 32 ? 4 : 5, lanes = 1 << bits, r = tid >> bits, part = tid & (lanes - 1);
+    const int bits = a.n > 64 || a.slices <= 8 ? 3 : a.n > 32 || a.slices <= 16 ? 4 : 5, lanes = 1 << bits, r = tid >> bits, part = tid & (lanes - 1);
     const bool there = r < a.n;
     const float score = there && part == 0 ? a.scores[item * a.n + r] : -INFINITY;
     const float2* p = a.part + ((int64_t)item * a.n + (there ? r : 0)) * a.slices;
@@ -854,7 +869,7 @@ template <typename T, bool MASK> struct Picker {
       if (tid == 0) s.n_groups = 0;
       __syncthreads();
       groups([&](float v, int r, int g) {
-        if (!(v > -INFINITY) || v < least || *const_cast<volatile int*>(&s.n_groups) > BP_GROUPS) return;
+        if (!(v > -INFINITY) || v < least || so_far(s.n_groups) > BP_GROUPS) return;
         const int to = atomicAdd(&s.n_groups, 1);
         if (to < BP_GROUPS) s.groups[to] = r * a.padded + g;
       });
@@ -862,7 +877,7 @@ template <typename T, bool MASK> struct Picker {
       return s.n_groups > BP_GROUPS;
     };
     const auto logits = [&](float least, auto&& f) {
-      each_logit(s.n_groups, [&](int r, int at, float x) {
+      each_logit_of_pieces(s.n_groups, [&](int r, int at, float x) {
         if (near(r, x) >= least) f(r, at, x);
       });
     };
@@ -872,6 +887,7 @@ template <typename T, bool MASK> struct Picker {
     float t = reached_among<false>(by_groups, a.k, s);
     const uint32_t top = __reduce_max_sync(0xffffffffu, s.word[lane]);  // the largest of all, of groups or logits
     if (too_many(t - least_slack(t))) {
+      if (float_key(t) >= top) return false;
       // the groups above the k-th one's bin, fewer than k, may have k logits; or a closer look at the groups shows that fewer will do
       const uint32_t above = s.above;
       too_many(nextafterf(key_float(above), INFINITY));
@@ -891,9 +907,12 @@ template <typename T, bool MASK> struct Picker {
       t = fmaxf(t, reached_among<true>(by_logits(least), a.k, s));
       if (tid == 0) s.n_list = 0;
       __syncthreads();
-      logits(t - least_slack(t), [&](int r, int at, float x) { add(r, at, x); });
+      logits(t - least_slack(t), [&](int r, int at, float x) {
+        if (so_far(s.n_list) <= BP_LIST) add(r, at, x);
+      });
       __syncthreads();
       if (s.n_list <= BP_LIST) return true;
+      if (float_key(t) >= top) return false;
       __syncthreads();
     }
     return false;
