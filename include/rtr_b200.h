@@ -461,12 +461,12 @@ int rtr_rotary(const rtr_rotary_rows* q, const rtr_rotary_rows* k, int64_t rows,
  * model of their own).  Item b has n beams: rows b * n .. of logits [items * n][logits_stride], scores [items][n].  The candidate
  * (i, v) is worth logits[i][v] - log sum_u exp logits[i][u] + scores[i] where allowed (bytes [items * n][allowed_stride],
  * NULL: everywhere; an allowed_stride of 0 is one row for all) is not 0, and minus infinity elsewhere.  all_* [items][k]: the k best, in
- * descending order, equal ones by i * vocab + v: token v, parent i, value rounded to float32.  next_* [items][beams]: the first
+ * descending order, equal ones by i * vocab + v: token v, parent i, value.  next_* [items][beams]: the first
  * `beams` of those whose token is not eos (eos < 0: none is).  A row whose score is minus infinity is not read.  A row
  * with a NaN or plus infinity among its logits, or such a score, is worth minus infinity throughout and sets 1 << 7 in `status` (a
- * device word).  The order is that of values computed in 64 bits (log sum exps that were
- * summed in 32 bits are summed again in 64 where two candidates are too close to tell).
- * A value below float32's range counts as minus infinity.
+ * device word).  The order is that of values computed in 64 bits: rows are summed in 32, and again in 64 where two candidates are
+ * closer than that may be off by.  The values are float32; those of rows that were not summed again are off by 1.4e-6 at most besides,
+ * and may differ in their last bits with the call's other rows.  A value below float32's range counts as minus infinity.
  * n 1 to 128, vocab 1 to 2^20, k 1 to 256 and at most n * vocab, beams at most k (with eos: k at least beams + n).  dtype float32 or bfloat16; the workspace (rtr_beam_select_workspace bytes, aligned to 16) is free again when the call's
  * kernels ran. */
 typedef struct {

@@ -59,8 +59,11 @@ class BeamSearch:
 
         Candidate (i, v) is worth ``log_softmax(logits[i])[v] + scores[i]`` where ``allowed`` (bool ``[items * n, vocab]``, or ``[vocab]`` for all
         rows) holds, minus infinity elsewhere: the softmax is over the whole vocabulary, as in the constrained request.
-        Equal ones rank by beam, then token.  The order is that of 64-bit arithmetic, the scores are rounded to float32 once.
-        A beam whose score is minus infinity has ended and is not read.  Beams with NaN or plus infinity among logits or
+        Equal ones rank by beam, then token.  The order within a call is that of 64-bit arithmetic.  The scores are float32, of sums
+        in 32 bits where nothing more was needed to tell candidates apart: off by 1.4e-6 at most besides their own rounding, and in their
+        last bits a row's may differ with the other rows of the call.
+        A beam whose score is minus infinity has ended and is not read; any other score is searched (-1e9 for beams that are to wait is right,
+        and slower where it leaves one beam alone).  Beams with NaN or plus infinity among logits or
         scores have nothing to offer, and ``check`` raises for them.  Where fewer than ``candidates`` are finite, the last have score minus
         infinity.  Returns ``BeamStep``.  The result carries no gradient.
         """

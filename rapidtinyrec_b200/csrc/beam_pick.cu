@@ -18,11 +18,14 @@
 // bound, both rows' sums are taken again in fp64 (rows whose fp32 sums are the same among them) and the list is put in order
 // again (two rows of 152,832: 63 us more by one block, some 25 by the four that are there in a batch; for one item in 80 or so): the
 // order is that of 64-bit arithmetic, however the rows were split.
-// What bounds it.  The first kernel: exponentials (XU 81 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 81 us, 5.96 TB/s;
+// What bounds it.  The first kernel: exponentials (XU 80 %) and issue slots (62 %), 1,600 rows of 152,832 in bf16 in 82 us, 5.96 TB/s;
 // without its exponentials it reads at 7.3 TB/s.  An eighth or a quarter of them on the FMA pipe instead: no change, and 3 us slower.
-// The second: latency, some 17,000 cycles, 8.5 us, for 50 beams: dependent loads (slices and groups, second bests, lanes' logits; 700
+// The second: latency, some 17,800 cycles, 9 us, for 50 beams: dependent loads (slices and groups, second bests, lanes' logits; 700
 // to 2,500 cycles each), code that comes from L2 as it is gone through once, and a dozen barriers of 1,024 threads (512 threads: 0.4 us
 // less for 4 beams, 0.9 more for 50).
+//
+// What the usual path is not made for: one beam far ahead of the others, masks that leave few groups (gather_closely, 25 to 50 us), and
+// ties that make its lists too long (gather_exactly: 0.4 ms for 4 rows of 8,192 equal logits, 1.8 ms for 50 of 152,832).
 #include <cuda_runtime.h>
 
 #include <cooperative_groups.h>
@@ -456,7 +459,7 @@ RTR_DEVICE int so_far(const int& count) { return *const_cast<const volatile int*
 
 // A value that at least k of many reach, and few more, or minus infinity where fewer are finite; each(f) calls f with a thread's
 // values.  They are counted by how far their keys lie behind the largest, in bins of 1/32 of that distance: one pass
-// and one scan (with one value a thread 600 cycles; finding the value bit by bit, with a barrier each, 2,600).  FINER: by how far they
+// and one scan (with one value a thread 1,200 cycles; finding the value bit by bit, with a barrier each, 2,600).  FINER: by how far they
 // lie behind s.above, which a call leaves where its bin ends above.  MANY: values may be the same, and a bin that has k counts no more.
 template <bool FINER, bool MANY = true, typename Each> RTR_DEVICE float reached_among(Each&& each, int k, PickShared& s) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1251,8 +1254,9 @@ int rtr_beam_select(const rtr_beam_step* step, void* workspace, int64_t workspac
   p.status = step->status;
   // Where there are eight items or more, of two rows at least (one row is never in doubt), an item is in doubt now and then (one in 80
   // or so), and summing its rows takes one block long where they are long (65,536 logits 14 us each): its block has others of a
-  // cluster beside it, on SMs that have no item.  (16 items of 10 rows of 32,003 without doubts: 14.7 us with one block each, 15.7
-  // with four.)
+  // cluster beside it, on SMs that have no item.  (One block : four, us, 24 calls.  16 items of 10 rows: of 32,003 without doubts 13.2 :
+  // 14.4, of 65,536, one with, 14.6 : 15.7, in the mean 15.7 : 16.2, and that one 41 : 27.  32 of 50 rows in the mean: of 32,003 49.8 : 49.7, of
+  // 65,536 60.3 : 58.5, of 131,072 96.2 : 87.4.)
   p.ranks = 1;
   if (step->items >= 8 && step->n > 1 && step->vocab >= 1 << 16)
     while (p.ranks < BP_RANKS && 2 * p.ranks * (int64_t)step->items <= on.sms) p.ranks *= 2;
