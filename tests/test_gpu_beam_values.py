@@ -247,3 +247,33 @@ def test_scores_and_logits_at_the_lowest_value(few, dtype):
     scores[2] = torch.finfo(torch.float32).min
     check_range(logits, scores, 8)
     check_range(logits, scores, 128)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('far', [-20.0, -1e9])
+@pytest.mark.parametrize('share', [0.5, 0.002])
+def test_beams_far_behind_with_lists_of_allowed_tokens(share, far, dtype):
+    """Rows that start at no multiple of 16 bytes, captured and replayed with other inputs."""
+    from rapidtinyrec_b200.beam_search import BeamSearch
+    items, n, vocab = 3, 30, 33001
+    room = torch.empty(items * n, vocab + 6, dtype=dtype, device='cuda')
+    logits, allowed = room[:, 3:3 + vocab], torch.empty(items * n, vocab, dtype=torch.bool, device='cuda')
+    scores = torch.zeros(items, n, device='cuda')
+    search = BeamSearch(n, eos=5)
+
+    def fill(seed):
+        made, _ = inputs(items, n, vocab, dtype, seed)
+        logits.copy_(made)
+        allowed.copy_(torch.rand(items * n, vocab, generator=generator(seed), device='cuda') < share)
+        scores.copy_(spread_scores(items, n, far, seed))
+
+    fill(71)
+    check_step(search.select(logits, scores, allowed=allowed), logits, scores, 2 * n, n, eos=5, allowed=allowed)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step = search.select(logits, scores, allowed=allowed)
+    for seed in (72, 73):
+        fill(seed)
+        graph.replay()
+        check_step(step, logits, scores, 2 * n, n, eos=5, allowed=allowed)
+    search.check()
